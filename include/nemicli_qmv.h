@@ -45,7 +45,8 @@ extern "C" {
 #define QMV_ERR_TOO_LARGE 8 /* a size beyond the fixed maximum of a no-allocation entry point */
 
 /* Bits of the device status word (qmv_device_status). */
-#define QMV_DEV_BAD_ADDRESS 1   /* an expert id was outside [0, n_exp) or an address-table entry misaligned */
+#define QMV_DEV_BAD_ADDRESS 1   /* an expert id was outside [0, n_exp) or an address-table entry misaligned; a cache
+                                   slot, page, position or length was out of range */
 
 int qmv_abi_version(void);
 const char* qmv_status_string(int status);
@@ -277,6 +278,89 @@ int64_t qmv_chain_workspace_bytes(void);
  * Replaces: nothing — it has no counterpart in the reference (whose decoder allocates through torch). */
 #define QMV_CHAIN_NOALLOC_MAX_STAGES 128
 int qmv_chain_noalloc(const qmv_stage* stages, int n_stages, void* stream);
+
+/* ---- quantised key / value cache and attention over it ---------------------------------------------- */
+
+/* A paged cache of n_kv heads of dim values (64, 96, 128 or 256).  A slot is page * P + place, P = `page` a
+ * power of two from 16 to 1024.  K and V are each Q4_0 (2) or Q8_0 (8), in blocks of 32 values along the head
+ * dimension with one fp16 scale: value = d * code.  Codes are stored with 8 or 128 added.  J = dim / 32, b = 4 (Q4_0)
+ * or 8 (Q8_0):
+ *   k       n_pages * n_kv * P * 4 * J * b bytes       [page][head][P][4 t][J][b]: values 8 t .. 8 t + 7 of block j
+ *   v       n_pages * n_kv * (P / 2) * 8 * J * b bytes [page][head][P / 2][8 g][J][b]: values 4 g .. 4 g + 3 of block j
+ *           of the tokens 2 i and 2 i + 1
+ *   scales  n_pages * n_kv * P * 2 * J fp16            [page][head][P][2][J]: K's, then V's
+ * In a Q4_0 K word value n sits at bit 16 (n & 1) + 4 (n >> 1), in a V word at bit 16 (token & 1) + 4 n; in the two
+ * Q8_0 K words in word n >> 2 at byte 2 (n & 1) + ((n & 3) >> 1), in the V words in word n >> 1 at byte
+ * 2 (token & 1) + (n & 1).  All three 16-byte aligned.  n_pages * P at most 2^40. */
+typedef struct qmv_kv_cache {
+    void* k;
+    void* v;
+    void* scales;
+    int64_t n_pages;
+    int n_kv;
+    int dim;
+    int page;
+    int k_type;
+    int v_type;
+} qmv_kv_cache;
+
+/* Quantise `rows` tokens into their slots: k, v rows of n_kv * dim values (dtype QMV_OUT_*), k_stride / v_stride
+ * values apart.  x is clamped to +-65504 and NaN counts as 0; Q4_0: d = fp16(x / -8) of the value of largest
+ * magnitude (the first), code = clamp(rint(x / d), -8, 7); Q8_0: d = fp16(max|x| / 127), code =
+ * clamp(rint(x / d), -127, 127); d = 0: code 0.  Slot -1 (any negative): a padding row, nothing written.  Slots of
+ * one call are distinct (of a slot named twice any mixture of the rows' blocks may stay).  With cos_table and
+ * sin_table ([n_positions][rot_dim / 2] fp32) K is rotated first by its row's position: value i pairs with
+ * i + rot_dim / 2, or 2 i with 2 i + 1 when paired != 0; y1 = x1 c - x2 s, y2 = x2 c + x1 s, each product and sum
+ * rounded to fp32; values from rot_dim on (a multiple of 8) stay.  With q (rows of n_q * dim values) the rotated
+ * queries go to q_out (dense, dtype's type; not q itself; without tables a copy).  Slots past the cache and
+ * positions outside the table: the row is not written (its queries become 0) and QMV_DEV_BAD_ADDRESS is set.  k, v, q:
+ * aligned to four values, strides multiples of 4; tables 16 bytes.  One launch.  Replaces: the cache write of
+ * ggufengine/mmvq.py:139-180 (rope_kv), whose cache is bf16. */
+int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride,
+                 long long v_stride, const long long* slots, long long rows, const float* cos_table,
+                 const float* sin_table, const long long* positions, long long n_positions, int rot_dim, int paired,
+                 const void* q, long long q_stride, int n_q, void* q_out, void* stream);
+
+/* The values d * code of the slots' tokens, rounded to dtype: k and v dense [rows][n_kv][dim], 16-byte aligned.
+ * Negative slots give zeros; slots past the cache too, and set QMV_DEV_BAD_ADDRESS.  One launch.  Replaces: nothing
+ * callable in the reference. */
+int qmv_kv_read(const qmv_kv_cache* cache, const long long* slots, long long rows, void* k, void* v, int dtype,
+                void* stream);
+
+/* Bytes of the workspace qmv_kv_attend needs for these sizes (0 for sizes it does not take). */
+int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, int n_seq, int max_new, int dtype);
+
+/* Causal attention of n_seq sequences over the cache: out = softmax(scale * q . k) v per query row and head, fp32
+ * statistics, q and out of type dtype (QMV_OUT_*).  Head h reads key head h / (n_heads / n_kv).  Sequence b: lens[b]
+ * tokens in the cache at the pages tables[b][0 .. table_width), the new ones (its query rows) last: rows
+ * starts[b] .. starts[b + 1] of q, or row b when starts is null.  Query i of n sits at position p = lens[b] - n + i and
+ * sees keys max(0, p - window + 1) .. p (window 0: from 0 on); one that sees none (p < 0) gives zeros.  q: rows of
+ * n_heads * dim values, q_stride apart (aligned to four values); out dense.  max_new: at least the longest run of new
+ * tokens (rows beyond it are not computed, QMV_DEV_BAD_ADDRESS is set).  Rows of out that no sequence covers stay
+ * as they are.  Table entries behind a sequence's last token are not read; pages outside the cache count as
+ * masked, lengths beyond the table are cut, and both set QMV_DEV_BAD_ADDRESS.  workspace: 256-byte aligned,
+ * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  The result does not depend on
+ * timing.  Replaces: ggufengine/mmvq.py:195-330 (attn1_teil, attn1_summe) over a quantised cache, for
+ * any number of tokens. */
+int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long q_stride, int n_heads,
+                  const int* tables, int table_width, const int* lens, const int* starts, int n_seq, long long n_rows,
+                  int max_new, float scale, int window, void* out, void* workspace, long long workspace_bytes,
+                  void* stream);
+
+/* The norms before and after a block with its gate and residual, any number of rows of n values (dtype QMV_OUT_*
+ * for y, h, gate, h_out and xn; norm weights fp32):
+ *     z = y rsqrt(mean(y^2) + eps) w_post     (w_post null: z = y)
+ *     h_out = h + rs * gate * z               (gate null: 1; gate_stride 0: one row for all)
+ *     xn = h_out rsqrt(mean(h_out^2) + eps) w_pre   (w_pre null: none)
+ * in fp32, each output rounded once (xn from the unrounded h_out).  y, h, gate: rows y_stride, h_stride, gate_stride
+ * values apart; h_out (may be h itself when h_stride == n) and xn dense.  With xq, xq2, xd, xs (n a multiple of 32)
+ * also the activation input of the fp32 xn.  n at most QMV_NORM_BLOCK_MAX.  One launch.  Replaces: norm_q8
+ * (ggufengine/mmvq.py:946-956) for blocks with a norm behind them and for several tokens. */
+#define QMV_NORM_BLOCK_MAX 32768
+int qmv_norm_block(const void* y, long long y_stride, const void* h, long long h_stride, const void* gate,
+                   long long gate_stride, const float* w_post, const float* w_pre, int dtype, float eps, float rs,
+                   long long rows, int n, void* h_out, void* xn, int8_t* xq, int8_t* xq2, float* xd, float* xs,
+                   void* stream);
 
 /* Values per unit of qmv_block_sums for a format (16 or 32; 0 for an unknown format). */
 int qmv_unit_values(int ggml_type);

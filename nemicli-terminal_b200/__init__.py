@@ -8,6 +8,7 @@ Module map (reference counterparts in ggufengine/):
     qlinear   -> qlinear.py       QuantLinear, build_quant_linear, quantizable
     layers    -> models/common.py PackedLinear, PackedExperts
     moe       -> models/moe.py    MoE FFN, router (models/baukasten.py:_auswahl)
+    kvcache   -> (new)            key / value cache held in 4 or 8 bits, attention over it
     shard     -> (new)            row-sharded projections and expert-sharded MoE over NCCL
 The CUDA kernels sit in csrc/ behind the C ABI of include/nemicli_qmv.h (libnemiqmv.so).
 """

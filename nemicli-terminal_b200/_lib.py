@@ -5,6 +5,7 @@ returns a non-zero status, a RuntimeError names the failure.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -49,6 +50,11 @@ _SIGNATURES = {
     "qmv_expert_combine": ([P, I, P, P, I, I, I, P, P], I),
     "qmv_mm_tc": ([I, P, I, I, P, I, I, P, P, LL, P], I),
     "qmv_moe_ffn": ([I, P, P, LL, I, P, LL, LL, P, P, I, I, P, I, LL, I, I, P, P, P], I),
+    "qmv_kv_write": ([P, P, P, I, LL, LL, P, LL, P, P, P, LL, I, I, P, LL, I, P, P], I),
+    "qmv_kv_read": ([P, P, LL, P, P, I, P], I),
+    "qmv_kv_attend_workspace_bytes": ([P, I, I, I, I], LL),
+    "qmv_kv_attend": ([P, P, I, LL, I, P, I, P, P, I, LL, I, ctypes.c_float, I, P, P, LL, P], I),
+    "qmv_norm_block": ([P, LL, P, LL, P, LL, P, P, I, ctypes.c_float, ctypes.c_float, LL, I, P, P, P, P, P, P, P], I),
 }
 
 ABI_VERSION = 2
@@ -104,6 +110,15 @@ def ptr(t) -> ctypes.c_void_p:
 
 def stream_ptr(device=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def on_device(device):
+    """Makes `device` the current one for a launch (a stream belongs to its own device only); nothing to do where it
+    is already."""
+    device = torch.device(device)
+    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def device_status(clear: bool = True, device=None) -> int:

@@ -10,6 +10,7 @@ meaning and return shapes, computed by this package's sm_100a kernels through th
 * `entpacken` — a block-format matrix unpacked to bf16 for long inputs (mmvq.py:931-940), every format.
 * `norm_q8`, `akt_q8` — the fused one-token producers of an Eingang (mmvq.py:946-966): RMS norm with the
   residual add, and the gated activation, each one launch that also quantises its output.
+* `norm_block` (new) — the norms before and after a block with its gate and residual, for any number of rows.
 * `mv_geteilt`, `mv_norm` (new) — up to four matrices on one single-token input in one launch;
   `mv_norm` forms norm_q8's RMS norm inside that launch (bit-identical to the two calls); with a
   `NextInput` the launch also forms the next matvec's input (quantised outputs, or SiLU·mul of two).
@@ -17,7 +18,8 @@ meaning and return shapes, computed by this package's sm_100a kernels through th
   layer (mmvq.py:969-1014) are not part of this package (the matvec path ends where attention begins).
   They are forwarded to an attention provider registered with `set_attention` (the reference's own
   module, for instance); without one `schritt_moeglich` is False and the reference's layer takes its
-  general path, whose projections still run here through PackedLinear / mv.
+  general path, whose projections still run here through PackedLinear / mv.  This package's own attention is
+  kvcache.KVCache (write, read, attend), over a paged cache held in 4 or 8 bits.
 
 Where the reference takes Q4_K and Q6_K only, these kernels take all twenty-six block formats of the path
 (`FORMATE`: the classic, K-quant, IQ, MXFP4, ternary and 1-bit formats).  Everything runs on torch's current stream and is CUDA-graph
@@ -430,6 +432,61 @@ def norm_q8(h: torch.Tensor, w: torch.Tensor, eps: float, rest: Optional[torch.T
                                        ctypes.c_float(eps), _lib.ptr(xn), *e.zeiger(), n, _lib.stream_ptr(h.device)),
                "qmv_norm_q8")
     return xn, e, (h_in if hn is None else hn)
+
+
+NORM_BLOCK_MAX = 32768                      # values a row of norm_block
+
+
+def norm_block(y: torch.Tensor, h: torch.Tensor, w_pre: Optional[torch.Tensor], eps: float,
+               w_post: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, rs: float = 1.0,
+               eingang: bool = False):
+    """The norms before and after a block with its gate and residual, in one launch, for M rows of n values:
+        z = RMS norm of the block's output y with w_post (without w_post: y)
+        h = h + rs * gate * z            (gate: (n,) for all rows or like y; None: 1)
+        x = RMS norm of the new h with w_pre, the next block's input (w_pre None: none)
+    y, h, gate: (M, n) or (n,) of one type (float32, bfloat16, float16), rows of any stride; w_post, w_pre
+    float32 (n,).  -> (x like y or None, Eingang of x or None, new h).  Sums and h are fp32 inside, each output is
+    rounded once.  eingang (n a multiple of 32): also the int8 activation input of the fp32 x, as norm_q8
+    gives it, for M rows.  New entry point: norm_q8 takes one row and has no norm behind the block."""
+    _need_cuda(y, "norm_block")
+    if y.dtype not in _OUT or y.dim() not in (1, 2) or y.shape[-1] == 0:
+        raise RuntimeError("norm_block: y (n,) or (M, n) of float32, bfloat16 or float16")
+    n = y.shape[-1]
+    if h.shape != y.shape or h.dtype != y.dtype or h.device != y.device:
+        raise RuntimeError(f"norm_block: h must be like y ({tuple(y.shape)}, {y.dtype}, {y.device})")
+    if gate is not None and (gate.shape not in (y.shape, (n,)) or gate.dtype != y.dtype or gate.device != y.device):
+        raise RuntimeError(f"norm_block: gate must be ({n},) or like y, of {y.dtype}")
+    for w in (w_post, w_pre):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (n,) or not w.is_contiguous() or w.device != y.device):
+            raise RuntimeError(f"norm_block: norm weights are contiguous float32 ({n},) on {y.device}")
+    if eingang and (w_pre is None or n % 32):
+        raise RuntimeError("norm_block: an Eingang needs w_pre and n a multiple of 32")
+    if n > NORM_BLOCK_MAX:
+        raise RuntimeError(f"norm_block: rows of at most {NORM_BLOCK_MAX} values (got {n})")
+
+    def rows(t):                          # the values of a row side by side, and the values between rows
+        t = t.reshape(1, n) if t.dim() == 1 else t
+        if t.stride(1) != 1 and n > 1 or t.shape[0] > 1 and t.stride(0) < n:
+            t = t.contiguous()
+        return t, (t.stride(0) if t.shape[0] > 1 else n)
+
+    M = 1 if y.dim() == 1 else y.shape[0]
+    y2, ys = rows(y)
+    h2, hs = rows(h)
+    g2, gs = (None, 0) if gate is None else rows(gate)
+    if gate is not None and gate.dim() < y.dim():
+        gs = 0
+    x = None if w_pre is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    new = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    e = Eingang(n=M * n, device=y.device) if eingang else None
+    if M:
+        with _lib.on_device(y.device):
+            _lib.check(_lib.load().qmv_norm_block(_lib.ptr(y2), ys, _lib.ptr(h2), hs, _lib.ptr(g2), gs, _lib.ptr(w_post),
+                                                  _lib.ptr(w_pre), _OUT[y.dtype], float(eps), float(rs), M, n,
+                                                  _lib.ptr(new), _lib.ptr(x),
+                                                  *(e.zeiger() if e else [_lib.ptr(None)] * 4),
+                                                  _lib.stream_ptr(y.device)), "qmv_norm_block")
+    return x, e, new
 
 
 def akt_q8(g: torch.Tensor, u: Optional[torch.Tensor], gelu: bool):

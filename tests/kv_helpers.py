@@ -1,0 +1,112 @@
+"""Plain 64-bit forms of the quantised cache and of attention over it, for the tests (numpy / torch fp64, written from the
+formulas and the byte layout in include/nemicli_qmv.h, sharing no code with the package)."""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+HALF_STEP = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
+
+
+def rotate(x: np.ndarray, cos: np.ndarray, sin: np.ndarray, pos: np.ndarray, paired: bool) -> np.ndarray:
+    """fp32 arithmetic, every product and sum rounded (numpy does not contract): x (rows, heads, dim) fp32."""
+    x = x.astype(np.float32)
+    half = cos.shape[1]
+    c, s = cos[pos][:, None], sin[pos][:, None]
+    y = x.copy()
+    ia, ib = (np.arange(half) * 2, np.arange(half) * 2 + 1) if paired else (np.arange(half), np.arange(half) + half)
+    a, b = x[..., ia], x[..., ib]
+    y[..., ia] = a * c - b * s
+    y[..., ib] = b * c + a * s
+    return y
+
+
+def quantise(x: np.ndarray, fmt: str):
+    """x (rows, heads, dim) fp32 -> codes (rows, heads, J, 32) with their offset, d (rows, heads, J) fp16."""
+    b = np.where(np.isnan(x), np.float32(0), np.clip(x, -65504, 65504)).astype(np.float32)
+    b = b.reshape(*x.shape[:-1], -1, 32)
+    first = np.abs(b).argmax(-1)[..., None]
+    m = np.take_along_axis(b, first, -1)[..., 0]
+    with np.errstate(over="ignore", under="ignore", divide="ignore", invalid="ignore"):
+        d = (m * np.float32(-0.125) if fmt == "Q4_0" else np.abs(m) / np.float32(127)).astype(np.float16)
+        df = d.astype(np.float32)[..., None]
+        q = np.where(df == 0, np.float32(0), np.rint(b / df))
+    lo, hi, off = (-8, 7, 8) if fmt == "Q4_0" else (-127, 127, 128)
+    return (np.clip(q, lo, hi) + off).astype(np.int64), d
+
+
+def codes_of(cache, slots: np.ndarray):
+    """(K codes, V codes (rows, heads, J, 32) with their offset, scales (rows, heads, 2, J)) read bit by bit out of
+    the cache's buffers."""
+    P, J = cache.page, cache.dim // 32
+    page, at = slots // P, slots % P
+    kc = cache.k_codes.cpu().numpy().astype(np.int64)[page, :, at]
+    vc = cache.v_codes.cpu().numpy().astype(np.int64)[page, :, at // 2]
+    rows, heads = kc.shape[:2]
+    k = np.empty((rows, heads, J, 32), np.int64)
+    v = np.empty_like(k)
+    odd = (at % 2)[:, None]
+    r, h = np.arange(rows)[:, None], np.arange(heads)[None]
+    for j in range(J):
+        for i in range(32):
+            t, n = divmod(i, 8)
+            if cache.k_fmt == "Q4_0":
+                bit = 16 * (n & 1) + 4 * (n >> 1)
+                k[..., j, i] = (kc[..., (t * J + j) * 4 + bit // 8] >> (bit % 8)) & 15
+            else:
+                k[..., j, i] = kc[..., (t * J + j) * 8 + 4 * (n >> 2) + 2 * (n & 1) + ((n & 3) >> 1)]
+            g, n = divmod(i, 4)
+            if cache.v_fmt == "Q4_0":
+                bit = 4 * n
+                v[..., j, i] = (vc[r, h, (g * J + j) * 4 + 2 * odd + bit // 8] >> (bit % 8)) & 15
+            else:
+                v[..., j, i] = vc[r, h, (g * J + j) * 8 + 4 * (n >> 1) + 2 * odd + (n & 1)]
+    return k, v, cache.scales.cpu().numpy()[page, :, at]
+
+
+def values(codes: np.ndarray, d: np.ndarray, fmt: str) -> np.ndarray:
+    off = 8 if fmt == "Q4_0" else 128
+    return ((codes - off) * d.astype(np.float64)[..., None]).reshape(*codes.shape[:-2], -1)
+
+
+def attention(q, k, v, pos, scale, window):
+    """One sequence: q (n, heads, dim), k, v (keys, n_kv, dim), pos (n,) in fp64 -> (out, sum p |v|, max over keys of
+    sum |q k| scale, per row and head).  Rows that see no key: zeros."""
+    n, heads, dim = q.shape
+    keys, n_kv, _ = k.shape
+    g = heads // n_kv
+    o = torch.zeros(n, heads, dim, dtype=torch.float64, device=q.device)
+    mag, qk = torch.zeros_like(o), torch.zeros(n, heads, dtype=torch.float64, device=q.device)
+    key = torch.arange(keys, device=q.device)
+    seen = key[None] <= pos[:, None]
+    if window:
+        seen &= key[None] > pos[:, None] - window
+    some = seen.any(1)
+    if keys == 0 or not bool(some.any()):
+        return o, mag, qk
+    for h in range(heads):
+        s = (q[:, h] @ k[:, h // g].T) * scale
+        s = s.masked_fill(~seen, -torch.inf)
+        p = torch.where(some[:, None], torch.softmax(s, 1), torch.zeros_like(s))
+        o[:, h] = p @ v[:, h // g]
+        mag[:, h] = p @ v[:, h // g].abs()
+        qk[:, h] = torch.where(seen, (q[:, h].abs() @ k[:, h // g].abs().T) * scale, torch.zeros_like(s)).amax(1)
+    return o, mag, qk
+
+
+def bound(mag, qk, o, dtype, keys, fmts, tiles):
+    """How far an output may be off, from the kernels' roundings (first order, worst case):
+    - a score is off by ds = qk * (e_q + e_k + 2^-23 * a): queries as two fp16 parts (2^-22; 16-bit types are exact),
+      keys d * code exact, or rounded to fp16 on the tile path (2^-11); fp32 sums of dim products, where the code
+      offset makes partial sums up to `a` times larger (16 for 4 bits, 3 for 8 bits, whose codes reach the offset;
+      none on the tile path) over dim / 16 = at most 16 accumulation steps;
+    - a weight exp(s - m) / sum changes by 2 ds relatively, and by its own rounding: to fp16 (2^-11) or two fp16
+      parts (2^-21), the value by 2^-11 on the tile path;
+    - the sums over the keys in steps of 16, with the offset again: keys / 16 * 2^-23 * a;
+    - exp2 and the final division: 2^-20; the output's own rounding, half a step."""
+    exact = dtype == torch.float32
+    a = 1.0 if tiles else 16.0 if "Q4_0" in fmts else 3.0
+    ds = qk * ((2.0 ** -22 if exact else 0.0) + (2.0 ** -11 if tiles else 0.0) + 16 * 2.0 ** -23 * a)
+    rel = 2 * ds[..., None] + (2.0 ** -21 if exact else 2.0 ** -11) + (2.0 ** -11 if tiles else 0.0) \
+        + (keys / 16 + 16) * 2.0 ** -23 * a + 2.0 ** -20
+    return mag * rel + o.abs() * HALF_STEP[dtype] + 2.0 ** -24 * (dtype == torch.float16) + 1e-30
