@@ -328,7 +328,8 @@ int qmv_kv_read(const qmv_kv_cache* cache, const long long* slots, long long row
                 void* stream);
 
 /* Bytes of the workspace qmv_kv_attend needs for these sizes (0 for sizes it does not take). */
-int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, int n_seq, int max_new, int dtype);
+int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, int n_seq, int max_new, int dtype,
+                                      int table_width, int window);
 
 /* Causal attention of n_seq sequences over the cache: out = softmax(scale * q . k) v per query row and head, fp32
  * statistics, q and out of type dtype (QMV_OUT_*).  Head h reads key head h / (n_heads / n_kv).  Sequence b: lens[b]

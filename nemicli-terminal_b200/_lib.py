@@ -52,7 +52,7 @@ _SIGNATURES = {
     "qmv_moe_ffn": ([I, P, P, LL, I, P, LL, LL, P, P, I, I, P, I, LL, I, I, P, P, P], I),
     "qmv_kv_write": ([P, P, P, I, LL, LL, P, LL, P, P, P, LL, I, I, P, LL, I, P, P], I),
     "qmv_kv_read": ([P, P, LL, P, P, I, P], I),
-    "qmv_kv_attend_workspace_bytes": ([P, I, I, I, I], LL),
+    "qmv_kv_attend_workspace_bytes": ([P, I, I, I, I, I, I], LL),
     "qmv_kv_attend": ([P, P, I, LL, I, P, I, P, P, I, LL, I, ctypes.c_float, I, P, P, LL, P], I),
     "qmv_norm_block": ([P, LL, P, LL, P, LL, P, P, I, ctypes.c_float, ctypes.c_float, LL, I, P, P, P, P, P, P, P], I),
 }

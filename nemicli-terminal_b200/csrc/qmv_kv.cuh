@@ -15,6 +15,9 @@
 // bit 16 (token & 1) + 4 n.  In the two Q8_0 K words value n sits in word n >> 2 at byte 2 (n & 1) + ((n & 3) >> 1);
 // in the V words in word n >> 1 at byte 2 (token & 1) + (n & 1).
 #pragma once
+#include <atomic>
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -69,6 +72,24 @@ inline int kv_view(const qmv_kv_cache* c, KvView& view) {
     view.vb = c->v_type == F_Q4_0 ? 4 : 8;
     return ST_OK;
 }
+
+// the right to more than 48 KB of shared memory (a kernel's fixed part, under 16 KB, counts too), asked for once a kernel and device
+struct SmemGrant {
+    std::atomic<uint64_t> done{0};
+    template <class Kernel>
+    int operator()(Kernel* kernel, size_t bytes) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (bytes <= 32 * 1024 || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return ST_OK;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+        if (e != cudaSuccess) {
+            set_last_cuda_error(int(e));
+            return ST_LAUNCH;
+        }
+        if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+        return ST_OK;
+    }
+};
 
 // element types of dense inputs and outputs (QMV_OUT_*): four consecutive values at a time
 template <int DT> struct Elem;

@@ -92,11 +92,9 @@ extern "C" int qmv_norm_block(const void* y, long long y_stride, const void* h, 
     return by_elem(dtype, [&](auto c) {
         constexpr int DT = decltype(c)::value;
         const size_t smem = size_t(n) * 4;
-        const cudaError_t e = cudaFuncSetAttribute(norm_block_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, QMV_NORM_BLOCK_MAX * 4);
-        if (e != cudaSuccess) {
-            set_last_cuda_error(int(e));
-            return int(ST_LAUNCH);
-        }
+        static SmemGrant grant;
+        if (smem > 32 * 1024)
+            if (const int e = grant(norm_block_kernel<DT>, size_t(QMV_NORM_BLOCK_MAX) * 4)) return e;
         return launch_pdl_smem(norm_block_kernel<DT>, dim3(unsigned(rows)), dim3(256), smem, static_cast<cudaStream_t>(stream), P);
     });
 }

@@ -187,12 +187,13 @@ class KVCache:
         lib = _lib.load()
         most = min(most, rows)
         with _lib.on_device(self.device):
-            nbytes = lib.qmv_kv_attend_workspace_bytes(self._ref, heads, n_seq, most, _DTYPES[q.dtype])
+            window = min(int(window), 2 ** 31 - 1)
+            nbytes = lib.qmv_kv_attend_workspace_bytes(self._ref, heads, n_seq, most, _DTYPES[q.dtype], width, window)
             if nbytes <= 0:
                 raise RuntimeError(f"KVCache.attend: {heads} heads, {n_seq} sequences of {most} new tokens not supported")
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             _lib.check(lib.qmv_kv_attend(self._ref, _lib.ptr(q), _DTYPES[q.dtype], qs, heads, _lib.ptr(tables), width,
                                          _lib.ptr(lens), _lib.ptr(starts), n_seq, rows, most,
-                                         self.dim ** -0.5 if scale is None else float(scale), min(int(window), 2 ** 31 - 1),
+                                         self.dim ** -0.5 if scale is None else float(scale), window,
                                          _lib.ptr(out), _lib.ptr(ws), nbytes, _lib.stream_ptr(self.device)), "qmv_kv_attend")
         return out

@@ -70,43 +70,49 @@ def values(codes: np.ndarray, d: np.ndarray, fmt: str) -> np.ndarray:
 
 
 def attention(q, k, v, pos, scale, window):
-    """One sequence: q (n, heads, dim), k, v (keys, n_kv, dim), pos (n,) in fp64 -> (out, sum p |v|, max over keys of
-    sum |q k| scale, per row and head).  Rows that see no key: zeros."""
+    """One sequence: q (n, heads, dim), k, v (keys, n_kv, dim), pos (n,) in fp64 -> (out, sizes): sizes = (sum p |v|,
+    sum p top(v), and over the keys the largest scale * sum |q k| and scale * sum |q| top(k)), where top is the
+    largest magnitude of the value's 32-value block.  Rows that see no key: zeros."""
     n, heads, dim = q.shape
     keys, n_kv, _ = k.shape
     g = heads // n_kv
     o = torch.zeros(n, heads, dim, dtype=torch.float64, device=q.device)
-    mag, qk = torch.zeros_like(o), torch.zeros(n, heads, dtype=torch.float64, device=q.device)
+    mag, top = torch.zeros_like(o), torch.zeros_like(o)
+    qk, qt = (torch.zeros(n, heads, dtype=torch.float64, device=q.device) for _ in range(2))
     key = torch.arange(keys, device=q.device)
     seen = key[None] <= pos[:, None]
     if window:
         seen &= key[None] > pos[:, None] - window
     some = seen.any(1)
     if keys == 0 or not bool(some.any()):
-        return o, mag, qk
+        return o, (mag, top, qk, qt)
+    kt, vt = (x.abs().unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1) for x in (k, v))
     for h in range(heads):
         s = (q[:, h] @ k[:, h // g].T) * scale
         s = s.masked_fill(~seen, -torch.inf)
         p = torch.where(some[:, None], torch.softmax(s, 1), torch.zeros_like(s))
         o[:, h] = p @ v[:, h // g]
         mag[:, h] = p @ v[:, h // g].abs()
-        qk[:, h] = torch.where(seen, (q[:, h].abs() @ k[:, h // g].abs().T) * scale, torch.zeros_like(s)).amax(1)
-    return o, mag, qk
+        top[:, h] = p @ vt[:, h // g]
+        for out, x in ((qk, k.abs()), (qt, kt)):
+            out[:, h] = torch.where(seen, (q[:, h].abs() @ x[:, h // g].T) * scale, torch.zeros_like(s)).amax(1)
+    return o, (mag, top, qk, qt)
 
 
-def bound(mag, qk, o, dtype, keys, fmts, tiles):
-    """How far an output may be off, from the kernels' roundings (first order, worst case):
-    - a score is off by ds = qk * (e_q + e_k + 2^-23 * a): queries as two fp16 parts (2^-22; 16-bit types are exact),
-      keys d * code exact, or rounded to fp16 on the tile path (2^-11); fp32 sums of dim products, where the code
-      offset makes partial sums up to `a` times larger (16 for 4 bits, 3 for 8 bits, whose codes reach the offset;
-      none on the tile path) over dim / 16 = at most 16 accumulation steps;
+def bound(sizes, o, dtype, keys, tiles):
+    """How far an output may be off, from the kernels' roundings (first order, worst case).  The sums over code bits run
+    before the codes' offset is taken off, so their partial sums are as large as the block's largest value times two
+    (codes 0 .. 15 against an offset of 8, 1 .. 255 against 128; the largest value's code lies at the offset's distance),
+    whatever the value itself is; a step of 16 products on the tensor cores is cut off at 2^-22 of them.
+    - a score is off by ds: queries as two fp16 parts (2^-22; 16-bit types are exact), keys d * code exact or rounded
+      to fp16 on the tile path (2^-11), and at most 16 such steps and block sums over the head's values;
     - a weight exp(s - m) / sum changes by 2 ds relatively, and by its own rounding: to fp16 (2^-11) or two fp16
-      parts (2^-21), the value by 2^-11 on the tile path;
-    - the sums over the keys in steps of 16, with the offset again: keys / 16 * 2^-23 * a;
-    - exp2 and the final division: 2^-20; the output's own rounding, half a step."""
+      parts (2^-21); the value by 2^-11 on the tile path; exp2 and the final division: 2^-20;
+    - the sums over the keys in steps of 16, and at most 16 joins of parts;
+    - the output's own rounding: half a step."""
+    mag, top, qk, qt = sizes
     exact = dtype == torch.float32
-    a = 1.0 if tiles else 16.0 if "Q4_0" in fmts else 3.0
-    ds = qk * ((2.0 ** -22 if exact else 0.0) + (2.0 ** -11 if tiles else 0.0) + 16 * 2.0 ** -23 * a)
-    rel = 2 * ds[..., None] + (2.0 ** -21 if exact else 2.0 ** -11) + (2.0 ** -11 if tiles else 0.0) \
-        + (keys / 16 + 16) * 2.0 ** -23 * a + 2.0 ** -20
-    return mag * rel + o.abs() * HALF_STEP[dtype] + 2.0 ** -24 * (dtype == torch.float16) + 1e-30
+    ds = qk * ((2.0 ** -22 if exact else 0.0) + (2.0 ** -11 if tiles else 0.0)) + 2 * qt * 16 * 2.0 ** -22
+    rel = 2 * ds[..., None] + (2.0 ** -21 if exact else 2.0 ** -11) + (2.0 ** -11 if tiles else 0.0) + 2.0 ** -20
+    return mag * rel + 2 * top * (keys / 16 + 16) * 2.0 ** -22 + o.abs() * HALF_STEP[dtype] \
+        + 2.0 ** -24 * (dtype == torch.float16) + 1e-30

@@ -166,8 +166,8 @@ def check(c, tables, held, lens, new, heads, dtype, window=0, seed=5, scale=None
             continue
         rows = slice(starts[b], starts[b + 1])
         pos = torch.arange(lens[b] - n, lens[b], device=dev)
-        o, mag, qk = KH.attention(q[rows].double(), *held[b], pos, scale or c.dim ** -0.5, window)
-        tol = KH.bound(mag, qk, o, dtype, max(lens[b], 1), (c.k_fmt, c.v_fmt), tiles)
+        o, sizes = KH.attention(q[rows].double(), *held[b], pos, scale or c.dim ** -0.5, window)
+        tol = KH.bound(sizes, o, dtype, max(lens[b], 1), tiles)
         err = (got[rows].double() - o).abs()
         assert torch.isfinite(got[rows]).all(), b
         assert (err <= tol).all(), (b, (err / tol).max().item())
@@ -280,8 +280,8 @@ def test_rows_nobody_covers_and_positions_before_the_start(cuda, new):
     if new > 3:
         assert not out[:new - 3].any()
         assert out[new - 3:new].any()
-    o, mag, qk = KH.attention(q[:new].double(), *held[0], torch.arange(3 - new, 3, device=cuda), 0.125, 0)
-    assert ((out[:new].double() - o).abs() <= KH.bound(mag, qk, o, BF16, 3, ("Q4_0", "Q4_0"), new > 16)).all()
+    o, sizes = KH.attention(q[:new].double(), *held[0], torch.arange(3 - new, 3, device=cuda), 0.125, 0)
+    assert ((out[:new].double() - o).abs() <= KH.bound(sizes, o, BF16, 3, new > 16)).all()
     assert _lib.device_status(device=cuda) == 0
 
 
@@ -305,8 +305,8 @@ def test_out_of_range_on_the_device(cuda, new):
         assert torch.equal(got[new:], want[new:]) and torch.isfinite(got).all()
         k, v = ([x[i] for i in range(96) if not 16 <= i < 32] for x in held[0])
         pos = torch.arange(80 - new, 80, device=cuda)
-        o, mag, qk = KH.attention(q[:new].double(), torch.stack(k), torch.stack(v), pos, 0.125, 0)
-        assert ((got[:new].double() - o).abs() <= KH.bound(mag, qk, o, BF16, 96, ("Q4_0", "Q4_0"), new > 16)).all()
+        o, sizes = KH.attention(q[:new].double(), torch.stack(k), torch.stack(v), pos, 0.125, 0)
+        assert ((got[:new].double() - o).abs() <= KH.bound(sizes, o, BF16, 96, new > 16)).all()
     got = c.attend(q, tables, torch.tensor([96, 1000], dtype=torch.int32, device=cuda), starts, max_new=new)
     assert _lib.device_status(device=cuda) == 1
     assert torch.equal(got, want)
@@ -452,8 +452,8 @@ def test_decoder_layer_step(cuda):
         for b in range(2):
             n = int(lens[b]) + 1
             held = [t.double() for t in c.read(slots_of(tables[b], n, page), F32)]
-            ref, mag, qk = KH.attention(qr[b:b + 1].double(), *held, torch.tensor([n - 1], device=cuda), dim ** -0.5, 0)
-            assert ((o[b:b + 1].double() - ref).abs() <= KH.bound(mag, qk, ref, F32, n, ("Q8_0", "Q4_0"), False)).all()
+            ref, sizes = KH.attention(qr[b:b + 1].double(), *held, torch.tensor([n - 1], device=cuda), dim ** -0.5, 0)
+            assert ((o[b:b + 1].double() - ref).abs() <= KH.bound(sizes, ref, F32, n, False)).all()
         z = y.double() / (y.double().square().mean(-1, keepdim=True) + 1e-6).sqrt() * w_post.double()
         z0 = ffn.double() / (ffn.double().square().mean(-1, keepdim=True) + 1e-6).sqrt() * w_post.double()
         ref = h.double() + 0.5 * z0 + 0.5 * z

@@ -35,7 +35,7 @@ def test_cache_descriptions_refused(bad, status):
     assert write(c) == status
     assert L.qmv_kv_read(c, A, 1, A, A, 0, None) == status
     assert L.qmv_kv_attend(c, A, 0, 256, 4, A, 1, A, None, 1, 1, 1, 1.0, 0, A, A, 1 << 30, None) == status
-    assert L.qmv_kv_attend_workspace_bytes(c, 4, 1, 1, 0) == 0
+    assert L.qmv_kv_attend_workspace_bytes(c, 4, 1, 1, 0, 1, 0) == 0
 
 
 @pytest.mark.parametrize("bad, status", [
@@ -96,10 +96,10 @@ def test_python_refuses_cpu_tensors_and_odd_shapes():
 def test_plain_attention_against_softmax_by_hand():
     q, k, v = (torch.randn(*s, dtype=torch.float64, generator=torch.Generator().manual_seed(i))
                for i, s in enumerate(((2, 2, 64), (3, 1, 64), (3, 1, 64))))
-    o, _, _ = KH.attention(q, k, v, torch.tensor([1, 2]), 0.5, 0)
+    o, _ = KH.attention(q, k, v, torch.tensor([1, 2]), 0.5, 0)
     w = torch.exp(0.5 * (k[:2, 0] @ q[0, 1]))
     assert torch.allclose(o[0, 1], (w / w.sum()) @ v[:2, 0], atol=1e-12)
-    o, _, _ = KH.attention(q, k, v, torch.tensor([-1, 2]), 0.5, 1)
+    o, _ = KH.attention(q, k, v, torch.tensor([-1, 2]), 0.5, 1)
     assert torch.equal(o[0], torch.zeros_like(o[0])) and torch.allclose(o[1, 0], v[2, 0], atol=1e-12)
 
 
