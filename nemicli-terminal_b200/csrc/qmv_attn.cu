@@ -1,5 +1,5 @@
 // Attention over a quantised key / value cache (layout: qmv_kv.cuh; C-ABI declarations: include/nemicli_qmv.h).
-#include "qmv_attn.cuh"
+#include "qmv_attn_tc.cuh"
 
 using namespace qmv;
 
@@ -12,6 +12,7 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
         return 0;
     if (dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16) return 0;
     if (table_width <= 0 || table_width > (0x7FFFFFFF >> c.page_shift) || window < 0) return 0;
+    if (attn_tc_used(c, dtype, n_heads, max_new)) return 256;     // no workspace
     const AttnPlan p = attn_plan(c, dtype, n_heads, n_seq, max_new, table_width, window);
     return p.grid ? p.bytes : 0;
 }
@@ -35,18 +36,30 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
     if (!aligned(q, four) || q_stride % 4 || !aligned(out, 16) || !aligned(tables, 4) || !aligned(lens, 4) ||
         !aligned(starts, 4) || !aligned(workspace, 256))
         return ST_BAD_ALIGN;
-    const AttnPlan pl = attn_plan(P.c, dtype, n_heads, n_seq, starts ? max_new : 1, table_width, window);
-    if (!pl.grid || workspace_bytes < pl.bytes) return ST_BAD_SHAPE;
+    if (!starts) max_new = 1;
+    const bool tiles = attn_tc_used(P.c, dtype, n_heads, max_new);
+    const AttnPlan pl = attn_plan(P.c, dtype, n_heads, n_seq, max_new, table_width, window);
+    if (tiles ? (long long)attn_tc_tiles(P.c, n_heads, max_new) * P.c.n_kv * n_seq > 0x7FFFFFFF : !pl.grid || workspace_bytes < pl.bytes)
+        return ST_BAD_SHAPE;
     if (n_rows == 0) return ST_OK;
     P.q = q, P.q_stride = q_stride, P.out = out;
     P.tables = tables, P.lens = lens, P.starts = starts;
     P.width = table_width, P.n_seq = n_seq, P.n_heads = n_heads, P.n_rows = int(n_rows);
-    P.max_new = starts ? max_new : 1, P.window = window, P.scale = scale;
+    P.max_new = max_new, P.window = window, P.scale = scale;
     P.row_tiles = pl.row_tiles, P.split = pl.split, P.by_segment = pl.by_segment;
     P.parts = static_cast<float*>(workspace);
     P.desc = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + pl.part_bytes);
     P.status = device_status_ptr();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (tiles) {
+        P.row_tiles = attn_tc_tiles(P.c, n_heads, max_new);
+        switch (P.c.J) {
+        case 2: return attn_tc_dispatch<2>(P, dtype, s);
+        case 3: return attn_tc_dispatch<3>(P, dtype, s);
+        case 4: return attn_tc_dispatch<4>(P, dtype, s);
+        case 8: return attn_tc_dispatch<8>(P, dtype, s);
+        }
+    }
     switch (P.c.J) {
     case 2: return attn_dispatch<2>(P, dtype, pl, s);
     case 3: return attn_dispatch<3>(P, dtype, pl, s);
