@@ -18,6 +18,8 @@
 // S NQ x BN columns, O NQ x D columns.  Every mbarrier wait is bounded; on expiry the CTA sets DEV_TIMEOUT, waits
 // (bounded) for its MMAs, frees its tensor memory and leaves.
 #pragma once
+#include <climits>
+
 #include "qmv_attn.cuh"
 
 namespace qmv {
@@ -25,14 +27,16 @@ namespace qmv {
 template <int J> struct AttnTcShape {
     static constexpr int D = 32 * J;
     static constexpr int NQ = J == 8 ? 1 : 2;                     // tiles of 128 query rows
-    static constexpr int BN = J == 8 ? 64 : 128;                  // keys a step
+    static constexpr int BN = 64;                                 // keys a step
+    static constexpr int PB = J == 8 ? 64 : 128;                  // keys the producers take at once: one or two steps' stages
+    static constexpr int KS = 2 * PB / BN;                        // stages of K and of V
     static constexpr int kThreads = NQ * 128 + 128 + 32;
     static constexpr int kQ = 128 * D * 2, kK = BN * D * 2, kV = D * BN * 2;      // bytes of one tile / stage
-    static constexpr int kScaleK = BN * J * 2, kScaleV = J * BN * 2;
-    static constexpr int kOffK = NQ * kQ, kOffV = kOffK + 2 * kK, kOffSK = kOffV + 2 * kV, kOffSV = kOffSK + 2 * kScaleK;
-    static constexpr int kOffBar = kOffSV + 2 * kScaleV;
-    static constexpr int kOffBad = kOffBar + 160;                 // [2][4] words: keys whose page is not of the cache
-    static constexpr int kSmem = kOffBar + 256;
+    static constexpr int kScaleK = PB * J * 2, kScaleV = J * PB * 2;
+    static constexpr int kOffK = NQ * kQ, kOffV = kOffK + KS * kK, kOffSK = kOffV + KS * kV, kOffSV = kOffSK + 2 * kScaleK;
+    static constexpr int kOffBar = kOffSV + 2 * kScaleV;          // mbarriers, the tensor-memory address
+    static constexpr int kOffBad = kOffBar + 256;                 // [2][4] words: keys whose page is not of the cache
+    static constexpr int kSmem = kOffBad + 32;
     static constexpr uint32_t kSboQ = D * 16, kSboK = D * 16, kSboV = BN * 16;    // bytes between 8-row groups
 };
 
@@ -53,6 +57,22 @@ __device__ __forceinline__ void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 __device__ __forceinline__ void at_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
 }
+__device__ __forceinline__ bool at_elect() {                      // true in one lane of the (whole) warp
+    uint32_t e;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(e));
+    return e != 0;
+}
+// a word of two bf16 or fp16 as fp32, and back (rounded to nearest)
+template <class T> __device__ __forceinline__ float2 raw_f2(uint32_t w);
+template <> __device__ __forceinline__ float2 raw_f2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+template <> __device__ __forceinline__ float2 raw_f2<__half>(uint32_t w) { return unpack_h2(w); }
+template <class T> __device__ __forceinline__ uint32_t pack_out(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack_out<__nv_bfloat16>(float x, float y) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t pack_out<__half>(float x, float y) { return pack_h2(x, y); }
 __device__ __forceinline__ void at_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void at_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void at_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -65,6 +85,38 @@ __device__ __forceinline__ void at_ld32(uint32_t a, uint32_t (&r)[32]) {
                    "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
                    "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(a));
+}
+__device__ __forceinline__ void at_ld16(uint32_t a, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(a));
+}
+// two fp32 at a time, and the larger of three
+__device__ __forceinline__ uint64_t pack_f2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ void at_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -143,7 +195,7 @@ template <int DT, int J, int KB, int VB>
 __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(const __grid_constant__ AttnParams P) {
     using T = typename Elem<DT>::type;
     using Sh = AttnTcShape<J>;
-    constexpr int D = Sh::D, NQ = Sh::NQ, BN = Sh::BN;
+    constexpr int D = Sh::D, NQ = Sh::NQ, BN = Sh::BN, KS = Sh::KS;
     extern __shared__ __align__(128) uint8_t tc_smem_[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -162,236 +214,301 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
     const int kt0 = first / BN, n_tiles = last < first ? 0 : last / BN - kt0 + 1;
 
     const uint32_t sm = smem_u32(tc_smem_);
-    const uint32_t bar = sm + Sh::kOffBar;
-    const uint32_t k_full = bar, k_free = bar + 16, v_full = bar + 32, v_free = bar + 48, s_full = bar + 64, p_full = bar + 80, o_full = bar + 96;
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBar + 128);
+    const uint32_t bar = sm + Sh::kOffBar;                        // stages: up to four each; S and P: two buffers a query tile
+    const uint32_t k_full = bar, k_free = bar + 32, v_full = bar + 64, v_free = bar + 96, s_full = bar + 128, p_full = bar + 160,
+                   o_full = bar + 192, q_full = bar + 224, done = bar + 232;
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBar + 240);
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tslot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(k_full + 8 * i, 4), mbar_init(k_free + 8 * i, 1);
-            mbar_init(v_full + 8 * i, 4), mbar_init(v_free + 8 * i, 1);
-            mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4);
+    if (warp == 4 && lane == 0) {
+        for (int i = 0; i < KS; ++i) {
+            mbar_init(k_full + 8 * i, 4 * BN / Sh::PB), mbar_init(k_free + 8 * i, 1);
+            mbar_init(v_full + 8 * i, 4 * BN / Sh::PB), mbar_init(v_free + 8 * i, 1);
         }
-        mbar_init(o_full, 1);
+        for (int i = 0; i < 2 * NQ; ++i) mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1);
+        mbar_init(done, 1);
+        mbar_init(q_full, 4 * NQ);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-
-    // the softmax threads' rows: query values to shared memory
-    const int qa = warp >> 2;                                     // which query tile (NQ and above: another role)
-    const int r = base + 128 * qa + 32 * (warp & 3) + lane;
-    float cs = 0.f;
-    int pos = -1;
-    if (qa < NQ) {
-        const bool live = r < rows;
-        const int tok = r / group;
-        if (live) pos = pos0 + tok;
-        const T* src = static_cast<const T*>(P.q) + (live ? (S.row0 + tok) * P.q_stride + (hk * group + r % group) * D : 0);
-        float top = 0.f;
-        for (int i = 0; i < D; i += 4) {
-            const float4 v = live ? load4(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-        const int ex = int((__float_as_uint(top) >> 23) & 255u);
-        const int e = ex == 0 || ex == 255 ? 0 : max(-110, min(110, ex - 127 - 8));     // 2^8 <= top 2^-e < 2^9
-        const float down = __uint_as_float(uint32_t(127 - e) << 23);
-        const float sgn = P.scale < 0.f ? -down : down;           // cs is not negative: the largest score is the largest product
-        cs = fabsf(P.scale) * 1.4426950408889634f * __uint_as_float(uint32_t(127 + e) << 23);
-        const int rl = 32 * (warp & 3) + lane;
-        const uint32_t dst = sm + qa * Sh::kQ + (rl >> 3) * Sh::kSboQ + (rl & 7) * 16;
-        for (int i = 0; i < D; i += 8) {
-            const float4 u = live ? load4(src + i) : make_float4(0.f, 0.f, 0.f, 0.f), v = live ? load4(src + i + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-            at_sts128(dst + (i >> 3) * 128, pack_h2(u.x * sgn, u.y * sgn), pack_h2(u.z * sgn, u.w * sgn), pack_h2(v.x * sgn, v.y * sgn),
-                      pack_h2(v.z * sgn, v.w * sgn));
-        }
-        at_fence_smem();
     }
     at_before();
     __syncthreads();
     at_after();
-    const uint32_t tmem = *tslot;
+    constexpr uint32_t tmem = 0;                                  // all 512 columns were asked for: they start at 0
+    constexpr uint32_t kO = NQ * 2 * BN;                          // S (and P over it): column (2 a + buffer) BN; O: kO + a D
+    const int qa = warp >> 2;                                     // query tile, NQ: producers, NQ + 1: MMA
     bool ok = true;                                               // no wait ran out so far
 
     if (qa < NQ) {
         // ---- softmax: one thread a row ----------------------------------------------------------
-        const uint32_t quad = tmem + (uint32_t(32 * (warp & 3)) << 16);
-        const uint32_t s_at = quad + qa * BN, o_at = quad + NQ * BN + qa * D;
+        const int wr = 32 * (warp & 3), r0 = base + 128 * qa + wr;        // the warp's first row
+        const int r = r0 + lane;
+        float cs = 0.f;
+        {   // the warp's 32 rows of queries, 8 at a time (four lanes a row), to fp16 after a power of two per row
+            constexpr int kCores = D / 32;                        // 16-byte pieces a lane
+            const int g = lane & 7, c = lane >> 3;
+            constexpr int kPass = J == 8 ? 2 : 4;
+            int mine = 0;                                         // exponent of row `lane`, found by lanes of pass lane / 8
+#pragma unroll 1
+            for (int q0 = 0; q0 < 4; q0 += kPass) {
+                uint32_t h[kPass][kCores][4];
+                int e[kPass];
+#pragma unroll
+                for (int q = 0; q < kPass; ++q) {
+                    const int rr = r0 + 8 * (q0 + q) + g;
+                    const bool live = rr < rows;
+                    const T* src = static_cast<const T*>(P.q) + (live ? (S.row0 + rr / group) * P.q_stride + (hk * group + rr % group) * D : 0);
+#pragma unroll
+                    for (int i = 0; i < kCores; ++i) {                // raw bits first: every load of the warp in flight
+                        const uint2* at = reinterpret_cast<const uint2*>(src + 8 * (4 * i + c));
+                        const uint2 u = live ? __ldg(at) : make_uint2(0u, 0u), v = live ? __ldg(at + 1) : make_uint2(0u, 0u);
+                        h[q][i][0] = u.x, h[q][i][1] = u.y, h[q][i][2] = v.x, h[q][i][3] = v.y;
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < kPass; ++q) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kCores; ++i)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const float2 x = raw_f2<T>(h[q][i][w]);
+                            top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const int ex = int((__float_as_uint(top) >> 23) & 255u);
+                    e[q] = ex == 0 || ex == 255 ? 0 : max(-110, min(110, ex - 127 - 8));      // 2^8 <= top 2^-e < 2^9
+                    const float down = __uint_as_float((uint32_t(127 - e[q]) << 23) | (P.scale < 0.f ? 0x80000000u : 0u));
+                    const int rl = wr + 8 * (q0 + q) + g;
+                    const uint32_t dst = sm + qa * Sh::kQ + (rl >> 3) * Sh::kSboQ + (rl & 7) * 16;
+#pragma unroll
+                    for (int i = 0; i < kCores; ++i) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const float2 x = raw_f2<T>(h[q][i][w]);
+                            o[w] = pack_h2(x.x * down, x.y * down);
+                        }
+                        at_sts128(dst + (4 * i + c) * 128, o[0], o[1], o[2], o[3]);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < kPass; ++q) {
+                    const int x = __shfl_sync(0xffffffffu, e[q], lane & 7);
+                    if (lane >> 3 == q0 + q) mine = x;
+                }
+            }
+            at_fence_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+            // positive (the sign went into the queries), so that masked scores stay -inf where the scale is 0
+            cs = fmaxf(fabsf(P.scale) * 1.4426950408889634f * __uint_as_float(uint32_t(127 + mine) << 23), 1e-30f);
+        }
+        const uint32_t quad = tmem + (uint32_t(wr) << 16), o_at = quad + kO + qa * D;
+        const int pos = r < rows ? pos0 + r / group : -1;
         float ref = kAttnNone, sum = 0.f;
         // keys that every row of this tile of 128 sees
         const int row_a = min(base + 128 * qa, rows - 1), row_b = min(base + 128 * qa + 127, rows - 1);
         const int full1 = pos0 + row_a / group, full0 = P.window > 0 ? pos0 + row_b / group - P.window + 1 : 0;
         const int low = P.window > 0 ? pos - P.window + 1 : 0;
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * qa, i & 1));      // the warp's lanes leave together
+        for (int i = 0; i < n_tiles; ++i) {
+            const int buf = i & 1;
+            const uint32_t s_at = quad + (2 * qa + buf) * BN;
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (2 * qa + buf), uint32_t(i >> 1) & 1u));      // the lanes leave together
             if (!ok) break;
             at_after();
+            uint32_t v[BN];                                       // the row's scores
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) at_ld32(s_at + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
             const int key = (kt0 + i) * BN;
             // keys of pages outside the cache are masked too (the words live as long as the tile's V stage)
-            uint32_t bad[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(bad[0]), "=r"(bad[1]), "=r"(bad[2]), "=r"(bad[3])
-                         : "r"(sm + Sh::kOffBad + 16 * (i & 1)) : "memory");
-            const bool whole = key >= full0 && key + BN - 1 <= full1 && !(bad[0] | bad[1] | bad[2] | bad[3]);
-            float top = -INFINITY;
+            uint32_t bad[2];
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(bad[0]), "=r"(bad[1])
+                         : "r"(sm + Sh::kOffBad + (Sh::PB == BN ? 16 * (i & 1) : 16 * ((i >> 1) & 1) + 8 * (i & 1))) : "memory");
+            const bool whole = key >= full0 && key + BN - 1 <= full1 && !(bad[0] | bad[1]);
+            at_wait_ld();
+            if (!whole) {                                         // what this row does not see becomes -inf
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t v[32];
-                at_ld32(s_at + c, v);
-                at_wait_ld();
-                if (whole) {
+                for (int c = 0; c < BN; c += 32) {
+                    const int lo = low - key - c, hi = pos - key - c;
+                    const uint32_t from = lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo, to = hi >= 31 ? ~0u : hi < 0 ? 0u : (2u << hi) - 1u;
+                    const uint32_t seen = from & to & ~bad[c / 32];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(v[k]));
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const int at = key + c + k;
-                        top = fmaxf(top, at <= pos && at >= low && !(bad[c / 32] >> k & 1u) ? __uint_as_float(v[k]) : -INFINITY);
-                    }
+                    for (int k = 0; k < 32; ++k)
+                        if (!(seen >> k & 1u)) v[c + k] = 0xFF800000u;
                 }
             }
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int k = 0; k < BN; k += 2) tops[(k >> 1) & 3] = max3(tops[(k >> 1) & 3], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+            const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
             const float m = top == -INFINITY ? kAttnNone : top * cs;
             const bool move = m > ref + 8.f;
             if (__any_sync(0xffffffffu, move)) {
                 const float f = move ? ex2(ref - m) : 1.f;
                 if (move) ref = m;
                 sum *= f;
-                if (i > 0) {                                      // O(i - 1) is complete: S(i) was issued after it
-#pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t v[32];
-                        at_ld32(o_at + c, v);
+                if (i > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * (2 * qa + (buf ^ 1)), uint32_t((i - 1) >> 1) & 1u));       // O(i - 1) is complete
+                    if (!ok) break;
+                    at_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t y[16];
+                        at_ld16(o_at + c, y);
                         at_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-                        at_st32(o_at + c, v);
+                        for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
+                        at_st16(o_at + c, y);
                     }
                 }
             }
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            uint64_t part[2] = {0ull, 0ull};                      // pairs of fp32 sums
+            const uint64_t cs2 = pack_f2(cs, cs), ref2 = pack_f2(-ref, -ref);
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) {                    // P over the scores already read
-                uint32_t v[32], h[16];
-                at_ld32(s_at + c, v);
-                at_wait_ld();
+            for (int c = 0; c < BN; c += 32) {                    // P over the scores
+                uint32_t h[16];
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
-                    float p0 = ex2(fmaf(__uint_as_float(v[k]), cs, -ref)), p1 = ex2(fmaf(__uint_as_float(v[k + 1]), cs, -ref));
-                    if (!whole) {
-                        const int at = key + c + k;
-                        if (at > pos || at < low || (bad[c / 32] >> k & 1u)) p0 = 0.f;
-                        if (at + 1 > pos || at + 1 < low || (bad[c / 32] >> k & 2u)) p1 = 0.f;
-                    }
-                    part[(k >> 1) & 1] += p0;
-                    part[2 + ((k >> 1) & 1)] += p1;
+                    const float2 x = unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c + k]), __uint_as_float(v[c + k + 1])), cs2, ref2));
+                    const float p0 = ex2(x.x), p1 = ex2(x.y);
+                    part[(k >> 1) & 1] = add_f2(part[(k >> 1) & 1], pack_f2(p0, p1));
                     h[k >> 1] = pack_h2(p0, p1);
                 }
                 at_st16(s_at + c / 2, h);
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            {
+                const float2 x = unpack_f2(add_f2(part[0], part[1]));
+                sum += x.x + x.y;
+            }
             at_wait_st();
             at_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 8 * qa);
+            if (lane == 0) mbar_arrive(p_full + 8 * (2 * qa + buf));
         }
-        if (ok && n_tiles) ok = __all_sync(0xffffffffu, mbar_wait(o_full, 0));
+        if (ok && n_tiles) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * (2 * qa + ((n_tiles - 1) & 1)), uint32_t((n_tiles - 1) >> 1) & 1u));
         at_after();
-        T* out = static_cast<T*>(P.out) + ((long long)(S.row0 + r / group) * P.n_heads + hk * group + r % group) * D;
+        // O / sum as the output's type to this warp's part of the query tile (nothing reads it any more), 16-byte pieces in
+        // an order that keeps lanes on different banks, and from there whole rows at a time
         const float inv = sum > 0.f ? __fdividef(1.f, sum) : sum == sum ? 0.f : sum;
+        const uint32_t stage = sm + qa * Sh::kQ + wr * D * 2;
+        if (ok) {
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-            uint32_t v[32];
-            if (n_tiles && ok) {
-                at_ld32(o_at + c, v);
-                at_wait_ld();
-            }
-            if (r < rows && ok) {
-#pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (inv != 0.f)
-                        y = make_float4(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv, __uint_as_float(v[k + 2]) * inv,
-                                        __uint_as_float(v[k + 3]) * inv);
-                    store4(out + c + k, y);
+            for (int c = 0; c < D; c += 32) {
+                uint32_t y[32];
+                if (n_tiles) {
+                    at_ld32(o_at + c, y);
+                    at_wait_ld();
                 }
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        o[w] = inv != 0.f ? pack_out<T>(__uint_as_float(y[k + 2 * w]) * inv, __uint_as_float(y[k + 2 * w + 1]) * inv) : 0u;
+                    const int piece = (c + k) / 8;
+                    at_sts128(stage + lane * D * 2 + (D % 64 ? piece : (piece & ~7) | ((piece ^ lane) & 7)) * 16, o[0], o[1], o[2], o[3]);
+                }
+            }
+            __syncwarp();
+            constexpr int kPieces = D / 8;                        // of a row
+            for (int i = lane; i < 32 * kPieces; i += 32) {
+                const int row = i / kPieces, piece = i - row * kPieces, rr = r0 + row;
+                if (rr >= rows) break;
+                const uint4 y = lds128(stage + row * D * 2 + (D % 64 ? piece : (piece & ~7) | ((piece ^ row) & 7)) * 16);
+                T* out = static_cast<T*>(P.out) + ((long long)(S.row0 + rr / group) * P.n_heads + hk * group + rr % group) * D;
+                reinterpret_cast<uint4*>(out)[piece] = y;
             }
         }
     } else if (qa == NQ) {
         // ---- producers -----------------------------------------------------------------------------
         const int pw = warp & 3, pt = tid - NQ * 128;             // producer warp and thread
-        constexpr int kRows = BN / 4, kGroups = kRows / 8;        // keys a warp, 8-key groups
+        constexpr int PB = Sh::PB, kPer = PB / BN;                // keys and stages a round
+        constexpr int kRows = PB / 4, kGroups = kRows / 8;        // keys a warp, 8-key groups
         constexpr int kWk = J * KB / 4;                           // words of a lane's K run
-        constexpr int JV = BN == 128 ? J : J / 2, kWv = JV * VB / 4;      // V blocks of a lane, words of a pair's run
+        constexpr int JV = PB == 128 ? J : J / 2, kWv = JV * VB / 4;      // V blocks of a lane, words of a pair's run
         uint32_t kw[kGroups][kWk], vw[4][kWv], sw[J], bad = 0;
         const int kk = lane & 7, kt = lane >> 3;                  // K: key within 8, run
-        const int vg = lane & 7, vkc = BN == 128 ? lane >> 3 : (lane >> 3) & 1, vj = BN == 128 ? 0 : (lane >> 4) * JV;
+        const int vg = lane & 7, vkc = PB == 128 ? lane >> 3 : (lane >> 3) & 1, vj = PB == 128 ? 0 : (lane >> 4) * JV;
         const int* table = P.tables + (long long)b * P.width;
-        // page of a 16-aligned run of keys, -1: nothing to see there
-        auto page_of = [&](int key) -> long long {
-            if (key > last || key + 15 < first) return -1;
-            const int p = __ldg(table + (key >> P.c.page_shift));
-            if (p >= 0 && p < P.c.n_pages) return p;
-            if (P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
-            return -1;
+        // The table entries of a tile's 16-key runs that this lane reads: asked for two tiles ahead and first looked at one
+        // tile later, so that no load waits for one.  kNoKey: nothing to see there.
+        constexpr int kNoKey = INT_MIN;
+        auto entry_of = [&](int key) { return key > last || key + 15 < first ? kNoKey : __ldg(table + (key >> P.c.page_shift)); };
+        auto valid = [&](int p) { return p >= 0 && p < P.c.n_pages; };
+        constexpr int kRuns = (kRows + 15) / 16;
+        int pk[kRuns], pv, ps;                                    // of K's runs, V's keys, the scale's key
+        auto ask = [&](int i) {
+            const int key = kt0 * BN + i * PB;
+#pragma unroll
+            for (int q = 0; q < kRuns; ++q) pk[q] = entry_of(key + kRows * pw + 16 * q);
+            pv = entry_of((key + kRows * pw + 8 * vkc) & ~15);
+            const int k = key + pt;
+            ps = pt < PB && k >= first && k <= last ? entry_of(k & ~15) : kNoKey;
         };
         auto load_k = [&](int i) {
-            const int key0 = (kt0 + i) * BN;
+            const int key0 = kt0 * BN + i * PB;
 #pragma unroll
             for (int q = 0; q < kGroups; ++q) {
-                const int key = key0 + kRows * pw + 8 * q;
-                const long long page = page_of(key & ~15);
-                if (page >= 0) {
+                const int key = key0 + kRows * pw + 8 * q, page = pk[q >> 1];
+                if (valid(page)) {
                     at_ldg<kWk>(kw[q], P.c.k + P.c.k_row(page, hk, (key & (P.c.page() - 1)) + kk) + kt * J * KB);
                 } else {
 #pragma unroll
                     for (int w = 0; w < kWk; ++w) kw[q][w] = 0u;
                 }
             }
-            // scales of key pt: nobody sees it: 0 (it may hold anything)
-            const int key = key0 + pt;
-            const bool seen = pt < BN && key >= first && key <= last;
-            const long long page = seen ? page_of(key & ~15) : -1;
-            bad = __ballot_sync(0xffffffffu, seen && page < 0);
-            if (page >= 0) {
-                at_ldg<J>(sw, reinterpret_cast<const uint8_t*>(P.c.sc + P.c.scale_row(page, hk, key & (P.c.page() - 1))));
+            // scales of key pt; nobody sees it: 0 (it may hold anything)
+            bad = __ballot_sync(0xffffffffu, ps != kNoKey && !valid(ps));
+            if (valid(ps)) {
+                at_ldg<J>(sw, reinterpret_cast<const uint8_t*>(P.c.sc + P.c.scale_row(ps, hk, (key0 + pt) & (P.c.page() - 1))));
             } else {
 #pragma unroll
                 for (int w = 0; w < J; ++w) sw[w] = 0u;
             }
         };
         auto load_v = [&](int i) {
-            const int key = (kt0 + i) * BN + kRows * pw + 8 * vkc;
-            const long long page = page_of(key & ~15);
+            const int key = kt0 * BN + i * PB + kRows * pw + 8 * vkc;
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                if (page >= 0) {
-                    at_ldg<kWv>(vw[p], P.c.v + P.c.v_pair(page, hk, ((key & (P.c.page() - 1)) >> 1) + p) + (vg * J + vj) * VB);
+                if (valid(pv)) {
+                    at_ldg<kWv>(vw[p], P.c.v + P.c.v_pair(pv, hk, ((key & (P.c.page() - 1)) >> 1) + p) + (vg * J + vj) * VB);
                 } else {
 #pragma unroll
                     for (int w = 0; w < kWv; ++w) vw[p][w] = 0u;
                 }
             }
         };
-        if (n_tiles) load_k(0), load_v(0);
-        for (int i = 0; i < n_tiles; ++i) {
-            const int st = i & 1;
+        if (n_tiles) {
+            ask(0);
+            load_k(0), load_v(0);
+            ask(1);
+        }
+        const int rounds = (n_tiles + kPer - 1) / kPer;
+        for (int i = 0; i < rounds; ++i) {
+            const int st = i & 1;                                 // stages kPer st ..
             const uint32_t par = uint32_t(i >> 1) & 1u;
             const uint32_t s_k = sm + Sh::kOffSK + st * Sh::kScaleK, s_v = sm + Sh::kOffSV + st * Sh::kScaleV;
-            if (i >= 2) ok = mbar_wait(k_free + 8 * st, par ^ 1u);
-            if (i >= 2 && ok) ok = mbar_wait(v_free + 8 * st, par ^ 1u);
+            if (i >= 2)
+#pragma unroll
+                for (int q = 0; q < kPer; ++q)
+                    ok = ok && mbar_wait(k_free + 8 * (kPer * st + q), par ^ 1u) && mbar_wait(v_free + 8 * (kPer * st + q), par ^ 1u);
             // scales: K's by key, V's by block (so that eight keys of a block are one word of 16 bytes)
-            if (pt < BN) {
+            if (pt < PB) {
                 __half* dk = reinterpret_cast<__half*>(tc_smem_ + Sh::kOffSK + st * Sh::kScaleK) + pt * J;
                 __half* dv = reinterpret_cast<__half*>(tc_smem_ + Sh::kOffSV + st * Sh::kScaleV) + pt;
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const uint32_t a = sw[j >> 1], c = sw[(J + j) >> 1];
                     dk[j] = __ushort_as_half((unsigned short)(j & 1 ? a >> 16 : a & 0xFFFFu));
-                    dv[j * BN] = __ushort_as_half((unsigned short)((J + j) & 1 ? c >> 16 : c & 0xFFFFu));
+                    dv[j * PB] = __ushort_as_half((unsigned short)((J + j) & 1 ? c >> 16 : c & 0xFFFFu));
                 }
             }
             uint32_t all;                                         // the four warps go on, or leave, together
             if (lane == 0) reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBad)[4 * st + pw] = bad;
+            if (bad && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
             asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.and.pred q, 1, 128, p; selp.u32 %0, 1, 0, q; }"
                          : "=r"(all) : "r"(uint32_t(ok)) : "memory");
             ok = all != 0;
@@ -399,84 +516,101 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
 #pragma unroll
             for (int q = 0; q < kGroups; ++q) {
                 const int key = kRows * pw + 8 * q + kk;
-                const uint32_t dst = sm + Sh::kOffK + st * Sh::kK + (key >> 3) * Sh::kSboK + (key & 7) * 16;
+                const uint32_t dst = sm + Sh::kOffK + kPer * st * Sh::kK + (key >> 3) * Sh::kSboK + (key & 7) * 16;     // stages side by side
+                uint32_t d2[(J + 1) / 2];
+                if constexpr (J == 3) {                           // three halves: at an odd key not on a word
+                    d2[0] = lds16u(s_k + key * 6) | (lds16u(s_k + key * 6 + 2) << 16), d2[1] = lds16u(s_k + key * 6 + 4);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < J / 2; ++w) d2[w] = lds32(s_k + key * 2 * J + 4 * w);
+                }
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    unsigned short d;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(d) : "r"(s_k + (key * J + j) * 2));
                     uint32_t o[4];
-                    unpack_k8<KB>(&kw[q][j * KB / 4], __half2half2(__ushort_as_half(d)), o);
+                    const __half2 d = bits_h2(d2[j >> 1]);
+                    unpack_k8<KB>(&kw[q][j * KB / 4], j & 1 ? __high2half2(d) : __low2half2(d), o);
                     at_sts128(dst + (4 * j + kt) * 128, o[0], o[1], o[2], o[3]);
                 }
             }
             at_fence_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(k_full + 8 * st);
-            if (i + 1 < n_tiles) load_k(i + 1);
+            if (lane == 0) mbar_arrive(k_full + 8 * (kPer * st + kRows * pw / BN));
+            if (i + 1 < rounds) load_k(i + 1);
             {
-                const int kc = (kRows / 8) * pw + vkc;            // 8-key core of the stage
+                const int kc = (kRows / 8) * pw + vkc;            // 8-key core of the round
+                const uint32_t dst = sm + Sh::kOffV + (kPer * st + kc / (BN / 8)) * Sh::kV + (kc % (BN / 8)) * 128;
 #pragma unroll
                 for (int j = 0; j < JV; ++j) {
                     uint32_t d[4];
                     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                                 : "r"(s_v + ((vj + j) * BN + 8 * kc) * 2));
+                                 : "r"(s_v + ((vj + j) * PB + 8 * kc) * 2));
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {                 // the value differs by lane: no two of eight lanes share a bank
                         const int e = (s + (vg >> 1)) & 3, n = 32 * (vj + j) + 4 * vg + e;
                         uint32_t o[4];
 #pragma unroll
                         for (int p = 0; p < 4; ++p) o[p] = unpack_v<VB>(&vw[p][j * VB / 4], e, bits_h2(d[p]));
-                        at_sts128(sm + Sh::kOffV + st * Sh::kV + (n >> 3) * Sh::kSboV + kc * 128 + (n & 7) * 16, o[0], o[1], o[2], o[3]);
+                        at_sts128(dst + (n >> 3) * Sh::kSboV + (n & 7) * 16, o[0], o[1], o[2], o[3]);
                     }
                 }
             }
             at_fence_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(v_full + 8 * st);
-            if (i + 1 < n_tiles) load_v(i + 1);
+            if (lane == 0) mbar_arrive(v_full + 8 * (kPer * st + kRows * pw / BN));
+            if (i + 1 < rounds) load_v(i + 1);
+            ask(i + 2);
         }
-    } else if (lane == 0) {
+    } else {
         // ---- MMA -----------------------------------------------------------------------------------
+        // The whole warp walks the loop and one elected lane issues: descriptors and addresses stay in uniform registers
+        // (issued by `if (lane == 0)` with the tensor-memory address read back, an MMA cost 116 clocks instead of 64).
+        // Scores run two steps ahead of the sums, so a tile's softmax finds the next scores ready.
         constexpr uint32_t id_s = at_idesc(BN), id_o = at_idesc(D);
-        auto scores = [&](int a, int i) {
-            const uint32_t q = sm + a * Sh::kQ, k = sm + Sh::kOffK + (i & 1) * Sh::kK;
-#pragma unroll
-            for (int s = 0; s < D / 16; ++s)
-                at_mma_ss(tmem + a * BN, at_desc(q + 256 * s, Sh::kSboQ), at_desc(k + 256 * s, Sh::kSboK), id_s, s > 0);
-            at_commit(s_full + 8 * a);
-        };
-        if (n_tiles) {
-            ok = mbar_wait(k_full, 0);
+        auto wait = [&](uint32_t b, int phase) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(b, uint32_t(phase) & 1u));
             at_after();
-            if (ok) {
-                for (int a = 0; a < NQ; ++a) scores(a, 0);
-                at_commit(k_free);
-            }
-        }
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            const int st = i & 1;
-            for (int a = 0; a < NQ && ok; ++a) {
-                ok = mbar_wait(p_full + 8 * a, i & 1);
-                if (a == 0 && ok) ok = mbar_wait(v_full + 8 * st, uint32_t(i >> 1) & 1u);
-                if (!ok) break;
-                at_after();
-                const uint32_t v = sm + Sh::kOffV + st * Sh::kV;
+            return ok;
+        };
+        auto scores = [&](int a, int i) {
+            if (at_elect()) {
+                const uint32_t q = sm + a * Sh::kQ, k = sm + Sh::kOffK + (i % KS) * Sh::kK, d = (2 * a + (i & 1)) * BN;
 #pragma unroll
-                for (int s = 0; s < BN / 16; ++s)
-                    at_mma_ts(tmem + NQ * BN + a * D, tmem + a * BN + 8 * s, at_desc(v + 256 * s, Sh::kSboV), id_o, i > 0 || s > 0);
-                if (a == NQ - 1) at_commit(v_free + 8 * st);
-                if (i + 1 < n_tiles) {
-                    if (a == 0) ok = mbar_wait(k_full + 8 * (st ^ 1), uint32_t((i + 1) >> 1) & 1u);
-                    if (!ok) break;
-                    at_after();
-                    scores(a, i + 1);
-                    if (a == NQ - 1) at_commit(k_free + 8 * (st ^ 1));
+                for (int s = 0; s < D / 16; ++s) at_mma_ss(d, at_desc(q + 256 * s, Sh::kSboQ), at_desc(k + 256 * s, Sh::kSboK), id_s, s > 0);
+                at_commit(s_full + 8 * (2 * a + (i & 1)));
+                if (a == NQ - 1) at_commit(k_free + 8 * (i % KS));
+            }
+            __syncwarp();
+        };
+        if (n_tiles) wait(q_full, 0);
+        for (int i = 0; i < min(2, n_tiles) && ok; ++i)
+            if (wait(k_full + 8 * i, 0))
+#pragma unroll
+                for (int a = 0; a < NQ; ++a) scores(a, i);
+        for (int i = 0; i < n_tiles && ok; ++i) {
+            const int st = i % KS;
+            const uint32_t v = sm + Sh::kOffV + st * Sh::kV;
+#pragma unroll
+            for (int a = 0; a < NQ; ++a) {
+                if (a == 0 && !wait(v_full + 8 * st, i / KS)) break;
+                if (!wait(p_full + 8 * (2 * a + (i & 1)), i >> 1)) break;
+                if (at_elect()) {
+#pragma unroll
+                    for (int s = 0; s < BN / 16; ++s)
+                        at_mma_ts(kO + a * D, (2 * a + (i & 1)) * BN + 8 * s, at_desc(v + 256 * s, Sh::kSboV), id_o, i > 0 || s > 0);
+                    at_commit(o_full + 8 * (2 * a + (i & 1)));
+                    if (a == NQ - 1) at_commit(v_free + 8 * st);
+                }
+                __syncwarp();
+                if (i + 2 < n_tiles) {
+                    if (a == 0 && !wait(k_full + 8 * ((i + 2) % KS), (i + 2) / KS)) break;
+                    scores(a, i + 2);
                 }
             }
         }
         if (n_tiles) {                                            // everything issued is done before the memory is given back
-            at_commit(o_full);
-            ok = mbar_wait(o_full, 0) && ok;
+            if (at_elect()) at_commit(done);
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, mbar_wait(done, 0)) && ok;
         }
     }
     if (!ok && lane == 0 && P.status) atomicOr(P.status, DEV_TIMEOUT);
