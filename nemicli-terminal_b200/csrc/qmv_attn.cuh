@@ -23,6 +23,7 @@
 // workspace and attn_join_kernel adds them in order.
 #pragma once
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "qmv_kv.cuh"
@@ -43,13 +44,13 @@ struct AttnParams {
     int split;                            // segments may be cut: parts, desc, attn_join_kernel follows
     int by_segment;                       // desc has an entry a segment (else a CTA)
     float* parts;                         // [2 a CTA][8 NT rows][dim + 2]: sums, then reference and weight
-    int4* desc;                           // first part, parts, (sequence, key head x row tiles + row tile)
+    int4* desc;                           // two an entry: first part's CTA, parts (0: nothing to join), sequence's first row, key head;
+                                          // first of the tile's rows, rows
     int* status;
 };
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnUnit = 64;             // keys a unit
-constexpr int kAttnMinUnits = 4;          // units a CTA takes at least before segments are cut
+constexpr int kAttnMinKeys = 256;         // keys a CTA takes at least before segments are cut
 constexpr float kAttnNone = -1e30f;       // reference of a row that has seen no key
 
 __device__ __forceinline__ float ex2(float x) {
@@ -57,96 +58,139 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// d = a b + c with c somewhere else (no copy of it), and in place
+__device__ __forceinline__ void mma16816(float (&d)[4], uint4 a, uint32_t b0, uint32_t b1, const float4& c) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t movm(uint32_t x) {            // 8 x 8 transpose of fp16 over the warp
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ float2 unpack_h2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// N words from p to the lane's places in shared memory (16-byte pieces of a warp side by side), asynchronously; p is
-// aligned to N words' largest power of two up to 16 bytes
-template <int N> constexpr int kPiece = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;     // words of a copy
-template <int N>
-__device__ __forceinline__ void stage_words(uint32_t dst, const void* p, int lane) {
-    constexpr int W = kPiece<N>;
-#pragma unroll
-    for (int i = 0; i < N; i += W) {
-        const uint32_t d = dst + (32 * i + W * lane) * 4;
-        if constexpr (W == 4)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(d), "l"(static_cast<const uint8_t*>(p) + 4 * i) : "memory");
-        else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" :: "r"(d), "l"(static_cast<const uint8_t*>(p) + 4 * i), "n"(4 * W) : "memory");
-    }
-}
-template <int N>
-__device__ __forceinline__ void staged_words(uint32_t (&w)[N], uint32_t src, int lane) {
-    constexpr int W = kPiece<N>;
-#pragma unroll
-    for (int i = 0; i < N; i += W) {
-        const uint32_t a = src + (32 * i + W * lane) * 4;
-        if constexpr (W == 4)
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(a));
-        else if constexpr (W == 2)
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(a));
-        else
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(a));
+// f(std::integral_constant<int, 0>) .. of N
+template <int N, int I = 0, class Fn>
+__device__ __forceinline__ void each(Fn&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        each<N, I + 1>(f);
     }
 }
 
-// The 16 keys of a warp's tile as a lane (g = lane / 4, t = lane % 4) uses them: run t of the K rows of keys g and g + 8,
-// run g of the V pairs t and t + 4, the scales of keys g and g + 8.  Each lane copies its own words to shared memory
-// some tiles ahead (cp.async), so nothing but its own copies has to be waited for and no register holds them.
-template <int J, int KB, int VB>
-struct AttnTile {
-    static constexpr int kK = J * KB / 4, kV = J * VB / 4, kWords = 2 * (kK + kV + J);     // words a lane
-    static constexpr int kBytes = 32 * 4 * kWords;
-    static __device__ __forceinline__ void issue(uint32_t buf, const KvView& c, long long page, int head, int at, int lane) {
-        const int g = lane >> 2, t = lane & 3;
-        const long long row = ((page * c.n_kv + head) << c.page_shift) + at;
-        const uint8_t* k = c.k + (row + g) * (4 * J * KB) + t * J * KB;
-        const uint8_t* v = c.v + ((row >> 1) + t) * (8 * J * VB) + g * J * VB;
-        const __half* sc = c.sc + (row + g) * (2 * J);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            stage_words<kK>(buf + 128 * h * kK, k + 8 * h * (4 * J * KB), lane);
-            stage_words<J>(buf + 128 * (2 * kK + h * J), sc + 8 * h * (2 * J), lane);
-            stage_words<kV>(buf + 128 * (2 * kK + 2 * J + h * kV), v + 4 * h * (8 * J * VB), lane);
+// N words of shared memory at a + O (aligned to N words' largest power of two up to 16 bytes; the constant part of an address
+// stays out of the register), from pieces S bytes apart (16: side by side)
+template <int N> constexpr int kPiece = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;     // words of a load
+template <int N, int O, int S = 0>
+__device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t a) {
+    constexpr int W = kPiece<N>;
+    constexpr int step = S ? S : 4 * W;
+    auto piece = [&](auto at) {
+        constexpr int i = decltype(at)::value * W, o = O + decltype(at)::value * step;
+        if constexpr (W == 4)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(a), "n"(o));
+        else if constexpr (W == 2)
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(a), "n"(o));
+        else
+            asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(w[i]) : "r"(a), "n"(o));
+    };
+    each<N / W>(piece);
+}
+// N words from global p + O to shared a + Q, in pieces 32 lanes' pieces apart, asynchronously
+template <int N, int O, int Q>
+__device__ __forceinline__ void copy_words(uint32_t a, const uint8_t* p) {
+    constexpr int W = kPiece<N>;
+    auto piece = [&](auto at) {
+        constexpr int i = decltype(at)::value;
+        if constexpr (W == 4)
+            asm volatile("cp.async.cg.shared.global [%0 + %1], [%2 + %3], 16;" :: "r"(a), "n"(Q + 128 * W * i), "l"(p), "n"(O + 4 * W * i) : "memory");
+        else
+            asm volatile("cp.async.ca.shared.global [%0 + %1], [%2 + %3], %4;" :: "r"(a), "n"(Q + 128 * W * i), "l"(p), "n"(O + 4 * W * i), "n"(4 * W) : "memory");
+    };
+    each<N / W>(piece);
+}
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// A slot of a warp's ring in shared memory: KT tiles of 16 keys.  A lane (g = lane / 4, t = lane % 4) uses run t of the K rows
+// of keys g and g + 8, run g of the V pairs t and t + 4, and the scales of keys 2 t, 2 t + 1, 2 t + 8 and 2 t + 9.  K and
+// scales come as they lie, in one bulk copy each that one lane starts.  V's runs would meet on the same banks that way (four
+// pairs, 128 bytes apart), so each lane copies its own, side by side with the other lanes'.  (Everything by the lanes: 376
+// instructions a tile, and 27 bytes a clock and SM at the start.  V pair by pair in bulk, padded: the lanes' copies go out one
+// after the other, 136 instructions a tile.)
+template <int J, int KB, int VB, int KT>
+struct AttnSlot {
+    static constexpr int kK = J * KB / 4, kV = J * VB / 4, kS = (J + 1) / 2;       // words of a lane's runs, of a key's K or V scales
+    static constexpr int kRowK = 4 * J * KB, kRowV = 8 * J * VB, kRowS = 4 * J;    // bytes of a key, a pair, a key's scales
+    static constexpr int kOffK = KT * 256 * kV, kOffS = kOffK + KT * 16 * kRowK, kBytes = kOffS + KT * 16 * kRowS;
+    template <int X>
+    static __device__ __forceinline__ void keys(uint32_t (&k)[2][kK], uint32_t at) {           // at: slot + lane's place (lane_k)
+        lds_words<kK, kOffK + 16 * X * kRowK>(k[0], at);
+        lds_words<kK, kOffK + (16 * X + 8) * kRowK>(k[1], at);
+    }
+    static __device__ __forceinline__ uint32_t lane_k(int g, int t) { return g * kRowK + t * J * KB; }
+    template <int X>
+    static __device__ __forceinline__ void vals(uint32_t (&v)[2][kV], uint32_t at) {           // at: slot + lane_v
+        lds_words<kV, 256 * kV * X, 128 * kPiece<kV>>(v[0], at);
+        lds_words<kV, 256 * kV * X + 128 * kV, 128 * kPiece<kV>>(v[1], at);
+    }
+    static __device__ __forceinline__ uint32_t lane_v(int lane) { return 4 * kPiece<kV> * lane; }
+    template <int X>
+    static __device__ __forceinline__ void copy_vals(uint32_t at, const uint8_t* from) {       // from: the tile's pair t, run g
+        copy_words<kV, 0, 256 * kV * X>(at, from);
+        copy_words<kV, 4 * kRowV, 256 * kV * X + 128 * kV>(at, from);
+    }
+    // K's (V: V's) scale words of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (J 3: the first of V's is half K's); at: slot + 2 t rows
+    template <int X, bool V>
+    static __device__ __forceinline__ void scales(uint32_t (&sc)[4][kS], uint32_t at) {
+        constexpr int o = kOffS + 16 * X * kRowS + (V ? 4 * (J - kS) : 0);
+        if constexpr (J == 3) {                                   // rows of 12 bytes: word by word
+            lds_words<1, o>(*reinterpret_cast<uint32_t(*)[1]>(sc[0]), at), lds_words<1, o + 4>(*reinterpret_cast<uint32_t(*)[1]>(sc[0] + 1), at);
+            lds_words<1, o + 12>(*reinterpret_cast<uint32_t(*)[1]>(sc[1]), at), lds_words<1, o + 16>(*reinterpret_cast<uint32_t(*)[1]>(sc[1] + 1), at);
+            lds_words<1, o + 96>(*reinterpret_cast<uint32_t(*)[1]>(sc[2]), at), lds_words<1, o + 100>(*reinterpret_cast<uint32_t(*)[1]>(sc[2] + 1), at);
+            lds_words<1, o + 108>(*reinterpret_cast<uint32_t(*)[1]>(sc[3]), at), lds_words<1, o + 112>(*reinterpret_cast<uint32_t(*)[1]>(sc[3] + 1), at);
+        } else {
+            lds_words<kS, o>(sc[0], at), lds_words<kS, o + kRowS>(sc[1], at);
+            lds_words<kS, o + 8 * kRowS>(sc[2], at), lds_words<kS, o + 9 * kRowS>(sc[3], at);
         }
     }
-    static __device__ __forceinline__ void keys(uint32_t (&k)[2][kK], uint32_t (&sc)[2][J], uint32_t buf, int lane) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            staged_words<kK>(k[h], buf + 128 * h * kK, lane);
-            staged_words<J>(sc[h], buf + 128 * (2 * kK + h * J), lane);
-        }
+    // scale j of those words
+    static __device__ __forceinline__ float scale(const uint32_t (&sc)[kS], int j, bool v) {
+        const int i = j + (v ? J % 2 : 0);
+        const __half2 h = bits_h2(sc[i >> 1]);
+        return i & 1 ? __high2float(h) : __low2float(h);
     }
-    static __device__ __forceinline__ void vals(uint32_t (&v)[2][kV], uint32_t buf, int lane) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) staged_words<kV>(v[h], buf + 128 * (2 * kK + 2 * J + h * kV), lane);
+    // V's scale j of two keys side by side
+    static __device__ __forceinline__ uint32_t pair(const uint32_t (&a)[kS], const uint32_t (&b)[kS], int j) {
+        const int i = j + J % 2;
+        return __byte_perm(a[i >> 1], b[i >> 1], i & 1 ? 0x7632 : 0x5410);
     }
 };
-// half i of a key's scales (K's J, then V's J)
-template <int J>
-__device__ __forceinline__ float scale_of(const uint32_t (&sc)[J], int i) {
-    return h2f(i & 1 ? sc[i >> 1] >> 16 : sc[i >> 1] & 0xFFFFu);
+// Tiles of 16 keys a warp works on at once (two: each instruction has another that does not wait for it, and the loop's and
+// the softmax's bookkeeping counts half), keys a unit, CTAs an SM is to hold, and the units a warp has in shared memory,
+// within 227 KB an SM.
+__host__ __device__ constexpr int attn_tiles(int J, int nt) { return J < 8 && nt == 1 ? 2 : 1; }
+__host__ __device__ constexpr int attn_unit(int J, int nt) { return 16 * kAttnWarps * attn_tiles(J, nt); }
+__host__ __device__ constexpr int attn_unit_bytes(int J, int kb, int vb, int nt) {
+    return kAttnWarps * attn_tiles(J, nt) * 64 * J * (vb + kb + 1);
 }
-
-// CTAs an SM is to hold, and the tiles a warp has in shared memory, within 227 KB an SM
-template <int DT, int J, int NT> constexpr int kAttnCtas = J == 8 || NT == 2 ? 2 : DT == QMV_OUT_F32 ? 3 : 4;
-template <int DT, int J, int KB, int VB, int NT>
-__host__ __device__ constexpr int attn_stages() {
-    const int room = (226 * 1024) / kAttnCtas<DT, J, NT> - 1024 - (DT == QMV_OUT_F32 ? 2 : 1) * NT * J * 512 - 256;
-    const int n = room / (kAttnWarps * AttnTile<J, KB, VB>::kBytes);
+__host__ __device__ constexpr int attn_room(bool hl, int J, int nt, int ctas) {
+    return (226 * 1024) / ctas - 1024 - J * 2048 - 256;      // less the fragments
+}
+__host__ __device__ constexpr int attn_ctas(bool hl, int J, int kb, int vb, int nt) {
+    return J < 8 && nt == 1 && attn_room(hl, J, nt, 3) >= 2 * attn_unit_bytes(J, kb, vb, nt) ? 3 : 2;
+}
+__host__ __device__ constexpr int attn_stages(bool hl, int J, int kb, int vb, int nt) {
+    const int n = attn_room(hl, J, nt, attn_ctas(hl, J, kb, vb, nt)) / attn_unit_bytes(J, kb, vb, nt);
     return n > 4 ? 4 : n;
 }
 
@@ -157,7 +201,7 @@ __host__ __device__ constexpr int attn_part_floats() { return 8 * NT * (32 * J +
 struct AttnSeq {
     int row0, n, len, first_unit, units;  // query rows, tokens in the cache, units of a segment
 };
-__device__ __forceinline__ AttnSeq attn_seq(const AttnParams& P, int b, bool report) {
+__device__ __forceinline__ AttnSeq attn_seq(const AttnParams& P, int b, bool report, int unit_keys) {
     AttnSeq s;
     int row1;
     if (P.starts) {
@@ -171,8 +215,8 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams& P, int b, bool rep
     s.len = min(max(len, 0), cap);
     if (report && P.status && (len < 0 || len > cap || s.n > P.max_new)) atomicOr(P.status, DEV_BAD_ADDRESS);
     const int first = s.n == 0 ? 0 : max(0, min(P.window > 0 ? s.len - s.n - P.window + 1 : 0, s.len));
-    s.first_unit = first / kAttnUnit;
-    s.units = s.n == 0 ? 1 : max(1, (s.len + kAttnUnit - 1) / kAttnUnit - s.first_unit);
+    s.first_unit = first / unit_keys;
+    s.units = s.n == 0 ? 1 : max(1, (s.len + unit_keys - 1) / unit_keys - s.first_unit);
     return s;
 }
 
@@ -201,82 +245,120 @@ __device__ __forceinline__ void attn_store(const AttnParams& P, int row0, int r,
 }
 
 template <int DT, int J, int KB, int VB, int NT>
-__global__ void __launch_bounds__(32 * kAttnWarps, (kAttnCtas<DT, J, NT>)) attn_kernel(const __grid_constant__ AttnParams P) {
+__global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32, J, KB, VB, NT))) attn_kernel(const __grid_constant__ AttnParams P) {
     using T = typename Elem<DT>::type;
-    constexpr bool HL = DT == QMV_OUT_F32;
+    // HL: queries and weights as two fp16 parts.  FAST: weights rounded to fp16 before they meet d_v, both then in fp16
+    // (two roundings of 2^-11 where the output's is 2^-8), half the instructions of the fp32 product and its rounding
+    constexpr bool HL = DT == QMV_OUT_F32, FAST = DT == QMV_OUT_BF16;
     constexpr int D = 32 * J, R = 8 * NT, kParts = HL ? 2 : 1;
     constexpr float kOffK = KB == 4 ? 8.f : 128.f;
+    constexpr float kTop = HL ? 4.f : 12.f;                      // p 2^-E at most 2^kTop (HL: small ones keep a second part's bits)
     constexpr uint32_t kOffV = VB == 4 ? 0x00080008u : 0x00800080u;
-    constexpr int S_ = attn_stages<DT, J, KB, VB, NT>();
-    using Tile = AttnTile<J, KB, VB>;
+    constexpr int S_ = attn_stages(HL, J, KB, VB, NT), KT = attn_tiles(J, NT), kUnit = attn_unit(J, NT);
+    using Slot = AttnSlot<J, KB, VB, KT>;
+    static_assert(kAttnWarps * Slot::kBytes == attn_unit_bytes(J, KB, VB, NT), "the launch's shared memory");
     extern __shared__ __align__(16) float s_part[];              // the warps' tiles [warps][S_]; then [warps][R (D + 2)]
-    __shared__ uint2 s_q[kParts][NT][J][2][32];                  // query fragments
+    constexpr bool two = HL || NT == 2;                          // the scores' rows g + 8 are used
+    // per block and lane, whole operands (put together in registers they cost a move a word): the queries of the two k steps, the
+    // scores' start, and the row of the offset's product
+    __shared__ uint4 s_q[J][2][32], s_one[J][32];
+    __shared__ float4 s_start[J][32];
     __shared__ long long s_scan[kAttnWarps + 1];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ uint64_t s_bar[kAttnWarps][4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t bar0 = smem_u32(s_bar[warp]);
+    if (lane == 0) {
+        for (int i = 0; i < S_; ++i) mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    bool dead = false;                                            // a copy did not come in time: this warp takes no more units
+    uint32_t phases = 0;                                          // bit i: the phase slot i of this warp's ring waits for
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int group = P.n_heads / P.c.n_kv, segs = P.c.n_kv * P.row_tiles;
 
-    // ---- this CTA's run of units: all units, then the sequence that holds the first one
+    // ---- this CTA's run of units: the list's length, and the sequence that holds the run's first one
     long long total = 0, u0 = 0, u1 = 0;
-    int ctas = gridDim.x;
+    int ctas = gridDim.x, b = 0, seg = 0, unit = 0;               // sequence, segment, unit: the next one
+    AttnSeq S;
     if (P.split) {
-        for (int b = tid; b < P.n_seq; b += 32 * kAttnWarps) total += attn_seq(P, b, blockIdx.x == 0).units;
+        long long before = 0;                                     // units of earlier sequences
+        if (P.n_seq == 1) {
+            S = attn_seq(P, 0, blockIdx.x == 0 && tid == 0, kUnit);
+            total = (long long)S.units * segs;
+        } else {
+            // sequences 128 at a time, a thread each; one round of them is looked at once
+            long long x = 0, inc = 0;
+            for (int b0 = 0; b0 < P.n_seq; b0 += 32 * kAttnWarps) {
+                x = b0 + tid < P.n_seq ? (long long)attn_seq(P, b0 + tid, blockIdx.x == 0, kUnit).units * segs : 0;
+                inc = x;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (lane == 0) s_scan[warp] = total;
-        __syncthreads();
-        total = 0;
+                for (int o = 1; o < 32; o *= 2) {
+                    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += y;
+                }
+                if (b0) __syncthreads();
+                if (lane == 31) s_scan[warp] = inc;
+                __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) total += s_scan[w];
-        total *= segs;
-        const long long most = max((total + kAttnMinUnits - 1) / kAttnMinUnits, (long long)P.n_seq * segs);
+                for (int w = 0; w < kAttnWarps; ++w) {
+                    if (w < warp) inc += s_scan[w];
+                    total += s_scan[w];
+                }
+            }
+            const long long most = max((total + kAttnMinKeys / kUnit - 1) / (kAttnMinKeys / kUnit), (long long)P.n_seq * segs);
+            if (most < ctas) ctas = int(most);
+            const long long first_u = total * blockIdx.x / ctas;
+            __syncthreads();
+            if (P.n_seq <= 32 * kAttnWarps) {
+                if (inc - x <= first_u && first_u < inc) s_scan[0] = tid, s_scan[1] = inc - x;
+                __syncthreads();
+            } else if (blockIdx.x < ctas) {
+                long long base = 0;
+                for (int b0 = 0; b0 < P.n_seq; b0 += 32 * kAttnWarps) {
+                    x = b0 + tid < P.n_seq ? (long long)attn_seq(P, b0 + tid, false, kUnit).units * segs : 0;
+                    inc = x;
+#pragma unroll
+                    for (int o = 1; o < 32; o *= 2) {
+                        const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+                        if (lane >= o) inc += y;
+                    }
+                    if (lane == 31) s_scan[warp] = inc;
+                    __syncthreads();
+                    long long all = base;
+                    inc += base;
+#pragma unroll
+                    for (int w = 0; w < kAttnWarps; ++w) {
+                        if (w < warp) inc += s_scan[w];
+                        all += s_scan[w];
+                    }
+                    __syncthreads();
+                    if (first_u < all) {                          // the same for every thread
+                        if (inc - x <= first_u && first_u < inc) s_scan[0] = b0 + tid, s_scan[1] = inc - x;
+                        __syncthreads();
+                        break;
+                    }
+                    base = all;
+                }
+            }
+            b = int(s_scan[0]);
+            before = s_scan[1];
+        }
+        const long long most = max((total + kAttnMinKeys / kUnit - 1) / (kAttnMinKeys / kUnit), (long long)P.n_seq * segs);
         if (most < ctas) ctas = int(most);
         if (blockIdx.x >= ctas) {
-            if (tid == 0 && !P.by_segment) P.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+            if (tid == 0 && !P.by_segment) P.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             return;
         }
         u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-    } else {
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    }
-    int b = 0, seg = 0, unit = 0;                                 // the next unit
-    AttnSeq S;
-    if (P.split) {
-        long long before = 0;                                     // units of earlier sequences
-        for (int b0 = 0; b0 < P.n_seq; b0 += 32 * kAttnWarps) {
-            const int mine = b0 + tid;
-            const long long x = mine < P.n_seq ? (long long)attn_seq(P, mine, false).units * segs : 0;
-            long long inc = x;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            __syncthreads();
-            if (lane == 31) s_scan[warp] = inc;
-            __syncthreads();
-            long long base = before;
-            for (int w = 0; w < warp; ++w) base += s_scan[w];
-            long long all = before;
-            for (int w = 0; w < kAttnWarps; ++w) all += s_scan[w];
-            if (u0 < all) {                                       // the same for every thread
-                const bool hit = base + inc - x <= u0 && u0 < base + inc;
-                __syncthreads();
-                if (hit) s_scan[0] = mine, s_scan[1] = base + inc - x;
-                __syncthreads();
-                b = int(s_scan[0]);
-                before = s_scan[1];
-                break;
-            }
-            before = all;
-        }
-        S = attn_seq(P, b, false);
+        if (P.n_seq > 1) S = attn_seq(P, b, false, kUnit);
         const long long in = u0 - before;
         seg = int(in / S.units), unit = int(in - (long long)seg * S.units);
     } else {                                                      // one CTA a segment
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         b = blockIdx.x / segs, seg = blockIdx.x - b * segs;
-        S = attn_seq(P, b, seg == 0 && tid == 0);
+        S = attn_seq(P, b, seg == 0 && tid == 0, kUnit);
         u1 = S.units;
     }
     bool owns = false;                                            // desc of this CTA written
@@ -292,12 +374,85 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (kAttnCtas<DT, J, NT>)) attn_
         // every row sees keys full0 .. full1
         const int full0 = P.window > 0 ? max(0, pos0 + tok1 - P.window + 1) : 0, full1 = pos0 + tok0;
 
-        float start[NT][J][2], cs[NT][2], M[NT][2], sum[NT][2], o[NT][J][2][4], off[NT][4];
-        int pos[NT][2];
+        float cs[NT], M[NT], rn[NT], sum[NT], o[NT][J][2][4], off[NT][4];        // of rows g, g + 8; o, off: columns 2 t, 2 t + 1
+        int pos[NT];
         float E = 0.f;
-        uint32_t lim = 0;
+        uint32_t lim = HL ? 0u : 0x48004800u;                     // d_v at most 8 until one larger is seen (two fp16)
         if (rows > 0) {
-            // queries: lane (g, t) holds row g's values 8 t .. 8 t + 7 of each block, scaled to fp16 by a power of two
+            // ---- this warp's tiles, KT a unit: the first units' copies start before the queries are looked at
+            const int turns = dead ? 0 : todo;
+            const int* table = P.tables + (long long)b * P.width;
+            const int key0 = (S.first_unit + unit) * kUnit + 16 * KT * warp;
+            const uint32_t ring = smem_u32(s_part) + warp * S_ * Slot::kBytes;
+            const uint32_t lane_k = Slot::lane_k(g, t), lane_v = Slot::lane_v(lane), lane_s = 2 * t * Slot::kRowS;
+            const int shift = P.c.page_shift, in_page = (1 << shift) - 1;
+            // this key head's rows of page 0, this lane's V run of it, and the bytes between pages
+            const uint8_t* head_k = P.c.k + ((long long)hk << shift) * Slot::kRowK;
+            const uint8_t* head_v = P.c.v + ((long long)hk << (shift - 1)) * Slot::kRowV + t * Slot::kRowV + g * J * VB;
+            const uint8_t* head_s = reinterpret_cast<const uint8_t*>(P.c.sc) + ((long long)hk << shift) * Slot::kRowS;
+            const uint32_t page_k = uint32_t(P.c.n_kv * Slot::kRowK) << shift, page_v = uint32_t(P.c.n_kv * Slot::kRowV) << (shift - 1),
+                           page_s = uint32_t(P.c.n_kv * Slot::kRowS) << shift;
+            constexpr int kNoKey = INT_MIN;                       // nothing to see there
+            struct Entry { int page[KT]; };                       // of a unit's tiles
+            auto look = [&](int u) {
+                Entry e;
+#pragma unroll
+                for (int x = 0; x < KT; ++x) {
+                    const int key = key0 + u * kUnit + 16 * x;
+                    e.page[x] = u < turns && key <= last && key + 15 >= first ? __ldg(table + (key >> shift)) : kNoKey;
+                }
+                return e;
+            };
+            uint32_t held = 0;                                    // bit KT i + x: tile x of slot i is there
+            auto ask = [&](int u, int slot, const Entry& e) {     // starts the copies of unit u's tiles
+                const uint32_t to = ring + slot * Slot::kBytes, bar = bar0 + 8 * slot;
+                uint32_t tiles = 0;
+#pragma unroll
+                for (int x = 0; x < KT; ++x) {
+                    const bool there = e.page[x] >= 0 && e.page[x] < P.c.n_pages;
+                    if (there) tiles |= 1u << x;
+                    else if (e.page[x] != kNoKey && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
+                }
+                held = (held & ~(((1u << KT) - 1u) << (KT * slot))) | tiles << (KT * slot);
+                const int at = (key0 + u * kUnit) & in_page;
+                if (tiles == (1u << KT) - 1u && (KT == 1 || shift > 4)) {          // one page holds the unit
+                    const uint32_t page = e.page[0];
+                    if (lane == 0) {
+                        mbar_arrive_tx(bar, KT * 16 * (Slot::kRowK + Slot::kRowS));
+                        copy_bulk(to + Slot::kOffK, head_k + (unsigned long long)page * page_k + at * Slot::kRowK, KT * 16 * Slot::kRowK, bar);
+                        copy_bulk(to + Slot::kOffS, head_s + (unsigned long long)page * page_s + at * Slot::kRowS, KT * 16 * Slot::kRowS, bar);
+                    }
+                    const uint8_t* from = head_v + (unsigned long long)page * page_v + (at >> 1) * Slot::kRowV;
+                    each<KT>([&](auto x) { Slot::template copy_vals<decltype(x)::value>(to + lane_v, from + decltype(x)::value * 8 * Slot::kRowV); });
+                } else {
+                    if (lane == 0) mbar_arrive_tx(bar, __popc(tiles) * 16 * (Slot::kRowK + Slot::kRowS));
+                    each<KT>([&](auto x) {
+                        constexpr int X = decltype(x)::value;
+                        if (tiles >> X & 1u) {
+                            const uint32_t page = e.page[X];
+                            const int a = (at + 16 * X) & in_page;
+                            if (lane == 0) {
+                                copy_bulk(to + Slot::kOffK + 16 * X * Slot::kRowK, head_k + (unsigned long long)page * page_k + a * Slot::kRowK, 16 * Slot::kRowK, bar);
+                                copy_bulk(to + Slot::kOffS + 16 * X * Slot::kRowS, head_s + (unsigned long long)page * page_s + a * Slot::kRowS, 16 * Slot::kRowS, bar);
+                            }
+                            Slot::template copy_vals<X>(to + lane_v, head_v + (unsigned long long)page * page_v + (a >> 1) * Slot::kRowV);
+                        }
+                    });
+                }
+            };
+            Entry entry[S_ - 1];                                  // of the units to ask for next (the loop: one, a unit ahead)
+#pragma unroll
+            for (int u = 0; u < S_ - 1; ++u) entry[u] = look(u);
+#pragma unroll
+            for (int u = 0; u < S_ - 1; ++u) {
+                if (u < turns) ask(u, u, entry[u]);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+            entry[0] = look(S_ - 1);
+            // Queries, scaled to fp16 by a power of two per row: lane (g, t) holds values 8 t .. 8 t + 7 of each block of row g
+            // as the product's rows g, and as rows g + 8 the second parts (HL) or row g + 8 (NT 2)
+            uint32_t part[2][J][2][2];                            // [rows g / g + 8][block][k step][half]
+            float start[NT][J];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int r = 8 * nt + g, rr = rt * R + r;
@@ -316,222 +471,275 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (kAttnCtas<DT, J, NT>)) attn_
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // 2^14 <= top 2^-e < 2^15; a row of zeros or with an infinity keeps its size
                 const int ex = int((__float_as_uint(top) >> 23) & 255u);
-                const int e = ex == 0 || ex == 255 ? 0 : ex - 127 - 14;
-                const float down = __uint_as_float(uint32_t(127 - max(-120, min(120, e))) << 23);
-                const float up = P.scale * 1.4426950408889634f * 16777216.f * __uint_as_float(uint32_t(127 + max(-120, min(120, e))) << 23);
-                cs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t);
-                cs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+                const int e = ex == 0 || ex == 255 ? 0 : max(-120, min(120, ex - 127 - 14));
+                // the scale's sign goes into the queries: cs is positive, and masked scores stay -inf
+                const float down = __uint_as_float((uint32_t(127 - e) << 23) | (P.scale < 0.f ? 0x80000000u : 0u));
+                cs[nt] = fmaxf(fabsf(P.scale) * 1.4426950408889634f * 16777216.f * __uint_as_float(uint32_t(127 + e) << 23), 1e-30f);
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    float part = 0.f;
+                    float all = 0.f;
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         constexpr float kHigh = KB == 4 ? 1.f / 16.f : 1.f;     // the upper nibbles arrive 16 times too large
                         const float a = x[j][m].x * down, b2 = x[j][m].y * down, c = x[j][m].z * down * kHigh, d = x[j][m].w * down * kHigh;
                         const uint32_t lo = pack_h2(a, b2), hi = pack_h2(c, d);
                         const float2 fl = unpack_h2(lo), fh = unpack_h2(hi);
-                        part += (fl.x + fl.y) + (fh.x + fh.y) * (1.f / kHigh);
-                        if (warp == 0) s_q[0][nt][j][m][lane] = make_uint2(lo, hi);
+                        all += (fl.x + fl.y) + (fh.x + fh.y) * (1.f / kHigh);
+                        part[nt][j][m][0] = lo, part[nt][j][m][1] = hi;
                         if constexpr (HL) {
                             const uint32_t lo2 = pack_h2(a - fl.x, b2 - fl.y), hi2 = pack_h2(c - fh.x, d - fh.y);
                             const float2 gl = unpack_h2(lo2), gh = unpack_h2(hi2);
-                            part += (gl.x + gl.y) + (gh.x + gh.y) * (1.f / kHigh);
-                            if (warp == 0) s_q[kParts - 1][nt][j][m][lane] = make_uint2(lo2, hi2);
+                            all += (gl.x + gl.y) + (gh.x + gh.y) * (1.f / kHigh);
+                            part[1][j][m][0] = lo2, part[1][j][m][1] = hi2;
                         }
                     }
-                    part += __shfl_xor_sync(0xffffffffu, part, 1);
-                    part += __shfl_xor_sync(0xffffffffu, part, 2);
-                    part *= -kOffK * 5.9604644775390625e-8f;
-                    start[nt][j][0] = __shfl_sync(0xffffffffu, part, 8 * t);
-                    start[nt][j][1] = __shfl_sync(0xffffffffu, part, 8 * t + 4);
+                    all += __shfl_xor_sync(0xffffffffu, all, 1);
+                    all += __shfl_xor_sync(0xffffffffu, all, 2);
+                    start[nt][j] = all * (-kOffK * 5.9604644775390625e-8f);
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[nt][j][m][i] = 0.f;
                 }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    M[nt][i] = kAttnNone, sum[nt][i] = 0.f;
-                    pos[nt][i] = pos0 + (rt * R + min(8 * nt + 2 * t + i, rows - 1)) / group;
-                }
+                M[nt] = kAttnNone, rn[nt] = -kAttnNone, sum[nt] = 0.f;
+                pos[nt] = pos0 + (rt * R + min(r, rows - 1)) / group;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) off[nt][i] = 0.f;
             }
+            if (warp == 0) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+                        s_q[j][m][lane] = make_uint4(part[0][j][m][0], two ? part[1][j][m][0] : 0u, part[0][j][m][1], two ? part[1][j][m][1] : 0u);
+                    const float second = NT == 2 ? start[NT - 1][j] : 0.f;
+                    s_start[j][lane] = make_float4(start[0][j], start[0][j], second, second);
+                    s_one[j][lane] = make_uint4(g == j ? kOffV : 0u, 0u, g == j ? kOffV : 0u, 0u);
+                }
+            }
             __syncthreads();
-            // ---- this warp's tiles: one a unit
-            const int* table = P.tables + (long long)b * P.width;
-            const int key0 = (S.first_unit + unit) * kAttnUnit + 16 * warp;
-            auto page_of = [&](int key) -> long long {            // -1: nothing to see here
-                if (key > last || key + 15 < first) return -1;
-                const int p = __ldg(table + (key >> P.c.page_shift));
-                if (p >= 0 && p < P.c.n_pages) return p;
-                if (lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
-                return -1;
-            };
-            const uint32_t buf0 = smem_u32(s_part) + warp * S_ * Tile::kBytes;
-            uint32_t held = 0;                                    // bit i: slot i of the ring holds a tile
-            auto ask = [&](int u) {                               // starts the copies of unit u's tile
-                const int key = key0 + u * kAttnUnit, slot = u % S_;
-                const long long page = u < todo ? page_of(key) : -1;
-                held = (held & ~(1u << slot)) | (page >= 0 ? 1u << slot : 0u);
-                if (page >= 0) Tile::issue(buf0 + slot * Tile::kBytes, P.c, page, hk, key & (P.c.page() - 1), lane);
+            int slot = 0, slot_in = S_ - 1;                       // of unit u, and of unit u + S_ - 1
+            for (int u = 0; u < turns; ++u) {
+                const int key = key0 + u * kUnit;
+                if (u + S_ - 1 < turns) ask(u + S_ - 1, slot_in, entry[0]);
                 asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-#pragma unroll
-            for (int u = 0; u < S_ - 1; ++u) ask(u);
-            for (int u = 0; u < todo; ++u) {
-                const int key = key0 + u * kAttnUnit;
-                ask(u + S_ - 1);
+                entry[0] = look(u + S_);
+                const uint32_t buf = ring + slot * Slot::kBytes;
+                const uint32_t here = held >> (KT * slot) & ((1u << KT) - 1u);
                 asm volatile("cp.async.wait_group %0;" :: "n"(S_ - 1) : "memory");
-                const uint32_t buf = buf0 + (u % S_) * Tile::kBytes;
-                if (held >> (u % S_) & 1u) {
-                    uint32_t kw[2][Tile::kK], sc[2][J];
-                    Tile::keys(kw, sc, buf, lane);
-                    // keys nobody sees hold anything (NaN scales too): scale 0, and their scores are masked
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < J; ++i)
-                            if (uint32_t(key + g + 8 * h - first) > uint32_t(last - first)) sc[h][i] = 0u;
-                    // scores: C row g / g + 8 = keys, columns 2 t, 2 t + 1 = query rows
-                    float s[NT][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        const float d0 = scale_of(sc[0], j), d1 = scale_of(sc[1], j);
-                        uint32_t a[2][4];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if constexpr (KB == 4) {
-                                const uint32_t w = kw[h][j], w8 = w >> 8;
-                                a[0][h] = w & 0x000F000Fu, a[0][2 + h] = w & 0x00F000F0u;
-                                a[1][h] = w8 & 0x000F000Fu, a[1][2 + h] = w8 & 0x00F000F0u;
-                            } else {
-                                const uint32_t w = kw[h][2 * j], x = kw[h][2 * j + 1];
-                                a[0][h] = w & 0x00FF00FFu, a[0][2 + h] = (w >> 8) & 0x00FF00FFu;
-                                a[1][h] = x & 0x00FF00FFu, a[1][2 + h] = (x >> 8) & 0x00FF00FFu;
-                            }
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            float c[4] = {start[nt][j][0], start[nt][j][1], start[nt][j][0], start[nt][j][1]};
-#pragma unroll
-                            for (int p = 0; p < kParts; ++p)
-#pragma unroll
-                                for (int m = 0; m < 2; ++m) {
-                                    const uint2 w = s_q[p][nt][j][m][lane];
-                                    mma16816(c, a[m][0], a[m][1], a[m][2], a[m][3], w.x, w.y);
-                                }
-                            s[nt][0] = fmaf(d0, c[0], s[nt][0]), s[nt][1] = fmaf(d0, c[1], s[nt][1]);
-                            s[nt][2] = fmaf(d1, c[2], s[nt][2]), s[nt][3] = fmaf(d1, c[3], s[nt][3]);
-                        }
+                if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * slot, phases >> slot & 1u))) {
+                    // a copy did not come: say so, give the others in flight their time, and leave
+                    dead = true;
+                    if (lane == 0 && P.status) atomicOr(P.status, DEV_TIMEOUT);
+                    for (int v = u + 1; v < min(u + S_, turns); ++v) {
+                        slot = slot + 1 == S_ ? 0 : slot + 1;
+                        mbar_wait(bar0 + 8 * slot, phases >> slot & 1u);
                     }
-                    // log2 scores; a tile that some row does not see whole is masked key by key
-                    const bool whole = key >= full0 && key + 15 <= full1;
-                    float top = kAttnNone;
-                    const float limit = 4.f + E;
+                    break;
+                }
+                phases ^= 1u << slot;
+                slot = slot + 1 == S_ ? 0 : slot + 1;
+                slot_in = slot_in + 1 == S_ ? 0 : slot_in + 1;
+                // A unit that some row does not see whole is masked key by key, in a copy of the code: in one, the masks were
+                // predicated instructions that every unit paid for (100 of a tile's 440)
+                auto work = [&](auto all_of_it) {
+                constexpr bool whole = decltype(all_of_it)::value;
+                // scores: C rows g / g + 8 = query rows (or their second parts), columns 2 t, 2 t + 1 = keys, of two 8-key tiles
+                float s[KT][NT][4];
+                uint32_t dv = 0;                                  // |d_v| as two fp16, every one of the unit's in some lane
+                uint32_t kw[KT][2][Slot::kK], sk[KT][4][Slot::kS];         // scales of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+                each<KT>([&](auto x) {
+                    Slot::template keys<decltype(x)::value>(kw[decltype(x)::value], buf + lane_k);
+                    Slot::template scales<decltype(x)::value, false>(sk[decltype(x)::value], buf + lane_s);
+                });
+#pragma unroll
+                for (int x = 0; x < KT; ++x) {
+                    // the words that hold V's scales: J / 2 a key (J 3: two, the first of them half K's)
+                    constexpr int kPer = Slot::kS, kFirst = J - kPer;
+#pragma unroll
+                    for (int i = 0; i < 16 * kPer; i += 32) {
+                        const int w = i + lane, key_w = w / kPer, at = kFirst + w % kPer;
+                        if (16 * kPer % 32 == 0 || w < 16 * kPer)
+                            if (whole || (here >> x & 1u && uint32_t(key + 16 * x + key_w - first) <= uint32_t(last - first)))
+                                dv = __vmaxu2(dv, lds32(buf + Slot::kOffS + ((16 * x + key_w) * J + at) * 4) & (J % 2 && at == kFirst ? 0x7FFF0000u : 0x7FFF7FFFu));
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[x][nt][i] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const uint4 q0 = s_q[j][0][lane], q1 = s_q[j][1][lane];
+                    const float4 begin = s_start[j][lane];
+#pragma unroll
+                    for (int x = 0; x < KT; ++x)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            uint32_t k0, k1, k2, k3;
+                            if constexpr (KB == 4) {
+                                const uint32_t w = kw[x][y][j], w8 = w >> 8;
+                                k0 = w & 0x000F000Fu, k1 = w & 0x00F000F0u, k2 = w8 & 0x000F000Fu, k3 = w8 & 0x00F000F0u;
+                            } else {
+                                const uint32_t w = kw[x][y][2 * j], z = kw[x][y][2 * j + 1];
+                                k0 = w & 0x00FF00FFu, k1 = (w >> 8) & 0x00FF00FFu, k2 = z & 0x00FF00FFu, k3 = (z >> 8) & 0x00FF00FFu;
+                            }
+                            float c[4];
+                            mma16816(c, q0, k0, k1, begin);
+                            mma16816(c, q1.x, q1.y, q1.z, q1.w, k2, k3);
+                            const float d0 = Slot::scale(sk[x][2 * y], j, false), d1 = Slot::scale(sk[x][2 * y + 1], j, false);
+                            if (HL) c[0] += c[2], c[1] += c[3];
+                            s[x][0][2 * y] = fmaf(d0, c[0], s[x][0][2 * y]), s[x][0][2 * y + 1] = fmaf(d1, c[1], s[x][0][2 * y + 1]);
+                            if (NT == 2)
+                                s[x][NT - 1][2 * y] = fmaf(d0, c[2], s[x][NT - 1][2 * y]), s[x][NT - 1][2 * y + 1] = fmaf(d1, c[3], s[x][NT - 1][2 * y + 1]);
+                        }
+                }
+                uint32_t gone = 0;                                // bit 4 x + i: key i of tile x is nobody's
+                if constexpr (!whole) {
+#pragma unroll
+                    for (int x = 0; x < KT; ++x)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            s[nt][i] *= cs[nt][i & 1];
-                            if (!whole) {
-                                const int k = key + g + 8 * (i >> 1), p = pos[nt][i & 1];
-                                if (k > p || k > last || (P.window > 0 && p - k >= P.window)) s[nt][i] = -INFINITY;
-                            }
-                            top = fmaxf(top, s[nt][i] - (M[nt][i & 1] - E));
+                            const int k = key + 16 * x + 2 * t + (i & 1) + 8 * (i >> 1);
+                            const bool there = here >> x & 1u && uint32_t(k - first) <= uint32_t(last - first);
+                            if (!there) gone |= 1u << (4 * x + i);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                if (!there || k > pos[nt] || (P.window > 0 && pos[nt] - k >= P.window)) s[x][nt][i] = -INFINITY;
                         }
-                    uint32_t dv = 0;                              // the largest |d_v| of the lane's keys, as fp16 bits
+                }
+                // p = 2^(s cs + rn); the references move only if some p or d_v would pass its limit
+                float p[KT][NT][4], top = kAttnNone;
+                auto weigh = [&]() {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = J / 2; i < J; ++i) dv = __vmaxu2(dv, sc[h][i] & (J % 2 && i == J / 2 ? 0x7FFF0000u : 0x7FFF7FFFu));
-                    dv = max(dv >> 16, dv & 0xFFFFu);
-                    if (__any_sync(0xffffffffu, top > limit || dv > lim)) {
-                        float old[NT][2];
+                    for (int x = 0; x < KT; ++x)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                old[nt][i] = M[nt][i] - E;
-                                float m = fmaxf(s[nt][i], s[nt][i + 2]);
+                            for (int i = 0; i < 4; ++i) p[x][nt][i] = fmaf(s[x][nt][i], cs[nt], rn[nt]);
+                };
+                weigh();
 #pragma unroll
-                                for (int w = 4; w < 32; w *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-                                M[nt][i] = fmaxf(M[nt][i], m);
-                            }
-                        dv = __reduce_max_sync(0xffffffffu, dv);
-                        if (dv > lim) {                           // up to 2^(ev - 11) with a factor of 8 to 16 to spare
-                            const uint32_t ev = max(1u, dv >> 10);
-                            lim = min((ev + 4) << 10, 0x7BFFu);
-                            E = float(22 - int(ev));
-                        }
+                for (int x = 0; x < KT; ++x)
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const float f0 = ex2(old[nt][0] - (M[nt][0] - E)), f1 = ex2(old[nt][1] - (M[nt][1] - E));
-                            sum[nt][0] *= f0, sum[nt][1] *= f1;
-                            off[nt][0] *= f0, off[nt][1] *= f1;
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int j = 0; j < J; ++j)
-#pragma unroll
-                                for (int m = 0; m < 2; ++m) {
-                                    o[nt][j][m][0] *= f0, o[nt][j][m][1] *= f1;
-                                    o[nt][j][m][2] *= f0, o[nt][j][m][3] *= f1;
-                                }
-                        }
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, p[x][nt][i]);
+                if (__any_sync(0xffffffffu, top > kTop + E || __vmaxu2(dv, lim) != lim)) {
+                    dv = __reduce_max_sync(0xffffffffu, max(dv >> 16, dv & 0xFFFFu));
+                    if (dv > (lim & 0xFFFFu)) {                   // up to 2^(ev - 11), a factor of 8 to 16 to spare; times 2^E it is 2^(15 - kTop)
+                        const uint32_t ev = max(1u, dv >> 10);
+                        lim = min((ev + 4) << 10, 0x7BFFu) * 0x10001u;
+                        E = 26.f - kTop - float(int(ev));
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
+                        float m = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[nt][i] = ex2(s[nt][i] - (M[nt][i & 1] - E));
-                        sum[nt][0] += s[nt][0] + s[nt][2], sum[nt][1] += s[nt][1] + s[nt][3];
+                        for (int x = 0; x < KT; ++x) m = fmaxf(m, fmaxf(fmaxf(s[x][nt][0], s[x][nt][1]), fmaxf(s[x][nt][2], s[x][nt][3])));
+                        m *= cs[nt];
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                        M[nt] = fmaxf(M[nt], m);
+                        const float n = kTop - 4.f + E - M[nt], f = ex2(n - rn[nt]);
+                        rn[nt] = n;
+                        sum[nt] *= f;
+                        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+                        off[nt][0] *= f0, off[nt][1] *= f1;
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                o[nt][j][h][0] *= f0, o[nt][j][h][1] *= f1;
+                                o[nt][j][h][2] *= f0, o[nt][j][h][3] *= f1;
+                            }
                     }
-                    uint32_t vw[2][Tile::kV];
-                    Tile::vals(vw, buf, lane);
-                    // output: rows = values g / g + 8 of two tiles a block, k = keys, columns = query rows
+                    weigh();
+                }
+                uint32_t ph[KT][NT][2], vw[KT][2][Slot::kV], sv[KT][4][Slot::kS];
 #pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        const float d0 = scale_of(sc[0], J + j), d1 = scale_of(sc[1], J + j);
+                for (int x = 0; x < KT; ++x) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[x][nt][i] = ex2(p[x][nt][i]);
+                        sum[nt] += (p[x][nt][0] + p[x][nt][1]) + (p[x][nt][2] + p[x][nt][3]);
+                        if (FAST) ph[x][nt][0] = pack_h2(p[x][nt][0], p[x][nt][1]), ph[x][nt][1] = pack_h2(p[x][nt][2], p[x][nt][3]);
+                    }
+                }
+                each<KT>([&](auto x) {
+                    Slot::template vals<decltype(x)::value>(vw[decltype(x)::value], buf + lane_v);
+                    Slot::template scales<decltype(x)::value, true>(sv[decltype(x)::value], buf + lane_s);
+                });
+                if (!whole) {                                     // keys nobody sees hold anything (NaN scales too): 0 times 0
+#pragma unroll
+                    for (int x = 0; x < KT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int w = 0; w < Slot::kS; ++w) sv[x][i][w] = gone >> (4 * x + i) & 1u ? 0u : sv[x][i][w];
+                }
+                // output: rows = values g / g + 8 of two tiles a block, k = keys, columns = query rows: the scores' layout is that of
+                // the second operand already
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const uint4 one = s_one[j][lane];             // row j of the offset's product
+#pragma unroll
+                    for (int x = 0; x < KT; ++x) {
                         uint32_t a[2][4];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {             // pair t (k 2 t, 2 t + 1), pair t + 4 (k 8 + 2 t, 9 + 2 t)
                             if constexpr (VB == 4) {
-                                const uint32_t w = vw[h][j], w8 = w >> 8;
+                                const uint32_t w = vw[x][h][j], w8 = w >> 8;
                                 a[0][2 * h] = w & 0x000F000Fu, a[0][2 * h + 1] = w & 0x00F000F0u;
                                 a[1][2 * h] = w8 & 0x000F000Fu, a[1][2 * h + 1] = w8 & 0x00F000F0u;
                             } else {
-                                const uint32_t w = vw[h][2 * j], x = vw[h][2 * j + 1];
+                                const uint32_t w = vw[x][h][2 * j], y = vw[x][h][2 * j + 1];
                                 a[0][2 * h] = w & 0x00FF00FFu, a[0][2 * h + 1] = (w >> 8) & 0x00FF00FFu;
-                                a[1][2 * h] = x & 0x00FF00FFu, a[1][2 * h + 1] = (x >> 8) & 0x00FF00FFu;
+                                a[1][2 * h] = y & 0x00FF00FFu, a[1][2 * h + 1] = (y >> 8) & 0x00FF00FFu;
                             }
                         }
-                        const uint32_t one = g == j ? kOffV : 0u; // row j of the offset's product
+                        float d[4];
+                        uint32_t d2[2];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (FAST) d2[i >> 1] = Slot::pair(sv[x][i & ~1], sv[x][i | 1], j);
+                            else d[i] = Slot::scale(sv[x][i], j, true);
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const float p0 = s[nt][0] * d0, p1 = s[nt][1] * d0, p2 = s[nt][2] * d1, p3 = s[nt][3] * d1;
-                            const uint32_t h0 = pack_h2(p0, p1), h1 = pack_h2(p2, p3);
+                            uint32_t bw[2], low[2];
 #pragma unroll
-                            for (int p = 0; p < kParts; ++p) {
-                                uint32_t x0 = h0, x1 = h1;
-                                if (p == 1) {
-                                    const float2 f0 = unpack_h2(h0), f1 = unpack_h2(h1);
-                                    x0 = pack_h2(p0 - f0.x, p1 - f0.y), x1 = pack_h2(p2 - f1.x, p3 - f1.y);
+                            for (int y = 0; y < 2; ++y) {
+                                if constexpr (FAST) {
+                                    bw[y] = h2_bits(__hmul2(bits_h2(ph[x][nt][y]), bits_h2(d2[y])));
+                                } else {
+                                    const float p0 = p[x][nt][2 * y] * d[2 * y], p1 = p[x][nt][2 * y + 1] * d[2 * y + 1];
+                                    bw[y] = pack_h2(p0, p1);
+                                    if (HL) {
+                                        const float2 f = unpack_h2(bw[y]);
+                                        low[y] = pack_h2(p0 - f.x, p1 - f.y);
+                                    }
                                 }
-                                const uint32_t b0 = movm(x0), b1 = movm(x1);
+                            }
+#pragma unroll
+                            for (int z = 0; z < kParts; ++z) {
+                                const uint32_t b0 = z ? low[0] : bw[0], b1 = z ? low[1] : bw[1];
                                 mma16816(o[nt][j][0], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
                                 mma16816(o[nt][j][1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
-                                mma16816(off[nt], one, 0u, one, 0u, b0, b1);
+                                mma16816(off[nt], one.x, one.y, one.z, one.w, b0, b1);
                             }
                         }
                     }
                 }
+                };
+                if (here == (1u << KT) - 1u && key >= full0 && key + 16 * KT - 1 <= full1) work(std::true_type{});
+                else if (here) work(std::false_type{});
+                __syncwarp();                                     // before other lanes copy into the slot again
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncthreads();                                      // every warp is done with its tiles
             // ---- the warps' sums side by side in shared memory
-            float* mine = s_part + warp * attn_part_floats<J, NT>();
+            float* own = s_part + warp * attn_part_floats<J, NT>();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -539,19 +747,13 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (kAttnCtas<DT, J, NT>)) attn_
                     constexpr float kUp = 16777216.f, kHigh = VB == 4 ? kUp / 16.f : kUp;
                     const float z0 = __shfl_sync(0xffffffffu, off[nt][0], 4 * j + t) * kUp, z1 = __shfl_sync(0xffffffffu, off[nt][1], 4 * j + t) * kUp;
                     const float(&x)[2][4] = o[nt][j];
-                    float* p = mine + (8 * nt + 2 * t) * D + 32 * j + 4 * g;
+                    float* p = own + (8 * nt + 2 * t) * D + 32 * j + 4 * g;
                     *reinterpret_cast<float4*>(p) = make_float4(fmaf(x[0][0], kUp, -z0), fmaf(x[0][2], kHigh, -z0), fmaf(x[1][0], kUp, -z0), fmaf(x[1][2], kHigh, -z0));
                     *reinterpret_cast<float4*>(p + D) = make_float4(fmaf(x[0][1], kUp, -z1), fmaf(x[0][3], kHigh, -z1), fmaf(x[1][1], kUp, -z1), fmaf(x[1][3], kHigh, -z1));
                 }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                    for (int w = 4; w < 32; w *= 2) sum[nt][i] += __shfl_xor_sync(0xffffffffu, sum[nt][i], w);
-                    if (g == 0) {
-                        mine[R * D + 8 * nt + 2 * t + i] = M[nt][i] - E;
-                        mine[R * D + R + 8 * nt + 2 * t + i] = sum[nt][i];
-                    }
-                }
+                sum[nt] += __shfl_xor_sync(0xffffffffu, sum[nt], 1);
+                sum[nt] += __shfl_xor_sync(0xffffffffu, sum[nt], 2);
+                if (t == 0) own[R * D + 8 * nt + g] = -rn[nt], own[R * D + R + 8 * nt + g] = sum[nt];
             }
         }
         // ---- and joined: the output, or this CTA's part of a cut segment
@@ -559,9 +761,12 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (kAttnCtas<DT, J, NT>)) attn_
         if (P.split && tid == 0 && !head_part) {                  // the segment starts here
             const long long end = u0 + S.units;                   // how many later CTAs work on it
             const int more = whole ? 0 : int(((end * ctas + total - 1) / total) - 1 - blockIdx.x);
-            const int4 d = make_int4(int(blockIdx.x), whole || rows == 0 ? 0 : more + 1, b, seg);
-            if (P.by_segment) P.desc[b * segs + seg] = d;
-            else if (!whole) P.desc[blockIdx.x] = d, owns = true;
+            const int at = P.by_segment ? b * segs + seg : int(blockIdx.x);
+            if (P.by_segment || !whole) {
+                P.desc[2 * at] = make_int4(int(blockIdx.x), whole ? 0 : more + 1, S.row0, hk);
+                P.desc[2 * at + 1] = make_int4(rt * R, rows, 0, 0);
+                owns = true;
+            }
         }
         if (rows > 0) {
             __syncthreads();
@@ -577,77 +782,91 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (kAttnCtas<DT, J, NT>)) attn_
                     if (i0 == 0) slot[R * D + r] = ref, slot[R * D + R + r] = weight;
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // these uses come before the next segment's copies
             __syncthreads();
         }
         u0 += todo;
         unit = 0;
         if (u0 < u1 && ++seg == segs) {
             seg = 0;
-            S = attn_seq(P, ++b, false);
+            S = attn_seq(P, ++b, false, kUnit);
         }
     }
     if (P.split) {
-        if (!P.by_segment && tid == 0 && !owns) P.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (!P.by_segment && tid == 0 && !owns) P.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
 }
 
-// Joins the parts of cut segments: block (entry, row), four warps share the parts, a lane 4 values (8 for wide heads).
+// Joins the parts of cut segments, in their order: block (entry, row), eight warps share the parts, a lane 4 values (8 of
+// wide heads).  A chain of three dependent reads: the entry, then references, weights and sums of up to four parts a warp at once.
 template <int DT, int J, int NT>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnParams P) {
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnParams P) {
     using T = typename Elem<DT>::type;
-    constexpr int D = 32 * J, R = 8 * NT, F = attn_part_floats<J, NT>();
-    __shared__ float4 s_o[4][D / 4];
-    __shared__ float s_sum[4];
+    constexpr int D = 32 * J, R = 8 * NT, F = attn_part_floats<J, NT>(), W = 8, V = (D + 127) / 128, B = 4;
+    __shared__ float4 s_o[W][D / 4];
+    __shared__ float s_ref[W], s_sum[W];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 d = P.desc[blockIdx.x];
-    if (d.y == 0) return;
-    const int group = P.n_heads / P.c.n_kv, hk = d.w / P.row_tiles, rt = d.w - hk * P.row_tiles;
-    const AttnSeq S = attn_seq(P, d.z, false);
+    const int4 d = P.desc[2 * blockIdx.x], e = P.desc[2 * blockIdx.x + 1];
     const int r = blockIdx.y;
-    if (rt * R + r >= min(S.n, P.max_new) * group) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // part k: the second slot of the segment's first CTA, then the first slots of the following ones
-    auto part = [&](int k) { return P.parts + (2LL * (d.x + k) + (k == 0)) * F; };
-    float ref = kAttnNone;
-    for (int k = lane; k < d.y; k += 32) ref = fmaxf(ref, part(k)[R * D + r]);
+    if (d.y == 0 || r >= e.y) return;
+    const int group = P.n_heads / P.c.n_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float ref = kAttnNone, sum = 0.f;
+    float4 o[V];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-    constexpr int V = (D + 127) / 128;
-    float4 x[V];
-    float sum = 0.f;
+    for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = warp; k0 < d.y; k0 += W * B) {                  // B parts in flight; each warp at its own reference
+        float rk[B], wk[B];
+        float4 x[B][V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = warp; k < d.y; k += 4) {
-        const float* p = part(k);
-        const float f = ex2(p[R * D + r] - ref);
-        sum = fmaf(f, p[R * D + R + r], sum);
+        for (int q = 0; q < B; ++q) {
+            const int k = k0 + W * q;
+            // part k: the second slot of the segment's first CTA, then the first slots of the following ones
+            const float* p = P.parts + (2LL * (d.x + k) + (k == 0)) * F;
+            const bool there = k < d.y;
+            rk[q] = there ? p[R * D + r] : kAttnNone;
+            wk[q] = there ? p[R * D + R + r] : 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int i = 128 * v + 4 * lane;
-            if (i < D) {
-                const float4 y = *reinterpret_cast<const float4*>(p + r * D + i);
-                x[v].x = fmaf(f, y.x, x[v].x), x[v].y = fmaf(f, y.y, x[v].y), x[v].z = fmaf(f, y.z, x[v].z), x[v].w = fmaf(f, y.w, x[v].w);
-            }
+            for (int v = 0; v < V; ++v)
+                x[q][v] = there && 128 * v + 4 * lane < D ? *reinterpret_cast<const float4*>(p + r * D + 128 * v + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float top = ref;
+#pragma unroll
+        for (int q = 0; q < B; ++q) top = fmaxf(top, rk[q]);
+        const float f = ex2(ref - top);
+        ref = top;
+        sum *= f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = make_float4(o[v].x * f, o[v].y * f, o[v].z * f, o[v].w * f);
+#pragma unroll
+        for (int q = 0; q < B; ++q) {
+            const float w = ex2(rk[q] - ref);
+            sum = fmaf(w, wk[q], sum);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                o[v] = make_float4(fmaf(w, x[q][v].x, o[v].x), fmaf(w, x[q][v].y, o[v].y), fmaf(w, x[q][v].z, o[v].z), fmaf(w, x[q][v].w, o[v].w));
         }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v)
-        if (128 * v + 4 * lane < D) s_o[warp][32 * v + lane] = x[v];
-    if (lane == 0) s_sum[warp] = sum;
+        if (128 * v + 4 * lane < D) s_o[warp][32 * v + lane] = o[v];
+    if (lane == 0) s_ref[warp] = ref, s_sum[warp] = sum;
     __syncthreads();
-    for (int i = threadIdx.x; i < D / 4; i += 128) {
-        float4 y = s_o[0][i];
-        float w = s_sum[0];
+    for (int i = threadIdx.x; i < D / 4; i += 32 * W) {
+        float top = s_ref[0];
 #pragma unroll
-        for (int k = 1; k < 4; ++k) {
+        for (int k = 1; k < W; ++k) top = fmaxf(top, s_ref[k]);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        float w = 0.f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float f = ex2(s_ref[k] - top);
             const float4 z = s_o[k][i];
-            y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
-            w += s_sum[k];
+            y = make_float4(fmaf(f, z.x, y.x), fmaf(f, z.y, y.y), fmaf(f, z.z, y.z), fmaf(f, z.w, y.w));
+            w = fmaf(f, s_sum[k], w);
         }
-        attn_store<T>(P, S.row0, rt * R + r, group, hk, 4 * i, y, w);
+        attn_store<T>(P, d.z, e.x + r, group, d.w, 4 * i, y, w);
     }
 }
 
@@ -660,38 +879,39 @@ struct AttnPlan {
 };
 inline AttnPlan attn_plan(const KvView& c, int dtype, int n_heads, int n_seq, int max_new, int width, int window) {
     AttnPlan p{};
-    const bool hl = dtype == QMV_OUT_F32, wide = c.J == 8;
+    const bool hl = dtype == QMV_OUT_F32;
     const long long rows = (long long)max_new * (n_heads / c.n_kv);
-    p.nt = rows > 8 && !hl && !wide ? 2 : 1;
+    p.nt = rows > 8 && !hl && c.J < 8 ? 2 : 1;
     p.row_tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const long long segs = (long long)n_seq * c.n_kv * p.row_tiles;
+    const int unit = attn_unit(c.J, p.nt), least = kAttnMinKeys / unit;
     long long keys = (long long)width << c.page_shift;
-    if (window > 0 && keys > (long long)window + max_new) keys = (long long)window + max_new + kAttnUnit;
-    const long long units = (keys + kAttnUnit - 1) / kAttnUnit;   // of a segment, at most
-    p.split = units > kAttnMinUnits;
-    const long long most = p.split ? std::max((segs * units + kAttnMinUnits - 1) / kAttnMinUnits, segs) : segs;
-    const int resident = sm_count() * (wide || p.nt == 2 ? 2 : hl ? 3 : 4);     // kAttnCtas
+    if (window > 0 && keys > (long long)window + max_new) keys = (long long)window + max_new + unit;
+    const long long units = (keys + unit - 1) / unit;             // of a segment, at most
+    p.split = units > least;
+    const long long most = p.split ? std::max((segs * units + least - 1) / least, segs) : segs;
+    const int resident = sm_count() * attn_ctas(hl, c.J, c.kb, c.vb, p.nt);
     p.grid = p.split ? int(std::min<long long>(most, resident)) : segs <= 0x7FFFFFFF ? int(segs) : 0;
     if (segs > 0x7FFFFFFF) p.grid = 0;                            // refused
     p.by_segment = p.split && segs <= p.grid;
     p.entries = p.by_segment ? int(segs) : p.grid;
     p.part_bytes = p.split ? 2LL * p.grid * (8LL * p.nt * (c.dim + 2)) * 4 : 0;
     p.part_bytes = (p.part_bytes + 255) / 256 * 256;
-    p.bytes = p.part_bytes + (p.split ? 16LL * p.entries : 0) + 256;
+    p.bytes = p.part_bytes + (p.split ? 32LL * p.entries : 0) + 256;
     return p;
 }
 
 template <int DT, int J, int KB, int VB, int NT>
 int attn_launch(const AttnParams& P, const AttnPlan& pl, cudaStream_t st) {
     const size_t smem = std::max(size_t(kAttnWarps) * attn_part_floats<J, NT>() * 4,
-                                 size_t(kAttnWarps) * attn_stages<DT, J, KB, VB, NT>() * AttnTile<J, KB, VB>::kBytes);
+                                 size_t(attn_stages(DT == QMV_OUT_F32, J, KB, VB, NT)) * attn_unit_bytes(J, KB, VB, NT));
     static SmemGrant grant;
     if (const int e = grant(attn_kernel<DT, J, KB, VB, NT>, smem)) return e;
     const int rc = launch_pdl_smem(attn_kernel<DT, J, KB, VB, NT>, dim3(pl.grid), dim3(32 * kAttnWarps), smem, st, P);
     if (rc || !pl.split) return rc;
     cudaLaunchConfig_t cfg = {};                                  // may start while the last parts are written
     cfg.gridDim = dim3(pl.entries, std::min<long long>(8 * NT, (long long)P.max_new * (P.n_heads / P.c.n_kv)));
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

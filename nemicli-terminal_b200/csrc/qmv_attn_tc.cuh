@@ -136,8 +136,6 @@ __device__ __forceinline__ void at_st32(uint32_t a, const uint32_t (&r)[32]) {
 __device__ __forceinline__ void at_sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 
 // words of N bytes-aligned-as-they-come (see load sites) read once from global memory
 template <int N>
@@ -205,7 +203,7 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
     const int hk = x % P.c.n_kv;
     x /= P.c.n_kv;
     const int qt = P.row_tiles - 1 - x % P.row_tiles, b = x / P.row_tiles;        // the tiles with most keys first
-    const AttnSeq S = attn_seq(P, b, tid == 0 && hk == 0 && qt == 0);
+    const AttnSeq S = attn_seq(P, b, tid == 0 && hk == 0 && qt == 0, BN);
     const int rows = min(S.n, P.max_new) * group, base = qt * 128 * NQ;
     if (base >= rows) return;
     const int pos0 = S.len - S.n, tok0 = base / group, tok1 = (min(base + 128 * NQ, rows) - 1) / group;

@@ -59,6 +59,7 @@ inline int kv_view(const qmv_kv_cache* c, KvView& view) {
     while (shift < 10 && (1 << shift) != c->page) ++shift;
     if ((1 << shift) != c->page || c->n_pages <= 0 || c->n_kv <= 0 || c->n_kv > 65535) return ST_BAD_SHAPE;
     if (c->n_pages > (1LL << 40) / c->page) return ST_BAD_SHAPE;
+    if ((long long)c->n_kv * c->dim * c->page > (1LL << 30)) return ST_BAD_SHAPE;      // a page's bytes fit 31 bits
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 16)) return ST_BAD_ALIGN;
     view.k = static_cast<uint8_t*>(c->k);
     view.v = static_cast<uint8_t*>(c->v);
