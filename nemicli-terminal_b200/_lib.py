@@ -112,13 +112,26 @@ def stream_ptr(device=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device):
     """Makes `device` the current one for a launch (a stream belongs to its own device only); nothing to do where it
     is already."""
-    device = torch.device(device)
-    if device.type != "cuda" or device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    index = device.index
+    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def addr(t) -> int:
+    """A tensor's address (0 for None) as the plain number that ctypes turns into a pointer: the short way of ptr, for calls
+    that take longer to prepare than to run."""
+    return 0 if t is None else t.data_ptr()
+
+
+def stream_of(device) -> int:
+    """torch's current stream of a CUDA device, as a plain number."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def device_status(clear: bool = True, device=None) -> int:

@@ -1,5 +1,6 @@
 // Writing a quantised key / value cache and reading it back (layout: qmv_kv.cuh; C-ABI declarations:
 // include/nemicli_qmv.h).
+#include <algorithm>
 #include <type_traits>
 
 #include "qmv_kv.cuh"
@@ -21,31 +22,20 @@ struct KvWriteParams {
     const long long* pos;
     long long n_pos;
     int rot, paired, n_q;
-    int rows;
+    int rows, parts, per_part;            // warps a row, blocks a warp (a multiple of 4)
     int* status;
 };
 
-// The four values 4 m .. 4 m + 3 of block j of one head, rotated: value i < rot pairs with i + rot / 2 (or,
-// paired, 2 i with 2 i + 1), angle i of the row's position.  y1 = x1 c - x2 s, y2 = x2 c + x1 s; every product and
-// sum is rounded on its own (no fused multiply-add), so the codes follow from the inputs bit for bit.
-template <class T>
-__device__ __forceinline__ float4 rotated(const T* row, int i0, const KvWriteParams& P, const float* c, const float* s) {
-    float4 x = load4(row + i0);
-    if (!c || i0 >= P.rot) return x;
-    if (P.paired) {
-        const float2 cc = __ldg(reinterpret_cast<const float2*>(c + i0 / 2)), ss = __ldg(reinterpret_cast<const float2*>(s + i0 / 2));
-        return make_float4(__fsub_rn(__fmul_rn(x.x, cc.x), __fmul_rn(x.y, ss.x)), __fadd_rn(__fmul_rn(x.y, cc.x), __fmul_rn(x.x, ss.x)),
-                           __fsub_rn(__fmul_rn(x.z, cc.y), __fmul_rn(x.w, ss.y)), __fadd_rn(__fmul_rn(x.w, cc.y), __fmul_rn(x.z, ss.y)));
-    }
-    const int half = P.rot / 2;
-    const bool first = i0 < half;
-    const int a = first ? i0 : i0 - half;
-    const float4 o = load4(row + (first ? i0 + half : a)), cc = load4(c + a), ss = load4(s + a);
-    if (first)
-        return make_float4(__fsub_rn(__fmul_rn(x.x, cc.x), __fmul_rn(o.x, ss.x)), __fsub_rn(__fmul_rn(x.y, cc.y), __fmul_rn(o.y, ss.y)),
-                           __fsub_rn(__fmul_rn(x.z, cc.z), __fmul_rn(o.z, ss.z)), __fsub_rn(__fmul_rn(x.w, cc.w), __fmul_rn(o.w, ss.w)));
-    return make_float4(__fadd_rn(__fmul_rn(x.x, cc.x), __fmul_rn(o.x, ss.x)), __fadd_rn(__fmul_rn(x.y, cc.y), __fmul_rn(o.y, ss.y)),
-                       __fadd_rn(__fmul_rn(x.z, cc.z), __fmul_rn(o.z, ss.z)), __fadd_rn(__fmul_rn(x.w, cc.w), __fmul_rn(o.w, ss.w)));
+// Four consecutive values x of a head, rotated: value i < rot pairs with i + rot / 2 (o: the partners, cos and sin of the
+// angles), or, paired, 2 i with 2 i + 1 (cos.x, cos.y: of the two pairs).  y1 = x1 c - x2 s, y2 = x2 c + x1 s; every product
+// and sum is rounded on its own (no fused multiply-add), so the codes follow from the inputs bit for bit.
+__device__ __forceinline__ float4 rotated(float4 x, float4 o, float4 c, float4 s, bool paired, bool first) {
+    if (paired)
+        return make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(x.y, s.x)), __fadd_rn(__fmul_rn(x.y, c.x), __fmul_rn(x.x, s.x)),
+                           __fsub_rn(__fmul_rn(x.z, c.y), __fmul_rn(x.w, s.y)), __fadd_rn(__fmul_rn(x.w, c.y), __fmul_rn(x.z, s.y)));
+    if (first) s = make_float4(-s.x, -s.y, -s.z, -s.w);           // a - b s = a + b (-s), exactly
+    return make_float4(__fadd_rn(__fmul_rn(x.x, c.x), __fmul_rn(o.x, s.x)), __fadd_rn(__fmul_rn(x.y, c.y), __fmul_rn(o.y, s.y)),
+                       __fadd_rn(__fmul_rn(x.z, c.z), __fmul_rn(o.z, s.z)), __fadd_rn(__fmul_rn(x.w, c.w), __fmul_rn(o.w, s.w)));
 }
 
 __device__ __forceinline__ float cleaned(float x) {          // NaN counts as 0, the rest is clamped to +-65504
@@ -78,73 +68,98 @@ __device__ __forceinline__ uint4 quantise4(float4 x, bool q4, __half& d) {
     return make_uint4(uint32_t(c[0]), uint32_t(c[1]), uint32_t(c[2]), uint32_t(c[3]));
 }
 
-// One 32-value block of one head of one row on eight lanes; rows x (K heads, V heads, rotated query heads) x J blocks.
-// Bound by memory for long prompts, by its launch for a decode step.
-template <int DT>
+// A warp takes some of one row's 32-value blocks (K heads, then V heads, then the queries to rotate), four at a time on eight
+// lanes each, and kAhead such passes' loads go out together.  Rows' angles are the same for all of a lane's passes where
+// a head has 2 or 4 blocks.  Bound by memory for long prompts (divisions and reductions are about as many clocks), by its
+// launch for a decode step.
+template <int DT, int J>
 __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvWriteParams P) {
     using T = typename Elem<DT>::type;
+    constexpr int kAhead = 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int J = P.c.J, kv = P.c.n_kv;
-    const int per_row = (2 * kv + P.n_q) * J;
-    const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-    const bool live = item < (long long)P.rows * per_row;     // idle groups still take part in the shuffles
-    const int m = threadIdx.x & 7;
-    const int row = live ? int(item / per_row) : 0, rem = live ? int(item - (long long)row * per_row) : 0;
-    int head = rem / J;
-    const int j = rem - head * J, i0 = 32 * j + 4 * m;
-    const int kind = head < kv ? 0 : head < 2 * kv ? 1 : 2;   // K, V, Q
-    head -= kind * kv;
-    const float* c = nullptr;
-    const float* s = nullptr;
-    bool bad = false;
+    const int kv = P.c.n_kv, blocks = (2 * kv + P.n_q) * J;
+    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int row = int(id / P.parts), part = int(id - (long long)row * P.parts);
+    if (row >= P.rows) return;                                    // whole warps
+    const int lane = threadIdx.x & 31, m = lane & 7;
+    const int b1 = min(blocks, (part + 1) * P.per_part);
+    const long long slot = __ldg(P.slots + row), page = slot >> P.c.page_shift;
+    const int at = int(slot & (P.c.page() - 1));
+    bool bad = slot >= 0 && page >= P.c.n_pages, lost = false;    // not to be written; queries without a position
+    const float* ct = nullptr;
+    const float* st = nullptr;
+    const int half = P.rot / 2;
     if (P.cos_t) {
         const long long p = __ldg(P.pos + row);
-        bad = p < 0 || p >= P.n_pos;
-        if (kind != 1) {
-            c = P.cos_t + (bad ? 0 : p) * (P.rot / 2);
-            s = P.sin_t + (bad ? 0 : p) * (P.rot / 2);
-        }
+        lost = p < 0 || p >= P.n_pos;
+        bad |= lost;
+        ct = P.cos_t + (lost ? 0 : p) * half;
+        st = P.sin_t + (lost ? 0 : p) * half;
     }
-    if (kind == 2) {
-        float4 x = rotated(static_cast<const T*>(P.q) + row * P.q_stride + head * P.c.dim, i0, P, c, s);
-        if (bad) x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (live) store4(static_cast<T*>(P.q_out) + ((long long)row * P.n_q + head) * P.c.dim + i0, x);
-    }
-    const T* src = kind == 1 ? static_cast<const T*>(P.v) + row * P.v_stride : static_cast<const T*>(P.k) + row * P.k_stride;
-    const bool q4 = (kind == 1 ? P.c.vb : P.c.kb) == 4;
-    __half d;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (kind != 2) x = rotated(src + head * P.c.dim, i0, P, c, s);
-    const uint4 n = quantise4(x, q4, d);
-    // K: lanes 2 t and 2 t + 1 share the 8 values of t
-    uint32_t word = q4 ? n.x | (n.y << 16) | (n.z << 4) | (n.w << 20) : n.x | (n.y << 16) | (n.z << 8) | (n.w << 24);
-    if (q4 && (m & 1)) word <<= 8;
-    const uint32_t both = word | __shfl_xor_sync(0xffffffffu, word, 1);
-    if (!live || kind == 2) {
-        if (live && bad && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
-        return;
-    }
-    const long long slot = __ldg(P.slots + row);
-    if (slot < 0) return;                                     // a padding row
-    const long long page = slot >> P.c.page_shift;
-    if (bad || page >= P.c.n_pages) {
-        if (P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
-        return;
-    }
-    const int at = int(slot & (P.c.page() - 1));
-    if (m == 0) P.c.sc[P.c.scale_row(page, head, at) + kind * J + j] = d;
-    if (kind == 0) {
-        uint8_t* dst = P.c.k + P.c.k_row(page, head, at) + ((m >> 1) * J + j) * P.c.kb;
-        if (!q4) *reinterpret_cast<uint32_t*>(dst + 4 * (m & 1)) = word;
-        else if (!(m & 1)) *reinterpret_cast<uint32_t*>(dst) = both;
-    } else {
-        uint8_t* dst = P.c.v + P.c.v_pair(page, head, at >> 1) + (m * J + j) * P.c.vb + 2 * (at & 1);
-        if (q4) {
-            *reinterpret_cast<uint16_t*>(dst) = uint16_t(n.x | (n.y << 4) | (n.z << 8) | (n.w << 12));
+    if (bad && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
+    const bool write = slot >= 0 && !bad;
+    auto angles = [&](int i0, float4& c, float4& s) {
+        if (P.paired) {
+            const float2 cc = __ldg(reinterpret_cast<const float2*>(ct + i0 / 2)), ss = __ldg(reinterpret_cast<const float2*>(st + i0 / 2));
+            c = make_float4(cc.x, cc.y, 0.f, 0.f), s = make_float4(ss.x, ss.y, 0.f, 0.f);
         } else {
-            *reinterpret_cast<uint16_t*>(dst) = uint16_t(n.x | (n.y << 8));
-            *reinterpret_cast<uint16_t*>(dst + 4) = uint16_t(n.z | (n.w << 8));
+            const int a = i0 < half ? i0 : i0 - half;
+            c = load4(ct + a), s = load4(st + a);
+        }
+    };
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f), s = c;
+    const int own = 32 * ((lane >> 3) % J) + 4 * m;               // 4 % J == 0: this lane's values of every head
+    if (4 % J == 0 && ct && own < P.rot) angles(own, c, s);
+    for (int b0 = part * P.per_part; b0 < b1; b0 += 4 * kAhead) {
+        float4 x[kAhead], o[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, i0 = 32 * (blk - h * J) + 4 * m;
+            x[q] = o[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (blk < b1) {
+                const T* src = h < kv ? static_cast<const T*>(P.k) + row * P.k_stride + h * (32 * J)
+                             : h < 2 * kv ? static_cast<const T*>(P.v) + row * P.v_stride + (h - kv) * (32 * J)
+                                          : static_cast<const T*>(P.q) + row * P.q_stride + (h - 2 * kv) * (32 * J);
+                x[q] = load4(src + i0);
+                if (ct && !P.paired && i0 < P.rot && (h < kv || h >= 2 * kv)) o[q] = load4(src + (i0 < half ? i0 + half : i0 - half));
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, j = blk - h * J, i0 = 32 * j + 4 * m;
+            if (b0 + 4 * q >= b1) break;                          // whole warps
+            const int kind = h < kv ? 0 : h < 2 * kv ? 1 : 2, head = h - kind * kv;
+            if (ct && kind != 1 && i0 < P.rot) {
+                if (4 % J != 0) angles(i0, c, s);
+                x[q] = rotated(x[q], o[q], c, s, P.paired, i0 < half);
+            }
+            const bool live = blk < b1;
+            if (kind == 2 && live)
+                store4(static_cast<T*>(P.q_out) + ((long long)row * P.n_q + head) * (32 * J) + i0, lost ? make_float4(0.f, 0.f, 0.f, 0.f) : x[q]);
+            if (!__any_sync(0xffffffffu, kind != 2 && live)) continue;
+            const bool q4 = (kind == 1 ? P.c.vb : P.c.kb) == 4;
+            __half d;
+            const uint4 n = quantise4(x[q], q4, d);
+            // K: lanes 2 t and 2 t + 1 share the 8 values of t
+            uint32_t word = q4 ? n.x | (n.y << 16) | (n.z << 4) | (n.w << 20) : n.x | (n.y << 16) | (n.z << 8) | (n.w << 24);
+            if (q4 && (m & 1)) word <<= 8;
+            const uint32_t both = word | __shfl_xor_sync(0xffffffffu, word, 1);
+            if (kind == 2 || !live || !write) continue;
+            if (m == 0) P.c.sc[P.c.scale_row(page, head, at) + kind * J + j] = d;
+            if (kind == 0) {
+                uint8_t* dst = P.c.k + P.c.k_row(page, head, at) + ((m >> 1) * J + j) * P.c.kb;
+                if (!q4) *reinterpret_cast<uint32_t*>(dst + 4 * (m & 1)) = word;
+                else if (!(m & 1)) *reinterpret_cast<uint32_t*>(dst) = both;
+            } else {
+                uint8_t* dst = P.c.v + P.c.v_pair(page, head, at >> 1) + (m * J + j) * P.c.vb + 2 * (at & 1);
+                if (q4) {
+                    *reinterpret_cast<uint16_t*>(dst) = uint16_t(n.x | (n.y << 4) | (n.z << 8) | (n.w << 12));
+                } else {
+                    *reinterpret_cast<uint16_t*>(dst) = uint16_t(n.x | (n.y << 8));
+                    *reinterpret_cast<uint16_t*>(dst + 4) = uint16_t(n.z | (n.w << 8));
+                }
+            }
         }
     }
 }
@@ -154,63 +169,88 @@ struct KvReadParams {
     const long long* slots;
     void* k;
     void* v;
-    int rows;
+    int rows, parts, per_part;
     int* status;
 };
 
-// four values of a block (the inverse of kv_write_kernel's stores): d * code, one rounded product each
-template <int DT>
+// The inverse of kv_write_kernel's stores, a warp some of one row's blocks: d * code, one rounded product each.
+template <int DT, int J>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadParams P) {
     using T = typename Elem<DT>::type;
+    constexpr int kAhead = 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int J = P.c.J, kv = P.c.n_kv, per_row = 2 * kv * J;
-    const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-    if (item >= (long long)P.rows * per_row) return;
-    const int m = threadIdx.x & 7;
-    const int row = int(item / per_row), rem = int(item - (long long)row * per_row);
-    int head = rem / J;
-    const int j = rem - head * J, kind = head < kv ? 0 : 1;
-    head -= kind * kv;
+    const int kv = P.c.n_kv, blocks = 2 * kv * J;
+    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int row = int(id / P.parts), part = int(id - (long long)row * P.parts);
+    if (row >= P.rows) return;
+    const int lane = threadIdx.x & 31, m = lane & 7, b1 = min(blocks, (part + 1) * P.per_part);
     const long long slot = __ldg(P.slots + row), page = slot >> P.c.page_shift;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (slot >= 0 && page < P.c.n_pages) {
-        const int at = int(slot & (P.c.page() - 1));
-        const float d = __half2float(P.c.sc[P.c.scale_row(page, head, at) + kind * J + j]);
-        uint32_t n[4];
-        if (kind == 0) {
-            const uint8_t* src = P.c.k + P.c.k_row(page, head, at) + ((m >> 1) * J + j) * P.c.kb;
-            if (P.c.kb == 4) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(src) >> (8 * (m & 1));
-                n[0] = w & 15u, n[1] = (w >> 16) & 15u, n[2] = (w >> 4) & 15u, n[3] = (w >> 20) & 15u;
+    const int at = int(slot & (P.c.page() - 1));
+    const bool there = slot >= 0 && page < P.c.n_pages;
+    if (slot >= 0 && !there && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
+    for (int b0 = part * P.per_part; b0 < b1; b0 += 4 * kAhead) {
+        uint32_t w[kAhead], u[kAhead];
+        float d[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, j = blk - h * J, kind = h < kv ? 0 : 1, head = h - kind * kv;
+            w[q] = u[q] = 0u, d[q] = 0.f;
+            if (!there || blk >= b1) continue;
+            d[q] = __half2float(P.c.sc[P.c.scale_row(page, head, at) + kind * J + j]);
+            if (kind == 0) {
+                const uint8_t* src = P.c.k + P.c.k_row(page, head, at) + ((m >> 1) * J + j) * P.c.kb;
+                w[q] = P.c.kb == 4 ? *reinterpret_cast<const uint32_t*>(src) >> (8 * (m & 1)) : *reinterpret_cast<const uint32_t*>(src + 4 * (m & 1));
             } else {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(src + 4 * (m & 1));
-                n[0] = w & 255u, n[1] = (w >> 16) & 255u, n[2] = (w >> 8) & 255u, n[3] = w >> 24;
-            }
-        } else {
-            const uint8_t* src = P.c.v + P.c.v_pair(page, head, at >> 1) + (m * J + j) * P.c.vb + 2 * (at & 1);
-            const uint32_t w = *reinterpret_cast<const uint16_t*>(src);
-            if (P.c.vb == 4) {
-                n[0] = w & 15u, n[1] = (w >> 4) & 15u, n[2] = (w >> 8) & 15u, n[3] = w >> 12;
-            } else {
-                const uint32_t u = *reinterpret_cast<const uint16_t*>(src + 4);
-                n[0] = w & 255u, n[1] = w >> 8, n[2] = u & 255u, n[3] = u >> 8;
+                const uint8_t* src = P.c.v + P.c.v_pair(page, head, at >> 1) + (m * J + j) * P.c.vb + 2 * (at & 1);
+                w[q] = *reinterpret_cast<const uint16_t*>(src);
+                if (P.c.vb == 8) u[q] = *reinterpret_cast<const uint16_t*>(src + 4);
             }
         }
-        const int off = (kind == 0 ? P.c.kb : P.c.vb) == 4 ? 8 : 128;
-        o = make_float4(__fmul_rn(d, float(int(n[0]) - off)), __fmul_rn(d, float(int(n[1]) - off)),
-                        __fmul_rn(d, float(int(n[2]) - off)), __fmul_rn(d, float(int(n[3]) - off)));
-    } else if (slot >= 0 && P.status) {
-        atomicOr(P.status, DEV_BAD_ADDRESS);
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, j = blk - h * J, kind = h < kv ? 0 : 1, head = h - kind * kv;
+            if (blk >= b1) continue;
+            uint32_t n[4];
+            const bool q4 = (kind == 0 ? P.c.kb : P.c.vb) == 4;
+            if (kind == 0) {
+                const int a = q4 ? 4 : 8, mask = q4 ? 15 : 255;
+                n[0] = w[q] & mask, n[1] = (w[q] >> 16) & mask, n[2] = (w[q] >> a) & mask, n[3] = (w[q] >> (16 + a)) & mask;
+            } else if (q4) {
+                n[0] = w[q] & 15u, n[1] = (w[q] >> 4) & 15u, n[2] = (w[q] >> 8) & 15u, n[3] = w[q] >> 12;
+            } else {
+                n[0] = w[q] & 255u, n[1] = w[q] >> 8, n[2] = u[q] & 255u, n[3] = u[q] >> 8;
+            }
+            const int off = q4 ? 8 : 128;
+            const float4 y = !there ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                    : make_float4(__fmul_rn(d[q], float(int(n[0]) - off)), __fmul_rn(d[q], float(int(n[1]) - off)),
+                                                  __fmul_rn(d[q], float(int(n[2]) - off)), __fmul_rn(d[q], float(int(n[3]) - off)));
+            store4(static_cast<T*>(kind == 0 ? P.k : P.v) + ((long long)row * kv + head) * (32 * J) + 32 * j + 4 * m, y);
+        }
     }
-    T* out = static_cast<T*>(kind == 0 ? P.k : P.v) + ((long long)row * kv + head) * P.c.dim + 32 * j + 4 * m;
-    store4(out, o);
 }
 
-// blocks of 256 threads for rows x per_row groups of eight lanes; 0 if that passes a launch's grid
-unsigned blocks_of(long long rows, long long per_row) {
-    const long long b = (rows * per_row + 31) / 32;
-    return b <= 0x7FFFFFFFLL ? unsigned(b) : 0u;
+// Warps a row and blocks a warp: rows on their own where they fill the GPU (16 warps an SM), else cut so that there are as
+// many, at least one pass of 4 blocks each; the launch's CTAs, 0 if they pass a grid.
+unsigned cut_rows(long long rows, int blocks, int& parts, int& per_part) {
+    const long long want = 16LL * sm_count();
+    const int passes = (blocks + 3) / 4;
+    parts = int(std::min<long long>(passes, std::max<long long>(1, want / rows)));
+    per_part = 4 * ((passes + parts - 1) / parts);
+    parts = (blocks + per_part - 1) / per_part;
+    const long long ctas = (rows * parts + 7) / 8;
+    return ctas <= 0x7FFFFFFFLL ? unsigned(ctas) : 0u;
+}
+// f(std::integral_constant<int, dim / 32>)
+template <class Fn>
+int by_blocks(int J, Fn&& f) {
+    switch (J) {
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    }
+    return ST_BAD_SHAPE;
 }
 
 }  // namespace
@@ -242,10 +282,12 @@ int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dt
     P.rot = rot_dim, P.paired = paired, P.n_q = q ? n_q : 0;
     P.rows = int(rows);
     P.status = device_status_ptr();
-    const unsigned blocks = blocks_of(rows, (long long)(2 * P.c.n_kv + P.n_q) * P.c.J);
-    if (!blocks) return ST_BAD_TOKENS;
+    const unsigned ctas = cut_rows(rows, (2 * P.c.n_kv + P.n_q) * P.c.J, P.parts, P.per_part);
+    if (!ctas) return ST_BAD_TOKENS;
     return by_elem(dtype, [&](auto c) {
-        return launch_pdl(kv_write_kernel<decltype(c)::value>, dim3(blocks), dim3(256), static_cast<cudaStream_t>(stream), P);
+        return by_blocks(P.c.J, [&](auto j) {
+            return launch_pdl(kv_write_kernel<decltype(c)::value, decltype(j)::value>, dim3(ctas), dim3(256), static_cast<cudaStream_t>(stream), P);
+        });
     });
 }
 
@@ -262,10 +304,12 @@ int qmv_kv_read(const qmv_kv_cache* cache, const long long* slots, long long row
     P.slots = slots, P.k = k, P.v = v;
     P.rows = int(rows);
     P.status = device_status_ptr();
-    const unsigned blocks = blocks_of(rows, 2LL * P.c.n_kv * P.c.J);
-    if (!blocks) return ST_BAD_TOKENS;
+    const unsigned ctas = cut_rows(rows, 2 * P.c.n_kv * P.c.J, P.parts, P.per_part);
+    if (!ctas) return ST_BAD_TOKENS;
     return by_elem(dtype, [&](auto c) {
-        return launch_pdl(kv_read_kernel<decltype(c)::value>, dim3(blocks), dim3(256), static_cast<cudaStream_t>(stream), P);
+        return by_blocks(P.c.J, [&](auto j) {
+            return launch_pdl(kv_read_kernel<decltype(c)::value, decltype(j)::value>, dim3(ctas), dim3(256), static_cast<cudaStream_t>(stream), P);
+        });
     });
 }
 

@@ -41,12 +41,14 @@ def _rows(t: torch.Tensor, heads: int, dim: int):
     """t (rows, heads, dim) as the kernels read it (the values of a row side by side, rows any multiple of 4
     values apart, a start on four values) and the values between rows."""
     row = heads * dim
-    if t.stride(2) != 1 or t.stride(1) != dim and heads > 1 or t.shape[0] > 1 and (t.stride(0) < row or t.stride(0) % 4) \
+    rows_apart, heads_apart, apart = t.stride()
+    if apart != 1 or heads_apart != dim and heads > 1 or t.shape[0] > 1 and (rows_apart < row or rows_apart % 4) \
             or t.data_ptr() % (4 * t.element_size()):
         t = t.contiguous()
         if t.data_ptr() % (4 * t.element_size()):
             t = t.clone()
-    return t, (t.stride(0) if t.shape[0] > 1 else row)
+        rows_apart = row
+    return t, (rows_apart if t.shape[0] > 1 else row)
 
 
 class KVCache:
@@ -83,21 +85,25 @@ class KVCache:
         self._c = _Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.scales.data_ptr(), n_pages, n_kv, dim, page,
                          TYPE_ID[k_fmt], TYPE_ID[v_fmt])
         self._ref = ctypes.byref(self._c)
+        self._need = {}                     # workspace bytes of the calls so far, by their sizes
+        self._none = None                   # stands for the workspace of calls that use none
 
     def _tokens(self, t: torch.Tensor, what: str, heads: Optional[int] = None, like: Optional[torch.Tensor] = None):
+        shape = t.shape
         if t.device != self.device:
             raise RuntimeError(f"{what}: tensor on {t.device}, the cache on {self.device}")
-        if t.dim() != 3 or t.shape[2] != self.dim or t.dtype not in _DTYPES or heads is not None and t.shape[1] != heads \
-                or t.shape[1] == 0:
+        if len(shape) != 3 or shape[2] != self.dim or t.dtype not in _DTYPES or heads is not None and shape[1] != heads \
+                or shape[1] == 0:
             raise RuntimeError(f"{what}: (rows, {heads or 'heads'}, {self.dim}) of float32, bfloat16 or float16 expected, "
-                               f"got {tuple(t.shape)} {t.dtype}")
-        if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
+                               f"got {tuple(shape)} {t.dtype}")
+        if like is not None and (t.dtype != like.dtype or shape[0] != like.shape[0]):
             raise RuntimeError(f"{what}: {like.shape[0]} rows of {like.dtype} expected")
 
     def _index(self, t: torch.Tensor, what: str, dtype, *shape):
-        if t.device != self.device or t.dtype != dtype or t.dim() != len(shape) or not t.is_contiguous() \
-                or any(s is not None and a != s for a, s in zip(t.shape, shape)):
-            raise RuntimeError(f"{what}: contiguous {dtype} {shape} on {self.device} expected, got {t.dtype} {tuple(t.shape)}")
+        got = t.shape
+        if t.device != self.device or t.dtype != dtype or len(got) != len(shape) or not t.is_contiguous() \
+                or any(want is not None and n != want for n, want in zip(got, shape)):
+            raise RuntimeError(f"{what}: contiguous {dtype} {shape} on {self.device} expected, got {t.dtype} {tuple(got)}")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, q: Optional[torch.Tensor] = None, rope=None,
               paired: bool = False) -> Optional[torch.Tensor]:
@@ -125,16 +131,17 @@ class KVCache:
         if q is not None:
             self._tokens(q, "KVCache.write q", None, k)
             n_q = q.shape[1]
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
             q, qs = _rows(q, n_q, self.dim)
         k, ks = _rows(k, self.n_kv, self.dim)
         v, vs = _rows(v, self.n_kv, self.dim)
         if rows:
             with _lib.on_device(self.device):
-                _lib.check(_lib.load().qmv_kv_write(self._ref, _lib.ptr(k), _lib.ptr(v), _DTYPES[k.dtype], ks, vs,
-                                                    _lib.ptr(slots), rows, _lib.ptr(cos), _lib.ptr(sin), _lib.ptr(pos),
-                                                    n_pos, rot, int(bool(paired)), _lib.ptr(q), qs, n_q, _lib.ptr(out),
-                                                    _lib.stream_ptr(self.device)), "qmv_kv_write")
+                st = _lib.load().qmv_kv_write(self._ref, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], ks, vs, slots.data_ptr(), rows,
+                                              _lib.addr(cos), _lib.addr(sin), _lib.addr(pos), n_pos, rot, int(bool(paired)),
+                                              _lib.addr(q), qs, n_q, _lib.addr(out), _lib.stream_of(self.device))
+            if st:
+                _lib.check(st, "qmv_kv_write")
         return out
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
@@ -142,11 +149,14 @@ class KVCache:
         self._index(slots, "KVCache.read slots", torch.int64, None)
         if dtype not in _DTYPES:
             raise RuntimeError(f"KVCache.read: dtype {dtype} (float32, bfloat16 or float16)")
-        k, v = (torch.empty(slots.shape[0], self.n_kv, self.dim, dtype=dtype, device=self.device) for _ in range(2))
-        if slots.shape[0]:
+        rows = slots.shape[0]
+        k, v = torch.empty((2, rows, self.n_kv, self.dim), dtype=dtype, device=self.device).unbind(0)
+        if rows:
             with _lib.on_device(self.device):
-                _lib.check(_lib.load().qmv_kv_read(self._ref, _lib.ptr(slots), slots.shape[0], _lib.ptr(k), _lib.ptr(v),
-                                                   _DTYPES[dtype], _lib.stream_ptr(self.device)), "qmv_kv_read")
+                st = _lib.load().qmv_kv_read(self._ref, slots.data_ptr(), rows, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
+                                             _lib.stream_of(self.device))
+            if st:
+                _lib.check(st, "qmv_kv_read")
         return k, v
 
     def attend(self, q: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None,
@@ -175,7 +185,7 @@ class KVCache:
         if window < 0 or most < 0:
             raise RuntimeError("KVCache.attend: window and max_new must not be negative")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() \
                 or out.data_ptr() % 16:
             raise RuntimeError(f"KVCache.attend: out must be a contiguous, 16-byte aligned {tuple(q.shape)} tensor of {q.dtype}")
@@ -185,15 +195,26 @@ class KVCache:
             raise RuntimeError("KVCache.attend: tables without a page")
         q, qs = _rows(q, heads, self.dim)
         lib = _lib.load()
-        most = min(most, rows)
+        most, window, dtype = min(most, rows), min(int(window), 2 ** 31 - 1), _DTYPES[q.dtype]
         with _lib.on_device(self.device):
-            window = min(int(window), 2 ** 31 - 1)
-            nbytes = lib.qmv_kv_attend_workspace_bytes(self._ref, heads, n_seq, most, _DTYPES[q.dtype], width, window)
-            if nbytes <= 0:
-                raise RuntimeError(f"KVCache.attend: {heads} heads, {n_seq} sequences of {most} new tokens not supported")
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            _lib.check(lib.qmv_kv_attend(self._ref, _lib.ptr(q), _DTYPES[q.dtype], qs, heads, _lib.ptr(tables), width,
-                                         _lib.ptr(lens), _lib.ptr(starts), n_seq, rows, most,
-                                         self.dim ** -0.5 if scale is None else float(scale), window,
-                                         _lib.ptr(out), _lib.ptr(ws), nbytes, _lib.stream_ptr(self.device)), "qmv_kv_attend")
+            sizes = (heads, n_seq, most, dtype, width, window)
+            nbytes = self._need.get(sizes)
+            if nbytes is None:
+                nbytes = lib.qmv_kv_attend_workspace_bytes(self._ref, *sizes)
+                if nbytes <= 0:
+                    raise RuntimeError(f"KVCache.attend: {heads} heads, {n_seq} sequences of {most} new tokens not supported")
+                if len(self._need) >= 4096:           # sizes that never come back
+                    self._need.clear()
+                self._need[sizes] = nbytes
+            if nbytes > 256:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            else:                                     # used by nothing
+                if self._none is None:
+                    self._none = torch.empty(256, dtype=torch.uint8, device=self.device)
+                ws = self._none
+            st = lib.qmv_kv_attend(self._ref, q.data_ptr(), dtype, qs, heads, tables.data_ptr(), width, lens.data_ptr(),
+                                   _lib.addr(starts), n_seq, rows, most, self.dim ** -0.5 if scale is None else float(scale), window,
+                                   out.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_of(self.device))
+        if st:
+            _lib.check(st, "qmv_kv_attend")
         return out

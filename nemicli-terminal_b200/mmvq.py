@@ -464,28 +464,30 @@ def norm_block(y: torch.Tensor, h: torch.Tensor, w_pre: Optional[torch.Tensor], 
     if n > NORM_BLOCK_MAX:
         raise RuntimeError(f"norm_block: rows of at most {NORM_BLOCK_MAX} values (got {n})")
 
-    def rows(t):                          # the values of a row side by side, and the values between rows
-        t = t.reshape(1, n) if t.dim() == 1 else t
-        if t.stride(1) != 1 and n > 1 or t.shape[0] > 1 and t.stride(0) < n:
-            t = t.contiguous()
-        return t, (t.stride(0) if t.shape[0] > 1 else n)
-
     M = 1 if y.dim() == 1 else y.shape[0]
+
+    def rows(t):                          # the values of a row side by side, and the values between rows
+        if t.is_contiguous():
+            return t, n
+        if t.stride(-1) != 1 and n > 1 or t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < n:
+            return t.contiguous(), n
+        return t, (t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else n)
+
     y2, ys = rows(y)
     h2, hs = rows(h)
     g2, gs = (None, 0) if gate is None else rows(gate)
     if gate is not None and gate.dim() < y.dim():
         gs = 0
-    x = None if w_pre is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    new = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    x = None if w_pre is None else torch.empty_like(y, memory_format=torch.contiguous_format)
+    new = torch.empty_like(y, memory_format=torch.contiguous_format)
     e = Eingang(n=M * n, device=y.device) if eingang else None
     if M:
         with _lib.on_device(y.device):
-            _lib.check(_lib.load().qmv_norm_block(_lib.ptr(y2), ys, _lib.ptr(h2), hs, _lib.ptr(g2), gs, _lib.ptr(w_post),
-                                                  _lib.ptr(w_pre), _OUT[y.dtype], float(eps), float(rs), M, n,
-                                                  _lib.ptr(new), _lib.ptr(x),
-                                                  *(e.zeiger() if e else [_lib.ptr(None)] * 4),
-                                                  _lib.stream_ptr(y.device)), "qmv_norm_block")
+            st = _lib.load().qmv_norm_block(y2.data_ptr(), ys, h2.data_ptr(), hs, _lib.addr(g2), gs, _lib.addr(w_post),
+                                            _lib.addr(w_pre), _OUT[y.dtype], eps, rs, M, n, new.data_ptr(), _lib.addr(x),
+                                            *(e.zeiger() if e else (0, 0, 0, 0)), _lib.stream_of(y.device))
+        if st:
+            _lib.check(st, "qmv_norm_block")
     return x, e, new
 
 
