@@ -22,7 +22,7 @@ struct KvWriteParams {
     const long long* pos;
     long long n_pos;
     int rot, paired, n_q;
-    int rows, parts, per_part;            // warps a row, blocks a warp (a multiple of 4)
+    int rows, parts, per_part;            // warps a row, passes a warp
     int* status;
 };
 
@@ -38,52 +38,83 @@ __device__ __forceinline__ float4 rotated(float4 x, float4 o, float4 c, float4 s
                        __fadd_rn(__fmul_rn(x.z, c.z), __fmul_rn(o.z, s.z)), __fadd_rn(__fmul_rn(x.w, c.w), __fmul_rn(o.w, s.w)));
 }
 
-__device__ __forceinline__ float cleaned(float x) {          // NaN counts as 0, the rest is clamped to +-65504
-    return x != x ? 0.f : fminf(fmaxf(x, -kKvMax), kKvMax);
-}
-
-// Eight lanes (m = 0..7) hold four values each of one 32-value block; the block's scale, and each lane's codes with their
-// offset.  Q4_0: d = fp16(x / -8) of the value of largest magnitude (the first of equal ones), codes
-// clamp(rint(x / d), -8, 7); Q8_0: d = fp16(max |x| / 127), codes clamp(rint(x / d), -127, 127).  Divisions are
-// IEEE, by the rounded d, the one the reader multiplies with.
-__device__ __forceinline__ uint4 quantise4(float4 x, bool q4, __half& d) {
-    x = make_float4(cleaned(x.x), cleaned(x.y), cleaned(x.z), cleaned(x.w));
-    float m = x.x;
-    if (fabsf(x.y) > fabsf(m)) m = x.y;
-    if (fabsf(x.z) > fabsf(m)) m = x.z;
-    if (fabsf(x.w) > fabsf(m)) m = x.w;
-    const int lane = threadIdx.x & 7;
+// Eight lanes (m = 0..7) hold four values each of one 32-value block; the block's scale, and each lane's codes without
+// offset, a byte each.  Q4_0: d = fp16(x / -8) of the value of largest magnitude (the first of equal ones), codes
+// clamp(rint(x / d), -8, 7); Q8_0: d = fp16(max |x| / 127), codes clamp(rint(x / d), -127, 127).  The quotient is the IEEE one by
+// the rounded d, the one the reader multiplies with.  It is formed as x (1 / d) first: that is within 2^-15 of it
+// (|x / d| <= 128, the reciprocal's error and a rounding), so only where that lies within 2^-11 of a border between codes is the division made.
+__device__ __forceinline__ uint32_t quantise4(float4 x, bool q4, __half& d) {
+    float v[4] = {x.x, x.y, x.z, x.w};
+    const bool odd = v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3];
+    if (__any_sync(0xffffffffu, odd)) {                           // NaN counts as 0
 #pragma unroll
-    for (int o = 1; o < 8; o *= 2) {
-        const float other = __shfl_xor_sync(0xffffffffu, m, o);
-        const bool lower = (lane & o) != 0;                   // the other lane's values come first
-        if (fabsf(other) > fabsf(m) || (lower && fabsf(other) == fabsf(m))) m = other;
+        for (int i = 0; i < 4; ++i) v[i] = v[i] != v[i] ? 0.f : v[i];
     }
-    d = __float2half_rn(q4 ? __fmul_rn(m, -0.125f) : __fdiv_rn(fabsf(m), 127.0f));
-    const float df = __half2float(d);
-    const float lo = q4 ? -8.f : -127.f, hi = q4 ? 7.f : 127.f, off = q4 ? 8.f : 128.f;
-    float c[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = (df == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(c[i], df)), lo), hi)) + off;
-    return make_uint4(uint32_t(c[0]), uint32_t(c[1]), uint32_t(c[2]), uint32_t(c[3]));
+    for (int i = 0; i < 4; ++i) v[i] = fminf(fmaxf(v[i], -kKvMax), kKvMax);
+    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+    for (int o = 1; o < 8; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // the sign of the first value of that magnitude, from the first lane of the eight that has one
+    const float first = fabsf(v[0]) == top ? v[0] : fabsf(v[1]) == top ? v[1] : fabsf(v[2]) == top ? v[2] : v[3];
+    const int group = threadIdx.x & 24;
+    const uint32_t has = __ballot_sync(0xffffffffu, fabsf(first) == top) >> group & 255u;
+    const uint32_t minus = __ballot_sync(0xffffffffu, first < 0.f) >> group;
+    const float m = minus >> (__ffs(has) - 1) & 1u ? -top : top;
+    d = __float2half_rn(q4 ? __fmul_rn(m, -0.125f) : __fdiv_rn(top, 127.0f));
+    const float df = __half2float(d);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(df));
+    if (df == 0.f) r = 0.f;
+    constexpr float kRound = 12582912.f;                          // 1.5 2^23: added, the sum's low bits are rint(t)
+    float t[4];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float p = v[i] * r;
+        t[i] = __fadd_rn(p, kRound);
+        near |= fabsf(__fsub_rn(p, __fsub_rn(t[i], kRound))) > 0.5f - 0.00048828125f;
+    }
+    if (__any_sync(0xffffffffu, near)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = __fadd_rn(df == 0.f ? 0.f : __fdiv_rn(v[i], df), kRound);
+    }
+    const float lo = kRound - (q4 ? 8.f : 127.f), hi = kRound + (q4 ? 7.f : 127.f);
+    uint32_t n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = __float_as_uint(fminf(fmaxf(t[i], lo), hi));
+    return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
 }
 
-// A warp takes some of one row's 32-value blocks (K heads, then V heads, then the queries to rotate), four at a time on eight
-// lanes each, and kAhead such passes' loads go out together.  Rows' angles are the same for all of a lane's passes where
-// a head has 2 or 4 blocks.  Bound by memory for long prompts (divisions and reductions are about as many clocks), by its
-// launch for a decode step.
+// four values of a row as they lie in memory
+template <int DT> struct Raw4 { using type = uint2; };
+template <> struct Raw4<QMV_OUT_F32> { using type = uint4; };
+__device__ __forceinline__ float4 raw4(uint4 w, float) { return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)); }
+__device__ __forceinline__ float4 raw4(uint2 w, __nv_bfloat16) {
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ float4 raw4(uint2 w, __half) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// A warp takes some of one row's passes of 128 consecutive values (four blocks, eight lanes each): K's, V's, then those of the
+// queries to rotate; kAhead passes' loads go out together.  Angles are the same for all of a lane's passes where a head
+// has 2 or 4 blocks.  Bound by memory for long prompts, by its launch for a decode step.
 template <int DT, int J>
 __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvWriteParams P) {
     using T = typename Elem<DT>::type;
-    constexpr int kAhead = 4;
+    using W = typename Raw4<DT>::type;
+    constexpr int D = 32 * J, kAhead = 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int kv = P.c.n_kv, blocks = (2 * kv + P.n_q) * J;
+    const int lane = threadIdx.x & 31, m = lane & 7;
     const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int row = int(id / P.parts), part = int(id - (long long)row * P.parts);
     if (row >= P.rows) return;                                    // whole warps
-    const int lane = threadIdx.x & 31, m = lane & 7;
-    const int b1 = min(blocks, (part + 1) * P.per_part);
+    const int kv = P.c.n_kv, n_kv = kv * D, n_q = P.n_q * D;      // values of a section
+    const int pk = (n_kv + 127) / 128, pq = (n_q + 127) / 128;
+    const int p1 = min(2 * pk + pq, (part + 1) * P.per_part);
     const long long slot = __ldg(P.slots + row), page = slot >> P.c.page_shift;
     const int at = int(slot & (P.c.page() - 1));
     bool bad = slot >= 0 && page >= P.c.n_pages, lost = false;    // not to be written; queries without a position
@@ -109,59 +140,84 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
         }
     };
     float4 c = make_float4(0.f, 0.f, 0.f, 0.f), s = c;
-    const int own = 32 * ((lane >> 3) % J) + 4 * m;               // 4 % J == 0: this lane's values of every head
-    if (4 % J == 0 && ct && own < P.rot) angles(own, c, s);
-    for (int b0 = part * P.per_part; b0 < b1; b0 += 4 * kAhead) {
-        float4 x[kAhead], o[kAhead];
+    constexpr bool kSame = 4 % J == 0;                            // this lane's place in every head
+    const int own = (4 * lane) % D;
+    if (kSame && ct && own < P.rot) angles(own, c, s);
+    // bytes between heads of a page (a page's bytes fit 31 bits), and this row's places in head 0
+    const uint32_t head_k = uint32_t(4 * J * P.c.kb) << P.c.page_shift, head_v = uint32_t(8 * J * P.c.vb) << (P.c.page_shift - 1),
+                   head_s = uint32_t(2 * J) << P.c.page_shift;
+    uint8_t* k_to = P.c.k + P.c.k_row(page, 0, at) + (m >> 1) * J * P.c.kb;
+    uint8_t* v_to = P.c.v + P.c.v_pair(page, 0, at >> 1) + 2 * (at & 1) + m * J * P.c.vb;
+    __half* s_to = P.c.sc + P.c.scale_row(page, 0, at);
+
+    // passes first .. last of a section of n values at src; KIND 0: K, 1: V, 2: queries
+    auto section = [&](auto kind_c, const T* src, int n, int first, int last) {
+        constexpr int KIND = decltype(kind_c)::value;
+        const bool q4 = (KIND == 1 ? P.c.vb : P.c.kb) == 4, turn = KIND != 1 && ct != nullptr;
+        auto batch = [&](int p0, auto count, bool check) {
+            constexpr int A = decltype(count)::value;
+            const T* at0 = src + 128 * p0 + 4 * lane;
+            W w[A], o[A];
 #pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, i0 = 32 * (blk - h * J) + 4 * m;
-            x[q] = o[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (blk < b1) {
-                const T* src = h < kv ? static_cast<const T*>(P.k) + row * P.k_stride + h * (32 * J)
-                             : h < 2 * kv ? static_cast<const T*>(P.v) + row * P.v_stride + (h - kv) * (32 * J)
-                                          : static_cast<const T*>(P.q) + row * P.q_stride + (h - 2 * kv) * (32 * J);
-                x[q] = load4(src + i0);
-                if (ct && !P.paired && i0 < P.rot && (h < kv || h >= 2 * kv)) o[q] = load4(src + (i0 < half ? i0 + half : i0 - half));
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, j = blk - h * J, i0 = 32 * j + 4 * m;
-            if (b0 + 4 * q >= b1) break;                          // whole warps
-            const int kind = h < kv ? 0 : h < 2 * kv ? 1 : 2, head = h - kind * kv;
-            if (ct && kind != 1 && i0 < P.rot) {
-                if (4 % J != 0) angles(i0, c, s);
-                x[q] = rotated(x[q], o[q], c, s, P.paired, i0 < half);
-            }
-            const bool live = blk < b1;
-            if (kind == 2 && live)
-                store4(static_cast<T*>(P.q_out) + ((long long)row * P.n_q + head) * (32 * J) + i0, lost ? make_float4(0.f, 0.f, 0.f, 0.f) : x[q]);
-            if (!__any_sync(0xffffffffu, kind != 2 && live)) continue;
-            const bool q4 = (kind == 1 ? P.c.vb : P.c.kb) == 4;
-            __half d;
-            const uint4 n = quantise4(x[q], q4, d);
-            // K: lanes 2 t and 2 t + 1 share the 8 values of t
-            uint32_t word = q4 ? n.x | (n.y << 16) | (n.z << 4) | (n.w << 20) : n.x | (n.y << 16) | (n.z << 8) | (n.w << 24);
-            if (q4 && (m & 1)) word <<= 8;
-            const uint32_t both = word | __shfl_xor_sync(0xffffffffu, word, 1);
-            if (kind == 2 || !live || !write) continue;
-            if (m == 0) P.c.sc[P.c.scale_row(page, head, at) + kind * J + j] = d;
-            if (kind == 0) {
-                uint8_t* dst = P.c.k + P.c.k_row(page, head, at) + ((m >> 1) * J + j) * P.c.kb;
-                if (!q4) *reinterpret_cast<uint32_t*>(dst + 4 * (m & 1)) = word;
-                else if (!(m & 1)) *reinterpret_cast<uint32_t*>(dst) = both;
-            } else {
-                uint8_t* dst = P.c.v + P.c.v_pair(page, head, at >> 1) + (m * J + j) * P.c.vb + 2 * (at & 1);
-                if (q4) {
-                    *reinterpret_cast<uint16_t*>(dst) = uint16_t(n.x | (n.y << 4) | (n.z << 8) | (n.w << 12));
-                } else {
-                    *reinterpret_cast<uint16_t*>(dst) = uint16_t(n.x | (n.y << 8));
-                    *reinterpret_cast<uint16_t*>(dst + 4) = uint16_t(n.z | (n.w << 8));
+            for (int a = 0; a < A; ++a) {
+                const int off = 128 * (p0 + a) + 4 * lane;
+                w[a] = o[a] = W{};
+                if (check && off >= n) continue;
+                w[a] = __ldg(reinterpret_cast<const W*>(at0 + 128 * a));
+                if (turn && !P.paired) {
+                    const int i0 = kSame ? own : off % D;
+                    if (i0 < P.rot) o[a] = __ldg(reinterpret_cast<const W*>(at0 + 128 * a + (i0 < half ? half : -half)));
                 }
             }
-        }
-    }
+#pragma unroll
+            for (int a = 0; a < A; ++a) {
+                const int off = 128 * (p0 + a) + 4 * lane, i0 = kSame ? own : off % D;
+                const bool live = !check || off < n;
+                float4 x = raw4(w[a], T{});
+                if (turn && i0 < P.rot) {
+                    if (!kSame) angles(i0, c, s);
+                    x = rotated(x, raw4(o[a], T{}), c, s, P.paired, i0 < half);
+                }
+                if constexpr (KIND == 2) {
+                    if (live) store4(static_cast<T*>(P.q_out) + (long long)row * n + off, lost ? make_float4(0.f, 0.f, 0.f, 0.f) : x);
+                } else {
+                    __half d;
+                    uint32_t b = quantise4(x, q4, d);
+                    b = q4 ? (b & 0x0F0F0F0Fu) ^ 0x08080808u : b ^ 0x80808080u;
+                    const uint32_t head = uint32_t(off) / D, j = (uint32_t(off) - head * D) / 32;
+                    if constexpr (KIND == 0) {
+                        // lanes 2 t and 2 t + 1 share the 8 values of t
+                        uint32_t word = q4 ? __byte_perm(b, 0u, 0x4140) | __byte_perm(b, 0u, 0x4342) << 4 : __byte_perm(b, 0u, 0x3120);
+                        if (q4 && (m & 1)) word <<= 8;
+                        const uint32_t both = word | __shfl_xor_sync(0xffffffffu, word, 1);
+                        if (!live || !write) continue;
+                        uint8_t* dst = k_to + (head * head_k + j * P.c.kb);
+                        if (!q4) *reinterpret_cast<uint32_t*>(dst + 4 * (m & 1)) = word;
+                        else if (!(m & 1)) *reinterpret_cast<uint32_t*>(dst) = both;
+                    } else {
+                        if (!live || !write) continue;
+                        uint8_t* dst = v_to + (head * head_v + j * P.c.vb);
+                        if (q4) {
+                            *reinterpret_cast<uint16_t*>(dst) = uint16_t(__byte_perm(b | b >> 4, 0u, 0x4420));
+                        } else {
+                            *reinterpret_cast<uint16_t*>(dst) = uint16_t(b);
+                            *reinterpret_cast<uint16_t*>(dst + 4) = uint16_t(b >> 16);
+                        }
+                    }
+                    if (m == 0) s_to[head * head_s + KIND * J + j] = d;
+                }
+            }
+        };
+        int p = first;
+        for (; p + kAhead <= last && 128 * (p + kAhead) <= n; p += kAhead) batch(p, std::integral_constant<int, kAhead>{}, false);
+        for (; p < last; ++p) batch(p, std::integral_constant<int, 1>{}, true);
+    };
+    const int q0 = part * P.per_part;
+    if (q0 < pk) section(std::integral_constant<int, 0>{}, static_cast<const T*>(P.k) + row * P.k_stride, n_kv, q0, min(p1, pk));
+    if (q0 < 2 * pk && p1 > pk)
+        section(std::integral_constant<int, 1>{}, static_cast<const T*>(P.v) + row * P.v_stride, n_kv, max(q0 - pk, 0), min(p1 - pk, pk));
+    if (p1 > 2 * pk)
+        section(std::integral_constant<int, 2>{}, static_cast<const T*>(P.q) + row * P.q_stride, n_q, max(q0 - 2 * pk, 0), p1 - 2 * pk);
 }
 
 struct KvReadParams {
@@ -173,74 +229,85 @@ struct KvReadParams {
     int* status;
 };
 
-// The inverse of kv_write_kernel's stores, a warp some of one row's blocks: d * code, one rounded product each.
+// The inverse of kv_write_kernel's stores, a warp some of one row's passes: d * code, one rounded product each.
 template <int DT, int J>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadParams P) {
     using T = typename Elem<DT>::type;
-    constexpr int kAhead = 4;
+    constexpr int D = 32 * J, kAhead = 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int kv = P.c.n_kv, blocks = 2 * kv * J;
+    const int lane = threadIdx.x & 31, m = lane & 7;
     const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int row = int(id / P.parts), part = int(id - (long long)row * P.parts);
     if (row >= P.rows) return;
-    const int lane = threadIdx.x & 31, m = lane & 7, b1 = min(blocks, (part + 1) * P.per_part);
+    const int n_kv = P.c.n_kv * D, pk = (n_kv + 127) / 128, p1 = min(2 * pk, (part + 1) * P.per_part);
     const long long slot = __ldg(P.slots + row), page = slot >> P.c.page_shift;
     const int at = int(slot & (P.c.page() - 1));
     const bool there = slot >= 0 && page < P.c.n_pages;
     if (slot >= 0 && !there && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
-    for (int b0 = part * P.per_part; b0 < b1; b0 += 4 * kAhead) {
-        uint32_t w[kAhead], u[kAhead];
-        float d[kAhead];
+    const uint32_t head_k = uint32_t(4 * J * P.c.kb) << P.c.page_shift, head_v = uint32_t(8 * J * P.c.vb) << (P.c.page_shift - 1),
+                   head_s = uint32_t(2 * J) << P.c.page_shift;
+    const uint8_t* k = P.c.k + P.c.k_row(page, 0, at) + (m >> 1) * J * P.c.kb;
+    const uint8_t* v = P.c.v + P.c.v_pair(page, 0, at >> 1) + 2 * (at & 1) + m * J * P.c.vb;
+    const __half* sc = P.c.sc + P.c.scale_row(page, 0, at);
+    auto section = [&](auto kind_c, int first, int last) {
+        constexpr int KIND = decltype(kind_c)::value;
+        const bool q4 = (KIND == 0 ? P.c.kb : P.c.vb) == 4;
+        T* out = static_cast<T*>(KIND == 0 ? P.k : P.v) + (long long)row * n_kv;
+        auto batch = [&](int p0, auto count, bool check) {
+            constexpr int A = decltype(count)::value;
+            uint32_t w[A];
+            __half d[A];
 #pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, j = blk - h * J, kind = h < kv ? 0 : 1, head = h - kind * kv;
-            w[q] = u[q] = 0u, d[q] = 0.f;
-            if (!there || blk >= b1) continue;
-            d[q] = __half2float(P.c.sc[P.c.scale_row(page, head, at) + kind * J + j]);
-            if (kind == 0) {
-                const uint8_t* src = P.c.k + P.c.k_row(page, head, at) + ((m >> 1) * J + j) * P.c.kb;
-                w[q] = P.c.kb == 4 ? *reinterpret_cast<const uint32_t*>(src) >> (8 * (m & 1)) : *reinterpret_cast<const uint32_t*>(src + 4 * (m & 1));
-            } else {
-                const uint8_t* src = P.c.v + P.c.v_pair(page, head, at >> 1) + (m * J + j) * P.c.vb + 2 * (at & 1);
-                w[q] = *reinterpret_cast<const uint16_t*>(src);
-                if (P.c.vb == 8) u[q] = *reinterpret_cast<const uint16_t*>(src + 4);
+            for (int a = 0; a < A; ++a) {
+                const uint32_t off = 128 * (p0 + a) + 4 * lane, head = off / D, j = (off - head * D) / 32;
+                w[a] = 0u, d[a] = __ushort_as_half(0);
+                if (!there || (check && int(off) >= n_kv)) continue;
+                d[a] = sc[head * head_s + KIND * J + j];
+                if constexpr (KIND == 0) {
+                    const uint8_t* src = k + (head * head_k + j * P.c.kb);
+                    w[a] = q4 ? *reinterpret_cast<const uint32_t*>(src) >> (8 * (m & 1)) : *reinterpret_cast<const uint32_t*>(src + 4 * (m & 1));
+                } else {
+                    const uint8_t* src = v + (head * head_v + j * P.c.vb);
+                    w[a] = *reinterpret_cast<const uint16_t*>(src);
+                    if (!q4) w[a] |= uint32_t(*reinterpret_cast<const uint16_t*>(src + 4)) << 16;
+                }
             }
-        }
 #pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-            const int blk = b0 + 4 * q + (lane >> 3), h = blk / J, j = blk - h * J, kind = h < kv ? 0 : 1, head = h - kind * kv;
-            if (blk >= b1) continue;
-            uint32_t n[4];
-            const bool q4 = (kind == 0 ? P.c.kb : P.c.vb) == 4;
-            if (kind == 0) {
-                const int a = q4 ? 4 : 8, mask = q4 ? 15 : 255;
-                n[0] = w[q] & mask, n[1] = (w[q] >> 16) & mask, n[2] = (w[q] >> a) & mask, n[3] = (w[q] >> (16 + a)) & mask;
-            } else if (q4) {
-                n[0] = w[q] & 15u, n[1] = (w[q] >> 4) & 15u, n[2] = (w[q] >> 8) & 15u, n[3] = w[q] >> 12;
-            } else {
-                n[0] = w[q] & 255u, n[1] = w[q] >> 8, n[2] = u[q] & 255u, n[3] = u[q] >> 8;
+            for (int a = 0; a < A; ++a) {
+                const int off = 128 * (p0 + a) + 4 * lane;
+                if (check && off >= n_kv) continue;
+                // the four codes as bytes, in order
+                uint32_t n = w[a];
+                if (q4) n = KIND == 0 ? (n & 0x000F000Fu) | (n & 0x00F000F0u) << 4 : (n & 0x000Fu) | (n & 0x00F0u) << 4 | (n & 0x0F00u) << 8 | (n & 0xF000u) << 12;
+                if (KIND == 0) n = __byte_perm(n, 0u, 0x3120);
+                const float f = there ? __half2float(d[a]) : 0.f;
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = there ? __fmul_rn(f, float(int(n >> (8 * i) & 255u) - (q4 ? 8 : 128))) : 0.f;
+                store4(out + off, make_float4(y[0], y[1], y[2], y[3]));
             }
-            const int off = q4 ? 8 : 128;
-            const float4 y = !there ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                    : make_float4(__fmul_rn(d[q], float(int(n[0]) - off)), __fmul_rn(d[q], float(int(n[1]) - off)),
-                                                  __fmul_rn(d[q], float(int(n[2]) - off)), __fmul_rn(d[q], float(int(n[3]) - off)));
-            store4(static_cast<T*>(kind == 0 ? P.k : P.v) + ((long long)row * kv + head) * (32 * J) + 32 * j + 4 * m, y);
-        }
-    }
+        };
+        int p = first;
+        for (; p + kAhead <= last && 128 * (p + kAhead) <= n_kv; p += kAhead) batch(p, std::integral_constant<int, kAhead>{}, false);
+        for (; p < last; ++p) batch(p, std::integral_constant<int, 1>{}, true);
+    };
+    const int q0 = part * P.per_part;
+    if (q0 < pk) section(std::integral_constant<int, 0>{}, q0, min(p1, pk));
+    if (p1 > pk) section(std::integral_constant<int, 1>{}, max(q0 - pk, 0), p1 - pk);
 }
 
-// Warps a row and blocks a warp: rows on their own where they fill the GPU (16 warps an SM), else cut so that there are as
-// many, at least one pass of 4 blocks each; the launch's CTAs, 0 if they pass a grid.
-unsigned cut_rows(long long rows, int blocks, int& parts, int& per_part) {
+// Warps a row and passes a warp: rows on their own where they fill the GPU (16 warps an SM), else cut so that there are as
+// many, one pass each at least; the launch's CTAs, 0 if they pass a grid.
+unsigned cut_rows(long long rows, int passes, int& parts, int& per_part) {
     const long long want = 16LL * sm_count();
-    const int passes = (blocks + 3) / 4;
     parts = int(std::min<long long>(passes, std::max<long long>(1, want / rows)));
-    per_part = 4 * ((passes + parts - 1) / parts);
-    parts = (blocks + per_part - 1) / per_part;
+    per_part = (passes + parts - 1) / parts;
+    parts = (passes + per_part - 1) / per_part;
     const long long ctas = (rows * parts + 7) / 8;
     return ctas <= 0x7FFFFFFFLL ? unsigned(ctas) : 0u;
 }
+int passes_of(int heads, int dim) { return (heads * dim + 127) / 128; }
 // f(std::integral_constant<int, dim / 32>)
 template <class Fn>
 int by_blocks(int J, Fn&& f) {
@@ -282,7 +349,7 @@ int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dt
     P.rot = rot_dim, P.paired = paired, P.n_q = q ? n_q : 0;
     P.rows = int(rows);
     P.status = device_status_ptr();
-    const unsigned ctas = cut_rows(rows, (2 * P.c.n_kv + P.n_q) * P.c.J, P.parts, P.per_part);
+    const unsigned ctas = cut_rows(rows, 2 * passes_of(P.c.n_kv, P.c.dim) + passes_of(P.n_q, P.c.dim), P.parts, P.per_part);
     if (!ctas) return ST_BAD_TOKENS;
     return by_elem(dtype, [&](auto c) {
         return by_blocks(P.c.J, [&](auto j) {
@@ -304,7 +371,7 @@ int qmv_kv_read(const qmv_kv_cache* cache, const long long* slots, long long row
     P.slots = slots, P.k = k, P.v = v;
     P.rows = int(rows);
     P.status = device_status_ptr();
-    const unsigned ctas = cut_rows(rows, 2 * P.c.n_kv * P.c.J, P.parts, P.per_part);
+    const unsigned ctas = cut_rows(rows, 2 * passes_of(P.c.n_kv, P.c.dim), P.parts, P.per_part);
     if (!ctas) return ST_BAD_TOKENS;
     return by_elem(dtype, [&](auto c) {
         return by_blocks(P.c.J, [&](auto j) {
