@@ -11,7 +11,8 @@
 // 4-bit pair costs one AND and no conversion; the factor 2^24 and the queries' 1 / 16 are folded into constants.
 // (tcgen05 would need the unpacked values written to shared memory first, more bytes a clock than an SM writes.)  The codes'
 // offset (8 or 128) comes out as its own term: in the scores it is the accumulator's start, -off sum_i q[i] per block,
-// in the output one more product with a constant row a block.  Scales stay out of the products: d_k multiplies a block's
+// in the output one more product with a constant row a block.  (fp32 queries take it off the codes first: the term is many
+// times the sum's size, and its rounding showed as 1e-5 of the result.)  Scales stay out of the products: d_k multiplies a block's
 // 16 x 8 scores in fp32, d_v goes into p before it is rounded to fp16.
 //
 // Queries are fp16 after a power of two per row (exact for bf16 and fp16); fp32 queries are two fp16 parts (HL), and so
@@ -75,6 +76,36 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ float2 unpack_h2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// The four fp16 pairs of a code word (8 bits: of two), as the products' operands.  Plain: the codes' bits, denormals c 2^-24 (the
+// upper nibbles 16 times that).  CENTRED: c - offset, exactly: an OR of fp16's 1024 gives 1024 + c, or 1024 + 16 c, and one
+// operation takes the rest off.
+template <int BYTES, bool CENTRED>
+__device__ __forceinline__ void code_pairs(const uint32_t* w, uint32_t (&o)[4]) {
+    if constexpr (BYTES == 4) {
+        const uint32_t a = w[0], b = w[0] >> 8;
+        if constexpr (CENTRED) {
+            const __half2 low = __float2half2_rn(-1032.f), high = __float2half2_rn(-72.f), sixteenth = __float2half2_rn(0.0625f);
+            o[0] = h2_bits(__hadd2(bits_h2((a & 0x000F000Fu) | 0x64006400u), low));
+            o[1] = h2_bits(__hfma2(bits_h2((a & 0x00F000F0u) | 0x64006400u), sixteenth, high));
+            o[2] = h2_bits(__hadd2(bits_h2((b & 0x000F000Fu) | 0x64006400u), low));
+            o[3] = h2_bits(__hfma2(bits_h2((b & 0x00F000F0u) | 0x64006400u), sixteenth, high));
+        } else {
+            o[0] = a & 0x000F000Fu, o[1] = a & 0x00F000F0u, o[2] = b & 0x000F000Fu, o[3] = b & 0x00F000F0u;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t a = w[i] & 0x00FF00FFu, b = (w[i] >> 8) & 0x00FF00FFu;
+            if constexpr (CENTRED) {
+                const __half2 low = __float2half2_rn(-1152.f);
+                o[2 * i] = h2_bits(__hadd2(bits_h2(a | 0x64006400u), low)), o[2 * i + 1] = h2_bits(__hadd2(bits_h2(b | 0x64006400u), low));
+            } else {
+                o[2 * i] = a, o[2 * i + 1] = b;
+            }
+        }
+    }
+}
 
 // f(std::integral_constant<int, 0>) .. of N
 template <int N, int I = 0, class Fn>
@@ -474,13 +505,13 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                 const int e = ex == 0 || ex == 255 ? 0 : max(-120, min(120, ex - 127 - 14));
                 // the scale's sign goes into the queries: cs is positive, and masked scores stay -inf
                 const float down = __uint_as_float((uint32_t(127 - e) << 23) | (P.scale < 0.f ? 0x80000000u : 0u));
-                cs[nt] = fmaxf(fabsf(P.scale) * 1.4426950408889634f * 16777216.f * __uint_as_float(uint32_t(127 + e) << 23), 1e-30f);
+                cs[nt] = fmaxf(fabsf(P.scale) * 1.4426950408889634f * (HL ? 1.f : 16777216.f) * __uint_as_float(uint32_t(127 + e) << 23), 1e-30f);
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     float all = 0.f;
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        constexpr float kHigh = KB == 4 ? 1.f / 16.f : 1.f;     // the upper nibbles arrive 16 times too large
+                        constexpr float kHigh = KB == 4 && !HL ? 1.f / 16.f : 1.f;      // the upper nibbles arrive 16 times too large
                         const float a = x[j][m].x * down, b2 = x[j][m].y * down, c = x[j][m].z * down * kHigh, d = x[j][m].w * down * kHigh;
                         const uint32_t lo = pack_h2(a, b2), hi = pack_h2(c, d);
                         const float2 fl = unpack_h2(lo), fh = unpack_h2(hi);
@@ -495,7 +526,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                     }
                     all += __shfl_xor_sync(0xffffffffu, all, 1);
                     all += __shfl_xor_sync(0xffffffffu, all, 2);
-                    start[nt][j] = all * (-kOffK * 5.9604644775390625e-8f);
+                    start[nt][j] = HL ? 0.f : all * (-kOffK * 5.9604644775390625e-8f);
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -576,17 +607,11 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                     for (int x = 0; x < KT; ++x)
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
-                            uint32_t k0, k1, k2, k3;
-                            if constexpr (KB == 4) {
-                                const uint32_t w = kw[x][y][j], w8 = w >> 8;
-                                k0 = w & 0x000F000Fu, k1 = w & 0x00F000F0u, k2 = w8 & 0x000F000Fu, k3 = w8 & 0x00F000F0u;
-                            } else {
-                                const uint32_t w = kw[x][y][2 * j], z = kw[x][y][2 * j + 1];
-                                k0 = w & 0x00FF00FFu, k1 = (w >> 8) & 0x00FF00FFu, k2 = z & 0x00FF00FFu, k3 = (z >> 8) & 0x00FF00FFu;
-                            }
+                            uint32_t k[4];
+                            code_pairs<KB, HL>(&kw[x][y][j * KB / 4], k);
                             float c[4];
-                            mma16816(c, q0, k0, k1, begin);
-                            mma16816(c, q1.x, q1.y, q1.z, q1.w, k2, k3);
+                            mma16816(c, q0, k[0], k[1], begin);
+                            mma16816(c, q1.x, q1.y, q1.z, q1.w, k[2], k[3]);
                             const float d0 = Slot::scale(sk[x][2 * y], j, false), d1 = Slot::scale(sk[x][2 * y + 1], j, false);
                             if (HL) c[0] += c[2], c[1] += c[3];
                             s[x][0][2 * y] = fmaf(d0, c[0], s[x][0][2 * y]), s[x][0][2 * y + 1] = fmaf(d1, c[1], s[x][0][2 * y + 1]);
@@ -689,15 +714,9 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                         uint32_t a[2][4];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {             // pair t (k 2 t, 2 t + 1), pair t + 4 (k 8 + 2 t, 9 + 2 t)
-                            if constexpr (VB == 4) {
-                                const uint32_t w = vw[x][h][j], w8 = w >> 8;
-                                a[0][2 * h] = w & 0x000F000Fu, a[0][2 * h + 1] = w & 0x00F000F0u;
-                                a[1][2 * h] = w8 & 0x000F000Fu, a[1][2 * h + 1] = w8 & 0x00F000F0u;
-                            } else {
-                                const uint32_t w = vw[x][h][2 * j], y = vw[x][h][2 * j + 1];
-                                a[0][2 * h] = w & 0x00FF00FFu, a[0][2 * h + 1] = (w >> 8) & 0x00FF00FFu;
-                                a[1][2 * h] = y & 0x00FF00FFu, a[1][2 * h + 1] = (y >> 8) & 0x00FF00FFu;
-                            }
+                            uint32_t v[4];
+                            code_pairs<VB, HL>(&vw[x][h][j * VB / 4], v);
+                            a[0][2 * h] = v[0], a[0][2 * h + 1] = v[1], a[1][2 * h] = v[2], a[1][2 * h + 1] = v[3];
                         }
                         float d[4];
                         uint32_t d2[2];
@@ -727,7 +746,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                                 const uint32_t b0 = z ? low[0] : bw[0], b1 = z ? low[1] : bw[1];
                                 mma16816(o[nt][j][0], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
                                 mma16816(o[nt][j][1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
-                                mma16816(off[nt], one.x, one.y, one.z, one.w, b0, b1);
+                                if constexpr (!HL) mma16816(off[nt], one.x, one.y, one.z, one.w, b0, b1);
                             }
                         }
                     }
@@ -744,7 +763,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    constexpr float kUp = 16777216.f, kHigh = VB == 4 ? kUp / 16.f : kUp;
+                    constexpr float kUp = HL ? 1.f : 16777216.f, kHigh = VB == 4 && !HL ? kUp / 16.f : kUp;
                     const float z0 = __shfl_sync(0xffffffffu, off[nt][0], 4 * j + t) * kUp, z1 = __shfl_sync(0xffffffffu, off[nt][1], 4 * j + t) * kUp;
                     const float(&x)[2][4] = o[nt][j];
                     float* p = own + (8 * nt + 2 * t) * D + 32 * j + 4 * g;
