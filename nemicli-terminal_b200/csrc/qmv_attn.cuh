@@ -152,35 +152,35 @@ __device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_
                  :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// A slot of a warp's ring in shared memory: KT tiles of 16 keys.  A lane (g = lane / 4, t = lane % 4) uses run t of the K rows
-// of keys g and g + 8, run g of the V pairs t and t + 4, and the scales of keys 2 t, 2 t + 1, 2 t + 8 and 2 t + 9.  K and
-// scales come as they lie, in one bulk copy each that one lane starts.  V's runs would meet on the same banks that way (four
-// pairs, 128 bytes apart), so each lane copies its own, side by side with the other lanes'.  (Everything by the lanes: 376
-// instructions a tile, and 27 bytes a clock and SM at the start.  V pair by pair in bulk, padded: the lanes' copies go out one
-// after the other, 136 instructions a tile.)
+// A slot of the CTA's ring in shared memory: a unit's 4 KT tiles of 16 keys, KT a warp.  A lane (g = lane / 4, t = lane % 4)
+// uses run t of the K rows of keys g and g + 8, run g of the V pairs t and t + 4, and the scales of keys 2 t, 2 t + 1, 2 t + 8
+// and 2 t + 9.  The warps take turns in asking for a unit.  K and scales come as they lie, page by page in bulk copies; V's runs
+// would meet on the same banks that way (four pairs, 128 bytes apart), so each lane copies the runs of its place, side by
+// side with the other lanes'.  (Every warp asking for its own tiles took 72 of a tile's 313 instructions; V pair by pair in
+// bulk, padded, 136: a bulk copy is one lane's.)
 template <int J, int KB, int VB, int KT>
 struct AttnSlot {
     static constexpr int kK = J * KB / 4, kV = J * VB / 4, kS = (J + 1) / 2;       // words of a lane's runs, of a key's K or V scales
     static constexpr int kRowK = 4 * J * KB, kRowV = 8 * J * VB, kRowS = 4 * J;    // bytes of a key, a pair, a key's scales
-    static constexpr int kOffK = KT * 256 * kV, kOffS = kOffK + KT * 16 * kRowK, kBytes = kOffS + KT * 16 * kRowS;
+    static constexpr int kTiles = kAttnWarps * KT, kTileV = 256 * kV;
+    static constexpr int kOffK = kTiles * kTileV, kOffS = kOffK + kTiles * 16 * kRowK, kBytes = kOffS + kTiles * 16 * kRowS;
     template <int X>
-    static __device__ __forceinline__ void keys(uint32_t (&k)[2][kK], uint32_t at) {           // at: slot + lane's place (lane_k)
+    static __device__ __forceinline__ void keys(uint32_t (&k)[2][kK], uint32_t at) {           // at: slot + lane_k
         lds_words<kK, kOffK + 16 * X * kRowK>(k[0], at);
         lds_words<kK, kOffK + (16 * X + 8) * kRowK>(k[1], at);
     }
-    static __device__ __forceinline__ uint32_t lane_k(int g, int t) { return g * kRowK + t * J * KB; }
+    static __device__ __forceinline__ uint32_t lane_k(int warp, int g, int t) { return (16 * KT * warp + g) * kRowK + t * J * KB; }
     template <int X>
-    static __device__ __forceinline__ void vals(uint32_t (&v)[2][kV], uint32_t at) {           // at: slot + lane_v
-        lds_words<kV, 256 * kV * X, 128 * kPiece<kV>>(v[0], at);
-        lds_words<kV, 256 * kV * X + 128 * kV, 128 * kPiece<kV>>(v[1], at);
+    static __device__ __forceinline__ void vals(uint32_t (&v)[2][kV], uint32_t at) {           // at: slot + KT warp tiles + lane_v
+        lds_words<kV, kTileV * X, 128 * kPiece<kV>>(v[0], at);
+        lds_words<kV, kTileV * X + 128 * kV, 128 * kPiece<kV>>(v[1], at);
     }
     static __device__ __forceinline__ uint32_t lane_v(int lane) { return 4 * kPiece<kV> * lane; }
-    template <int X>
     static __device__ __forceinline__ void copy_vals(uint32_t at, const uint8_t* from) {       // from: the tile's pair t, run g
-        copy_words<kV, 0, 256 * kV * X>(at, from);
-        copy_words<kV, 4 * kRowV, 256 * kV * X + 128 * kV>(at, from);
+        copy_words<kV, 0, 0>(at, from);
+        copy_words<kV, 4 * kRowV, 128 * kV>(at, from);
     }
-    // K's (V: V's) scale words of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (J 3: the first of V's is half K's); at: slot + 2 t rows
+    // K's (V: V's) scale words of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (J 3: the first of V's is half K's); at: slot + the warp's and 2 t rows
     template <int X, bool V>
     static __device__ __forceinline__ void scales(uint32_t (&sc)[4][kS], uint32_t at) {
         constexpr int o = kOffS + 16 * X * kRowS + (V ? 4 * (J - kS) : 0);
@@ -207,8 +207,8 @@ struct AttnSlot {
     }
 };
 // Tiles of 16 keys a warp works on at once (two: each instruction has another that does not wait for it, and the loop's and
-// the softmax's bookkeeping counts half), keys a unit, CTAs an SM is to hold, and the units a warp has in shared memory,
-// within 227 KB an SM.
+// the softmax's bookkeeping counts half), keys a unit, CTAs an SM is to hold (heads of 128 values: two, whose registers hold
+// everything; three spill, 104 us against 96 for 32 sequences of 8175 keys), and the units in a CTA's ring, within 227 KB an SM.
 __host__ __device__ constexpr int attn_tiles(int J, int nt) { return J < 8 && nt == 1 ? 2 : 1; }
 __host__ __device__ constexpr int attn_unit(int J, int nt) { return 16 * kAttnWarps * attn_tiles(J, nt); }
 __host__ __device__ constexpr int attn_unit_bytes(int J, int kb, int vb, int nt) {
@@ -218,7 +218,7 @@ __host__ __device__ constexpr int attn_room(bool hl, int J, int nt, int ctas) {
     return (226 * 1024) / ctas - 1024 - J * 2048 - 256;      // less the fragments
 }
 __host__ __device__ constexpr int attn_ctas(bool hl, int J, int kb, int vb, int nt) {
-    return J < 8 && nt == 1 && attn_room(hl, J, nt, 3) >= 2 * attn_unit_bytes(J, kb, vb, nt) ? 3 : 2;
+    return J < 4 && nt == 1 && attn_room(hl, J, nt, 3) >= 2 * attn_unit_bytes(J, kb, vb, nt) ? 3 : 2;
 }
 __host__ __device__ constexpr int attn_stages(bool hl, int J, int kb, int vb, int nt) {
     const int n = attn_room(hl, J, nt, attn_ctas(hl, J, kb, vb, nt)) / attn_unit_bytes(J, kb, vb, nt);
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
     constexpr uint32_t kOffV = VB == 4 ? 0x00080008u : 0x00800080u;
     constexpr int S_ = attn_stages(HL, J, KB, VB, NT), KT = attn_tiles(J, NT), kUnit = attn_unit(J, NT);
     using Slot = AttnSlot<J, KB, VB, KT>;
-    static_assert(kAttnWarps * Slot::kBytes == attn_unit_bytes(J, KB, VB, NT), "the launch's shared memory");
+    static_assert(Slot::kBytes == attn_unit_bytes(J, KB, VB, NT), "the launch's shared memory");
     extern __shared__ __align__(16) float s_part[];              // the warps' tiles [warps][S_]; then [warps][R (D + 2)]
     constexpr bool two = HL || NT == 2;                          // the scores' rows g + 8 are used
     // per block and lane, whole operands (put together in registers they cost a move a word): the queries of the two k steps, the
@@ -295,16 +295,21 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
     __shared__ uint4 s_q[J][2][32], s_one[J][32];
     __shared__ float4 s_start[J][32];
     __shared__ long long s_scan[kAttnWarps + 1];
-    __shared__ uint64_t s_bar[kAttnWarps][4];
+    __shared__ uint64_t s_bar[2][4];
+    __shared__ uint32_t s_held[4];                               // the unit's runs of keys in one page that were copied, a bit each
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const uint32_t bar0 = smem_u32(s_bar[warp]);
-    if (lane == 0) {
-        for (int i = 0; i < S_; ++i) mbar_init(bar0 + 8 * i, 1);
+    const uint32_t full0 = smem_u32(s_bar[0]), empty0 = smem_u32(s_bar[1]), ring = smem_u32(s_part);
+    if (tid == 0) {
+        for (int i = 0; i < S_; ++i) mbar_init(full0 + 8 * i, 33), mbar_init(empty0 + 8 * i, kAttnWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncwarp();
+    __syncthreads();
+    // slots of the next unit to work on and to ask for, and the phase of its full (its empty, the one before) barrier
+    constexpr int kAhead = S_ > 2 ? S_ - 2 : 1;                  // units asked for ahead: S_ - 2 leaves the other warps a unit's time
+    int slot = 0, slot_in = 0;
+    uint32_t phase = 0, phase_in = 1;
     bool dead = false;                                            // a copy did not come in time: this warp takes no more units
-    uint32_t phases = 0;                                          // bit i: the phase slot i of this warp's ring waits for
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the join finds room as CTAs leave, and waits for the last
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int group = P.n_heads / P.c.n_kv, segs = P.c.n_kv * P.row_tiles;
 
@@ -379,7 +384,6 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
         if (most < ctas) ctas = int(most);
         if (blockIdx.x >= ctas) {
             if (tid == 0 && !P.by_segment) P.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             return;
         }
         u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
@@ -387,7 +391,6 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
         const long long in = u0 - before;
         seg = int(in / S.units), unit = int(in - (long long)seg * S.units);
     } else {                                                      // one CTA a segment
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         b = blockIdx.x / segs, seg = blockIdx.x - b * segs;
         S = attn_seq(P, b, seg == 0 && tid == 0, kUnit);
         u1 = S.units;
@@ -402,21 +405,23 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
         const int tok0 = rt * R / group, tok1 = (rt * R + max(rows, 1) - 1) / group;
         const int last = min(pos0 + tok1, S.len - 1);             // keys of interest: first .. last
         const int first = P.window > 0 ? max(0, pos0 + tok0 - P.window + 1) : 0;
-        // every row sees keys full0 .. full1
-        const int full0 = P.window > 0 ? max(0, pos0 + tok1 - P.window + 1) : 0, full1 = pos0 + tok0;
+        // every row sees keys seen0 .. seen1
+        const int seen0 = P.window > 0 ? max(0, pos0 + tok1 - P.window + 1) : 0, seen1 = pos0 + tok0;
 
         float cs[NT], M[NT], rn[NT], sum[NT], o[NT][J][2][4], off[NT][4];        // of rows g, g + 8; o, off: columns 2 t, 2 t + 1
         int pos[NT];
         float E = 0.f;
         uint32_t lim = HL ? 0u : 0x48004800u;                     // d_v at most 8 until one larger is seen (two fp16)
         if (rows > 0) {
-            // ---- this warp's tiles, KT a unit: the first units' copies start before the queries are looked at
+            // ---- the units' copies; the first ones start before the queries are looked at
             const int turns = dead ? 0 : todo;
             const int* table = P.tables + (long long)b * P.width;
-            const int key0 = (S.first_unit + unit) * kUnit + 16 * KT * warp;
-            const uint32_t ring = smem_u32(s_part) + warp * S_ * Slot::kBytes;
-            const uint32_t lane_k = Slot::lane_k(g, t), lane_v = Slot::lane_v(lane), lane_s = 2 * t * Slot::kRowS;
+            const int key0 = (S.first_unit + unit) * kUnit;
+            const uint32_t lane_k = Slot::lane_k(warp, g, t), lane_v = KT * warp * Slot::kTileV + Slot::lane_v(lane),
+                           lane_s = (16 * KT * warp + 2 * t) * Slot::kRowS;
             const int shift = P.c.page_shift, in_page = (1 << shift) - 1;
+            constexpr int kUnitShift = kUnit == 64 ? 6 : 7;
+            const int run = min(shift, kUnitShift), runs = 1 << (kUnitShift - run);         // log2 of a run's keys, runs a unit
             // this key head's rows of page 0, this lane's V run of it, and the bytes between pages
             const uint8_t* head_k = P.c.k + ((long long)hk << shift) * Slot::kRowK;
             const uint8_t* head_v = P.c.v + ((long long)hk << (shift - 1)) * Slot::kRowV + t * Slot::kRowV + g * J * VB;
@@ -424,62 +429,52 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
             const uint32_t page_k = uint32_t(P.c.n_kv * Slot::kRowK) << shift, page_v = uint32_t(P.c.n_kv * Slot::kRowV) << (shift - 1),
                            page_s = uint32_t(P.c.n_kv * Slot::kRowS) << shift;
             constexpr int kNoKey = INT_MIN;                       // nothing to see there
-            struct Entry { int page[KT]; };                       // of a unit's tiles
-            auto look = [&](int u) {
-                Entry e;
-#pragma unroll
-                for (int x = 0; x < KT; ++x) {
-                    const int key = key0 + u * kUnit + 16 * x;
-                    e.page[x] = u < turns && key <= last && key + 15 >= first ? __ldg(table + (key >> shift)) : kNoKey;
-                }
-                return e;
+            auto look = [&](int u) {                              // lane c: the page of unit u's run c
+                const int key = key0 + u * kUnit + (lane << run);
+                return u < turns && lane < runs && key <= last && key + (1 << run) > first ? __ldg(table + (key >> shift)) : kNoKey;
             };
-            uint32_t held = 0;                                    // bit KT i + x: tile x of slot i is there
-            auto ask = [&](int u, int slot, const Entry& e) {     // starts the copies of unit u's tiles
-                const uint32_t to = ring + slot * Slot::kBytes, bar = bar0 + 8 * slot;
-                uint32_t tiles = 0;
-#pragma unroll
-                for (int x = 0; x < KT; ++x) {
-                    const bool there = e.page[x] >= 0 && e.page[x] < P.c.n_pages;
-                    if (there) tiles |= 1u << x;
-                    else if (e.page[x] != kNoKey && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
+            auto ask = [&](int u, int entry) {                    // one warp: starts the copies of unit u into slot_in
+                const bool there = entry >= 0 && entry < P.c.n_pages;
+                if (!there && entry != kNoKey && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
+                const uint32_t mask = __ballot_sync(0xffffffffu, there), full = full0 + 8 * slot_in;
+                if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * slot_in, phase_in))) {
+                    if (lane == 0 && P.status) atomicOr(P.status, DEV_TIMEOUT);
+                    return;                                       // the unit never gets full: every warp gives up there
                 }
-                held = (held & ~(((1u << KT) - 1u) << (KT * slot))) | tiles << (KT * slot);
-                const int at = (key0 + u * kUnit) & in_page;
-                if (tiles == (1u << KT) - 1u && (KT == 1 || shift > 4)) {          // one page holds the unit
-                    const uint32_t page = e.page[0];
+                const uint32_t to = ring + slot_in * Slot::kBytes;
+                if (lane == 0) {
+                    s_held[slot_in] = mask;
+                    mbar_arrive_tx(full, __popc(mask) * ((Slot::kRowK + Slot::kRowS) << run));
+                }
+                const int at = (key0 + u * kUnit) & in_page;      // within a page that holds the whole unit (else 0)
+                for (int c = 0; c < runs; ++c) {
+                    if (!(mask >> c & 1u)) continue;
+                    const uint32_t page = __shfl_sync(0xffffffffu, entry, c);
+                    const int first_key = c << run;
                     if (lane == 0) {
-                        mbar_arrive_tx(bar, KT * 16 * (Slot::kRowK + Slot::kRowS));
-                        copy_bulk(to + Slot::kOffK, head_k + (unsigned long long)page * page_k + at * Slot::kRowK, KT * 16 * Slot::kRowK, bar);
-                        copy_bulk(to + Slot::kOffS, head_s + (unsigned long long)page * page_s + at * Slot::kRowS, KT * 16 * Slot::kRowS, bar);
+                        copy_bulk(to + Slot::kOffK + first_key * Slot::kRowK, head_k + (unsigned long long)page * page_k + at * Slot::kRowK, Slot::kRowK << run, full);
+                        copy_bulk(to + Slot::kOffS + first_key * Slot::kRowS, head_s + (unsigned long long)page * page_s + at * Slot::kRowS, Slot::kRowS << run, full);
                     }
                     const uint8_t* from = head_v + (unsigned long long)page * page_v + (at >> 1) * Slot::kRowV;
-                    each<KT>([&](auto x) { Slot::template copy_vals<decltype(x)::value>(to + lane_v, from + decltype(x)::value * 8 * Slot::kRowV); });
-                } else {
-                    if (lane == 0) mbar_arrive_tx(bar, __popc(tiles) * 16 * (Slot::kRowK + Slot::kRowS));
-                    each<KT>([&](auto x) {
-                        constexpr int X = decltype(x)::value;
-                        if (tiles >> X & 1u) {
-                            const uint32_t page = e.page[X];
-                            const int a = (at + 16 * X) & in_page;
-                            if (lane == 0) {
-                                copy_bulk(to + Slot::kOffK + 16 * X * Slot::kRowK, head_k + (unsigned long long)page * page_k + a * Slot::kRowK, 16 * Slot::kRowK, bar);
-                                copy_bulk(to + Slot::kOffS + 16 * X * Slot::kRowS, head_s + (unsigned long long)page * page_s + a * Slot::kRowS, 16 * Slot::kRowS, bar);
-                            }
-                            Slot::template copy_vals<X>(to + lane_v, head_v + (unsigned long long)page * page_v + (a >> 1) * Slot::kRowV);
-                        }
-                    });
+                    uint32_t dst = to + (first_key >> 4) * Slot::kTileV + Slot::lane_v(lane);
+#pragma unroll 4
+                    for (int x = 0; x < 1 << (run - 4); ++x, from += 8 * Slot::kRowV, dst += Slot::kTileV) Slot::copy_vals(dst, from);
                 }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(full) : "memory");
             };
-            Entry entry[S_ - 1];                                  // of the units to ask for next (the loop: one, a unit ahead)
+            auto next_in = [&]() {
+                if (++slot_in == S_) slot_in = 0, phase_in ^= 1u;
+            };
+            int entry = look(warp);                               // of the next unit this warp asks for: warp, warp + 4, ...
 #pragma unroll
-            for (int u = 0; u < S_ - 1; ++u) entry[u] = look(u);
-#pragma unroll
-            for (int u = 0; u < S_ - 1; ++u) {
-                if (u < turns) ask(u, u, entry[u]);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
-            entry[0] = look(S_ - 1);
+            for (int u = 0; u < kAhead; ++u)
+                if (u < turns) {
+                    if ((u & (kAttnWarps - 1)) == warp) {
+                        ask(u, entry);
+                        entry = look(u + kAttnWarps);
+                    }
+                    next_in();
+                }
             // Queries, scaled to fp16 by a power of two per row: lane (g, t) holds values 8 t .. 8 t + 7 of each block of row g
             // as the product's rows g, and as rows g + 8 the second parts (HL) or row g + 8 (NT 2)
             uint32_t part[2][J][2][2];                            // [rows g / g + 8][block][k step][half]
@@ -549,28 +544,28 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                 }
             }
             __syncthreads();
-            int slot = 0, slot_in = S_ - 1;                       // of unit u, and of unit u + S_ - 1
             for (int u = 0; u < turns; ++u) {
-                const int key = key0 + u * kUnit;
-                if (u + S_ - 1 < turns) ask(u + S_ - 1, slot_in, entry[0]);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                entry[0] = look(u + S_);
-                const uint32_t buf = ring + slot * Slot::kBytes;
-                const uint32_t here = held >> (KT * slot) & ((1u << KT) - 1u);
-                asm volatile("cp.async.wait_group %0;" :: "n"(S_ - 1) : "memory");
-                if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * slot, phases >> slot & 1u))) {
-                    // a copy did not come: say so, give the others in flight their time, and leave
+                const int key = key0 + u * kUnit + 16 * KT * warp;        // this warp's first key
+                if (u + kAhead < turns) {
+                    if (((u + kAhead) & (kAttnWarps - 1)) == warp) {
+                        ask(u + kAhead, entry);
+                        entry = look(u + kAhead + kAttnWarps);
+                    }
+                    next_in();
+                }
+                const uint32_t buf = ring + slot * Slot::kBytes, empty = empty0 + 8 * slot;
+                if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * slot, phase))) {
+                    // a copy did not come in time: say so and take no more units (the other warps find the same)
                     dead = true;
                     if (lane == 0 && P.status) atomicOr(P.status, DEV_TIMEOUT);
-                    for (int v = u + 1; v < min(u + S_, turns); ++v) {
-                        slot = slot + 1 == S_ ? 0 : slot + 1;
-                        mbar_wait(bar0 + 8 * slot, phases >> slot & 1u);
-                    }
                     break;
                 }
-                phases ^= 1u << slot;
-                slot = slot + 1 == S_ ? 0 : slot + 1;
-                slot_in = slot_in + 1 == S_ ? 0 : slot_in + 1;
+                const uint32_t mask = s_held[slot];
+                uint32_t here = 0;                                // bit x: tile x is there and some row sees some of it
+#pragma unroll
+                for (int x = 0; x < KT; ++x)
+                    if (mask >> ((16 * (KT * warp + x)) >> run) & 1u && key + 16 * x <= last && key + 16 * x + 15 >= first) here |= 1u << x;
+                if (++slot == S_) slot = 0, phase ^= 1u;
                 // A unit that some row does not see whole is masked key by key, in a copy of the code: in one, the masks were
                 // predicated instructions that every unit paid for (100 of a tile's 440)
                 auto work = [&](auto all_of_it) {
@@ -592,7 +587,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                         const int w = i + lane, key_w = w / kPer, at = kFirst + w % kPer;
                         if (16 * kPer % 32 == 0 || w < 16 * kPer)
                             if (whole || (here >> x & 1u && uint32_t(key + 16 * x + key_w - first) <= uint32_t(last - first)))
-                                dv = __vmaxu2(dv, lds32(buf + Slot::kOffS + ((16 * x + key_w) * J + at) * 4) & (J % 2 && at == kFirst ? 0x7FFF0000u : 0x7FFF7FFFu));
+                                dv = __vmaxu2(dv, lds32(buf + Slot::kOffS + ((16 * (KT * warp + x) + key_w) * J + at) * 4) & (J % 2 && at == kFirst ? 0x7FFF0000u : 0x7FFF7FFFu));
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
@@ -708,7 +703,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                 // the second operand already
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    const uint4 one = s_one[j][lane];             // row j of the offset's product
+                    [[maybe_unused]] const uint4 one = s_one[j][lane];       // row j of the offset's product
 #pragma unroll
                     for (int x = 0; x < KT; ++x) {
                         uint32_t a[2][4];
@@ -752,9 +747,10 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                     }
                 }
                 };
-                if (here == (1u << KT) - 1u && key >= full0 && key + 16 * KT - 1 <= full1) work(std::true_type{});
+                if (here == (1u << KT) - 1u && key >= seen0 && key + 16 * KT - 1 <= seen1) work(std::true_type{});
                 else if (here) work(std::false_type{});
-                __syncwarp();                                     // before other lanes copy into the slot again
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty);                // the slot may be filled again
             }
             __syncthreads();                                      // every warp is done with its tiles
             // ---- the warps' sums side by side in shared memory
@@ -811,10 +807,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
             S = attn_seq(P, ++b, false, kUnit);
         }
     }
-    if (P.split) {
-        if (!P.by_segment && tid == 0 && !owns) P.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    }
+    if (P.split && !P.by_segment && tid == 0 && !owns) P.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
 // Joins the parts of cut segments, in their order: block (entry, row), eight warps share the parts, a lane 4 values (8 of
