@@ -337,7 +337,8 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
  * starts[b] .. starts[b + 1] of q, or row b when starts is null.  Query i of n sits at position p = lens[b] - n + i and
  * sees keys max(0, p - window + 1) .. p (window 0: from 0 on); one that sees none (p < 0) gives zeros.  q: rows of
  * n_heads * dim values, q_stride apart (aligned to four values); out dense.  max_new: at least the longest run of new
- * tokens (rows beyond it are not computed, QMV_DEV_BAD_ADDRESS is set).  Rows of out that no sequence covers stay
+ * tokens (rows beyond it are not computed, QMV_DEV_BAD_ADDRESS is set; n_seq * max_new also decides between two
+ * kernels, so a tight bound is the faster one; with starts null it counts as 1, for the workspace too).  Rows of out that no sequence covers stay
  * as they are.  Table entries behind a sequence's last token are not read; pages outside the cache count as
  * masked, lengths beyond the table are cut, and both set QMV_DEV_BAD_ADDRESS.  workspace: 256-byte aligned,
  * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  The result does not depend on

@@ -12,7 +12,7 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
         return 0;
     if (dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16) return 0;
     if (table_width <= 0 || table_width > (0x7FFFFFFF >> c.page_shift) || window < 0) return 0;
-    if (attn_tc_used(c, dtype, n_heads, max_new)) return 256;     // no workspace
+    if (attn_tc_used(c, dtype, n_heads, n_seq, max_new)) return 1;       // no workspace
     const AttnPlan p = attn_plan(c, dtype, n_heads, n_seq, max_new, table_width, window);
     return p.grid ? p.bytes : 0;
 }
@@ -37,7 +37,7 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
         !aligned(starts, 4) || !aligned(workspace, 256))
         return ST_BAD_ALIGN;
     if (!starts) max_new = 1;
-    const bool tiles = attn_tc_used(P.c, dtype, n_heads, max_new);
+    const bool tiles = attn_tc_used(P.c, dtype, n_heads, n_seq, max_new);
     const AttnPlan pl = attn_plan(P.c, dtype, n_heads, n_seq, max_new, table_width, window);
     if (tiles ? (long long)attn_tc_tiles(P.c, n_heads, max_new) * P.c.n_kv * n_seq > 0x7FFFFFFF : !pl.grid || workspace_bytes < pl.bytes)
         return ST_BAD_SHAPE;

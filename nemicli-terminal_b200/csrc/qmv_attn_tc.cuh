@@ -4,18 +4,22 @@
 //   S = Q K^T,  P = 2^(S scale log2 e - ref),  O += P V,  l += sum P   per tile of BN keys, then O / l
 //
 // A CTA takes NQ tiles of 128 query rows of one sequence and key head (row = token * group + head of the group, so
-// the cache is unpacked once for the whole group) over all their keys.  Bound by the tensor cores and the special
-// function units about equally: 128 x 128 scores of 128 values take 1024 clocks of MMA (both products) and
-// 1024 of exp2.  Roles:
-//   producers  4 warps: words of the cache -> d * code in fp16 (one rounding) -> shared memory, in the MMA's K-major core
+// the cache is unpacked once for the whole group) over all their keys.  For two tiles, 64 keys and 128 values a step of both
+// takes 2048 clocks of exp2 (16 a clock and SM) and 2048 of MMA (both products), which run side by side; measured about 2200
+// (8192 tokens, 32 heads: 0.58 to 0.61 ms, 900 TFLOP/s).  Roles:
+//   producers  NP x 4 warps: words of the cache -> d * code in fp16 (one rounding) -> shared memory, in the MMA's K-major core
 //              matrices (8 rows x 16 bytes; K: rows = keys, V: rows = values of the head, so a V word, whose halves
-//              are two tokens, lands transposed without a shuffle).  Two stages each, loads one tile ahead in registers.
-//   MMA        one thread: S(i + 1) of a tile follows its O(i), the other tile's softmax runs meanwhile.
+//              are two tokens, lands transposed without a shuffle).  Loads one round ahead in registers, page numbers two.
+//              Heads of 256 values have one query tile's time for twice the unpacking: two groups take the rounds in turn
+//              (6 prompts of up to 1500 tokens on up to 6001, window 1024, 16 heads on 8: 287 -> 262 us), and V's stage is waited
+//              for behind K's (-> 240).
+//   MMA        one warp: the scores run two steps ahead of the sums, the other tile's softmax runs meanwhile.
 //   softmax    NQ x 4 warps, one thread a row: scores from tensor memory, P as fp16 over them, and the row's
 //              reference, sum and mask in registers.  The reference moves only when the row's maximum passes it by 2^8;
 //              then the warp rescales its rows of O in tensor memory.
+// A quarter of the exponentials as a cubic on the other units gained nothing (595 us without, 610 with it).
 // Queries are fp16 after a power of two per row (exact but for values 2^-32 below the row's largest).  Tensor memory:
-// S NQ x BN columns, O NQ x D columns.  Every mbarrier wait is bounded; on expiry the CTA sets DEV_TIMEOUT, waits
+// S NQ x 2 x BN columns, O NQ x D columns.  Every mbarrier wait is bounded; on expiry the CTA sets DEV_TIMEOUT, waits
 // (bounded) for its MMAs, frees its tensor memory and leaves.
 #pragma once
 #include <climits>
@@ -30,13 +34,14 @@ template <int J> struct AttnTcShape {
     static constexpr int BN = 64;                                 // keys a step
     static constexpr int PB = J == 8 ? 64 : 128;                  // keys the producers take at once: one or two steps' stages
     static constexpr int KS = 2 * PB / BN;                        // stages of K and of V
-    static constexpr int kThreads = NQ * 128 + 128 + 32;
+    static constexpr int NP = J == 8 ? 2 : 1;                    // groups of producers (two: each sees every phase of its stage)
+    static constexpr int kThreads = (NQ + NP) * 128 + 32;
     static constexpr int kQ = 128 * D * 2, kK = BN * D * 2, kV = D * BN * 2;      // bytes of one tile / stage
     static constexpr int kScaleK = PB * J * 2, kScaleV = J * PB * 2;
     static constexpr int kOffK = NQ * kQ, kOffV = kOffK + KS * kK, kOffSK = kOffV + KS * kV, kOffSV = kOffSK + 2 * kScaleK;
-    static constexpr int kOffBar = kOffSV + 2 * kScaleV;          // mbarriers, the tensor-memory address
-    static constexpr int kOffBad = kOffBar + 256;                 // [2][4] words: keys whose page is not of the cache
-    static constexpr int kSmem = kOffBad + 32;
+    static constexpr int kOffBar = kOffSV + 4 * kScaleV;          // mbarriers, the tensor-memory address
+    static constexpr int kOffBad = kOffBar + 256;                 // [4][4] words: keys whose page is not of the cache
+    static constexpr int kSmem = kOffBad + 64;
     static constexpr uint32_t kSboQ = D * 16, kSboK = D * 16, kSboV = BN * 16;    // bytes between 8-row groups
 };
 
@@ -193,7 +198,7 @@ template <int DT, int J, int KB, int VB>
 __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(const __grid_constant__ AttnParams P) {
     using T = typename Elem<DT>::type;
     using Sh = AttnTcShape<J>;
-    constexpr int D = Sh::D, NQ = Sh::NQ, BN = Sh::BN, KS = Sh::KS;
+    constexpr int D = Sh::D, NQ = Sh::NQ, BN = Sh::BN, KS = Sh::KS, NP = Sh::NP;
     extern __shared__ __align__(128) uint8_t tc_smem_[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -235,7 +240,7 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
     at_after();
     constexpr uint32_t tmem = 0;                                  // all 512 columns were asked for: they start at 0
     constexpr uint32_t kO = NQ * 2 * BN;                          // S (and P over it): column (2 a + buffer) BN; O: kO + a D
-    const int qa = warp >> 2;                                     // query tile, NQ: producers, NQ + 1: MMA
+    const int qa = warp >> 2;                                     // query tile, from NQ on producers, NQ + NP: MMA
     bool ok = true;                                               // no wait ran out so far
 
     if (qa < NQ) {
@@ -321,10 +326,10 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
 #pragma unroll
             for (int c = 0; c < BN; c += 32) at_ld32(s_at + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
             const int key = (kt0 + i) * BN;
-            // keys of pages outside the cache are masked too (the words live as long as the tile's V stage)
+            // keys of pages outside the cache are masked too (the words stay for four rounds)
             uint32_t bad[2];
             asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(bad[0]), "=r"(bad[1])
-                         : "r"(sm + Sh::kOffBad + (Sh::PB == BN ? 16 * (i & 1) : 16 * ((i >> 1) & 1) + 8 * (i & 1))) : "memory");
+                         : "r"(sm + Sh::kOffBad + (Sh::PB == BN ? 16 * (i & 3) : 16 * ((i >> 1) & 3) + 8 * (i & 1))) : "memory");
             const bool whole = key >= full0 && key + BN - 1 <= full1 && !(bad[0] | bad[1]);
             at_wait_ld();
             if (!whole) {                                         // what this row does not see becomes -inf
@@ -420,9 +425,9 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
                 reinterpret_cast<uint4*>(out)[piece] = y;
             }
         }
-    } else if (qa == NQ) {
+    } else if (qa < NQ + NP) {
         // ---- producers -----------------------------------------------------------------------------
-        const int pw = warp & 3, pt = tid - NQ * 128;             // producer warp and thread
+        const int pw = warp & 3, pt = tid & 127, pg = qa - NQ;    // producer warp, thread and group: rounds pg, pg + NP, ..
         constexpr int PB = Sh::PB, kPer = PB / BN;                // keys and stages a round
         constexpr int kRows = PB / 4, kGroups = kRows / 8;        // keys a warp, 8-key groups
         constexpr int kWk = J * KB / 4;                           // words of a lane's K run
@@ -435,7 +440,13 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
         // tile later, so that no load waits for one.  kNoKey: nothing to see there.
         constexpr int kNoKey = INT_MIN;
         auto entry_of = [&](int key) { return key > last || key + 15 < first ? kNoKey : __ldg(table + (key >> P.c.page_shift)); };
-        auto valid = [&](int p) { return p >= 0 && p < P.c.n_pages; };
+        auto valid = [&](int p) { return uint32_t(p) < uint32_t(P.c.n_pages); };
+        // this lane's bytes of page 0, and the pages' strides (below 2^31 bytes: a page has at most 2^30 values)
+        const uint8_t* const k0 = P.c.k + P.c.k_row(0, hk, kk) + kt * J * KB;
+        const uint8_t* const v0 = P.c.v + P.c.v_pair(0, hk, 0) + (vg * J + vj) * VB;
+        const uint8_t* const s0 = reinterpret_cast<const uint8_t*>(P.c.sc + P.c.scale_row(0, hk, 0));
+        const uint32_t in_page = P.c.page() - 1, rows_page = uint32_t(P.c.n_kv) << P.c.page_shift;
+        const uint32_t k_page = rows_page * (4 * J * KB), v_page = rows_page * (4 * J * VB), s_page = rows_page * (4 * J);
         constexpr int kRuns = (kRows + 15) / 16;
         int pk[kRuns], pv, ps;                                    // of K's runs, V's keys, the scale's key
         auto ask = [&](int i) {
@@ -452,7 +463,7 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
             for (int q = 0; q < kGroups; ++q) {
                 const int key = key0 + kRows * pw + 8 * q, page = pk[q >> 1];
                 if (valid(page)) {
-                    at_ldg<kWk>(kw[q], P.c.k + P.c.k_row(page, hk, (key & (P.c.page() - 1)) + kk) + kt * J * KB);
+                    at_ldg<kWk>(kw[q], k0 + ((unsigned long long)page * k_page + (key & in_page) * (4 * J * KB)));
                 } else {
 #pragma unroll
                     for (int w = 0; w < kWk; ++w) kw[q][w] = 0u;
@@ -461,7 +472,7 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
             // scales of key pt; nobody sees it: 0 (it may hold anything)
             bad = __ballot_sync(0xffffffffu, ps != kNoKey && !valid(ps));
             if (valid(ps)) {
-                at_ldg<J>(sw, reinterpret_cast<const uint8_t*>(P.c.sc + P.c.scale_row(ps, hk, (key0 + pt) & (P.c.page() - 1))));
+                at_ldg<J>(sw, s0 + ((unsigned long long)ps * s_page + ((key0 + pt) & in_page) * (4 * J)));
             } else {
 #pragma unroll
                 for (int w = 0; w < J; ++w) sw[w] = 0u;
@@ -469,34 +480,36 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
         };
         auto load_v = [&](int i) {
             const int key = kt0 * BN + i * PB + kRows * pw + 8 * vkc;
+            if (valid(pv)) {
+                const uint8_t* at = v0 + ((unsigned long long)pv * v_page + (key & in_page) * (4 * J * VB));
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                if (valid(pv)) {
-                    at_ldg<kWv>(vw[p], P.c.v + P.c.v_pair(pv, hk, ((key & (P.c.page() - 1)) >> 1) + p) + (vg * J + vj) * VB);
-                } else {
+                for (int p = 0; p < 4; ++p) at_ldg<kWv>(vw[p], at + p * (8 * J * VB));
+            } else {
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
 #pragma unroll
                     for (int w = 0; w < kWv; ++w) vw[p][w] = 0u;
-                }
             }
         };
         if (n_tiles) {
-            ask(0);
-            load_k(0), load_v(0);
-            ask(1);
+            ask(pg);
+            load_k(pg), load_v(pg);
+            ask(pg + NP);
         }
         const int rounds = (n_tiles + kPer - 1) / kPer;
-        for (int i = 0; i < rounds; ++i) {
+        for (int i = pg; i < rounds; i += NP) {
             const int st = i & 1;                                 // stages kPer st ..
             const uint32_t par = uint32_t(i >> 1) & 1u;
-            const uint32_t s_k = sm + Sh::kOffSK + st * Sh::kScaleK, s_v = sm + Sh::kOffSV + st * Sh::kScaleV;
+            const uint32_t s_k = sm + Sh::kOffSK + st * Sh::kScaleK, s_v = sm + Sh::kOffSV + (i & 3) * Sh::kScaleV;
             if (i >= 2)
 #pragma unroll
                 for (int q = 0; q < kPer; ++q)
-                    ok = ok && mbar_wait(k_free + 8 * (kPer * st + q), par ^ 1u) && mbar_wait(v_free + 8 * (kPer * st + q), par ^ 1u);
-            // scales: K's by key, V's by block (so that eight keys of a block are one word of 16 bytes)
+                    ok = ok && mbar_wait(k_free + 8 * (kPer * st + q), par ^ 1u);
+            // scales: K's by key, V's by block (so that eight keys of a block are one word of 16 bytes); four buffers of V's,
+            // since a warp may be here while another still reads the ones of this group's last round
             if (pt < PB) {
                 __half* dk = reinterpret_cast<__half*>(tc_smem_ + Sh::kOffSK + st * Sh::kScaleK) + pt * J;
-                __half* dv = reinterpret_cast<__half*>(tc_smem_ + Sh::kOffSV + st * Sh::kScaleV) + pt;
+                __half* dv = reinterpret_cast<__half*>(tc_smem_ + Sh::kOffSV + (i & 3) * Sh::kScaleV) + pt;
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const uint32_t a = sw[j >> 1], c = sw[(J + j) >> 1];
@@ -505,10 +518,10 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
                 }
             }
             uint32_t all;                                         // the four warps go on, or leave, together
-            if (lane == 0) reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBad)[4 * st + pw] = bad;
+            if (lane == 0) reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBad)[4 * (i & 3) + pw] = bad;
             if (bad && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
-            asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.and.pred q, 1, 128, p; selp.u32 %0, 1, 0, q; }"
-                         : "=r"(all) : "r"(uint32_t(ok)) : "memory");
+            asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.and.pred q, %2, 128, p; selp.u32 %0, 1, 0, q; }"
+                         : "=r"(all) : "r"(uint32_t(ok)), "r"(1 + pg) : "memory");
             ok = all != 0;
             if (!ok) break;
 #pragma unroll
@@ -533,8 +546,14 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
             at_fence_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(k_full + 8 * (kPer * st + kRows * pw / BN));
-            if (i + 1 < rounds) load_k(i + 1);
-            {
+            if (i + NP < rounds) load_k(i + NP);
+            // V's stage is free one step later than K's: waited for here, the scores of this round are not held up by it
+            if (i >= 2) {
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) ok = ok && mbar_wait(v_free + 8 * (kPer * st + q), par ^ 1u);
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            if (ok) {                                             // (if not: all leave at the next round's barrier)
                 const int kc = (kRows / 8) * pw + vkc;            // 8-key core of the round
                 const uint32_t dst = sm + Sh::kOffV + (kPer * st + kc / (BN / 8)) * Sh::kV + (kc % (BN / 8)) * 128;
 #pragma unroll
@@ -554,9 +573,9 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
             }
             at_fence_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(v_full + 8 * (kPer * st + kRows * pw / BN));
-            if (i + 1 < rounds) load_v(i + 1);
-            ask(i + 2);
+            if (ok && lane == 0) mbar_arrive(v_full + 8 * (kPer * st + kRows * pw / BN));
+            if (i + NP < rounds) load_v(i + NP);
+            ask(i + 2 * NP);
         }
     } else {
         // ---- MMA -----------------------------------------------------------------------------------
@@ -622,16 +641,22 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
 // ---- host -------------------------------------------------------------------------------------------
 
 
-// Rows of a sequence (new tokens x heads of a key head) from which the tiles are used.
-constexpr int kAttnTcRows = 65;
-
-inline bool attn_tc_used(const KvView& c, int dtype, int n_heads, int max_new) {
-    return dtype != QMV_OUT_F32 && (long long)max_new * (n_heads / c.n_kv) >= kAttnTcRows;
-}
 inline int attn_tc_tiles(const KvView& c, int n_heads, int max_new) {
     const long long rows = (long long)max_new * (n_heads / c.n_kv);
     const int per = c.J == 8 ? 128 : 256;
     return int((rows + per - 1) / per);
+}
+// Whether the tiles are used (else attn_kernel).  A tile walks all its keys at a cost that its rows do not change, one CTA an
+// SM: 14.5 ns a key for heads of 64 values, 17.8 for 128, 18.5 for 256.  attn_kernel spreads any work over the GPU, at a cost
+// that goes with the rows: 2.3, 3.3 and 11 ps a key and row.  So the tiles gain from as many rows a round of CTAs as the
+// ratio of the two.  Measured in us, tiles / attn_kernel, heads of 128 values, 8 key heads, 4 query heads each:
+//   1 sequence of 32768 keys, 16 new tokens (512 rows): 584 / 68     64 tokens (2048 rows): 586 / 229
+//   8 sequences of 4096 keys, 16 tokens (4096 rows): 80 / 75         24 tokens (6144 rows): 80.5 / 107
+//   and 4 key heads of 256 values, 8 x 4096 keys, 8 tokens (1024 rows): 86 / 63      16 tokens (2048 rows): 86 / 112
+inline bool attn_tc_used(const KvView& c, int dtype, int n_heads, int n_seq, int max_new) {
+    if (dtype == QMV_OUT_F32) return false;                       // fp16 products lack its accuracy
+    const long long heads = (long long)n_seq * c.n_kv, rounds = (heads * attn_tc_tiles(c, n_heads, max_new) + sm_count() - 1) / sm_count();
+    return heads * max_new * (n_heads / c.n_kv) >= rounds * (c.J == 2 ? 6400 : c.J == 8 ? 1700 : 5400);
 }
 
 template <int DT, int J, int KB, int VB>

@@ -1,9 +1,11 @@
 """Plain 64-bit forms of the quantised cache and of attention over it, for the tests (numpy / torch fp64, written from the
-formulas and the byte layout in include/nemicli_qmv.h, sharing no code with the package)."""
+formulas and the byte layout in include/nemicli_qmv.h, sharing no arithmetic with the package)."""
 from __future__ import annotations
 
 import numpy as np
 import torch
+
+from nemicli_terminal_b200 import _lib
 
 HALF_STEP = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
 
@@ -97,6 +99,12 @@ def attention(q, k, v, pos, scale, window):
         for out, x in ((qk, k.abs()), (qt, kt)):
             out[:, h] = torch.where(seen, (q[:, h].abs() @ x[:, h // g].T) * scale, torch.zeros_like(s)).amax(1)
     return o, (mag, top, qk, qt)
+
+
+def tiled(c, heads, n_seq, max_new, dtype, width, window=0):
+    """Whether attend takes tiles of 128 rows for such a call (then one byte of workspace)."""
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    return _lib.load().qmv_kv_attend_workspace_bytes(c._ref, heads, n_seq, max_new, code, width, window) == 1
 
 
 def bound(sizes, o, dtype, keys, tiles):

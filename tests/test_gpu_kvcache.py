@@ -150,16 +150,25 @@ def filled(cuda, lens, n_kv, dim, page, kf, vf, seed=0, extra=2, poison=True):
     return c, tables, held
 
 
-def check(c, tables, held, lens, new, heads, dtype, window=0, seed=5, scale=None, tiles=False, q=None, out=None, one=False):
-    """attend for new[b] tokens of each sequence against the 64-bit form; -> the output."""
+MANY = 20000                    # query rows, and bound on a sequence's, that make any batch one for the tiles
+
+
+def check(c, tables, held, lens, new, heads, dtype, window=0, seed=5, scale=None, most=None, q=None, out=None, one=False):
+    """attend for new[b] tokens of each sequence against the 64-bit form; -> the output.  most: the bound given, and MANY
+    rows of q, which nothing covers."""
     dev = c.device
     starts = [0]
     for n in new:
         starts.append(starts[-1] + n)
     if q is None:
         q = torch.randn(starts[-1], heads, c.dim, generator=gen(seed, dev), device=dev).to(dtype)
+    if most == MANY:
+        q = torch.cat([q, q.new_full((MANY - q.shape[0], heads, c.dim), 3.0)])
+    most = most or max(new)
+    tiles = KH.tiled(c, heads, len(new), most, dtype, tables.shape[1])
+    assert tiles or most < MANY or dtype == F32
     got = c.attend(q, tables, torch.tensor(lens, dtype=torch.int32, device=dev),
-                   starts=None if one else torch.tensor(starts, dtype=torch.int32, device=dev), max_new=max(new), window=window,
+                   starts=None if one else torch.tensor(starts, dtype=torch.int32, device=dev), max_new=most, window=window,
                    scale=scale, out=out)
     for b, n in enumerate(new):
         if n == 0:
@@ -223,35 +232,39 @@ def test_few_tokens(cuda, dtype, new, window):
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("dim, n_kv, group", [(64, 2, 7), (96, 1, 3), (128, 2, 4), (256, 1, 2), (128, 3, 1), (64, 1, 32)])
 @pytest.mark.parametrize("kf, vf", [("Q4_0", "Q4_0"), ("Q8_0", "Q4_0"), ("Q4_0", "Q8_0"), ("Q8_0", "Q8_0")])
-def test_prompts(cuda, dtype, dim, n_kv, group, kf, vf):
+@pytest.mark.parametrize("most", [None, MANY])
+def test_prompts(cuda, dtype, dim, n_kv, group, kf, vf, most):
     """Prompts of unequal length behind what the cache holds already, a fresh one (all of its tokens new), a single token."""
     lens, new = [300, 65, 257, 129, 1], [100, 65, 33, 1, 1]
     c, tables, held = filled(cuda, lens, n_kv, dim, 16, kf, vf)
-    check(c, tables, held, lens, new, n_kv * group, dtype, tiles=True)
+    check(c, tables, held, lens, new, n_kv * group, dtype, most=most)
     assert _lib.device_status(device=cuda) == 0
 
 
 @pytest.mark.parametrize("window", [1, 64, 130, 4000])
 @pytest.mark.parametrize("dim", [128, 256])
-def test_prompt_windows(cuda, window, dim):
+@pytest.mark.parametrize("most", [None, MANY])
+def test_prompt_windows(cuda, window, dim, most):
     lens, new = [700, 200], [600, 200]
     c, tables, held = filled(cuda, lens, 1, dim, 64, "Q4_0", "Q4_0")
-    check(c, tables, held, lens, new, 4, BF16, window=window, tiles=True)
+    check(c, tables, held, lens, new, 4, BF16, window=window, most=most)
 
 
 @pytest.mark.parametrize("n", [17, 128, 255, 511])
-def test_prompt_lengths(cuda, n):
+@pytest.mark.parametrize("most", [None, MANY])
+def test_prompt_lengths(cuda, n, most):
     c, tables, held = filled(cuda, [n], 2, 128, 16, "Q4_0", "Q4_0")
-    check(c, tables, held, [n], [n], 2, BF16, tiles=True)
+    check(c, tables, held, [n], [n], 2, BF16, most=most)
 
 
-def test_long_prompt(cuda):
+@pytest.mark.parametrize("most", [None, MANY])
+def test_long_prompt(cuda, most):
     c, tables, held = filled(cuda, [2500], 2, 128, 64, "Q4_0", "Q4_0")
-    check(c, tables, held, [2500], [2100], 4, BF16, tiles=True)
+    check(c, tables, held, [2500], [2100], 4, BF16, most=most)
 
 
-@pytest.mark.parametrize("new", [1, 6, 90])
-def test_extreme_scores(cuda, new):
+@pytest.mark.parametrize("new, most", [(1, None), (6, None), (90, None), (90, MANY), (1, MANY)])
+def test_extreme_scores(cuda, new, most):
     """Scores far apart (one key takes all the weight), all equal (zero queries: the mean of the values), and values and
     queries of very different sizes among the heads."""
     lens = [200, 150]
@@ -262,39 +275,42 @@ def test_extreme_scores(cuda, new):
     q[:, 1] = 0
     q[:, 2] *= 1e-6
     q[:, 5] *= 1e-3
-    check(c, tables, held, lens, [new, new], 8, BF16, q=q, tiles=new > 16)
+    check(c, tables, held, lens, [new, new], 8, BF16, q=q, most=most)
 
 
-@pytest.mark.parametrize("new", [1, 5, 70])
-def test_rows_nobody_covers_and_positions_before_the_start(cuda, new):
+@pytest.mark.parametrize("new, most", [(1, 1), (5, 5), (70, 70), (70, MANY)])
+def test_rows_nobody_covers_and_positions_before_the_start(cuda, new, most):
     """Rows behind the last sequence stay as they were; more new tokens than the cache holds: those before its start see no
     key and give zeros."""
     lens = [3, 80]
     c, tables, held = filled(cuda, lens, 1, 64, 16, "Q4_0", "Q4_0")
-    q = torch.randn(2 * new + 4, 2, 64, generator=gen(2, cuda), device=cuda).bfloat16()
+    q = torch.randn(max(2 * new + 4, most), 2, 64, generator=gen(2, cuda), device=cuda).bfloat16()
+    assert KH.tiled(c, 2, 2, most, BF16, tables.shape[1]) == (most == MANY)
     out = torch.full_like(q, 7.0)
     lens_t = torch.tensor(lens, dtype=torch.int32, device=cuda)
     starts = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=cuda)
-    assert c.attend(q, tables, lens_t, starts, max_new=new, out=out) is out
+    assert c.attend(q, tables, lens_t, starts, max_new=most, out=out) is out
     assert (out[2 * new:] == 7).all()
     if new > 3:
         assert not out[:new - 3].any()
         assert out[new - 3:new].any()
     o, sizes = KH.attention(q[:new].double(), *held[0], torch.arange(3 - new, 3, device=cuda), 0.125, 0)
-    assert ((out[:new].double() - o).abs() <= KH.bound(sizes, o, BF16, 3, new > 16)).all()
+    assert ((out[:new].double() - o).abs() <= KH.bound(sizes, o, BF16, 3, most == MANY)).all()
     assert _lib.device_status(device=cuda) == 0
 
 
-@pytest.mark.parametrize("new", [1, 40])
-def test_out_of_range_on_the_device(cuda, new):
+@pytest.mark.parametrize("new, seqs", [(1, 2), (40, 2), (40, 100)])
+def test_out_of_range_on_the_device(cuda, new, seqs):
     """Pages outside the cache count as masked, lengths beyond the table are cut, runs longer than max_new are not computed
     beyond it: each sets the status, and nothing else is touched."""
-    lens = [96, 96]
+    lens = [96] * seqs                        # (100: the tiles)
+    tiles = seqs > 2
     c, tables, held = filled(cuda, lens, 1, 64, 16, "Q4_0", "Q4_0", poison=False)
     _lib.device_status(device=cuda)
-    q = torch.randn(2 * new, 2, 64, generator=gen(2, cuda), device=cuda).bfloat16()
-    starts = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=cuda)
+    q = torch.randn(seqs * new, 2, 64, generator=gen(2, cuda), device=cuda).bfloat16()
+    starts = torch.arange(seqs + 1, dtype=torch.int32, device=cuda) * new
     lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    assert KH.tiled(c, 2, seqs, new, BF16, tables.shape[1]) == KH.tiled(c, 2, seqs, max(1, new - 3), BF16, tables.shape[1]) == tiles
     want = c.attend(q, tables, lt, starts, max_new=new)
     assert _lib.device_status(device=cuda) == 0
     for wrong in (-5, c.n_pages, 2 ** 31 - 1):
@@ -306,8 +322,8 @@ def test_out_of_range_on_the_device(cuda, new):
         k, v = ([x[i] for i in range(96) if not 16 <= i < 32] for x in held[0])
         pos = torch.arange(80 - new, 80, device=cuda)
         o, sizes = KH.attention(q[:new].double(), torch.stack(k), torch.stack(v), pos, 0.125, 0)
-        assert ((got[:new].double() - o).abs() <= KH.bound(sizes, o, BF16, 96, new > 16)).all()
-    got = c.attend(q, tables, torch.tensor([96, 1000], dtype=torch.int32, device=cuda), starts, max_new=new)
+        assert ((got[:new].double() - o).abs() <= KH.bound(sizes, o, BF16, 96, tiles)).all()
+    got = c.attend(q, tables, torch.tensor([96, 1000] + lens[2:], dtype=torch.int32, device=cuda), starts, max_new=new)
     assert _lib.device_status(device=cuda) == 1
     assert torch.equal(got, want)
     if new > 1:
@@ -328,41 +344,44 @@ def test_strided_queries_scale_and_out(cuda):
     check(c, tables, held, lens, [1, 1], 8, F32, q=odd, one=True)
 
 
-@pytest.mark.parametrize("new", [1, 3, 60])
-def test_same_bits_every_time_and_on_another_stream(cuda, new):
+@pytest.mark.parametrize("new, most", [(1, 1), (3, 3), (60, 60), (60, MANY)])
+def test_same_bits_every_time_and_on_another_stream(cuda, new, most):
     lens = [5000, 777, 64]
     c, tables, _ = filled(cuda, lens, 2, 128, 64, "Q4_0", "Q4_0")
-    q = torch.randn(3 * new, 8, 128, generator=gen(6, cuda), device=cuda).bfloat16()
+    assert KH.tiled(c, 8, 3, most, BF16, tables.shape[1]) == (most == MANY)
+    q = torch.randn(max(3 * new, most), 8, 128, generator=gen(6, cuda), device=cuda).bfloat16()
     lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
     starts = torch.arange(4, dtype=torch.int32, device=cuda) * new
-    want = c.attend(q, tables, lt, starts, max_new=new)
+    attend = lambda: c.attend(q, tables, lt, starts, max_new=most)[:3 * new]      # noqa: E731
+    want = attend()
     side = torch.cuda.Stream(cuda)
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        outs = [c.attend(q, tables, lt, starts, max_new=new) for _ in range(3)]
-    here = c.attend(q, tables, lt, starts, max_new=new)           # at the same time as the side stream's
+        outs = [attend() for _ in range(3)]
+    here = attend()           # at the same time as the side stream's
     torch.cuda.current_stream().wait_stream(side)
     for o in outs + [here]:
         assert torch.equal(o, want)
 
 
-@pytest.mark.parametrize("new", [1, 30])
-def test_graph_with_growing_sequences(cuda, new):
+@pytest.mark.parametrize("new, most", [(1, 1), (30, 30), (30, MANY)])
+def test_graph_with_growing_sequences(cuda, new, most):
     """A captured write + attend, replayed as the cache grows (lengths, slots and tables change in place), two graphs in
     turn and overlapping on two streams."""
     lens = [40, 400, 63]
     c, tables, _ = filled(cuda, [n + 200 for n in lens], 2, 128, 16, "Q4_0", "Q4_0")
     lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
     starts = torch.arange(4, dtype=torch.int32, device=cuda) * new
+    assert KH.tiled(c, 8, 3, most, BF16, tables.shape[1]) == (most == MANY)
     st = []
     for i in range(2):
         g = gen(20 + i, cuda)
-        st.append([torch.randn(3 * new, h, 128, generator=g, device=cuda).bfloat16() for h in (8, 2, 2)])
+        st.append([torch.randn(n, h, 128, generator=g, device=cuda).bfloat16() for n, h in ((max(3 * new, most), 8), (3 * new, 2), (3 * new, 2))])
     slots = torch.arange(3 * new, device=cuda)
 
     def step(q, k, v):
         c.write(k, v, slots)
-        return c.attend(q, tables, lt, starts, max_new=new)
+        return c.attend(q, tables, lt, starts, max_new=most)[:3 * new]
 
     step(*st[0])
     graphs, outs = [], []
@@ -382,10 +401,10 @@ def test_graph_with_growing_sequences(cuda, new):
     # the same slots and inputs on two streams: each graph has its own workspace
     a, b = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
     with torch.cuda.graph(a):
-        oa = c.attend(st[0][0], tables, lt, starts, max_new=new)
+        oa = c.attend(st[0][0], tables, lt, starts, max_new=most)[:3 * new]
     with torch.cuda.graph(b):
-        ob = c.attend(st[1][0], tables, lt, starts, max_new=new)
-    want = [c.attend(s[0], tables, lt, starts, max_new=new) for s in st]
+        ob = c.attend(st[1][0], tables, lt, starts, max_new=most)[:3 * new]
+    want = [c.attend(s[0], tables, lt, starts, max_new=most)[:3 * new] for s in st]
     side = torch.cuda.Stream(cuda)
     torch.cuda.synchronize()
     for _ in range(5):
@@ -409,8 +428,8 @@ def test_offsets_past_32_bits(cuda):
     c.write(k, v, s)
     held = [[x.double() for x in c.read(s, F32)]]
     assert (held[0][0] - k).abs().max() < 0.05
-    for new in (1, 4, 80):
-        check(c, tables, held, [n], [new], 8, BF16, tiles=new > 16)
+    for new, most in ((1, None), (4, None), (80, MANY)):
+        check(c, tables, held, [n], [new], 8, BF16, most=most)
 
 
 def test_decoder_layer_step(cuda):
