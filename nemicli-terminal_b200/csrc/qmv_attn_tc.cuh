@@ -248,9 +248,14 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
         const int wr = 32 * (warp & 3), r0 = base + 128 * qa + wr;        // the warp's first row
         const int r = r0 + lane;
         float cs = 0.f;
-        {   // the warp's 32 rows of queries, 8 at a time (four lanes a row), to fp16 after a power of two per row
+        const int tok = r / group, head = hk * group + r - tok * group;
+        {   // The warp's 32 rows of queries, 8 at a time, to fp16 after a power of two per row.  Read by four neighbouring lanes a
+            // row (64 bytes side by side: two tiles in 6200 clocks, with eight rows in neighbouring lanes 7500; one load a piece where
+            // rows start on 16 bytes: 5000),
+            // stored by eight rows in neighbouring lanes (no two on a bank), exchanged in between.
             constexpr int kCores = D / 32;                        // 16-byte pieces a lane
-            const int g = lane & 7, c = lane >> 3;
+            const bool wide = !((reinterpret_cast<uintptr_t>(P.q) | uintptr_t(P.q_stride) * sizeof(T)) & 15u);
+            const int g = lane >> 2, c = lane & 3, from = 4 * (lane & 7) + (lane >> 3);
             constexpr int kPass = J == 8 ? 2 : 4;
             int mine = 0;                                         // exponent of row `lane`, found by lanes of pass lane / 8
 #pragma unroll 1
@@ -261,12 +266,19 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
                 for (int q = 0; q < kPass; ++q) {
                     const int rr = r0 + 8 * (q0 + q) + g;
                     const bool live = rr < rows;
-                    const T* src = static_cast<const T*>(P.q) + (live ? (S.row0 + rr / group) * P.q_stride + (hk * group + rr % group) * D : 0);
+                    const int t = __shfl_sync(0xffffffffu, tok, 8 * (q0 + q) + g), hd = __shfl_sync(0xffffffffu, head, 8 * (q0 + q) + g);
+                    const T* src = static_cast<const T*>(P.q) + (live ? (S.row0 + t) * P.q_stride + hd * D : 0);
 #pragma unroll
                     for (int i = 0; i < kCores; ++i) {                // raw bits first: every load of the warp in flight
-                        const uint2* at = reinterpret_cast<const uint2*>(src + 8 * (4 * i + c));
-                        const uint2 u = live ? __ldg(at) : make_uint2(0u, 0u), v = live ? __ldg(at + 1) : make_uint2(0u, 0u);
-                        h[q][i][0] = u.x, h[q][i][1] = u.y, h[q][i][2] = v.x, h[q][i][3] = v.y;
+                        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                        if (live && wide) {
+                            u = __ldg(reinterpret_cast<const uint4*>(src + 8 * (4 * i + c)));
+                        } else if (live) {
+                            const uint2* at = reinterpret_cast<const uint2*>(src + 8 * (4 * i + c));
+                            const uint2 a = __ldg(at), b2 = __ldg(at + 1);
+                            u = make_uint4(a.x, a.y, b2.x, b2.y);
+                        }
+                        h[q][i][0] = u.x, h[q][i][1] = u.y, h[q][i][2] = u.z, h[q][i][3] = u.w;
                     }
                 }
 #pragma unroll
@@ -279,12 +291,12 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
                             const float2 x = raw_f2<T>(h[q][i][w]);
                             top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
                         }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     const int ex = int((__float_as_uint(top) >> 23) & 255u);
                     e[q] = ex == 0 || ex == 255 ? 0 : max(-110, min(110, ex - 127 - 8));      // 2^8 <= top 2^-e < 2^9
                     const float down = __uint_as_float((uint32_t(127 - e[q]) << 23) | (P.scale < 0.f ? 0x80000000u : 0u));
-                    const int rl = wr + 8 * (q0 + q) + g;
+                    const int rl = wr + 8 * (q0 + q) + (lane & 7);
                     const uint32_t dst = sm + qa * Sh::kQ + (rl >> 3) * Sh::kSboQ + (rl & 7) * 16;
 #pragma unroll
                     for (int i = 0; i < kCores; ++i) {
@@ -292,14 +304,14 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
                             const float2 x = raw_f2<T>(h[q][i][w]);
-                            o[w] = pack_h2(x.x * down, x.y * down);
+                            o[w] = __shfl_sync(0xffffffffu, pack_h2(x.x * down, x.y * down), from);
                         }
-                        at_sts128(dst + (4 * i + c) * 128, o[0], o[1], o[2], o[3]);
+                        at_sts128(dst + (4 * i + (lane >> 3)) * 128, o[0], o[1], o[2], o[3]);
                     }
                 }
 #pragma unroll
                 for (int q = 0; q < kPass; ++q) {
-                    const int x = __shfl_sync(0xffffffffu, e[q], lane & 7);
+                    const int x = __shfl_sync(0xffffffffu, e[q], 4 * (lane & 7));
                     if (lane >> 3 == q0 + q) mine = x;
                 }
             }
@@ -310,7 +322,7 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
             cs = fmaxf(fabsf(P.scale) * 1.4426950408889634f * __uint_as_float(uint32_t(127 + mine) << 23), 1e-30f);
         }
         const uint32_t quad = tmem + (uint32_t(wr) << 16), o_at = quad + kO + qa * D;
-        const int pos = r < rows ? pos0 + r / group : -1;
+        const int pos = r < rows ? pos0 + tok : -1;
         float ref = kAttnNone, sum = 0.f;
         // keys that every row of this tile of 128 sees
         const int row_a = min(base + 128 * qa, rows - 1), row_b = min(base + 128 * qa + 127, rows - 1);
@@ -418,10 +430,11 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
             __syncwarp();
             constexpr int kPieces = D / 8;                        // of a row
             for (int i = lane; i < 32 * kPieces; i += 32) {
-                const int row = i / kPieces, piece = i - row * kPieces, rr = r0 + row;
-                if (rr >= rows) break;
+                const int row = i / kPieces, piece = i - row * kPieces;
+                const int t = __shfl_sync(0xffffffffu, tok, row), hd = __shfl_sync(0xffffffffu, head, row);
+                if (r0 + row >= rows) continue;
                 const uint4 y = lds128(stage + row * D * 2 + (D % 64 ? piece : (piece & ~7) | ((piece ^ row) & 7)) * 16);
-                T* out = static_cast<T*>(P.out) + ((long long)(S.row0 + rr / group) * P.n_heads + hk * group + rr % group) * D;
+                T* out = static_cast<T*>(P.out) + ((long long)(S.row0 + t) * P.n_heads + hd) * D;
                 reinterpret_cast<uint4*>(out)[piece] = y;
             }
         }

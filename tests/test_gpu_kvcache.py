@@ -162,7 +162,7 @@ def check(c, tables, held, lens, new, heads, dtype, window=0, seed=5, scale=None
         starts.append(starts[-1] + n)
     if q is None:
         q = torch.randn(starts[-1], heads, c.dim, generator=gen(seed, dev), device=dev).to(dtype)
-    if most == MANY:
+    if most == MANY and q.shape[0] < MANY:
         q = torch.cat([q, q.new_full((MANY - q.shape[0], heads, c.dim), 3.0)])
     most = most or max(new)
     tiles = KH.tiled(c, heads, len(new), most, dtype, tables.shape[1])
@@ -342,6 +342,17 @@ def test_strided_queries_scale_and_out(cuda):
     assert check(c, tables, held, lens, [1, 1], 8, F32, scale=0.3, q=q, out=out, one=True).data_ptr() == out.data_ptr()
     odd = torch.randn(2 * 8 * 64 + 1, generator=gen(8, cuda), device=cuda)[1:].view(2, 8, 64)     # starts off four values
     check(c, tables, held, lens, [1, 1], 8, F32, q=odd, one=True)
+
+
+@pytest.mark.parametrize("off", [4, 8])
+@pytest.mark.parametrize("dim", [96, 128, 256])
+def test_strided_queries_of_the_tiles(cuda, off, dim):
+    """Rows apart that start on 8 bytes (not 16) or on 16."""
+    lens, new = [150, 90], [70, 90]
+    c, tables, held = filled(cuda, lens, 2, dim, 16, "Q4_0", "Q8_0")
+    fused = torch.randn(MANY, 4 * dim + off + 8, generator=gen(8, cuda), device=cuda).to(F16)
+    q = fused[:, off:off + 4 * dim].unflatten(1, (4, dim))
+    check(c, tables, held, lens, new, 4, F16, q=q, most=MANY)
 
 
 @pytest.mark.parametrize("new, most", [(1, 1), (3, 3), (60, 60), (60, MANY)])
