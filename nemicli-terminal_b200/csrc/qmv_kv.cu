@@ -43,25 +43,30 @@ __device__ __forceinline__ float4 rotated(float4 x, float4 o, float4 c, float4 s
 // clamp(rint(x / d), -8, 7); Q8_0: d = fp16(max |x| / 127), codes clamp(rint(x / d), -127, 127).  The quotient is the IEEE one by
 // the rounded d, the one the reader multiplies with.  It is formed as x (1 / d) first: that is within 2^-15 of it
 // (|x / d| <= 128, the reciprocal's error and a rounding), so only where that lies within 2^-11 of a border between codes is the division made.
-__device__ __forceinline__ uint32_t quantise4(float4 x, bool q4, __half& d) {
+template <bool Q4>
+__device__ __forceinline__ uint32_t quantise4(float4 x, __half& d) {
     float v[4] = {x.x, x.y, x.z, x.w};
-    const bool odd = v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3];
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd |= !(fabsf(v[i]) <= kKvMax);
     if (__any_sync(0xffffffffu, odd)) {                           // NaN counts as 0
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = v[i] != v[i] ? 0.f : v[i];
+        for (int i = 0; i < 4; ++i) v[i] = v[i] != v[i] ? 0.f : fminf(fmaxf(v[i], -kKvMax), kKvMax);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fminf(fmaxf(v[i], -kKvMax), kKvMax);
     float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
     for (int o = 1; o < 8; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // the sign of the first value of that magnitude, from the first lane of the eight that has one
-    const float first = fabsf(v[0]) == top ? v[0] : fabsf(v[1]) == top ? v[1] : fabsf(v[2]) == top ? v[2] : v[3];
-    const int group = threadIdx.x & 24;
-    const uint32_t has = __ballot_sync(0xffffffffu, fabsf(first) == top) >> group & 255u;
-    const uint32_t minus = __ballot_sync(0xffffffffu, first < 0.f) >> group;
-    const float m = minus >> (__ffs(has) - 1) & 1u ? -top : top;
-    d = __float2half_rn(q4 ? __fmul_rn(m, -0.125f) : __fdiv_rn(top, 127.0f));
+    if constexpr (Q4) {
+        // the sign of the first value of that magnitude, from the first lane of the eight that has one
+        const float first = fabsf(v[0]) == top ? v[0] : fabsf(v[1]) == top ? v[1] : fabsf(v[2]) == top ? v[2] : v[3];
+        const int group = threadIdx.x & 24;
+        const uint32_t has = __ballot_sync(0xffffffffu, fabsf(first) == top) >> group & 255u;
+        const uint32_t minus = __ballot_sync(0xffffffffu, first < 0.f) >> group;
+        const float m = minus >> (__ffs(has) - 1) & 1u ? -top : top;
+        d = __float2half_rn(__fmul_rn(m, -0.125f));
+    } else {
+        d = __float2half_rn(__fdiv_rn(top, 127.0f));
+    }
     const float df = __half2float(d);
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(df));
@@ -79,7 +84,7 @@ __device__ __forceinline__ uint32_t quantise4(float4 x, bool q4, __half& d) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) t[i] = __fadd_rn(df == 0.f ? 0.f : __fdiv_rn(v[i], df), kRound);
     }
-    const float lo = kRound - (q4 ? 8.f : 127.f), hi = kRound + (q4 ? 7.f : 127.f);
+    const float lo = kRound - (Q4 ? 8.f : 127.f), hi = kRound + (Q4 ? 7.f : 127.f);
     uint32_t n[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) n[i] = __float_as_uint(fminf(fmaxf(t[i], lo), hi));
@@ -100,7 +105,10 @@ __device__ __forceinline__ float4 raw4(uint2 w, __half) {
 
 // A warp takes some of one row's passes of 128 consecutive values (four blocks, eight lanes each): K's, V's, then those of the
 // queries to rotate; kAhead passes' loads go out together.  Angles are the same for all of a lane's passes where a head
-// has 2 or 4 blocks.  Bound by memory for long prompts, by its launch for a decode step.
+// has 2 or 4 blocks.  The formats are template choices (tested value by value they cost 12 of 58 us).  16381 bf16 tokens of 8
+// key heads of 128 values: 46 us (50 in Q4_0), bound by the 142 instructions for four values a lane; with 32 query heads rotated
+// along 88, where the queries' part moves at 6.4 TB/s.  Five or six CTAs an SM (fewer registers) instead of four: 88 and 94.
+// A decode step is bound by its launch (64 tokens written and read, 12 us for both).
 template <int DT, int J>
 __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvWriteParams P) {
     using T = typename Elem<DT>::type;
@@ -151,9 +159,10 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     __half* s_to = P.c.sc + P.c.scale_row(page, 0, at);
 
     // passes first .. last of a section of n values at src; KIND 0: K, 1: V, 2: queries
-    auto section = [&](auto kind_c, const T* src, int n, int first, int last) {
+    auto section = [&](auto kind_c, auto q4_c, const T* src, int n, int first, int last) {
         constexpr int KIND = decltype(kind_c)::value;
-        const bool q4 = (KIND == 1 ? P.c.vb : P.c.kb) == 4, turn = KIND != 1 && ct != nullptr;
+        constexpr bool q4 = decltype(q4_c)::value;
+        const bool turn = KIND != 1 && ct != nullptr;
         auto batch = [&](int p0, auto count, bool check) {
             constexpr int A = decltype(count)::value;
             const T* at0 = src + 128 * p0 + 4 * lane;
@@ -182,7 +191,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
                     if (live) store4(static_cast<T*>(P.q_out) + (long long)row * n + off, lost ? make_float4(0.f, 0.f, 0.f, 0.f) : x);
                 } else {
                     __half d;
-                    uint32_t b = quantise4(x, q4, d);
+                    uint32_t b = quantise4<q4>(x, d);
                     b = q4 ? (b & 0x0F0F0F0Fu) ^ 0x08080808u : b ^ 0x80808080u;
                     const uint32_t head = uint32_t(off) / D, j = (uint32_t(off) - head * D) / 32;
                     if constexpr (KIND == 0) {
@@ -213,11 +222,15 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
         for (; p < last; ++p) batch(p, std::integral_constant<int, 1>{}, true);
     };
     const int q0 = part * P.per_part;
-    if (q0 < pk) section(std::integral_constant<int, 0>{}, static_cast<const T*>(P.k) + row * P.k_stride, n_kv, q0, min(p1, pk));
+    auto by_format = [&](auto kind_c, int bytes, const T* src, int first, int last) {
+        if (bytes == 4) section(kind_c, std::true_type{}, src, n_kv, first, last);
+        else section(kind_c, std::false_type{}, src, n_kv, first, last);
+    };
+    if (q0 < pk) by_format(std::integral_constant<int, 0>{}, P.c.kb, static_cast<const T*>(P.k) + row * P.k_stride, q0, min(p1, pk));
     if (q0 < 2 * pk && p1 > pk)
-        section(std::integral_constant<int, 1>{}, static_cast<const T*>(P.v) + row * P.v_stride, n_kv, max(q0 - pk, 0), min(p1 - pk, pk));
+        by_format(std::integral_constant<int, 1>{}, P.c.vb, static_cast<const T*>(P.v) + row * P.v_stride, max(q0 - pk, 0), min(p1 - pk, pk));
     if (p1 > 2 * pk)
-        section(std::integral_constant<int, 2>{}, static_cast<const T*>(P.q) + row * P.q_stride, n_q, max(q0 - 2 * pk, 0), p1 - 2 * pk);
+        section(std::integral_constant<int, 2>{}, std::false_type{}, static_cast<const T*>(P.q) + row * P.q_stride, n_q, max(q0 - 2 * pk, 0), p1 - 2 * pk);
 }
 
 struct KvReadParams {
@@ -229,7 +242,8 @@ struct KvReadParams {
     int* status;
 };
 
-// The inverse of kv_write_kernel's stores, a warp some of one row's passes: d * code, one rounded product each.
+// The inverse of kv_write_kernel's stores, a warp some of one row's passes: d * code, one rounded product each.  16381
+// tokens as above to bf16: 21 us (4.4 TB/s of codes read and values written).
 template <int DT, int J>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadParams P) {
     using T = typename Elem<DT>::type;
@@ -250,9 +264,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
     const uint8_t* k = P.c.k + P.c.k_row(page, 0, at) + (m >> 1) * J * P.c.kb;
     const uint8_t* v = P.c.v + P.c.v_pair(page, 0, at >> 1) + 2 * (at & 1) + m * J * P.c.vb;
     const __half* sc = P.c.sc + P.c.scale_row(page, 0, at);
-    auto section = [&](auto kind_c, int first, int last) {
+    auto section = [&](auto kind_c, auto q4_c, int first, int last) {
         constexpr int KIND = decltype(kind_c)::value;
-        const bool q4 = (KIND == 0 ? P.c.kb : P.c.vb) == 4;
+        constexpr bool q4 = decltype(q4_c)::value;
         T* out = static_cast<T*>(KIND == 0 ? P.k : P.v) + (long long)row * n_kv;
         auto batch = [&](int p0, auto count, bool check) {
             constexpr int A = decltype(count)::value;
@@ -293,8 +307,12 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
         for (; p < last; ++p) batch(p, std::integral_constant<int, 1>{}, true);
     };
     const int q0 = part * P.per_part;
-    if (q0 < pk) section(std::integral_constant<int, 0>{}, q0, min(p1, pk));
-    if (p1 > pk) section(std::integral_constant<int, 1>{}, max(q0 - pk, 0), p1 - pk);
+    auto by_format = [&](auto kind_c, int bytes, int first, int last) {
+        if (bytes == 4) section(kind_c, std::true_type{}, first, last);
+        else section(kind_c, std::false_type{}, first, last);
+    };
+    if (q0 < pk) by_format(std::integral_constant<int, 0>{}, P.c.kb, q0, min(p1, pk));
+    if (p1 > pk) by_format(std::integral_constant<int, 1>{}, P.c.vb, max(q0 - pk, 0), p1 - pk);
 }
 
 // Warps a row and passes a warp: rows on their own where they fill the GPU (16 warps an SM), else cut so that there are as
