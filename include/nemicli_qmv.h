@@ -341,8 +341,8 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
  * kernels, so a tight bound is the faster one; with starts null it counts as 1, for the workspace too).  Rows of out that no sequence covers stay
  * as they are.  Table entries behind a sequence's last token are not read; pages outside the cache count as
  * masked, lengths beyond the table are cut, and both set QMV_DEV_BAD_ADDRESS.  workspace: 256-byte aligned,
- * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  The result does not depend on
- * timing.  Replaces: ggufengine/mmvq.py:195-330 (attn1_teil, attn1_summe) over a quantised cache, for
+ * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  At most 2^30 rows, and 2^30 tokens a
+ * table (table_width * page).  The result does not depend on timing.  Replaces: ggufengine/mmvq.py:195-330 (attn1_teil, attn1_summe) over a quantised cache, for
  * any number of tokens. */
 int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long q_stride, int n_heads,
                   const int* tables, int table_width, const int* lens, const int* starts, int n_seq, long long n_rows,

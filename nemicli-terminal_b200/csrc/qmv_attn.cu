@@ -3,6 +3,13 @@
 
 using namespace qmv;
 
+namespace {
+constexpr int kMostKeys = 1 << 30;        // tokens a table may hold and query rows: positions, windows and tiles' ends stay in 31 bits
+bool bad_table(const KvView& c, int width, int window) { return width <= 0 || width > kMostKeys >> c.page_shift || window < 0; }
+// a window no shorter than the table is none
+int real_window(const KvView& c, int width, int window) { return window >= width << c.page_shift ? 0 : window; }
+}  // namespace
+
 extern "C" {
 
 int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, int n_seq, int max_new, int dtype,
@@ -11,7 +18,8 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
     if (kv_view(cache, c) || n_heads <= 0 || n_heads > 65535 || n_heads % c.n_kv || n_seq <= 0 || n_seq > 65535 || max_new <= 0)
         return 0;
     if (dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16) return 0;
-    if (table_width <= 0 || table_width > (0x7FFFFFFF >> c.page_shift) || window < 0) return 0;
+    if (bad_table(c, table_width, window)) return 0;
+    window = real_window(c, table_width, window);
     if (attn_tc_used(c, dtype, n_heads, n_seq, max_new)) return 1;       // no workspace
     const AttnPlan p = attn_plan(c, dtype, n_heads, n_seq, max_new, table_width, window);
     return p.grid ? p.bytes : 0;
@@ -26,10 +34,9 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
     if (st) return st;
     if (!q || !tables || !lens || !out || !workspace) return ST_NULL;
     if (dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16) return ST_BAD_SHAPE;
-    if (n_heads <= 0 || n_heads > 65535 || n_heads % P.c.n_kv || table_width <= 0 ||
-        table_width > (0x7FFFFFFF >> P.c.page_shift) || window < 0)
-        return ST_BAD_SHAPE;
-    if (n_seq <= 0 || n_seq > 65535 || n_rows < 0 || n_rows > 0x7FFFFFFFLL || max_new <= 0 || (!starts && n_rows < n_seq))
+    if (n_heads <= 0 || n_heads > 65535 || n_heads % P.c.n_kv || bad_table(P.c, table_width, window)) return ST_BAD_SHAPE;
+    window = real_window(P.c, table_width, window);
+    if (n_seq <= 0 || n_seq > 65535 || n_rows < 0 || n_rows > kMostKeys || max_new <= 0 || (!starts && n_rows < n_seq))
         return ST_BAD_TOKENS;
     if (q_stride < (long long)n_heads * P.c.dim) return ST_BAD_SHAPE;
     const uintptr_t four = 4 * elem_bytes(dtype);

@@ -6,7 +6,7 @@
 //
 // Bound by reading the cache once (4.5 or 8.5 bits a value), so what counts is instructions per value: at 6.5 TB/s an SM
 // sees about 40 four-bit values a clock.  Both products run on mma.sync m16n8k16 (fp16 in, fp32 sums) with the cache as
-// the 16-row operand, straight from global memory: the codes' bits ARE the operand.  A code c masked out of its word
+// the 16-row operand, as it lies: the codes' bits ARE the operand.  A code c masked out of its word
 // is the fp16 denormal c 2^-24 (16 c 2^-24 for the upper nibble of a byte), which the tensor cores multiply exactly, so a
 // 4-bit pair costs one AND and no conversion; the factor 2^24 and the queries' 1 / 16 are folded into constants.
 // (tcgen05 would need the unpacked values written to shared memory first, more bytes a clock than an SM writes.)  The codes'
@@ -19,7 +19,7 @@
 // is p d_v then, which keeps fp32's accuracy.  The softmax reference only moves when a score passes it by 2^4 or a d_v
 // its limit (checked with one vote a tile): p d_v 2^E stays below 2^15.  Sums and statistics are fp32.
 //
-// Work: units of 64 keys (16 a warp) of segments (sequence, key head, tile of 8 NT rows); the list of all units is cut into
+// Work: units of 64 or 128 keys (one or two tiles of 16 a warp) of segments (sequence, key head, tile of 8 NT rows); the list of all units is cut into
 // equal runs, one a CTA, so unequal lengths do not unbalance it.  A segment cut over several CTAs leaves its parts in the
 // workspace and attn_join_kernel adds them in order.
 #pragma once
@@ -51,7 +51,7 @@ struct AttnParams {
 };
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnMinKeys = 256;         // keys a CTA takes at least before segments are cut
+constexpr int kAttnMinKeys = 256;         // keys a CTA takes at least before segments are cut (128 and 512 took the same time)
 constexpr float kAttnNone = -1e30f;       // reference of a row that has seen no key
 
 __device__ __forceinline__ float ex2(float x) {
@@ -207,8 +207,10 @@ struct AttnSlot {
     }
 };
 // Tiles of 16 keys a warp works on at once (two: each instruction has another that does not wait for it, and the loop's and
-// the softmax's bookkeeping counts half), keys a unit, CTAs an SM is to hold (heads of 128 values: two, whose registers hold
-// everything; three spill, 104 us against 96 for 32 sequences of 8175 keys), and the units in a CTA's ring, within 227 KB an SM.
+// the softmax's bookkeeping counts half; 64 sequences of up to 8191 keys, 8 heads of 128: 115 us, with one 139), keys a unit, CTAs
+// an SM is to hold (heads of 64 or 96 values: three, 64 sequences of 8192 keys 104 and 130 us against 122 and 145 with two; of 128:
+// two, whose registers hold everything, three spill, 104 us against 96 for 32 sequences of 8175 keys), and the units in a
+// CTA's ring, within 227 KB an SM.
 __host__ __device__ constexpr int attn_tiles(int J, int nt) { return J < 8 && nt == 1 ? 2 : 1; }
 __host__ __device__ constexpr int attn_unit(int J, int nt) { return 16 * kAttnWarps * attn_tiles(J, nt); }
 __host__ __device__ constexpr int attn_unit_bytes(int J, int kb, int vb, int nt) {
@@ -279,7 +281,8 @@ template <int DT, int J, int KB, int VB, int NT>
 __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32, J, KB, VB, NT))) attn_kernel(const __grid_constant__ AttnParams P) {
     using T = typename Elem<DT>::type;
     // HL: queries and weights as two fp16 parts.  FAST: weights rounded to fp16 before they meet d_v, both then in fp16
-    // (two roundings of 2^-11 where the output's is 2^-8), half the instructions of the fp32 product and its rounding
+    // (two roundings of 2^-11 where the output's is 2^-8), half the instructions of the fp32 product and its rounding (64
+    // sequences: 115 us, with fp32 products 117)
     constexpr bool HL = DT == QMV_OUT_F32, FAST = DT == QMV_OUT_BF16;
     constexpr int D = 32 * J, R = 8 * NT, kParts = HL ? 2 : 1;
     constexpr float kOffK = KB == 4 ? 8.f : 128.f;
@@ -540,7 +543,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                         s_q[j][m][lane] = make_uint4(part[0][j][m][0], two ? part[1][j][m][0] : 0u, part[0][j][m][1], two ? part[1][j][m][1] : 0u);
                     const float second = NT == 2 ? start[NT - 1][j] : 0.f;
                     s_start[j][lane] = make_float4(start[0][j], start[0][j], second, second);
-                    s_one[j][lane] = make_uint4(g == j ? kOffV : 0u, 0u, g == j ? kOffV : 0u, 0u);
+                    if (!HL) s_one[j][lane] = make_uint4(g == j ? kOffV : 0u, 0u, g == j ? kOffV : 0u, 0u);
                 }
             }
             __syncthreads();
@@ -807,6 +810,13 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
             S = attn_seq(P, ++b, false, kUnit);
         }
     }
+    if (dead) {                                                   // copies of units asked for ahead may still be on their way here
+        for (int i = 0; i <= kAhead; ++i) {
+            mbar_wait(full0 + 8 * slot, phase);                   // bounded too
+            if (++slot == S_) slot = 0, phase ^= 1u;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
     if (P.split && !P.by_segment && tid == 0 && !owns) P.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
@@ -893,6 +903,8 @@ inline AttnPlan attn_plan(const KvView& c, int dtype, int n_heads, int n_seq, in
     AttnPlan p{};
     const bool hl = dtype == QMV_OUT_F32;
     const long long rows = (long long)max_new * (n_heads / c.n_kv);
+    // Two tiles of 8 rows share a cache tile's unpacked words (8 sequences of 4096 keys, 8 heads of 128: 16 rows 30 us against 33, 64
+    // rows 75 against 91); not where their sums do not fit the registers (heads of 256) or both parts of fp32 queries use the rows.
     p.nt = rows > 8 && !hl && c.J < 8 ? 2 : 1;
     p.row_tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const long long segs = (long long)n_seq * c.n_kv * p.row_tiles;

@@ -333,6 +333,19 @@ def test_out_of_range_on_the_device(cuda, new, seqs):
         assert (out[new - 3:new] == 7).all() and not (out[:new - 3] == 7).all()
 
 
+@pytest.mark.parametrize("new", [5, 70])
+def test_window_of_any_size(cuda, new):
+    """A window as long as an int holds is none, for queries before the sequence's start too."""
+    c, tables, _ = filled(cuda, [3, 80], 1, 64, 16, "Q4_0", "Q4_0")
+    lens = torch.tensor([3, 80], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, new, 2 * new], dtype=torch.int32, device=cuda)
+    for rows in (2 * new, MANY):
+        q = torch.randn(rows, 2, 64, generator=gen(4, cuda), device=cuda).bfloat16()
+        want = c.attend(q, tables, lens, starts, max_new=rows)[:2 * new]
+        for window in (10 ** 6, 2 ** 31 - 1, 2 ** 40):
+            assert torch.equal(c.attend(q, tables, lens, starts, max_new=rows, window=window)[:2 * new], want)
+
+
 def test_strided_queries_scale_and_out(cuda):
     lens = [50, 77]
     c, tables, held = filled(cuda, lens, 2, 64, 16, "Q8_0", "Q4_0")
