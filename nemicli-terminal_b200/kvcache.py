@@ -101,8 +101,12 @@ class KVCache:
 
     def _index(self, t: torch.Tensor, what: str, dtype, *shape):
         got = t.shape
-        if t.device != self.device or t.dtype != dtype or len(got) != len(shape) or not t.is_contiguous() \
-                or any(want is not None and n != want for n, want in zip(got, shape)):
+        ok = t.device == self.device and t.dtype == dtype and len(got) == len(shape) and t.is_contiguous()
+        if ok:
+            for n, want in zip(got, shape):
+                if want is not None and n != want:
+                    ok = False
+        if not ok:
             raise RuntimeError(f"{what}: contiguous {dtype} {shape} on {self.device} expected, got {t.dtype} {tuple(got)}")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, q: Optional[torch.Tensor] = None, rope=None,
@@ -150,7 +154,7 @@ class KVCache:
         if dtype not in _DTYPES:
             raise RuntimeError(f"KVCache.read: dtype {dtype} (float32, bfloat16 or float16)")
         rows = slots.shape[0]
-        k, v = torch.empty((2, rows, self.n_kv, self.dim), dtype=dtype, device=self.device).unbind(0)
+        k, v = (self.scales.new_empty((rows, self.n_kv, self.dim), dtype=dtype) for _ in range(2))
         if rows:
             with _lib.on_device(self.device):
                 st = _lib.load().qmv_kv_read(self._ref, slots.data_ptr(), rows, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],

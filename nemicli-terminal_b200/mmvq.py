@@ -449,22 +449,23 @@ def norm_block(y: torch.Tensor, h: torch.Tensor, w_pre: Optional[torch.Tensor], 
     rounded once.  eingang (n a multiple of 32): also the int8 activation input of the fp32 x, as norm_q8
     gives it, for M rows.  New entry point: norm_q8 takes one row and has no norm behind the block."""
     _need_cuda(y, "norm_block")
-    if y.dtype not in _OUT or y.dim() not in (1, 2) or y.shape[-1] == 0:
+    shape, dtype, device = y.shape, y.dtype, y.device
+    if dtype not in _OUT or len(shape) not in (1, 2) or shape[-1] == 0:
         raise RuntimeError("norm_block: y (n,) or (M, n) of float32, bfloat16 or float16")
-    n = y.shape[-1]
-    if h.shape != y.shape or h.dtype != y.dtype or h.device != y.device:
-        raise RuntimeError(f"norm_block: h must be like y ({tuple(y.shape)}, {y.dtype}, {y.device})")
-    if gate is not None and (gate.shape not in (y.shape, (n,)) or gate.dtype != y.dtype or gate.device != y.device):
-        raise RuntimeError(f"norm_block: gate must be ({n},) or like y, of {y.dtype}")
+    n = shape[-1]
+    if h.shape != shape or h.dtype != dtype or h.device != device:
+        raise RuntimeError(f"norm_block: h must be like y ({tuple(shape)}, {dtype}, {device})")
+    if gate is not None and (gate.shape not in (shape, (n,)) or gate.dtype != dtype or gate.device != device):
+        raise RuntimeError(f"norm_block: gate must be ({n},) or like y, of {dtype}")
     for w in (w_post, w_pre):
-        if w is not None and (w.dtype != torch.float32 or w.shape != (n,) or not w.is_contiguous() or w.device != y.device):
-            raise RuntimeError(f"norm_block: norm weights are contiguous float32 ({n},) on {y.device}")
+        if w is not None and (w.dtype != torch.float32 or w.shape != (n,) or not w.is_contiguous() or w.device != device):
+            raise RuntimeError(f"norm_block: norm weights are contiguous float32 ({n},) on {device}")
     if eingang and (w_pre is None or n % 32):
         raise RuntimeError("norm_block: an Eingang needs w_pre and n a multiple of 32")
     if n > NORM_BLOCK_MAX:
         raise RuntimeError(f"norm_block: rows of at most {NORM_BLOCK_MAX} values (got {n})")
 
-    M = 1 if y.dim() == 1 else y.shape[0]
+    M = 1 if len(shape) == 1 else shape[0]
 
     def rows(t):                          # the values of a row side by side, and the values between rows
         if t.is_contiguous():
@@ -476,16 +477,16 @@ def norm_block(y: torch.Tensor, h: torch.Tensor, w_pre: Optional[torch.Tensor], 
     y2, ys = rows(y)
     h2, hs = rows(h)
     g2, gs = (None, 0) if gate is None else rows(gate)
-    if gate is not None and gate.dim() < y.dim():
+    if gate is not None and gate.dim() < len(shape):
         gs = 0
     x = None if w_pre is None else torch.empty_like(y, memory_format=torch.contiguous_format)
     new = torch.empty_like(y, memory_format=torch.contiguous_format)
-    e = Eingang(n=M * n, device=y.device) if eingang else None
+    e = Eingang(n=M * n, device=device) if eingang else None
     if M:
-        with _lib.on_device(y.device):
+        with _lib.on_device(device):
             st = _lib.load().qmv_norm_block(y2.data_ptr(), ys, h2.data_ptr(), hs, _lib.addr(g2), gs, _lib.addr(w_post),
-                                            _lib.addr(w_pre), _OUT[y.dtype], eps, rs, M, n, new.data_ptr(), _lib.addr(x),
-                                            *(e.zeiger() if e else (0, 0, 0, 0)), _lib.stream_of(y.device))
+                                            _lib.addr(w_pre), _OUT[dtype], eps, rs, M, n, new.data_ptr(), _lib.addr(x),
+                                            *(e.zeiger() if e else (0, 0, 0, 0)), _lib.stream_of(device))
         if st:
             _lib.check(st, "qmv_norm_block")
     return x, e, new
