@@ -291,7 +291,7 @@ int qmv_chain_noalloc(const qmv_stage* stages, int n_stages, void* stream);
  *   scales  n_pages * n_kv * P * 2 * J fp16            [page][head][P][2][J]: K's, then V's
  * In a Q4_0 K word value n sits at bit 16 (n & 1) + 4 (n >> 1), in a V word at bit 16 (token & 1) + 4 n; in the two
  * Q8_0 K words in word n >> 2 at byte 2 (n & 1) + ((n & 3) >> 1), in the V words in word n >> 1 at byte
- * 2 (token & 1) + (n & 1).  All three 16-byte aligned.  n_pages * P at most 2^40. */
+ * 2 (token & 1) + (n & 1).  All three 16-byte aligned.  n_pages * P at most 2^40, n_kv * dim * P at most 2^30. */
 typedef struct qmv_kv_cache {
     void* k;
     void* v;

@@ -219,6 +219,33 @@ def test_one_token_many_short_sequences(cuda):
     check(c, tables, held, lens, [1] * 300, 4, F32, one=True)
 
 
+@pytest.mark.parametrize("n_seq", [127, 128, 129, 300])
+def test_many_sequences_cut_over_the_gpu(cuda, n_seq):
+    """More sequences than a CTA has threads, lengths long enough to be cut between CTAs, some empty or without new tokens."""
+    lens = [(397 * b) % 1500 * (b % 7 > 0) for b in range(n_seq)]
+    c, tables, held = filled(cuda, lens, 1, 64, 16, "Q4_0", "Q4_0")
+    check(c, tables, held, lens, [1] * n_seq, 4, BF16, one=True)
+    new = [b % 3 if n > 2 else 0 for b, n in enumerate(lens)]
+    check(c, tables, held, lens, new, 4, BF16)
+
+
+@pytest.mark.parametrize("most", [3, MANY])
+def test_rows_between_sequences(cuda, most):
+    """Rows before the first sequence's stay as they were, and a sequence without new tokens writes none."""
+    lens = [40, 200, 33]
+    c, tables, held = filled(cuda, lens, 2, 128, 16, "Q8_0", "Q4_0")
+    q = torch.randn(max(most, 12), 8, 128, generator=gen(3, cuda), device=cuda).bfloat16()
+    out = torch.full_like(q, 7.0)
+    starts = torch.tensor([4, 7, 7, 9], dtype=torch.int32, device=cuda)
+    c.attend(q, tables, torch.tensor(lens, dtype=torch.int32, device=cuda), starts, max_new=most, out=out)
+    assert (out[:4] == 7).all() and (out[9:] == 7).all()
+    for b, rows in ((0, slice(4, 7)), (2, slice(7, 9))):
+        n = rows.stop - rows.start
+        o, sizes = KH.attention(q[rows].double(), *held[b], torch.arange(lens[b] - n, lens[b], device=cuda), 128 ** -0.5, 0)
+        assert ((out[rows].double() - o).abs() <= KH.bound(sizes, o, BF16, lens[b], most == MANY)).all()
+    assert _lib.device_status(device=cuda) == 0
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("new", [[2, 3, 1, 5], [16, 16, 16, 16], [4, 0, 9, 1]])
 @pytest.mark.parametrize("window", [0, 7])
