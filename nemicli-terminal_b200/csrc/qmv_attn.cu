@@ -20,7 +20,8 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
     if (dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16) return 0;
     if (bad_table(c, table_width, window)) return 0;
     window = real_window(c, table_width, window);
-    if (attn_tc_used(c, dtype, n_heads, n_seq, max_new)) return 1;       // no workspace
+    const AttnTcPlan tc = attn_tc_plan(c, dtype, n_heads, n_seq, max_new, table_width, window);
+    if (tc.used) return tc.grid > 0x7FFFFFFF ? 0 : tc.bytes + 1;      // (no workspace: one byte)
     const AttnPlan p = attn_plan(c, dtype, n_heads, n_seq, max_new, table_width, window);
     return p.grid ? p.bytes : 0;
 }
@@ -44,10 +45,9 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
         !aligned(starts, 4) || !aligned(workspace, 256))
         return ST_BAD_ALIGN;
     if (!starts) max_new = 1;
-    const bool tiles = attn_tc_used(P.c, dtype, n_heads, n_seq, max_new);
+    const AttnTcPlan tc = attn_tc_plan(P.c, dtype, n_heads, n_seq, max_new, table_width, window);
     const AttnPlan pl = attn_plan(P.c, dtype, n_heads, n_seq, max_new, table_width, window);
-    if (tiles ? (long long)attn_tc_tiles(P.c, n_heads, max_new) * P.c.n_kv * n_seq > 0x7FFFFFFF : !pl.grid || workspace_bytes < pl.bytes)
-        return ST_BAD_SHAPE;
+    if (tc.used ? tc.grid > 0x7FFFFFFF || workspace_bytes < tc.bytes : !pl.grid || workspace_bytes < pl.bytes) return ST_BAD_SHAPE;
     if (n_rows == 0) return ST_OK;
     P.q = q, P.q_stride = q_stride, P.out = out;
     P.tables = tables, P.lens = lens, P.starts = starts;
@@ -58,8 +58,8 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
     P.desc = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + pl.part_bytes);
     P.status = device_status_ptr();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tiles) {
-        P.row_tiles = attn_tc_tiles(P.c, n_heads, max_new);
+    if (tc.used) {
+        P.row_tiles = tc.row_tiles, P.split = tc.split;
         switch (P.c.J) {
         case 2: return attn_tc_dispatch<2>(P, dtype, s);
         case 3: return attn_tc_dispatch<3>(P, dtype, s);

@@ -42,6 +42,7 @@ template <int J> struct AttnTcShape {
     static constexpr int kOffBar = kOffSV + 4 * kScaleV;          // mbarriers, the tensor-memory address
     static constexpr int kOffBad = kOffBar + 256;                 // [4][4] words: keys whose page is not of the cache
     static constexpr int kSmem = kOffBad + 64;
+    static constexpr int kPart = (D + 2) * 128 * NQ;              // floats of a CTA's part: [D / 4][rows][4], references, weights
     static constexpr uint32_t kSboQ = D * 16, kSboK = D * 16, kSboV = BN * 16;    // bytes between 8-row groups
 };
 
@@ -205,6 +206,8 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = P.n_heads / P.c.n_kv;
     int x = blockIdx.x;
+    const int sp = x % P.split;                                   // of the tile's keys
+    x /= P.split;
     const int hk = x % P.c.n_kv;
     x /= P.c.n_kv;
     const int qt = P.row_tiles - 1 - x % P.row_tiles, b = x / P.row_tiles;        // the tiles with most keys first
@@ -214,7 +217,11 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
     const int pos0 = S.len - S.n, tok0 = base / group, tok1 = (min(base + 128 * NQ, rows) - 1) / group;
     const int last = min(pos0 + tok1, S.len - 1);
     const int first = P.window > 0 ? max(0, pos0 + tok0 - P.window + 1) : 0;
-    const int kt0 = first / BN, n_tiles = last < first ? 0 : last / BN - kt0 + 1;
+    int kt0 = first / BN, n_tiles = last < first ? 0 : last / BN - kt0 + 1;
+    if (P.split > 1) {                                            // steps of this CTA
+        const int per = (n_tiles + P.split - 1) / P.split;
+        kt0 += sp * per, n_tiles = max(0, min(per, n_tiles - sp * per));
+    }
 
     const uint32_t sm = smem_u32(tc_smem_);
     const uint32_t bar = sm + Sh::kOffBar;                        // stages: up to four each; S and P: two buffers a query tile
@@ -409,7 +416,22 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
         // an order that keeps lanes on different banks, and from there whole rows at a time
         const float inv = sum > 0.f ? __fdividef(1.f, sum) : sum == sum ? 0.f : sum;
         const uint32_t stage = sm + qa * Sh::kQ + wr * D * 2;
-        if (ok) {
+        if (ok && P.split > 1) {                                  // sums, reference and weight for attn_tc_join_kernel
+            float* part = P.parts + (long long)blockIdx.x * Sh::kPart + 128 * qa + wr + lane;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+                uint32_t y[16] = {};
+                if (n_tiles) {
+                    at_ld16(o_at + c, y);
+                    at_wait_ld();
+                }
+                float4* to = reinterpret_cast<float4*>(P.parts + (long long)blockIdx.x * Sh::kPart) + c / 4 * (128 * NQ) + 128 * qa + wr + lane;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (r < rows) to[k * 128 * NQ] = make_float4(__uint_as_float(y[4 * k]), __uint_as_float(y[4 * k + 1]), __uint_as_float(y[4 * k + 2]), __uint_as_float(y[4 * k + 3]));
+            }
+            part[D * 128 * NQ] = ref, part[(D + 1) * 128 * NQ] = sum;
+        } else if (ok) {
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 uint32_t y[32];
@@ -651,25 +673,71 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
 }
 
+// Joins the parts of tiles whose keys were cut: block (32 rows and 32 of their values, key head, sequence), a lane a row, a warp four
+// values.
+template <int DT, int J>
+__global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant__ AttnParams P) {
+    using T = typename Elem<DT>::type;
+    using Sh = AttnTcShape<J>;
+    constexpr int R = 128 * Sh::NQ, D = Sh::D;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int b = blockIdx.z, hk = blockIdx.y, group = P.n_heads / P.c.n_kv, lane = threadIdx.x & 31;
+    const int c = blockIdx.x % J * 8 + (threadIdx.x >> 5);        // values 4 c ..
+    const AttnSeq S = attn_seq(P, b, false, Sh::BN);
+    const int rows = min(S.n, P.max_new) * group, r = 32 * int(blockIdx.x / J) + lane, qt = r / R, at = r % R;
+    if (r >= rows) return;
+    const float* part = P.parts + ((long long)(b * P.row_tiles + P.row_tiles - 1 - qt) * P.c.n_kv + hk) * P.split * Sh::kPart;
+    float ref = kAttnNone, sum = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < P.split; ++k) ref = fmaxf(ref, part[(long long)k * Sh::kPart + D * R + at]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < P.split; ++k) {
+        const float* p = part + (long long)k * Sh::kPart;
+        const float w = ex2(p[D * R + at] - ref);
+        const float4 y = reinterpret_cast<const float4*>(p)[c * R + at];
+        sum = fmaf(w, p[(D + 1) * R + at], sum);
+        o = make_float4(fmaf(w, y.x, o.x), fmaf(w, y.y, o.y), fmaf(w, y.z, o.z), fmaf(w, y.w, o.w));
+    }
+    const float inv = sum > 0.f ? __fdividef(1.f, sum) : sum == sum ? 0.f : sum;
+    T* out = static_cast<T*>(P.out) + ((long long)(S.row0 + r / group) * P.n_heads + hk * group + r % group) * D + 4 * c;
+    store4(out, inv != 0.f ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
+}
+
 // ---- host -------------------------------------------------------------------------------------------
 
-
-inline int attn_tc_tiles(const KvView& c, int n_heads, int max_new) {
-    const long long rows = (long long)max_new * (n_heads / c.n_kv);
+// Whether a call takes the tiles (else attn_kernel), and how.  A tile walks its keys at a cost that its rows do not change, one
+// CTA an SM: 14.5 ns a key for heads of 64 values, 17.8 for 128, 18.5 for 256.  attn_kernel spreads any work over the GPU, at
+// a cost that goes with the rows: 2.3, 3.3 and 11 ps a key and row.  So the tiles gain from as many rows a round of CTAs as
+// the ratio of the two.  Where the tiles fill at most half the SMs and there are keys enough to pay for a second launch
+// (512 a part: 9 us of work, the launch 4 to 5), each one's keys are cut into as many parts as fill the GPU, and
+// attn_tc_join_kernel adds them.  Measured in us, cut / uncut / attn_kernel, heads of 128 values, 8 key heads, 4 query heads each:
+//   1 sequence of 32768 keys, 16 new tokens: 49 / 584 / 68      64 tokens: 52 / 586 / 228
+//   8 sequences of 4096 keys, 16 tokens: 47 / 80 / 75           64 tokens: 53 / 82 / 250
+//   1 sequence of 4096 keys, 16 tokens: not used, 22            64 tokens: 22 / 81 / 44
+//   32 sequences of 1024 keys, 24 tokens: - / 51 / 126
+// and 4 key heads of 256 values, 8 sequences of 4096 keys, 4 tokens: 32 / 85 / 38
+struct AttnTcPlan {
+    bool used;
+    int row_tiles, split;
+    long long grid, bytes;                                        // workspace: the parts
+};
+inline AttnTcPlan attn_tc_plan(const KvView& c, int dtype, int n_heads, int n_seq, int max_new, int width, int window) {
+    AttnTcPlan p{};
+    if (dtype == QMV_OUT_F32) return p;                           // fp16 products lack its accuracy
     const int per = c.J == 8 ? 128 : 256;
-    return int((rows + per - 1) / per);
-}
-// Whether the tiles are used (else attn_kernel).  A tile walks all its keys at a cost that its rows do not change, one CTA an
-// SM: 14.5 ns a key for heads of 64 values, 17.8 for 128, 18.5 for 256.  attn_kernel spreads any work over the GPU, at a cost
-// that goes with the rows: 2.3, 3.3 and 11 ps a key and row.  So the tiles gain from as many rows a round of CTAs as the
-// ratio of the two.  Measured in us, tiles / attn_kernel, heads of 128 values, 8 key heads, 4 query heads each:
-//   1 sequence of 32768 keys, 16 new tokens (512 rows): 584 / 68     64 tokens (2048 rows): 586 / 229
-//   8 sequences of 4096 keys, 16 tokens (4096 rows): 80 / 75         24 tokens (6144 rows): 80.5 / 107
-//   and 4 key heads of 256 values, 8 x 4096 keys, 8 tokens (1024 rows): 86 / 63      16 tokens (2048 rows): 86 / 112
-inline bool attn_tc_used(const KvView& c, int dtype, int n_heads, int n_seq, int max_new) {
-    if (dtype == QMV_OUT_F32) return false;                       // fp16 products lack its accuracy
-    const long long heads = (long long)n_seq * c.n_kv, rounds = (heads * attn_tc_tiles(c, n_heads, max_new) + sm_count() - 1) / sm_count();
-    return heads * max_new * (n_heads / c.n_kv) >= rounds * (c.J == 2 ? 6400 : c.J == 8 ? 1700 : 5400);
+    const long long rows = (long long)max_new * (n_heads / c.n_kv), heads = (long long)n_seq * c.n_kv, tiles = (rows + per - 1) / per;
+    long long keys = (long long)width << c.page_shift;
+    if (window > 0) keys = std::min<long long>(keys, (long long)window + max_new);
+    p.split = int(std::max<long long>(1, std::min<long long>(sm_count() / std::min<long long>(heads * tiles, sm_count()), keys / 512)));
+    const long long rounds = (heads * tiles + sm_count() - 1) / sm_count();
+    p.used = heads * rows >= rounds * (c.J == 2 ? 6400 : c.J == 8 ? 1700 : 5400) / p.split;
+    p.grid = heads * tiles * p.split;
+    if (tiles > INT_MAX) p.grid = LLONG_MAX;                      // refused
+    p.row_tiles = int(std::min<long long>(tiles, INT_MAX));
+    p.bytes = p.split > 1 ? p.grid * (c.dim + 2) * per * 4 : 0;
+    return p;
 }
 
 template <int DT, int J, int KB, int VB>
@@ -677,7 +745,19 @@ int attn_tc_go(const AttnParams& P, cudaStream_t st) {
     using Sh = AttnTcShape<J>;
     static SmemGrant grant;
     if (const int e = grant(attn_tc_kernel<DT, J, KB, VB>, Sh::kSmem)) return e;
-    return launch_pdl_smem(attn_tc_kernel<DT, J, KB, VB>, dim3(P.row_tiles * P.c.n_kv * P.n_seq), dim3(Sh::kThreads), Sh::kSmem, st, P);
+    const int rc = launch_pdl_smem(attn_tc_kernel<DT, J, KB, VB>, dim3(P.row_tiles * P.c.n_kv * P.n_seq * P.split), dim3(Sh::kThreads), Sh::kSmem, st, P);
+    if (rc || P.split == 1) return rc;
+    cudaLaunchConfig_t cfg = {};                                  // may start while the last parts are written
+    cfg.gridDim = dim3(P.row_tiles * Sh::NQ * 4 * J, P.c.n_kv, P.n_seq);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, attn_tc_join_kernel<DT, J>, P);
+    return launched();
 }
 
 template <int J>

@@ -102,9 +102,9 @@ def attention(q, k, v, pos, scale, window):
 
 
 def tiled(c, heads, n_seq, max_new, dtype, width, window=0):
-    """Whether attend takes tiles of 128 rows for such a call (then one byte of workspace)."""
+    """Whether attend takes tiles of 128 rows for such a call: its workspace then has an odd number of bytes."""
     code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
-    return _lib.load().qmv_kv_attend_workspace_bytes(c._ref, heads, n_seq, max_new, code, width, window) == 1
+    return _lib.load().qmv_kv_attend_workspace_bytes(c._ref, heads, n_seq, max_new, code, width, window) % 2 == 1
 
 
 def bound(sizes, o, dtype, keys, tiles):

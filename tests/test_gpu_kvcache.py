@@ -290,6 +290,45 @@ def test_long_prompt(cuda, most):
     check(c, tables, held, [2500], [2100], 4, BF16, most=most)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim, n_kv, group", [(64, 2, 8), (96, 3, 3), (128, 2, 4), (256, 1, 5)])
+@pytest.mark.parametrize("window", [0, 700, 1500])
+def test_tiles_with_keys_cut(cuda, dtype, dim, n_kv, group, window):
+    """Few tiles with many keys: each tile's keys are cut over several CTAs; lengths that leave some of them no key."""
+    lens, new = [5000, 1, 2049, 130, 0, 700], [120, 1, 97, 130, 0, 3]
+    c, tables, held = filled(cuda, lens, n_kv, dim, 16, "Q4_0", "Q8_0")
+    assert KH.tiled(c, n_kv * group, 6, 130, dtype, tables.shape[1])
+    cut = _lib.load().qmv_kv_attend_workspace_bytes(c._ref, n_kv * group, 6, 130, 1, tables.shape[1], window) > 1
+    assert cut == (window != 700)             # too few keys to cut
+    check(c, tables, held, lens, new, n_kv * group, dtype, window=window)
+    assert _lib.device_status(device=cuda) == 0
+
+
+def test_tiles_with_keys_cut_from_graphs(cuda):
+    """Two captured calls with cut keys replayed at the same time: each has its own parts."""
+    lens, new = [5000, 3000], [60, 64]
+    c, tables, _ = filled(cuda, lens, 2, 128, 64, "Q4_0", "Q4_0")
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, 60, 124], dtype=torch.int32, device=cuda)
+    assert KH.tiled(c, 8, 2, 64, BF16, tables.shape[1])
+    qs = [torch.randn(124, 8, 128, generator=gen(30 + i, cuda), device=cuda).bfloat16() for i in range(2)]
+    want = [c.attend(q, tables, lt, starts, max_new=64) for q in qs]
+    graphs, outs = [], []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(c.attend(q, tables, lt, starts, max_new=64))
+        graphs.append(g)
+    side = torch.cuda.Stream(cuda)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
 @pytest.mark.parametrize("new, most", [(1, None), (6, None), (90, None), (90, MANY), (1, MANY)])
 def test_extreme_scores(cuda, new, most):
     """Scores far apart (one key takes all the weight), all equal (zero queries: the mean of the values), and values and
@@ -399,7 +438,7 @@ def test_strided_queries_of_the_tiles(cuda, off, dim):
 def test_same_bits_every_time_and_on_another_stream(cuda, new, most):
     lens = [5000, 777, 64]
     c, tables, _ = filled(cuda, lens, 2, 128, 64, "Q4_0", "Q4_0")
-    assert KH.tiled(c, 8, 3, most, BF16, tables.shape[1]) == (most == MANY)
+    assert KH.tiled(c, 8, 3, most, BF16, tables.shape[1]) == (new == 60)      # (60, 60): keys cut over the GPU
     q = torch.randn(max(3 * new, most), 8, 128, generator=gen(6, cuda), device=cuda).bfloat16()
     lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
     starts = torch.arange(4, dtype=torch.int32, device=cuda) * new
