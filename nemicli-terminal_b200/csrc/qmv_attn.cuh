@@ -42,9 +42,9 @@ struct AttnParams {
     int width, n_seq, n_heads, n_rows, max_new, window;
     float scale;
     int row_tiles;                        // tiles of query rows (token-major over the heads of a key head)
-    int split;                            // segments may be cut: parts, desc, attn_join_kernel follows
+    int split;                            // segments may be cut: parts, desc, attn_join_kernel follows (attn_tc_kernel: parts of a tile's keys)
     int by_segment;                       // desc has an entry a segment (else a CTA)
-    float* parts;                         // [2 a CTA][8 NT rows][dim + 2]: sums, then reference and weight
+    float* parts;                         // [2 a CTA][8 NT rows][dim + 2]: sums, then reference and weight (attn_tc_kernel: its kPart a CTA)
     int4* desc;                           // two an entry: first part's CTA, parts (0: nothing to join), sequence's first row, key head;
                                           // first of the tile's rows, rows
     int* status;

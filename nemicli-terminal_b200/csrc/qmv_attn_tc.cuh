@@ -4,9 +4,11 @@
 //   S = Q K^T,  P = 2^(S scale log2 e - ref),  O += P V,  l += sum P   per tile of BN keys, then O / l
 //
 // A CTA takes NQ tiles of 128 query rows of one sequence and key head (row = token * group + head of the group, so
-// the cache is unpacked once for the whole group) over all their keys.  For two tiles, 64 keys and 128 values a step of both
-// takes 2048 clocks of exp2 (16 a clock and SM) and 2048 of MMA (both products), which run side by side; measured about 2200
-// (8192 tokens, 32 heads: 0.58 to 0.61 ms, 900 TFLOP/s).  Roles:
+// the cache is unpacked once for the whole group) over all their keys.  For two tiles, 64 keys and 128 values a step takes
+// 1024 clocks of MMA (both products), 1024 of exp2 (16 a clock and SM) and about 1540 of shared memory (the operands of the
+// scores, queries among them, 768; V 512; the producers' stores 256), all side by side; measured about 2200 (8192 tokens, 32 heads:
+// 0.58 to 0.61 ms, 900 TFLOP/s), the MMAs' issue waiting for their operands.  Scores of 128 keys at a time would read the
+// queries half as often, but two buffers of them do not fit tensor memory beside the sums.  Roles:
 //   producers  NP x 4 warps: words of the cache -> d * code in fp16 (one rounding) -> shared memory, in the MMA's K-major core
 //              matrices (8 rows x 16 bytes; K: rows = keys, V: rows = values of the head, so a V word, whose halves
 //              are two tokens, lands transposed without a shuffle).  Loads one round ahead in registers, page numbers two.
@@ -17,7 +19,7 @@
 //   softmax    NQ x 4 warps, one thread a row: scores from tensor memory, P as fp16 over them, and the row's
 //              reference, sum and mask in registers.  The reference moves only when the row's maximum passes it by 2^8;
 //              then the warp rescales its rows of O in tensor memory.
-// A quarter of the exponentials as a cubic on the other units gained nothing (595 us without, 610 with it).
+// The exponentials are not the bound: a quarter of them as a cubic on the other units gained nothing (595 us without, 610 with it).
 // Queries are fp16 after a power of two per row (exact but for values 2^-32 below the row's largest).  Tensor memory:
 // S NQ x 2 x BN columns, O NQ x D columns.  Every mbarrier wait is bounded; on expiry the CTA sets DEV_TIMEOUT, waits
 // (bounded) for its MMAs, frees its tensor memory and leaves.

@@ -66,6 +66,12 @@ def test_attend_refusals(bad, status):
     assert attend(**bad) == status
 
 
+def test_attend_refuses_a_short_workspace_for_cut_tiles():
+    need = _lib.load().qmv_kv_attend_workspace_bytes(cache(), 4, 1, 2000, 1, 1000, 0)
+    assert need % 2 == 1 and need > 1
+    assert attend(dtype=1, new=2000, rows=2000, width=1000, nbytes=need - 2) == 2
+
+
 def test_attend_of_no_rows_is_no_launch():
     assert attend(rows=0) == 0
 
