@@ -170,7 +170,8 @@ class KVCache:
         reads key head h // (heads // n_kv)); tables int32 (sequences, width): the pages of each sequence in order;
         lens int32 (sequences,): its tokens in the cache, the new ones among them (write comes first).  One row a
         sequence, or with starts int32 (sequences + 1,) rows starts[b] .. starts[b + 1] for sequence b, its last tokens;
-        max_new: at least the most new tokens of a sequence (default: all rows).  scale: default dim ** -0.5.  window: a
+        max_new: at least the most new tokens of a sequence (default: all rows; it chooses between two kernels, so a
+        tight bound is the faster one).  scale: default dim ** -0.5.  window: a
         query sees that many keys up to its own (0: all).  -> like q, rows side by side; in `out` (contiguous) if
         given; rows that no sequence covers keep what out held (without `out` they are undefined).  Queries that
         see no key give zeros.  float32 queries are computed to float32's precision."""
