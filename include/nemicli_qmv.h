@@ -340,7 +340,8 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
  * tokens (rows beyond it are not computed, QMV_DEV_BAD_ADDRESS is set; n_seq * max_new also decides between two
  * kernels, so a tight bound is the faster one; with starts null it counts as 1, for the workspace too).  Rows of out that no sequence covers stay
  * as they are.  Table entries behind a sequence's last token are not read; pages outside the cache count as
- * masked, lengths beyond the table are cut, and both set QMV_DEV_BAD_ADDRESS.  workspace: 256-byte aligned,
+ * masked, lengths beyond the table are cut, and both set QMV_DEV_BAD_ADDRESS.  Held values beyond +-65504 (a Q8_0 block
+ * of clamped values holds 65532) may count as +-65504.  workspace: 256-byte aligned,
  * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  At most 2^30 rows, and 2^30 tokens a
  * table (table_width * page).  The result does not depend on timing.  Replaces: ggufengine/mmvq.py:195-330 (attn1_teil, attn1_summe) over a quantised cache, for
  * any number of tokens. */

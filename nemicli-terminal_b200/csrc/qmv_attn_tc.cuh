@@ -43,7 +43,8 @@ template <int J> struct AttnTcShape {
     static constexpr int kOffK = NQ * kQ, kOffV = kOffK + KS * kK, kOffSK = kOffV + KS * kV, kOffSV = kOffSK + 2 * kScaleK;
     static constexpr int kOffBar = kOffSV + 4 * kScaleV;          // mbarriers, the tensor-memory address
     static constexpr int kOffBad = kOffBar + 256;                 // [4][4] words: keys whose page is not of the cache
-    static constexpr int kSmem = kOffBad + 64;
+    static constexpr int kOffBig = kOffBad + 64;                  // [4][4] words: bit 0 a large K scale among the warp's keys, bit 1 V
+    static constexpr int kSmem = kOffBig + 64;
     static constexpr int kPart = (D + 2) * 128 * NQ;              // floats of a CTA's part: [D / 4][rows][4], references, weights
     static constexpr uint32_t kSboQ = D * 16, kSboK = D * 16, kSboV = BN * 16;    // bytes between 8-row groups
 };
@@ -165,6 +166,18 @@ __device__ __forceinline__ void at_ldg(uint32_t* w, const uint8_t* p) {
         for (int i = 0; i < N; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p + 4 * i));
     }
 }
+
+// d * code stays within fp16: Q8_0's clamped values are 127 times fp16(65504 / 127) = 516, and 65532 rounds to an infinity, which a
+// weight of 0 would turn into NaN for the queries that must not see it.  65504 is that value within its rounding, 2^-11.  Only
+// rounds of keys with a larger scale than big_scale go over the eight values that a thread has stored at a (unpacking in two
+// versions instead: 24.7 us for 517 tokens from a cold start against 22.7, the instructions' fetch)
+__device__ __forceinline__ void at_clamp8(uint32_t a) {
+    const __half2 most = __float2half2_rn(65504.f), least = __float2half2_rn(-65504.f);
+    uint4 w = lds128(a);
+    auto in = [&](uint32_t x) { return h2_bits(__hmax2_nan(__hmin2_nan(bits_h2(x), most), least)); };
+    at_sts128(a, in(w.x), in(w.y), in(w.z), in(w.w));
+}
+__host__ __device__ constexpr uint32_t big_scale(int b) { return b == 4 ? 0x6FFFu : 0x5FFFu; }      // 8188, 511.75 (fp16 bits): 8 and 128 times that are 65504
 
 // Eight K values of one word (two for Q8_0) times d: an OR of fp16's 1024 turns a code into 1024 + c (the upper nibbles
 // into 1024 + 16 c), the subtraction is exact, and the product with d is the one rounding
@@ -554,13 +567,28 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
                     dv[j * PB] = __ushort_as_half((unsigned short)((J + j) & 1 ? c >> 16 : c & 0xFFFFu));
                 }
             }
+            uint32_t most[2] = {0u, 0u};                          // |scales| of K and of V, two fp16 each
+#pragma unroll
+            for (int w = 0; w < J; ++w) {
+                const uint32_t of_k = (2 * w < J ? 0x7FFFu : 0u) | (2 * w + 1 < J ? 0x7FFF0000u : 0u);
+                if (of_k) most[0] = __vmaxu2(most[0], sw[w] & of_k);
+                if (of_k != 0x7FFF7FFFu) most[1] = __vmaxu2(most[1], sw[w] & (of_k ^ 0x7FFF7FFFu));
+            }
+            const uint32_t big_k = max(most[0] >> 16, most[0] & 0xFFFFu) > big_scale(KB) ? 1u : 0u,
+                           big_v = max(most[1] >> 16, most[1] & 0xFFFFu) > big_scale(VB) ? 2u : 0u;
+            const uint32_t big = __reduce_or_sync(0xffffffffu, big_k | big_v);
             uint32_t all;                                         // the four warps go on, or leave, together
-            if (lane == 0) reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBad)[4 * (i & 3) + pw] = bad;
+            if (lane == 0) {
+                reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBad)[4 * (i & 3) + pw] = bad;
+                reinterpret_cast<uint32_t*>(tc_smem_ + Sh::kOffBig)[4 * (i & 3) + pw] = big;
+            }
             if (bad && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
             asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.and.pred q, %2, 128, p; selp.u32 %0, 1, 0, q; }"
                          : "=r"(all) : "r"(uint32_t(ok)), "r"(1 + pg) : "memory");
             ok = all != 0;
             if (!ok) break;
+            const uint4 bigs = lds128(sm + Sh::kOffBig + 16 * (i & 3));
+            const uint32_t any_big = bigs.x | bigs.y | bigs.z | bigs.w;
 #pragma unroll
             for (int q = 0; q < kGroups; ++q) {
                 const int key = kRows * pw + 8 * q + kk;
@@ -579,6 +607,12 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
                     unpack_k8<KB>(&kw[q][j * KB / 4], j & 1 ? __high2half2(d) : __low2half2(d), o);
                     at_sts128(dst + (4 * j + kt) * 128, o[0], o[1], o[2], o[3]);
                 }
+            }
+            if (any_big & 1u) {
+                const int key = kRows * pw + kk;
+                const uint32_t dst = sm + Sh::kOffK + kPer * st * Sh::kK + (key >> 3) * Sh::kSboK + (key & 7) * 16 + kt * 128;
+#pragma unroll 1
+                for (int x = 0; x < kGroups * J; ++x) at_clamp8(dst + x / J * Sh::kSboK + x % J * 512);
             }
             at_fence_smem();
             __syncwarp();
@@ -605,6 +639,13 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
 #pragma unroll
                         for (int p = 0; p < 4; ++p) o[p] = unpack_v<VB>(&vw[p][j * VB / 4], e, bits_h2(d[p]));
                         at_sts128(dst + (n >> 3) * Sh::kSboV + (n & 7) * 16, o[0], o[1], o[2], o[3]);
+                    }
+                }
+                if (any_big & 2u) {
+#pragma unroll 1
+                    for (int x = 0; x < 4 * JV; ++x) {
+                        const int n = 32 * (vj + x / 4) + 4 * vg + x % 4;
+                        at_clamp8(dst + (n >> 3) * Sh::kSboV + (n & 7) * 16);
                     }
                 }
             }
