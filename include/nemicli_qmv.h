@@ -321,7 +321,8 @@ int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dt
                  const float* sin_table, const long long* positions, long long n_positions, int rot_dim, int paired,
                  const void* q, long long q_stride, int n_q, void* q_out, void* stream);
 
-/* The values d * code of the slots' tokens, rounded to dtype: k and v dense [rows][n_kv][dim], 16-byte aligned.
+/* The values d * code of the slots' tokens, rounded to dtype (float16: at most +-65504, also where a Q8_0 block of clamped
+ * values holds 65532): k and v dense [rows][n_kv][dim], 16-byte aligned.
  * Negative slots give zeros; slots past the cache too, and set QMV_DEV_BAD_ADDRESS.  One launch.  Replaces: nothing
  * callable in the reference. */
 int qmv_kv_read(const qmv_kv_cache* cache, const long long* slots, long long rows, void* k, void* v, int dtype,
@@ -341,7 +342,8 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
  * kernels, so a tight bound is the faster one; with starts null it counts as 1, for the workspace too).  Rows of out that no sequence covers stay
  * as they are.  Table entries behind a sequence's last token are not read; pages outside the cache count as
  * masked, lengths beyond the table are cut, and both set QMV_DEV_BAD_ADDRESS.  Held values beyond +-65504 (a Q8_0 block
- * of clamped values holds 65532) may count as +-65504.  workspace: 256-byte aligned,
+ * of clamped values holds 65532) may count as +-65504,
+ * and float16 outputs end there.  workspace: 256-byte aligned,
  * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  At most 2^30 rows, and 2^30 tokens a
  * table (table_width * page).  The result does not depend on timing.  Replaces: ggufengine/mmvq.py:195-330 (attn1_teil, attn1_summe) over a quantised cache, for
  * any number of tokens. */

@@ -274,7 +274,7 @@ template <class T>
 __device__ __forceinline__ void attn_store(const AttnParams& P, int row0, int r, int group, int hk, int i0, float4 o, float sum) {
     const float inv = sum > 0.f ? __fdividef(1.f, sum) : 0.f;     // no key: zeros
     T* out = static_cast<T*>(P.out) + ((long long)(row0 + r / group) * P.n_heads + hk * group + r % group) * P.c.dim + i0;
-    store4(out, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    store4_held(out, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 template <int DT, int J, int KB, int VB, int NT>

@@ -81,7 +81,7 @@ template <> __device__ __forceinline__ uint32_t pack_out<__nv_bfloat16>(float x,
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
     return r;
 }
-template <> __device__ __forceinline__ uint32_t pack_out<__half>(float x, float y) { return pack_h2(x, y); }
+template <> __device__ __forceinline__ uint32_t pack_out<__half>(float x, float y) { return pack_held(x, y); }
 __device__ __forceinline__ void at_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void at_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void at_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
     }
     const float inv = sum > 0.f ? __fdividef(1.f, sum) : sum == sum ? 0.f : sum;
     T* out = static_cast<T*>(P.out) + ((long long)(S.row0 + r / group) * P.n_heads + hk * group + r % group) * D + 4 * c;
-    store4(out, inv != 0.f ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
+    store4_held(out, inv != 0.f ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
 }
 
 // ---- host -------------------------------------------------------------------------------------------

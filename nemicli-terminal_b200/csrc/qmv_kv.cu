@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
                 float y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) y[i] = there ? __fmul_rn(f, float(int(n >> (8 * i) & 255u) - (q4 ? 8 : 128))) : 0.f;
-                store4(out + off, make_float4(y[0], y[1], y[2], y[3]));
+                store4_held(out + off, make_float4(y[0], y[1], y[2], y[3]));
             }
         };
         int p = first;

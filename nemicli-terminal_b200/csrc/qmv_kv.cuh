@@ -120,6 +120,18 @@ __device__ __forceinline__ void store4(__half* p, float4 v) {
     __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
 }
+// Four values that a cache holds, or a mean of such: fp16 ends at 65504 (a Q8_0 block of clamped values holds 65532, which would
+// round to an infinity)
+__device__ __forceinline__ uint32_t pack_held(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void store4_held(T* p, float4 v) {
+    if constexpr (std::is_same_v<T, __half>) *reinterpret_cast<uint2*>(p) = make_uint2(pack_held(v.x, v.y), pack_held(v.z, v.w));
+    else store4(p, v);
+}
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

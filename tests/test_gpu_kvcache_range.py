@@ -5,7 +5,7 @@ import torch
 from nemicli_terminal_b200 import kvcache
 
 from tests import kv_helpers as KH
-from tests.test_gpu_kvcache import BF16, F32, MANY, gen, slots_of, tables_of
+from tests.test_gpu_kvcache import BF16, F16, F32, MANY, gen, slots_of, tables_of
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,25 @@ def test_clamped_values(cuda, dtype, dim, kf, vf, most):
     got, tiles = attend(c, tables, q, [90], [90], most)
     assert tiles == (most == MANY and dtype == BF16)
     compare(got, tiles, q, held, [90], [90], dim ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", ["Q4_0", "Q8_0"])
+def test_clamped_values_in_float16(cuda, fmt):
+    """65532 rounds to an infinity of float16: read and the attention's float16 outputs stay at 65504, half a step away."""
+    k = torch.zeros(1, 1, 64, device=cuda)
+    v = torch.ones(1, 1, 64, device=cuda)
+    v[..., 0], v[..., 40] = float("inf"), -1e30
+    k[..., 3] = float("inf")
+    c = kvcache.KVCache(200, 1, 64, 16, fmt, fmt, cuda)
+    c.write(k.expand(2, 1, 64).contiguous(), v.expand(2, 1, 64).contiguous(), torch.arange(2, device=cuda))
+    want = torch.zeros(64, device=cuda)
+    want[0], want[40] = 65504, -65504
+    for x in c.read(torch.arange(2, device=cuda), F16):
+        assert torch.isfinite(x).all()
+    assert torch.equal(c.read(torch.arange(2, device=cuda), F16)[1][0, 0], want.half())
+    table = torch.zeros(1, 1, dtype=torch.int32, device=cuda)
+    wide = torch.zeros(1, 200, dtype=torch.int32, device=cuda)             # a table this long: keys cut over the GPU
+    for t, new, most in ((table, 1, 1), (table, 2, 2), (table, 2, MANY), (wide, 1, 1), (wide, 2, 400)):
+        q = torch.zeros(new, 4, 64, dtype=F16, device=cuda)
+        got, _ = attend(c, t, q, [2], [new], most)
+        assert torch.equal(got, want.half().expand(new, 4, 64))
