@@ -16,8 +16,11 @@
 // 16 x 8 scores in fp32, d_v goes into p before it is rounded to fp16.
 //
 // Queries are fp16 after a power of two per row (exact for bf16 and fp16); fp32 queries are two fp16 parts (HL), and so
-// is p d_v then, which keeps fp32's accuracy.  The softmax reference only moves when a score passes it by 2^4 or a d_v
-// its limit (checked with one vote a tile): p d_v 2^E stays below 2^15.  Sums and statistics are fp32.
+// is p d_v then, which keeps fp32's accuracy.  The softmax reference only moves when a score passes it by 2^4 or a d_v the
+// next power of two (checked with one vote a tile).  p d_v is rounded to fp16 once: it stays below 2^15 and is 2^10 at least for the
+// reference and the largest d_v, whatever V's size, so 2^-24 of that is still a normal number.  (p as fp16 times d_v as fp16 took 112
+// us for 64 sequences of bf16 queries where this takes 116, but holds no p large enough for a small d_v.)  Sums and statistics are
+// fp32.
 //
 // Work: units of 64 or 128 keys (one or two tiles of 16 a warp) of segments (sequence, key head, tile of 8 NT rows); the list of all units is cut into
 // equal runs, one a CTA, so unequal lengths do not unbalance it.  A segment cut over several CTAs leaves its parts in the
@@ -200,11 +203,6 @@ struct AttnSlot {
         const __half2 h = bits_h2(sc[i >> 1]);
         return i & 1 ? __high2float(h) : __low2float(h);
     }
-    // V's scale j of two keys side by side
-    static __device__ __forceinline__ uint32_t pair(const uint32_t (&a)[kS], const uint32_t (&b)[kS], int j) {
-        const int i = j + J % 2;
-        return __byte_perm(a[i >> 1], b[i >> 1], i & 1 ? 0x7632 : 0x5410);
-    }
 };
 // Tiles of 16 keys a warp works on at once (two: each instruction has another that does not wait for it, and the loop's and
 // the softmax's bookkeeping counts half; 64 sequences of up to 8191 keys, 8 heads of 128: 115 us, with one 139), keys a unit, CTAs
@@ -280,13 +278,9 @@ __device__ __forceinline__ void attn_store(const AttnParams& P, int row0, int r,
 template <int DT, int J, int KB, int VB, int NT>
 __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32, J, KB, VB, NT))) attn_kernel(const __grid_constant__ AttnParams P) {
     using T = typename Elem<DT>::type;
-    // HL: queries and weights as two fp16 parts.  FAST: weights rounded to fp16 before they meet d_v, both then in fp16
-    // (two roundings of 2^-11 where the output's is 2^-8), half the instructions of the fp32 product and its rounding (64
-    // sequences: 115 us, with fp32 products 117)
-    constexpr bool HL = DT == QMV_OUT_F32, FAST = DT == QMV_OUT_BF16;
+    constexpr bool HL = DT == QMV_OUT_F32;                       // queries and weights as two fp16 parts
     constexpr int D = 32 * J, R = 8 * NT, kParts = HL ? 2 : 1;
     constexpr float kOffK = KB == 4 ? 8.f : 128.f;
-    constexpr float kTop = HL ? 4.f : 12.f;                      // p 2^-E at most 2^kTop (HL: small ones keep a second part's bits)
     constexpr uint32_t kOffV = VB == 4 ? 0x00080008u : 0x00800080u;
     constexpr int S_ = attn_stages(HL, J, KB, VB, NT), KT = attn_tiles(J, NT), kUnit = attn_unit(J, NT);
     using Slot = AttnSlot<J, KB, VB, KT>;
@@ -413,8 +407,8 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
 
         float cs[NT], M[NT], rn[NT], sum[NT], o[NT][J][2][4], off[NT][4];        // of rows g, g + 8; o, off: columns 2 t, 2 t + 1
         int pos[NT];
-        float E = 0.f;
-        uint32_t lim = HL ? 0u : 0x48004800u;                     // d_v at most 8 until one larger is seen (two fp16)
+        float top_p = 0.f;                                        // log2 of the largest p allowed
+        uint32_t lim = 0u;                                        // ... while every |d_v| is at most this (two fp16)
         if (rows > 0) {
             // ---- the units' copies; the first ones start before the queries are looked at
             const int turns = dead ? 0 : todo;
@@ -648,12 +642,12 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top = fmaxf(top, p[x][nt][i]);
-                if (__any_sync(0xffffffffu, top > kTop + E || __vmaxu2(dv, lim) != lim)) {
+                if (__any_sync(0xffffffffu, top > top_p || __vmaxu2(dv, lim) != lim)) {
                     dv = __reduce_max_sync(0xffffffffu, max(dv >> 16, dv & 0xFFFFu));
-                    if (dv > (lim & 0xFFFFu)) {                   // up to 2^(ev - 11), a factor of 8 to 16 to spare; times 2^E it is 2^(15 - kTop)
-                        const uint32_t ev = max(1u, dv >> 10);
-                        lim = min((ev + 4) << 10, 0x7BFFu) * 0x10001u;
-                        E = 26.f - kTop - float(int(ev));
+                    if (dv > (lim & 0xFFFFu)) {                   // the next power of two, 2^(ev - 14); times 2^top_p it is 2^15
+                        const int bits = 31 - __clz(dv), ev = dv < 1024u ? bits - 9 : int(dv >> 10);        // (below 2^-14 denormal)
+                        lim = (dv < 1024u ? 2u << bits : min(uint32_t(ev + 1) << 10, 0x7BFFu)) * 0x10001u;
+                        top_p = float(29 - ev);
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -664,7 +658,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                         M[nt] = fmaxf(M[nt], m);
-                        const float n = kTop - 4.f + E - M[nt], f = ex2(n - rn[nt]);
+                        const float n = top_p - 4.f - M[nt], f = ex2(n - rn[nt]);
                         rn[nt] = n;
                         sum[nt] *= f;
                         const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
@@ -679,7 +673,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                     }
                     weigh();
                 }
-                uint32_t ph[KT][NT][2], vw[KT][2][Slot::kV], sv[KT][4][Slot::kS];
+                uint32_t vw[KT][2][Slot::kV], sv[KT][4][Slot::kS];
 #pragma unroll
                 for (int x = 0; x < KT; ++x) {
 #pragma unroll
@@ -687,7 +681,6 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
 #pragma unroll
                         for (int i = 0; i < 4; ++i) p[x][nt][i] = ex2(p[x][nt][i]);
                         sum[nt] += (p[x][nt][0] + p[x][nt][1]) + (p[x][nt][2] + p[x][nt][3]);
-                        if (FAST) ph[x][nt][0] = pack_h2(p[x][nt][0], p[x][nt][1]), ph[x][nt][1] = pack_h2(p[x][nt][2], p[x][nt][3]);
                     }
                 }
                 each<KT>([&](auto x) {
@@ -717,26 +710,18 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                             a[0][2 * h] = v[0], a[0][2 * h + 1] = v[1], a[1][2 * h] = v[2], a[1][2 * h + 1] = v[3];
                         }
                         float d[4];
-                        uint32_t d2[2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (FAST) d2[i >> 1] = Slot::pair(sv[x][i & ~1], sv[x][i | 1], j);
-                            else d[i] = Slot::scale(sv[x][i], j, true);
-                        }
+                        for (int i = 0; i < 4; ++i) d[i] = Slot::scale(sv[x][i], j, true);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             uint32_t bw[2], low[2];
 #pragma unroll
                             for (int y = 0; y < 2; ++y) {
-                                if constexpr (FAST) {
-                                    bw[y] = h2_bits(__hmul2(bits_h2(ph[x][nt][y]), bits_h2(d2[y])));
-                                } else {
-                                    const float p0 = p[x][nt][2 * y] * d[2 * y], p1 = p[x][nt][2 * y + 1] * d[2 * y + 1];
-                                    bw[y] = pack_h2(p0, p1);
-                                    if (HL) {
-                                        const float2 f = unpack_h2(bw[y]);
-                                        low[y] = pack_h2(p0 - f.x, p1 - f.y);
-                                    }
+                                const float p0 = p[x][nt][2 * y] * d[2 * y], p1 = p[x][nt][2 * y + 1] * d[2 * y + 1];
+                                bw[y] = pack_h2(p0, p1);
+                                if (HL) {
+                                    const float2 f = unpack_h2(bw[y]);
+                                    low[y] = pack_h2(p0 - f.x, p1 - f.y);
                                 }
                             }
 #pragma unroll

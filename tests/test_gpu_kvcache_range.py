@@ -41,11 +41,15 @@ def compare(got, tiles, q, held, lens, new, scale, window=0, tol_of=None):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("dim", [64, 96, 128, 256])
 @pytest.mark.parametrize("kf, vf", [("Q8_0", "Q8_0"), ("Q4_0", "Q8_0"), ("Q8_0", "Q4_0")])
-@pytest.mark.parametrize("most", [MANY])
+@pytest.mark.parametrize("most", [90, MANY])
 def test_clamped_values(cuda, dtype, dim, kf, vf, most):
     """Infinities and values past fp16 are held as the largest code times fp16(65504 / 127), which is 65532: finite for every
     query that sees them, and nothing to those before.  The queries' share of K's clamped channel is small, so that its score
-    is an ordinary one."""
+    is an ordinary one.
+    One bound more than KH.bound's where the codes' bits are the operand (16-bit queries, no tiles): the tensor cores align a
+    step's 16 products at the largest exponent and cut each off there, 2^-23 of it, and a code c 2^-24, a denormal, counts as
+    2^-14: each loses up to 2^-37 p d, or 2^-13 p d once 2^24 is taken off; 16 of a step 2^-9 p d, for the codes and for
+    their offset 2^-8 p d together.  A block's largest value is 8 d at least: 2^-11 of it."""
     g = gen(1, cuda)
     tables, pages = tables_of([90], 16, 1, cuda)
     c = kvcache.KVCache(pages, 2, dim, 16, kf, vf, cuda)
@@ -62,7 +66,9 @@ def test_clamped_values(cuda, dtype, dim, kf, vf, most):
     q = q.to(dtype)
     got, tiles = attend(c, tables, q, [90], [90], most)
     assert tiles == (most == MANY and dtype == BF16)
-    compare(got, tiles, q, held, [90], [90], dim ** -0.5)
+    bits = dtype == BF16 and not tiles
+    compare(got, tiles, q, held, [90], [90], dim ** -0.5,
+            tol_of=lambda sizes, o, keys: KH.bound(sizes, o, dtype, keys, tiles) + 2.0 ** -11 * sizes[1] * bits)
 
 
 @pytest.mark.parametrize("fmt", ["Q4_0", "Q8_0"])
@@ -85,3 +91,71 @@ def test_clamped_values_in_float16(cuda, fmt):
         q = torch.zeros(new, 4, 64, dtype=F16, device=cuda)
         got, _ = attend(c, t, q, [2], [new], most)
         assert torch.equal(got, want.half().expand(new, 4, 64))
+
+
+# ---- weights far apart, values of any size ---------------------------------------------------------------
+
+def sink(cuda, lens, gap, small, kf, vf, dim=64, n_kv=2, heads=4, page=16):
+    """Caches whose first key stands `gap` above all others in the score of a head's queries (half of it for odd heads) and
+    whose first value is 0; the others' values are `small` times 1 to 1.25.  -> cache, tables, held, the queries' row, scale.
+    Queries are one power of two on channel 0, and K there an integer times a power of two, so every score is exact."""
+    g = gen(2, cuda)
+    tables, pages = tables_of(lens, page, 1, cuda)
+    c = kvcache.KVCache(pages, n_kv, dim, page, kf, vf, cuda)
+    held = []
+    for b, n in enumerate(lens):
+        k = torch.zeros(n, n_kv, dim, device=cuda)
+        top, d, most = (100, 0.125, 127) if kf == "Q8_0" else (7, 0.5, -8)
+        k[..., 31] = most * d                                  # the block's scale is d
+        k[0, :, 0] = top * d
+        v = small * (1 + 0.25 * torch.rand(n, n_kv, dim, generator=g, device=cuda))
+        v[0] = 0
+        s = slots_of(tables[b], n, page)
+        c.write(k, v, s)
+        held.append([x.double() for x in c.read(s, F32)])
+        assert torch.equal(held[-1][0], k.double())
+    q = torch.zeros(heads, dim, device=cuda)
+    q[:, 0] = 1.0
+    q[1::2, 0] = 0.5
+    scale = torch.tensor(gap / (top * d)).float().item()
+    return c, tables, held, q, scale
+
+
+def sink_bound(dtype, tiles):
+    """The scores are exact, so a weight 2^x is off by x's rounding: x = s cs + reference, |x| <= 32: 2^-19 for the sum, three
+    roundings of 2^-24 in cs times at most 25, ln 2 times both is 5e-6; ex2's 2^-22; twice, for the sum that it is divided by:
+    2^-16.  Weights in fp16 2^-11 (float32: two parts, 2^-21), V in fp16 2^-11 on the tiles; sums and the output as in KH.bound."""
+    rel = 2.0 ** -16 + (2.0 ** -21 if dtype == F32 else 2.0 ** -11) + (2.0 ** -11 if tiles else 0.0)
+
+    def tol(sizes, o, keys):
+        mag, top, _, _ = sizes
+        return mag * rel + 2 * top * (keys / 16 + 16) * 2.0 ** -22 + o.abs() * KH.HALF_STEP[dtype] + 2.0 ** -24 * (dtype == F16) + 1e-30
+    return tol
+
+
+CALLS = [([1500, 900], 1, 1), ([1500, 900], 6, 6), ([1500, 900], 60, MANY), ([5000], 200, 200)]     # the last: keys cut over the GPU
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("small", [1.0, 1e-2, 1e-3, 3e-5])
+@pytest.mark.parametrize("kf, vf", [("Q8_0", "Q8_0"), ("Q4_0", "Q4_0")])
+@pytest.mark.parametrize("lens, new, most", CALLS)
+def test_small_values_keep_small_weights(cuda, dtype, small, kf, vf, lens, new, most):
+    """The output does not depend on V's size."""
+    c, tables, held, q, scale = sink(cuda, lens, 10.0, small, kf, vf)
+    q = q.expand(new * len(lens), 4, 64).to(dtype)
+    got, tiles = attend(c, tables, q, lens, [new] * len(lens), most, scale)
+    assert tiles == (new >= 60 and dtype != F32)
+    compare(got, tiles, q, held, lens, [new] * len(lens), scale, tol_of=sink_bound(dtype, tiles))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("gap", [12.0, 14.0, 15.0])
+@pytest.mark.parametrize("lens, new, most", CALLS[:2])
+def test_many_weights_under_one_key(cuda, dtype, gap, lens, new, most):
+    """Weights down to 2^-24 of the row's largest hold their bits: a first key without a value (an attention sink) far above
+    many equal ones."""
+    c, tables, held, q, scale = sink(cuda, lens, gap, 1.0, "Q8_0", "Q8_0")
+    q = q.expand(new * len(lens), 4, 64).to(dtype)
+    got, tiles = attend(c, tables, q, lens, [new] * len(lens), most, scale)
+    compare(got, tiles, q, held, lens, [new] * len(lens), scale, tol_of=sink_bound(dtype, tiles))
