@@ -17,8 +17,10 @@
 //              for behind K's (-> 240).
 //   MMA        one warp: the scores run two steps ahead of the sums, the other tile's softmax runs meanwhile.
 //   softmax    NQ x 4 warps, one thread a row: scores from tensor memory, P as fp16 over them, and the row's
-//              reference, sum and mask in registers.  The reference moves only when the row's maximum passes it by 2^8;
-//              then the warp rescales its rows of O in tensor memory.
+//              reference, sum and mask in registers.  P is 2^9 where the reference was set and moves it only past 2^15 (then the
+//              warp rescales its rows of O in tensor memory), so weights down to 2^-23 of the row's largest are normal numbers of
+//              fp16 (set at 1 and moved past 2^8, the sum kept weights below 2^-14 that P lost).  Set at 2^11, 8192 tokens take 631
+//              us, at 2^9 618, at 2^7 617; with 256 values and a window 258, 244 and 242.
 // The exponentials are not the bound: a quarter of them as a cubic on the other units gained nothing (595 us without, 610 with it).
 // Queries are fp16 after a power of two per row (exact but for values 2^-32 below the row's largest).  Tensor memory:
 // S NQ x 2 x BN columns, O NQ x D columns.  Every mbarrier wait is bounded; on expiry the CTA sets DEV_TIMEOUT, waits
@@ -382,10 +384,10 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
             for (int k = 0; k < BN; k += 2) tops[(k >> 1) & 3] = max3(tops[(k >> 1) & 3], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
             const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
             const float m = top == -INFINITY ? kAttnNone : top * cs;
-            const bool move = m > ref + 8.f;
+            const bool move = m > ref + 15.f;
             if (__any_sync(0xffffffffu, move)) {
-                const float f = move ? ex2(ref - m) : 1.f;
-                if (move) ref = m;
+                const float f = move ? ex2(ref - (m - 9.f)) : 1.f;
+                if (move) ref = m - 9.f;
                 sum *= f;
                 if (i > 0) {
                     ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * (2 * qa + (buf ^ 1)), uint32_t((i - 1) >> 1) & 1u));       // O(i - 1) is complete
