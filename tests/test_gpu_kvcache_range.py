@@ -95,9 +95,9 @@ def test_clamped_values_in_float16(cuda, fmt):
 
 # ---- weights far apart, values of any size ---------------------------------------------------------------
 
-def sink(cuda, lens, gap, small, kf, vf, dim=64, n_kv=2, heads=4, page=16):
+def sink(cuda, lens, gap, small, kf, vf, same=False, dim=64, n_kv=2, heads=4, page=16):
     """Caches whose first key stands `gap` above all others in the score of a head's queries (half of it for odd heads) and
-    whose first value is 0; the others' values are `small` times 1 to 1.25.  -> cache, tables, held, the queries' row, scale.
+    whose first value is 0; the others' values are `small` times 1 to 1.25 (same: one row for all of them).  -> cache, tables, held, the queries' row, scale.
     Queries are one power of two on channel 0, and K there an integer times a power of two, so every score is exact."""
     g = gen(2, cuda)
     tables, pages = tables_of(lens, page, 1, cuda)
@@ -109,6 +109,8 @@ def sink(cuda, lens, gap, small, kf, vf, dim=64, n_kv=2, heads=4, page=16):
         k[..., 31] = most * d                                  # the block's scale is d
         k[0, :, 0] = top * d
         v = small * (1 + 0.25 * torch.rand(n, n_kv, dim, generator=g, device=cuda))
+        if same:
+            v[:] = v[1]
         v[0] = 0
         s = slots_of(tables[b], n, page)
         c.write(k, v, s)
@@ -125,12 +127,13 @@ def sink_bound(dtype, tiles, small=1.0):
     """The scores are exact, so a weight 2^x is off by x's rounding: x = s cs + reference, |x| <= 32: 2^-19 for the sum, three
     roundings of 2^-24 in cs times at most 25, ln 2 times both is 5e-6; ex2's 2^-22; twice, for the sum that it is divided by:
     2^-16.  Weights in fp16 2^-11 (float32: two parts, 2^-21), V in fp16 2^-11 on the tiles; sums and the output as in KH.bound.
-    In fp16 a weight is off by 2^-25 at least, where the largest one is 2^9 or more: 2^-34 a key, times V, at most 1.25 `small`."""
+    A product of a weight (and V's scale) in fp16, or its second part, is off by 2^-25 at least, where the largest weight has 2^9
+    or more (2^10 with V's scale, as float32 queries have it): 2^-34 a key (2^-35), times V, at most 1.25 `small`."""
     rel = 2.0 ** -16 + (2.0 ** -21 if dtype == F32 else 2.0 ** -11) + (2.0 ** -11 if tiles else 0.0)
 
     def tol(sizes, o, keys):
         mag, top, _, _ = sizes
-        return mag * rel + (0.0 if dtype == F32 else keys * 2.0 ** -34 * 1.25 * small) + 2 * top * (keys / 16 + 16) * 2.0 ** -22 + o.abs() * KH.HALF_STEP[dtype] + 2.0 ** -24 * (dtype == F16) + 1e-30
+        return mag * rel + keys * 2.0 ** (-35 if dtype == F32 else -34) * 1.25 * small + 2 * top * (keys / 16 + 16) * 2.0 ** -22 + o.abs() * KH.HALF_STEP[dtype] + 2.0 ** -24 * (dtype == F16) + 1e-30
     return tol
 
 
@@ -152,11 +155,12 @@ def test_small_values_keep_small_weights(cuda, dtype, small, kf, vf, lens, new, 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("gap", [12.0, 14.0, 15.0, 17.0])
+@pytest.mark.parametrize("same", [False, True])
 @pytest.mark.parametrize("lens, new, most", CALLS)
-def test_many_weights_under_one_key(cuda, dtype, gap, lens, new, most):
-    """Weights down to 2^-23 of the row's largest hold their bits, those below 2^-34 of it: a first key without a value (an attention sink) far above
+def test_many_weights_under_one_key(cuda, dtype, gap, same, lens, new, most):
+    """Weights down to 2^-23 of the row's largest hold their bits, those below to 2^-34 of it: a first key without a value (an attention sink) far above
     many equal ones."""
-    c, tables, held, q, scale = sink(cuda, lens, gap, 1.0, "Q8_0", "Q8_0")
+    c, tables, held, q, scale = sink(cuda, lens, gap, 1.0, "Q8_0", "Q8_0", same)
     q = q.expand(new * len(lens), 4, 64).to(dtype)
     got, tiles = attend(c, tables, q, lens, [new] * len(lens), most, scale)
     compare(got, tiles, q, held, lens, [new] * len(lens), scale, tol_of=sink_bound(dtype, tiles))
