@@ -15,12 +15,14 @@
 // times the sum's size, and its rounding showed as 1e-5 of the result.)  Scales stay out of the products: d_k multiplies a block's
 // 16 x 8 scores in fp32, d_v goes into p before it is rounded to fp16.
 //
-// Queries are fp16 after a power of two per row (exact for bf16 and fp16); fp32 queries are two fp16 parts (HL), and so
-// is p d_v then: 22 bits, down to 2^-35 of a row's largest product.  (Second parts 2^11 times as large against codes 2^-11 times as
-// large would go down to 2^-46; they take 44 us for one sequence of 65519 tokens where this takes 40.)  The softmax reference only moves when a score passes it by 2^4 or a d_v the
-// next power of two (checked with one vote a tile).  p d_v is rounded to fp16 once: it stays below 2^15 and is 2^10 at least for the
-// reference and the largest d_v, whatever V's size, so 2^-24 of that is still a normal number.  (p as fp16 times d_v as fp16 took 112
-// us for 64 sequences of bf16 queries where this takes 116, but holds no p large enough for a small d_v.)  Sums and statistics are
+// Queries are fp16 after a power of two per row, which puts the largest at 2^14: bf16 values are exact down to 2^-31 of it, fp16's
+// down to 2^-28, smaller ones are off by up to 2^-39 of it (those that meet the upper nibbles of 4-bit keys go in 1 / 16 as large:
+// 2^-27, 2^-24, 2^-35); fp32 queries are two fp16 parts (HL), and so is p d_v then: 22 bits, down to 2^-35 of a row's largest
+// product. (Second parts 2^11 times as large against codes 2^-11 times as large would go down to 2^-46; they take 44 us for one
+// sequence of 65519 tokens where this takes 40.) The softmax reference only moves when a score passes it by 2^4 or a d_v the next
+// power of two (checked with one vote a tile). p d_v is rounded to fp16 once: it stays below 2^15 and is 2^10 at least for the
+// reference and the largest d_v, whatever V's size, so 2^-24 of that is still a normal number. (p as fp16 times d_v as fp16 took 112
+// us for 64 sequences of bf16 queries where this takes 116, but holds no p large enough for a small d_v.) Sums and statistics are
 // fp32.
 //
 // Work: units of 64 or 128 keys (one or two tiles of 16 a warp) of segments (sequence, key head, tile of 8 NT rows); the list of all units is cut into
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // 2^14 <= top 2^-e < 2^15; a row of zeros or with an infinity keeps its size
                 const int ex = int((__float_as_uint(top) >> 23) & 255u);
-                const int e = ex == 0 || ex == 255 ? 0 : max(-120, min(120, ex - 127 - 14));
+                const int e = ex == 0 || ex == 255 ? 0 : max(-120, ex - 127 - 14);
                 // the scale's sign goes into the queries: cs is positive, and masked scores stay -inf
                 const float down = __uint_as_float((uint32_t(127 - e) << 23) | (P.scale < 0.f ? 0x80000000u : 0u));
                 cs[nt] = fmaxf(fabsf(P.scale) * 1.4426950408889634f * (HL ? 1.f : 16777216.f) * __uint_as_float(uint32_t(127 + e) << 23), 1e-30f);

@@ -22,9 +22,9 @@
 //              fp16 (set at 1 and moved past 2^8, the sum kept weights below 2^-14 that P lost).  Set at 2^11, 8192 tokens take 631
 //              us, at 2^9 618, at 2^7 617; with 256 values and a window 258, 244 and 242.
 // The exponentials are not the bound: a quarter of them as a cubic on the other units gained nothing (595 us without, 610 with it).
-// Queries are fp16 after a power of two per row (exact but for values 2^-32 below the row's largest).  Tensor memory:
-// S NQ x 2 x BN columns, O NQ x D columns.  Every mbarrier wait is bounded; on expiry the CTA sets DEV_TIMEOUT, waits
-// (bounded) for its MMAs, frees its tensor memory and leaves.
+// Queries are fp16 after a power of two per row, which puts the largest at 2^14: bf16 values are exact down to 2^-31 of it, fp16's
+// down to 2^-28, smaller ones are off by up to 2^-39 of it. Tensor memory: S NQ x 2 x BN columns, O NQ x D columns. Every mbarrier
+// wait is bounded; on expiry the CTA sets DEV_TIMEOUT, waits (bounded) for its MMAs, frees its tensor memory and leaves.
 #pragma once
 #include <climits>
 
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(AttnTcShape<J>::kThreads, 1) attn_tc_kernel(co
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     const int ex = int((__float_as_uint(top) >> 23) & 255u);
-                    e[q] = ex == 0 || ex == 255 ? 0 : max(-110, min(110, ex - 127 - 8));      // 2^8 <= top 2^-e < 2^9
+                    e[q] = ex == 0 || ex == 255 ? 0 : max(-120, ex - 127 - 14);       // 2^14 <= top 2^-e < 2^15
                     const float down = __uint_as_float((uint32_t(127 - e[q]) << 23) | (P.scale < 0.f ? 0x80000000u : 0u));
                     const int rl = wr + 8 * (q0 + q) + (lane & 7);
                     const uint32_t dst = sm + qa * Sh::kQ + (rl >> 3) * Sh::kSboQ + (rl & 7) * 16;

@@ -5,7 +5,7 @@ import torch
 from nemicli_terminal_b200 import kvcache
 
 from tests import kv_helpers as KH
-from tests.test_gpu_kvcache import BF16, F16, F32, MANY, gen, slots_of, tables_of
+from tests.test_gpu_kvcache import BF16, F16, F32, MANY, filled, gen, slots_of, tables_of
 
 pytestmark = pytest.mark.gpu
 
@@ -164,3 +164,44 @@ def test_many_weights_under_one_key(cuda, dtype, gap, same, lens, new, most):
     q = q.expand(new * len(lens), 4, 64).to(dtype)
     got, tiles = attend(c, tables, q, lens, [new] * len(lens), most, scale)
     compare(got, tiles, q, held, lens, [new] * len(lens), scale, tol_of=sink_bound(dtype, tiles))
+
+
+# ---- queries --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("kf", ["Q4_0", "Q8_0"])
+@pytest.mark.parametrize("new, most", [(1, 1), (6, 6), (70, MANY)])
+def test_queries_of_far_sizes_in_a_row(cuda, dtype, kf, new, most):
+    """One value of a row 2^30 (2^27 with Q4_0's upper nibbles, float16: 2^23) above the others, where K holds zeros: the others
+    count in full."""
+    lens, g = [200, 150], gen(3, cuda)
+    tables, pages = tables_of(lens, 16, 1, cuda)
+    c = kvcache.KVCache(pages, 1, 96, 16, kf, "Q8_0", cuda)
+    held = []
+    for b, n in enumerate(lens):
+        k, v = (torch.randn(n, 1, 96, generator=g, device=cuda) for _ in range(2))
+        k[..., :32] = 0
+        s = slots_of(tables[b], n, 16)
+        c.write(k, v, s)
+        held.append([x.double() for x in c.read(s, F32)])
+    far = 23 if dtype == F16 else 30 if kf == "Q8_0" else 27
+    q = torch.randn(2 * new, 4, 96, generator=g, device=cuda)
+    q = torch.sign(q) * q.abs().clamp(0.5, 1.9) * 2.0 ** (13 - far)
+    q[..., 5] = 1.9 * 2.0 ** 13
+    q = q.to(dtype)
+    scale = 2.0 ** (far - 13) / 8
+    got, tiles = attend(c, tables, q, lens, [new, new], most, scale)
+    compare(got, tiles, q, held, lens, [new, new], scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [2.0 ** 125])
+@pytest.mark.parametrize("new, most", [(1, 1), (6, 6), (70, MANY)])
+def test_queries_of_any_size(cuda, dtype, size, new, most):
+    """Queries near both ends of bf16's range, with a scale that makes their scores ordinary."""
+    lens = [200, 150]
+    c, tables, held = filled(cuda, lens, 1, 128, 16, "Q8_0", "Q8_0")
+    q = (torch.randn(2 * new, 4, 128, generator=gen(4, cuda), device=cuda).clamp(-3.9, 3.9) * size).to(dtype)
+    scale = 2.0 ** -3 / size
+    got, tiles = attend(c, tables, q, lens, [new, new], most, scale)
+    compare(got, tiles, q, held, lens, [new, new], scale)
