@@ -500,7 +500,9 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
                 const int e = ex == 0 || ex == 255 ? 0 : max(-120, ex - 127 - 14);
                 // the scale's sign goes into the queries: cs is positive, and masked scores stay -inf
                 const float down = __uint_as_float((uint32_t(127 - e) << 23) | (P.scale < 0.f ? 0x80000000u : 0u));
-                cs[nt] = fmaxf(fabsf(P.scale) * 1.4426950408889634f * (HL ? 1.f : 16777216.f) * __uint_as_float(uint32_t(127 + e) << 23), 1e-30f);
+                // (2^e first, in halves: a scale near fp32's end times 2^24 would pass it though its queries are as small)
+                const float up = __uint_as_float(uint32_t(127 + e / 2) << 23);
+                cs[nt] = fmaxf(fabsf(P.scale) * 1.4426950408889634f * up * (HL ? 1.f : 16777216.f) * __uint_as_float(uint32_t(127 + e - e / 2) << 23), 1e-30f);
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     float all = 0.f;

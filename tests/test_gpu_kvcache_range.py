@@ -195,7 +195,7 @@ def test_queries_of_far_sizes_in_a_row(cuda, dtype, kf, new, most):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("size", [2.0 ** 125])
+@pytest.mark.parametrize("size", [2.0 ** 125, 2.0 ** -120])
 @pytest.mark.parametrize("new, most", [(1, 1), (6, 6), (70, MANY)])
 def test_queries_of_any_size(cuda, dtype, size, new, most):
     """Queries near both ends of bf16's range, with a scale that makes their scores ordinary."""
