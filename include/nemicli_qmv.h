@@ -347,8 +347,8 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
  * masked, lengths beyond the table are cut, and both set QMV_DEV_BAD_ADDRESS.  Held values beyond +-65504 (a Q8_0 block
  * of clamped values holds 65532) may count as +-65504,
  * and float16 outputs end there.  workspace: 256-byte aligned,
- * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  At most 2^30 rows, and 2^30 tokens a
- * table (table_width * page).  The result does not depend on timing.  Replaces: ggufengine/mmvq.py:195-330 (attn1_teil, attn1_summe) over a quantised cache, for
+ * qmv_kv_attend_workspace_bytes long; calls that may overlap need separate ones.  At most 2^30 rows, 2^30 tokens a
+ * table (table_width * page), and max_new * (n_heads / n_kv) 2^30.  The result does not depend on timing.  Replaces: ggufengine/mmvq.py:195-330 (attn1_teil, attn1_summe) over a quantised cache, for
  * any number of tokens. */
 int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long q_stride, int n_heads,
                   const int* tables, int table_width, const int* lens, const int* starts, int n_seq, long long n_rows,

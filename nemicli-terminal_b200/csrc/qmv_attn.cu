@@ -4,7 +4,8 @@
 using namespace qmv;
 
 namespace {
-constexpr int kMostKeys = 1 << 30;        // tokens a table may hold and query rows: positions, windows and tiles' ends stay in 31 bits
+constexpr int kMostKeys = 1 << 30;        // tokens a table may hold, query rows, rows a key head (max_new times its heads):
+                                          // positions, windows and tiles' ends stay in 31 bits
 bool bad_table(const KvView& c, int width, int window) { return width <= 0 || width > kMostKeys >> c.page_shift || window < 0; }
 // a window no shorter than the table is none
 int real_window(const KvView& c, int width, int window) { return window >= width << c.page_shift ? 0 : window; }
@@ -18,7 +19,7 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
     if (kv_view(cache, c) || n_heads <= 0 || n_heads > 65535 || n_heads % c.n_kv || n_seq <= 0 || n_seq > 65535 || max_new <= 0)
         return 0;
     if (dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16) return 0;
-    if (bad_table(c, table_width, window)) return 0;
+    if (bad_table(c, table_width, window) || max_new > kMostKeys / (n_heads / c.n_kv)) return 0;
     window = real_window(c, table_width, window);
     const AttnTcPlan tc = attn_tc_plan(c, dtype, n_heads, n_seq, max_new, table_width, window);
     if (tc.used) return tc.grid > 0x7FFFFFFF ? 0 : tc.bytes + 1;      // (no workspace: one byte)
@@ -45,6 +46,7 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
         !aligned(starts, 4) || !aligned(workspace, 256))
         return ST_BAD_ALIGN;
     if (!starts) max_new = 1;
+    if (max_new > kMostKeys / (n_heads / P.c.n_kv)) return ST_BAD_TOKENS;
     const AttnTcPlan tc = attn_tc_plan(P.c, dtype, n_heads, n_seq, max_new, table_width, window);
     const AttnPlan pl = attn_plan(P.c, dtype, n_heads, n_seq, max_new, table_width, window);
     if (tc.used ? tc.grid > 0x7FFFFFFF || workspace_bytes < tc.bytes : !pl.grid || workspace_bytes < pl.bytes) return ST_BAD_SHAPE;
