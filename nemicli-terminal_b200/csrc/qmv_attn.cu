@@ -1,4 +1,6 @@
 // Attention over a quantised key / value cache (layout: qmv_kv.cuh; C-ABI declarations: include/nemicli_qmv.h).
+#include <cmath>
+
 #include "qmv_attn_tc.cuh"
 
 using namespace qmv;
@@ -37,6 +39,7 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
     if (!q || !tables || !lens || !out || !workspace) return ST_NULL;
     if (dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16) return ST_BAD_SHAPE;
     if (n_heads <= 0 || n_heads > 65535 || n_heads % P.c.n_kv || bad_table(P.c, table_width, window)) return ST_BAD_SHAPE;
+    if (!std::isfinite(scale)) return ST_BAD_SHAPE;           // (its kernels would take NaN for the smallest scale)
     window = real_window(P.c, table_width, window);
     if (n_seq <= 0 || n_seq > 65535 || n_rows < 0 || n_rows > kMostKeys || max_new <= 0 || (!starts && n_rows < n_seq))
         return ST_BAD_TOKENS;

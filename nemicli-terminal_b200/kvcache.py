@@ -188,6 +188,8 @@ class KVCache:
         elif rows < n_seq:
             raise RuntimeError(f"KVCache.attend: {rows} query rows for {n_seq} sequences")
         most = 1 if starts is None else (rows if max_new is None else int(max_new))
+        if scale is not None and not abs(scale) < 3.5e38:          # float32's end, and NaN
+            raise RuntimeError(f"KVCache.attend: scale {scale} is not finite")
         if window < 0 or most < 0:
             raise RuntimeError("KVCache.attend: window and max_new must not be negative")
         if out is None:

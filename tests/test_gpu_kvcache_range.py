@@ -205,3 +205,11 @@ def test_queries_of_any_size(cuda, dtype, size, new, most):
     scale = 2.0 ** -3 / size
     got, tiles = attend(c, tables, q, lens, [new, new], most, scale)
     compare(got, tiles, q, held, lens, [new, new], scale)
+
+
+def test_scale_must_be_finite(cuda):
+    c, tables, _ = filled(cuda, [3], 1, 64, 16, "Q4_0", "Q4_0")
+    q, lens = torch.zeros(1, 2, 64, device=cuda), torch.tensor([3], dtype=torch.int32, device=cuda)
+    for scale in (float("nan"), float("inf"), -1e39, 1e300):
+        with pytest.raises(RuntimeError):
+            c.attend(q, tables, lens, scale=scale)

@@ -3,7 +3,7 @@ import pytest
 
 from nemicli_terminal_b200 import _lib
 
-from tests.test_kvcache import attend, cache
+from tests.test_kvcache import A, attend, cache
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
@@ -15,3 +15,11 @@ def test_more_rows_than_positions_are_refused(dtype, heads, new):
     assert attend(dtype=dtype, heads=heads, qs=64 * heads, new=new) == 4
     at_most = (1 << 30) // (heads // 2)
     assert need(cache(), heads, 1, at_most, dtype, 1, 0) > 0
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_scales_without_a_size_are_refused(scale):
+    L = _lib.load()
+    call = lambda s: L.qmv_kv_attend(cache(), A, 0, 256, 4, A, 1, A, A, 1, 0, 1, s, 0, A, A, 1 << 34, None)      # noqa: E731
+    assert call(scale) == 2
+    assert call(0.0) == call(-1e38) == 0             # (no rows: no launch)
