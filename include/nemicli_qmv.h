@@ -340,7 +340,7 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
  * tokens in the cache at the pages tables[b][0 .. table_width), the new ones (its query rows) last: rows
  * starts[b] .. starts[b + 1] of q, or row b when starts is null.  Query i of n sits at position p = lens[b] - n + i and
  * sees keys max(0, p - window + 1) .. p (window 0: from 0 on); one that sees none (p < 0) gives zeros.  q: rows of
- * n_heads * dim values, q_stride apart (aligned to four values); out dense.  scale: finite.  max_new: at least the longest run of new
+ * n_heads * dim values, q_stride apart (aligned to four values); out dense (q itself too, where that is dense).  scale: finite.  max_new: at least the longest run of new
  * tokens (rows beyond it are not computed, QMV_DEV_BAD_ADDRESS is set; n_seq * max_new also decides between two
  * kernels, so a tight bound is the faster one; with starts null it counts as 1, for the workspace too).  Rows of out that no sequence covers stay
  * as they are.  Table entries behind a sequence's last token are not read; pages outside the cache count as

@@ -26,7 +26,6 @@
 
 namespace qmv {
 
-constexpr int kKvMaxDim = 256;
 constexpr float kKvMax = 65504.0f;        // values are clamped to fp16's range before they are quantised
 
 struct KvView {

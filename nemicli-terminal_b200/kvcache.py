@@ -172,8 +172,8 @@ class KVCache:
         sequence, or with starts int32 (sequences + 1,) rows starts[b] .. starts[b + 1] for sequence b, its last tokens;
         max_new: at least the most new tokens of a sequence (default: all rows; it chooses between two kernels, so a
         tight bound is the faster one).  scale: default dim ** -0.5.  window: a
-        query sees that many keys up to its own (0: all).  -> like q, rows side by side; in `out` (contiguous) if
-        given; rows that no sequence covers keep what out held (without `out` they are undefined).  Queries that
+        query sees that many keys up to its own (0: all).  -> like q, rows side by side; in `out` (contiguous; q itself if
+        that is) if given; rows that no sequence covers keep what out held (without `out` they are undefined).  Queries that
         see no key give zeros.  16-bit queries: weights are held in float16 (2^-11 of themselves, or 2^-34 of the row's largest),
         many rows' keys and values too; float32 queries: two float16 parts (2^-21, or 2^-35 of the largest)."""
         self._tokens(q, "KVCache.attend q")

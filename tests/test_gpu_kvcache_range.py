@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from nemicli_terminal_b200 import kvcache
+from nemicli_terminal_b200 import _lib, kvcache
 
 from tests import kv_helpers as KH
 from tests.test_gpu_kvcache import BF16, F16, F32, MANY, filled, gen, slots_of, tables_of
@@ -213,3 +213,41 @@ def test_scale_must_be_finite(cuda):
     for scale in (float("nan"), float("inf"), -1e39, 1e300):
         with pytest.raises(RuntimeError):
             c.attend(q, tables, lens, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("window", [0, 30])
+@pytest.mark.parametrize("new, most", [(1, 1), (6, 6), (70, MANY)])
+def test_scale_zero_and_negative(cuda, dtype, scale, window, new, most):
+    """Masked keys stay masked whatever the scale's sign, the causal and the window's border inside a unit of keys."""
+    lens = [200, 77]
+    c, tables, held = filled(cuda, lens, 2, 128, 16, "Q8_0", "Q4_0")
+    q = torch.randn(2 * new, 8, 128, generator=gen(5, cuda), device=cuda).to(dtype)
+    got, tiles = attend(c, tables, q, lens, [new, new], most, scale, window)
+    compare(got, tiles, q, held, lens, [new, new], scale, window)
+
+
+def test_no_rows(cuda):
+    c = kvcache.KVCache(2, 1, 64, 16, "Q8_0", "Q8_0", cuda)
+    x, s = torch.randn(0, 1, 64, device=cuda), torch.arange(0, device=cuda)
+    assert c.write(x, x, s) is None
+    assert c.write(x, x, s, q=torch.randn(0, 3, 64, device=cuda)).shape == (0, 3, 64)
+    k, v = c.read(s, F32)
+    assert k.shape == (0, 1, 64) and v.shape == (0, 1, 64)
+    assert _lib.device_status(device=cuda) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens, new, most", CALLS)
+def test_out_over_the_queries(cuda, dtype, lens, new, most):
+    """out may be q itself: a row's queries are read before it is written, by every part of a cut sequence too."""
+    c, tables, held = filled(cuda, lens, 2, 64, 16, "Q8_0", "Q4_0")
+    n = [new] * len(lens)
+    q = torch.randn(most if most == MANY else new * len(lens), 8, 64, generator=gen(6, cuda), device=cuda).to(dtype)
+    starts = torch.arange(len(lens) + 1, dtype=torch.int32, device=cuda) * new
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    want = c.attend(q, tables, lt, starts, max_new=most)[:sum(n)]
+    out = q.clone()
+    assert torch.equal(c.attend(out, tables, lt, starts, max_new=most, out=out)[:sum(n)], want)
+    assert torch.equal(out[sum(n):], q[sum(n):])
