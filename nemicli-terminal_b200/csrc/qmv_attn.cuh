@@ -7,8 +7,9 @@
 // Bound by reading the cache once (4.5 or 8.5 bits a value), so what counts is instructions per value: at 6.5 TB/s an SM
 // sees about 40 four-bit values a clock.  Both products run on mma.sync m16n8k16 (fp16 in, fp32 sums) with the cache as
 // the 16-row operand, as it lies: the codes' bits ARE the operand.  A code c masked out of its word
-// is the fp16 denormal c 2^-24 (16 c 2^-24 for the upper nibble of a byte), which the tensor cores multiply exactly, so a
-// 4-bit pair costs one AND and no conversion; the factor 2^24 and the queries' 1 / 16 are folded into constants.
+// is the fp16 denormal c 2^-24 (16 c 2^-24 for the upper nibble of a byte, c 2^-18 for V's nibbles), which the tensor cores
+// multiply exactly, so a 4-bit pair costs one AND (V's a shift too) and no conversion; these factors and the queries' 1 / 16 are folded
+// into constants.
 // (tcgen05 would need the unpacked values written to shared memory first, more bytes a clock than an SM writes.)  The codes'
 // offset (8 or 128) comes out as its own term: in the scores it is the accumulator's start, -off sum_i q[i] per block,
 // in the output one more product with a constant row a block.  (fp32 queries take it off the codes first: the term is many
@@ -111,6 +112,14 @@ __device__ __forceinline__ void code_pairs(const uint32_t* w, uint32_t (&o)[4]) 
             }
         }
     }
+}
+
+// V's four nibbles a half for the second product, each at bits 6 to 9: c 2^-18.  The tensor cores align a step's products at the largest
+// exponent before they cut them off, and a denormal counts there as 2^-14, whatever its bits.  At c 2^-24 a step of 16 keys lost up to
+// 2^-11 of a block's largest value (2^-16 on random data, all one way in the upper nibbles), at c 2^-18 2^-17; 64 sequences 113 ->
+// 116 us for the shifts.  K's codes stay as they are: the queries' signs keep what is cut off from adding up.
+__device__ __forceinline__ void v_pairs(uint32_t w, uint32_t (&o)[4]) {
+    o[0] = (w << 6) & 0x03C003C0u, o[1] = (w << 2) & 0x03C003C0u, o[2] = (w >> 2) & 0x03C003C0u, o[3] = (w >> 6) & 0x03C003C0u;
 }
 
 // f(std::integral_constant<int, 0>) .. of N
@@ -284,7 +293,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
     constexpr bool HL = DT == QMV_OUT_F32;                       // queries and weights as two fp16 parts
     constexpr int D = 32 * J, R = 8 * NT, kParts = HL ? 2 : 1;
     constexpr float kOffK = KB == 4 ? 8.f : 128.f;
-    constexpr uint32_t kOffV = VB == 4 ? 0x00080008u : 0x00800080u;
+    constexpr uint32_t kOffV = VB == 4 ? 0x02000200u : 0x00800080u;
     constexpr int S_ = attn_stages(HL, J, KB, VB, NT), KT = attn_tiles(J, NT), kUnit = attn_unit(J, NT);
     using Slot = AttnSlot<J, KB, VB, KT>;
     static_assert(Slot::kBytes == attn_unit_bytes(J, KB, VB, NT), "the launch's shared memory");
@@ -711,7 +720,8 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {             // pair t (k 2 t, 2 t + 1), pair t + 4 (k 8 + 2 t, 9 + 2 t)
                             uint32_t v[4];
-                            code_pairs<VB, HL>(&vw[x][h][j * VB / 4], v);
+                            if constexpr (VB == 4 && !HL) v_pairs(vw[x][h][j], v);
+                            else code_pairs<VB, HL>(&vw[x][h][j * VB / 4], v);
                             a[0][2 * h] = v[0], a[0][2 * h + 1] = v[1], a[1][2 * h] = v[2], a[1][2 * h + 1] = v[3];
                         }
                         float d[4];
@@ -752,12 +762,12 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    constexpr float kUp = HL ? 1.f : 16777216.f, kHigh = VB == 4 && !HL ? kUp / 16.f : kUp;
+                    constexpr float kUp = HL ? 1.f : VB == 4 ? 262144.f : 16777216.f;
                     const float z0 = __shfl_sync(0xffffffffu, off[nt][0], 4 * j + t) * kUp, z1 = __shfl_sync(0xffffffffu, off[nt][1], 4 * j + t) * kUp;
                     const float(&x)[2][4] = o[nt][j];
                     float* p = own + (8 * nt + 2 * t) * D + 32 * j + 4 * g;
-                    *reinterpret_cast<float4*>(p) = make_float4(fmaf(x[0][0], kUp, -z0), fmaf(x[0][2], kHigh, -z0), fmaf(x[1][0], kUp, -z0), fmaf(x[1][2], kHigh, -z0));
-                    *reinterpret_cast<float4*>(p + D) = make_float4(fmaf(x[0][1], kUp, -z1), fmaf(x[0][3], kHigh, -z1), fmaf(x[1][1], kUp, -z1), fmaf(x[1][3], kHigh, -z1));
+                    *reinterpret_cast<float4*>(p) = make_float4(fmaf(x[0][0], kUp, -z0), fmaf(x[0][2], kUp, -z0), fmaf(x[1][0], kUp, -z0), fmaf(x[1][2], kUp, -z0));
+                    *reinterpret_cast<float4*>(p + D) = make_float4(fmaf(x[0][1], kUp, -z1), fmaf(x[0][3], kUp, -z1), fmaf(x[1][1], kUp, -z1), fmaf(x[1][3], kUp, -z1));
                 }
                 sum[nt] += __shfl_xor_sync(0xffffffffu, sum[nt], 1);
                 sum[nt] += __shfl_xor_sync(0xffffffffu, sum[nt], 2);

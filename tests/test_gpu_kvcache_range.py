@@ -47,9 +47,10 @@ def test_clamped_values(cuda, dtype, dim, kf, vf, most):
     query that sees them, and nothing to those before.  The queries' share of K's clamped channel is small, so that its score
     is an ordinary one.
     One bound more than KH.bound's where the codes' bits are the operand (16-bit queries, no tiles): the tensor cores align a
-    step's 16 products at the largest exponent and cut each off there, 2^-23 of it, and a code c 2^-24, a denormal, counts as
-    2^-14: each loses up to 2^-37 p d, or 2^-13 p d once 2^24 is taken off; 16 of a step 2^-9 p d, for the codes and for
-    their offset 2^-8 p d together.  A block's largest value is 8 d at least: 2^-11 of it."""
+    step's 16 products at the largest exponent and cut each off there, 2^-23 of it, and a code c 2^-24 (8 bits; 4 bits:
+    c 2^-18), a denormal, counts as 2^-14: each loses up to 2^-37 p d, or 2^-13 p d (2^-19) once 2^24 (2^18) is taken off; 16
+    of a step 2^-9 p d (2^-15), codes and offset together 2^-8 (2^-14).  A block's largest value is 127 d (7 d): 2^-15 of
+    it (2^-16)."""
     g = gen(1, cuda)
     tables, pages = tables_of([90], 16, 1, cuda)
     c = kvcache.KVCache(pages, 2, dim, 16, kf, vf, cuda)
@@ -68,7 +69,7 @@ def test_clamped_values(cuda, dtype, dim, kf, vf, most):
     assert tiles == (most == MANY and dtype == BF16)
     bits = dtype == BF16 and not tiles
     compare(got, tiles, q, held, [90], [90], dim ** -0.5,
-            tol_of=lambda sizes, o, keys: KH.bound(sizes, o, dtype, keys, tiles) + 2.0 ** -11 * sizes[1] * bits)
+            tol_of=lambda sizes, o, keys: KH.bound(sizes, o, dtype, keys, tiles) + 2.0 ** (-15 if vf == "Q8_0" else -16) * sizes[1] * bits)
 
 
 @pytest.mark.parametrize("fmt", ["Q4_0", "Q8_0"])
@@ -91,6 +92,21 @@ def test_clamped_values_in_float16(cuda, fmt):
         q = torch.zeros(new, 4, 64, dtype=F16, device=cuda)
         got, _ = attend(c, t, q, [2], [new], most)
         assert torch.equal(got, want.half().expand(new, 4, 64))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("kf", ["Q4_0", "Q8_0"])
+@pytest.mark.parametrize("vf", ["Q4_0", "Q8_0"])
+@pytest.mark.parametrize("dim, n_kv, group", [(64, 8, 1), (128, 3, 8), (256, 2, 7), (96, 2, 4)])
+def test_values_under_a_larger_key(cuda, dtype, kf, vf, dim, n_kv, group):
+    """Sums near 0 beside a key whose values are far larger: few keys, so that a step's largest product stands alone."""
+    lens, new = [21, 22, 37, 53, 14, 33, 112, 24], [3, 9, 4, 1, 3, 3, 10, 1]
+    for seed in range(6):
+        c, tables, held = filled(cuda, lens, n_kv, dim, 32, kf, vf, seed=seed)
+        q = torch.randn(sum(new), n_kv * group, dim, generator=gen(seed, cuda), device=cuda).to(dtype)
+        got, tiles = attend(c, tables, q, lens, new, max(new))
+        assert not tiles
+        compare(got, tiles, q, held, lens, new, dim ** -0.5)
 
 
 # ---- weights far apart, values of any size ---------------------------------------------------------------
