@@ -22,8 +22,8 @@
 // product. (Second parts 2^11 times as large against codes 2^-11 times as large would go down to 2^-46; they take 44 us for one
 // sequence of 65519 tokens where this takes 40.) The softmax reference only moves when a score passes it by 2^4 or a d_v the next
 // power of two (checked with one vote a tile). p d_v is rounded to fp16 once: it stays below 2^15 and is 2^10 at least for the
-// reference and the largest d_v, whatever V's size, so 2^-24 of that is still a normal number. (p as fp16 times d_v as fp16 took 112
-// us for 64 sequences of bf16 queries where this takes 116, but holds no p large enough for a small d_v.) Sums and statistics are
+// reference and the largest d_v, whatever V's size, so 2^-24 of that is still a normal number. (p as fp16 times d_v as fp16 took 3 %
+// less for 64 sequences of bf16 queries, but holds no p large enough for a small d_v.) Sums and statistics are
 // fp32.
 //
 // Work: units of 64 or 128 keys (one or two tiles of 16 a warp) of segments (sequence, key head, tile of 8 NT rows); the list of all units is cut into
@@ -116,8 +116,8 @@ __device__ __forceinline__ void code_pairs(const uint32_t* w, uint32_t (&o)[4]) 
 
 // V's four nibbles a half for the second product, each at bits 6 to 9: c 2^-18.  The tensor cores align a step's products at the largest
 // exponent before they cut them off, and a denormal counts there as 2^-14, whatever its bits.  At c 2^-24 a step of 16 keys lost up to
-// 2^-11 of a block's largest value (2^-16 on random data, all one way in the upper nibbles), at c 2^-18 2^-17; 64 sequences 113 ->
-// 116 us for the shifts.  K's codes stay as they are: the queries' signs keep what is cut off from adding up.
+// 2^-11 of a block's largest value (2^-16 on random data, all one way in the upper nibbles), at c 2^-18 2^-17; the
+// shifts cost 3 % for 64 sequences.  K's codes stay as they are: the queries' signs keep what is cut off from adding up.
 __device__ __forceinline__ void v_pairs(uint32_t w, uint32_t (&o)[4]) {
     o[0] = (w << 6) & 0x03C003C0u, o[1] = (w << 2) & 0x03C003C0u, o[2] = (w >> 2) & 0x03C003C0u, o[3] = (w >> 6) & 0x03C003C0u;
 }
@@ -217,9 +217,9 @@ struct AttnSlot {
     }
 };
 // Tiles of 16 keys a warp works on at once (two: each instruction has another that does not wait for it, and the loop's and
-// the softmax's bookkeeping counts half; 64 sequences of up to 8191 keys, 8 heads of 128: 115 us, with one 139), keys a unit, CTAs
-// an SM is to hold (heads of 64 or 96 values: three, 64 sequences of 8192 keys 104 and 130 us against 122 and 145 with two; of 128:
-// two, whose registers hold everything, three spill, 104 us against 96 for 32 sequences of 8175 keys), and the units in a
+// the softmax's bookkeeping counts half; 64 sequences of 8191 keys, 8 heads of 128: 174 us, with one 220), keys a unit, CTAs
+// an SM is to hold (heads of 64 or 96 values: three, 64 sequences of 8192 keys 112 and 142 us against 131 and 157 with two; of 128:
+// two, whose registers hold everything, three spill, 101 us against 95 for 32 sequences of 8175 keys), and the units in a
 // CTA's ring, within 227 KB an SM.
 __host__ __device__ constexpr int attn_tiles(int J, int nt) { return J < 8 && nt == 1 ? 2 : 1; }
 __host__ __device__ constexpr int attn_unit(int J, int nt) { return 16 * kAttnWarps * attn_tiles(J, nt); }
@@ -903,8 +903,8 @@ inline AttnPlan attn_plan(const KvView& c, int dtype, int n_heads, int n_seq, in
     AttnPlan p{};
     const bool hl = dtype == QMV_OUT_F32;
     const long long rows = (long long)max_new * (n_heads / c.n_kv);
-    // Two tiles of 8 rows share a cache tile's unpacked words (8 sequences of 4096 keys, 8 heads of 128: 16 rows 30 us against 33, 64
-    // rows 75 against 91); not where their sums do not fit the registers (heads of 256) or both parts of fp32 queries use the rows.
+    // Two tiles of 8 rows share a cache tile's unpacked words (8 sequences of 4096 keys, 8 heads of 128: 16 rows 34 us against 36);
+    // not where their sums do not fit the registers (heads of 256) or both parts of fp32 queries use the rows.
     p.nt = rows > 8 && !hl && c.J < 8 ? 2 : 1;
     p.row_tiles = int((rows + 8 * p.nt - 1) / (8 * p.nt));
     const long long segs = (long long)n_seq * c.n_kv * p.row_tiles;

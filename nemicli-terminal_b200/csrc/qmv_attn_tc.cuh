@@ -5,16 +5,16 @@
 //
 // A CTA takes NQ tiles of 128 query rows of one sequence and key head (row = token * group + head of the group, so
 // the cache is unpacked once for the whole group) over all their keys.  For two tiles, 64 keys and 128 values a step takes
-// 1024 clocks of MMA (both products), 1024 of exp2 (16 a clock and SM) and about 1540 of shared memory (the operands of the
-// scores, queries among them, 768; V 512; the producers' stores 256), all side by side; measured about 2200 (8192 tokens, 32 heads:
-// 0.58 to 0.61 ms, 900 TFLOP/s), the MMAs' issue waiting for their operands.  Scores of 128 keys at a time would read the
-// queries half as often, but two buffers of them do not fit tensor memory beside the sums.  Roles:
+// 1280 clocks of MMA (the scores 768: one of 64 keys from shared memory takes 48 clocks, not 32; the sums 512), 1024 of exp2 (16 a
+// clock and SM) and 1280 of shared memory (128 bytes a clock: the scores' operands 768, V 256, the producers' stores 256), all side by
+// side; measured about 2200 (8192 tokens, 32 heads: 0.58 to 0.62 ms, 880 to 900 TFLOP/s): no pipe is full, each role waits for another.
+// Scores of 128 keys would take their 64 clocks an MMA and half the waits, with one buffer a query tile and the two tiles in turn.  Roles:
 //   producers  NP x 4 warps: words of the cache -> d * code in fp16 (one rounding) -> shared memory, in the MMA's K-major core
 //              matrices (8 rows x 16 bytes; K: rows = keys, V: rows = values of the head, so a V word, whose halves
 //              are two tokens, lands transposed without a shuffle).  Loads one round ahead in registers, page numbers two.
 //              Heads of 256 values have one query tile's time for twice the unpacking: two groups take the rounds in turn
 //              (6 prompts of up to 1500 tokens on up to 6001, window 1024, 16 heads on 8: 287 -> 262 us), and V's stage is waited
-//              for behind K's (-> 240).
+//              for behind K's (-> 240; 236 to 244 now).
 //   MMA        one warp: the scores run two steps ahead of the sums, the other tile's softmax runs meanwhile.
 //   softmax    NQ x 4 warps, one thread a row: scores from tensor memory, P as fp16 over them, and the row's
 //              reference, sum and mask in registers.  P is 2^9 where the reference was set and moves it only past 2^15 (then the
@@ -753,16 +753,16 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
 // ---- host -------------------------------------------------------------------------------------------
 
 // Whether a call takes the tiles (else attn_kernel), and how.  A tile walks its keys at a cost that its rows do not change, one
-// CTA an SM: 14.5 ns a key for heads of 64 values, 17.8 for 128, 18.5 for 256.  attn_kernel spreads any work over the GPU, at
-// a cost that goes with the rows: 2.3, 3.3 and 11 ps a key and row.  So the tiles gain from as many rows a round of CTAs as
+// CTA an SM: 14.7 ns a key for heads of 64 values, 17.9 for 128, 20.4 for 256.  attn_kernel spreads any work over the GPU, at
+// a cost that goes with the rows: 2.6, 3.5 and 11.4 ps a key and row (both measured on 128 tokens and 32768 keys).  So the tiles gain from as many rows a round of CTAs as
 // the ratio of the two.  Where the tiles fill at most half the SMs and there are keys enough to pay for a second launch
 // (512 a part: 9 us of work, the launch 4 to 5), each one's keys are cut into as many parts as fill the GPU, and
 // attn_tc_join_kernel adds them.  Measured in us, cut / uncut / attn_kernel, heads of 128 values, 8 key heads, 4 query heads each:
-//   1 sequence of 32768 keys, 16 new tokens: 49 / 584 / 68      64 tokens: 52 / 586 / 228
-//   8 sequences of 4096 keys, 16 tokens: 47 / 80 / 75           64 tokens: 53 / 82 / 250
-//   1 sequence of 4096 keys, 16 tokens: not used, 22            64 tokens: 22 / 81 / 44
-//   32 sequences of 1024 keys, 24 tokens: - / 51 / 126
-// and 4 key heads of 256 values, 8 sequences of 4096 keys, 4 tokens: 32 / 85 / 38
+//   1 sequence of 32768 keys, 16 new tokens: 53 / 585 / 75      64 tokens: 56 / 586 / 248
+//   8 sequences of 4096 keys, 16 tokens: 51 / 82 / 81           64 tokens: 57 / 83 / 267
+//   1 sequence of 4096 keys, 16 tokens: 21 / 81 / 26 (the last is taken)    64 tokens: 25 / 82 / 50
+//   32 sequences of 1024 keys, 24 tokens: - / 55 / 136
+// and 64 heads on 4 of 256 values, 8 sequences of 4096 keys, 4 tokens: 37 / 90 / 119
 struct AttnTcPlan {
     bool used;
     int row_tiles, split;

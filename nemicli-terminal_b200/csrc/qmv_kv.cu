@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
 }
 
 // Warps a row and passes a warp: rows on their own where they fill the GPU (32 warps an SM), else cut so that there are as
-// many, one pass each at least (512 bf16 rows of 8 key heads of 128 with 32 query heads: 7.4 us, uncut 12.4, for 16 warps an SM
+// many, one pass each at least (512 bf16 rows of 8 key heads of 128 with 32 query heads, calls in a graph: 7.7 us, uncut 12.4, for 16 warps an SM
 // 8.4, for 64 8.1; 64 rows: 3.2, uncut 12.2); the launch's CTAs, 0 if they pass a grid.
 unsigned cut_rows(long long rows, int passes, int& parts, int& per_part) {
     const long long want = 32LL * sm_count();

@@ -267,7 +267,7 @@ extern "C" int qmv_norm_block(const void* y, long long y_stride, const void* h, 
         constexpr int DT = decltype(c)::value;
         if (whole) {
             // Pieces a thread: for rows that fill the GPU CTAs of about 256 threads (8192 rows of 4096 values: bf16 52 us, fp32 83;
-            // of up to 1024 threads 74 and 104), else the fewest (one row: fp32 2.8 us, with 256 threads 3.4).  C 4 with up
+            // of up to 1024 threads 74 and 104), else the fewest (one row, 200 calls in a graph: fp32 2.6 us a call, with 256 threads 3.4).  C 4 with up
             // to 512 threads has the registers for it.  Rows of more than 4096 pieces are left to the other kernel
             const int pieces = n * int(one) / 16, most = rows >= 2LL * sm_count() ? 256 : 1024;
             const int C = pieces <= most ? 1 : pieces <= 2 * most ? 2 : 4;
