@@ -335,8 +335,9 @@ int64_t qmv_kv_attend_workspace_bytes(const qmv_kv_cache* cache, int n_heads, in
 /* Causal attention of n_seq sequences over the cache: out = softmax(scale * q . k) v per query row and head, scores,
  * statistics and sums fp32, q and out of type dtype (QMV_OUT_*).  Rounded on the way: with 16-bit queries the weights (where
  * few rows are computed: weight times V's scale) to float16, where many rows are K and V too (d * code); float32 queries have two
- * float16 parts in each of these places.  A weight is held to 2^-11 of itself (float32: 2^-21) or 2^-34 (2^-35) of the row's
- * largest, whichever is more.  Head h reads key head h / (n_heads / n_kv).  Sequence b: lens[b]
+ * float16 parts in each of these places.  These products are held to 2^-11 of themselves
+ * (float32: 2^-21) or 2^-34 (2^-35) of the row's largest weight, times the largest V scale where V's scale is in them, whichever is
+ * more.  Head h reads key head h / (n_heads / n_kv).  Sequence b: lens[b]
  * tokens in the cache at the pages tables[b][0 .. table_width), the new ones (its query rows) last: rows
  * starts[b] .. starts[b + 1] of q, or row b when starts is null.  Query i of n sits at position p = lens[b] - n + i and
  * sees keys max(0, p - window + 1) .. p (window 0: from 0 on); one that sees none (p < 0) gives zeros.  q: rows of

@@ -174,8 +174,9 @@ class KVCache:
         tight bound is the faster one).  scale: default dim ** -0.5.  window: a
         query sees that many keys up to its own (0: all).  -> like q, rows side by side; in `out` (contiguous; q itself if
         that is) if given; rows that no sequence covers keep what out held (without `out` they are undefined).  Queries that
-        see no key give zeros.  16-bit queries: weights are held in float16 (2^-11 of themselves, or 2^-34 of the row's largest),
-        many rows' keys and values too; float32 queries: two float16 parts (2^-21, or 2^-35 of the largest)."""
+        see no key give zeros.  16-bit queries: weights (few rows: times V's scales) are held in float16,
+        to 2^-11 of themselves or 2^-34 of the largest in the row, many rows' keys and values too; float32 queries: two float16
+        parts, 2^-21 or 2^-35 of the largest."""
         self._tokens(q, "KVCache.attend q")
         rows, heads, _ = q.shape
         if heads % self.n_kv:
