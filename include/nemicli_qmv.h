@@ -356,6 +356,106 @@ int qmv_kv_attend(const qmv_kv_cache* cache, const void* q, int dtype, long long
                   int max_new, float scale, int window, void* out, void* workspace, long long workspace_bytes,
                   void* stream);
 
+/* qmv_kv_write for tokens that have a position on each of up to four axes (time, height and width of a picture): positions
+ * [n_axes][rows], axes [rot_dim / 2] (host memory, read by the call) names the axis of each frequency: frequency f of a row turns by
+ * cos_table, sin_table[positions[axes[f]][row]][f].  A row with a position outside the tables on any axis is not written.  Everything
+ * else as there.  Replaces: nothing (the reference's cache write takes one position a token). */
+int qmv_kv_write_axes(const qmv_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride,
+                      long long v_stride, const long long* slots, long long rows, const float* cos_table,
+                      const float* sin_table, const long long* positions, long long n_positions, int rot_dim, int paired,
+                      const uint8_t* axes, int n_axes, const void* q, long long q_stride, int n_q, void* q_out,
+                      void* stream);
+
+/* Copies the first used[i] tokens (null: all; rounded up to two for V, whose tokens lie in pairs) of page src[i] to page dst[i],
+ * i < n, all key heads; a negative src or dst: nothing.  Pages outside the cache are skipped and set QMV_DEV_BAD_ADDRESS.  No page is
+ * the target of two copies, nor target and source.  One launch.  Replaces: nothing. */
+int qmv_kv_copy(const qmv_kv_cache* cache, const int* src, const int* dst, const int* used, int n, void* stream);
+
+/* Boxes around the keys of pages: bounds [n_pages][n_kv][2][dim] fp16 (16-byte aligned), the least and the largest value of each
+ * channel over a page's keys, rounded outwards, within +-65504.  Written for the pages that the newest tokens of each sequence
+ * completed: places (lens[b] - new) / page .. lens[b] / page - 1 of tables[b], new = starts[b + 1] - starts[b] (null: 1).  max_new: at
+ * least the most new tokens of a sequence (pages beyond what it allows are left, and QMV_DEV_BAD_ADDRESS is set, as by pages outside
+ * the cache and lengths beyond the table).  One launch.  Replaces: nothing. */
+int qmv_kv_bounds(const qmv_kv_cache* cache, const int* tables, int table_width, const int* lens, const int* starts, int n_seq,
+                  int max_new, void* bounds, void* stream);
+
+/* Bytes of the workspace qmv_kv_choose needs for these sizes (0 for sizes it does not take). */
+int64_t qmv_kv_choose_workspace_bytes(const qmv_kv_cache* cache, int table_width, long long n_rows, int keep);
+
+/* The pages that each query row looks at, for each key head: chosen [n_rows][n_kv][keep], in the order of the sequence, -1 behind
+ * them, and held [n_rows] the tokens in them up to the query's own.  A query at position p has the pages 0 .. p / page of its
+ * sequence; where these are more than keep, the first `first`, the last `last` (at least 1: the query's own, whose box need not be
+ * written) and of the others those with the largest
+ *     max over the key head's query heads of sum_c max(q[c] lo[c], q[c] hi[c])
+ * (no product q . k of the page is larger), computed in fp64, the earlier page first among equals; NaN counts as least.  q, tables,
+ * lens, starts as for qmv_kv_attend; rows that no sequence covers, or with p < 0, get no page and held 0.  At most 65535 rows and
+ * 64 query heads a key head.  workspace: 256-byte aligned, qmv_kv_choose_workspace_bytes long.  Two launches.  Replaces: nothing. */
+int qmv_kv_choose(const qmv_kv_cache* cache, const void* q, int dtype, long long q_stride, int n_heads, const void* bounds,
+                  const int* tables, int table_width, const int* lens, const int* starts, int n_seq, long long n_rows, int keep,
+                  int first, int last, int* chosen, int* held, void* workspace, long long workspace_bytes, void* stream);
+
+/* Bytes of the workspace qmv_kv_attend_chosen needs for these sizes (0 for sizes it does not take). */
+int64_t qmv_kv_attend_chosen_workspace_bytes(const qmv_kv_cache* cache, int n_heads, long long n_rows, int dtype, int keep);
+
+/* Attention of each query row over its chosen pages, as qmv_kv_attend computes it: row r and key head h see the first held[r] tokens
+ * of the pages chosen[r][h][0 .. keep).  Rows with held 0 give zeros.  At most 65535 rows.  Replaces: nothing. */
+int qmv_kv_attend_chosen(const qmv_kv_cache* cache, const void* q, int dtype, long long q_stride, int n_heads, const int* chosen,
+                         int keep, const int* held, long long n_rows, float scale, void* out, void* workspace,
+                         long long workspace_bytes, void* stream);
+
+/* ---- page tables of such a cache ---------------------------------------------------------------------- */
+
+/* Free pages are a stack: free_pages [n_pages], of which the first counts[0] count and the last is taken first; counts[1] is a
+ * running number of pages that were asked for in vain.  All arrays are device memory, the outputs are not the inputs' own (free_pages
+ * and the tables apart, as named), and the same call on the same inputs gives the same again.  Pages of 16 to 1024 tokens (a power of
+ * two), at most 65535 sequences and 2^30 tokens a table. */
+
+/* A step's bookkeeping: sequence b holds lens[b] tokens and gets add[b] more.  The pages it lacks are taken from the stack, in the
+ * order of sequences, and written to its table (tables [n_seq][table_width]); lens_out[b] = lens[b] + add[b], starts [n_seq + 1]: the
+ * first row of each sequence.  Row r < rows is a new token, slots[r] its slot and positions[r] its place in the sequence; rows behind the last token have slot -1
+ * and position 0.  Tokens beyond the table's end are dropped (they have no row), as are negative numbers of tokens; tokens beyond `rows`
+ * have a page but no row; tokens whose page is missing have slot -1 and a table entry -1: each of these sets
+ * QMV_DEV_BAD_ADDRESS.  counts_out: what is left.  One launch.  Replaces: nothing. */
+int qmv_page_plan(const int* lens, const int* add, int* tables, int n_seq, int table_width, int page, const int* free_pages,
+                  int n_pages, const int* counts, long long rows, long long* slots, long long* positions, int* starts,
+                  int* lens_out, int* counts_out, void* stream);
+
+/* The pages of the sequences with done[b] != 0 go onto the stack, in order; lens_out[b] = 0 there and lens[b] elsewhere.  The tables
+ * stay.  Pages beyond n_pages are dropped and set QMV_DEV_BAD_ADDRESS.  One launch.  Replaces: nothing. */
+int qmv_page_release(const uint8_t* done, const int* lens, const int* tables, int n_seq, int table_width, int page,
+                     int* free_pages, int n_pages, const int* counts, int* lens_out, int* counts_out, void* stream);
+
+/* Bytes of the workspace qmv_page_reorder needs for these sizes (0 for sizes it does not take). */
+int64_t qmv_page_reorder_workspace_bytes(int n_req, int beams, int table_width);
+
+/* The next step's tables of a beam search: beam j of request r goes on from beam parents[r][j] (-1: ends) of the tables [n_req][beams]
+ * [table_width] and lens [n_req][beams].  Beams of a request share whole pages, at the same place of their tables; pages that no
+ * beam holds any more become free, in the order of place, then beam (the first own[r] places are not the request's and stay; own null:
+ * 0).  Of the beams that would write to the same partly filled page the first keeps it and the others get a copy (all of them
+ * where the page is not the request's): src, dst, used [n_req][beams] name the page to copy, the new one and its tokens
+ * (-1, -1, 0: none), for qmv_kv_copy of each layer.  New pages are the request's own freed ones, in order, then the stack's, onto which all the
+ * other freed ones went before; -1 where none is left (counts_out[1] counts them).  tables_out, lens_out: as tables and lens, -1 behind a beam's pages.  Parents
+ * outside the request count as -1 and set QMV_DEV_BAD_ADDRESS.  At most 64 beams and 65535 in all.  workspace: 256-byte aligned.  Two launches.
+ * Replaces: nothing. */
+int qmv_page_reorder(const int* parents, const int* lens, const int* tables, const int* own, int n_req, int beams, int table_width,
+                     int page, int* free_pages, int n_pages, const int* counts, int* tables_out, int* lens_out, int* src,
+                     int* dst, int* used, int* counts_out, void* workspace, long long workspace_bytes, void* stream);
+
+/* ---- beam search's choice ------------------------------------------------------------------------------- */
+
+/* Bytes of the workspace qmv_beam_select needs for these sizes (0 for sizes it does not take). */
+int64_t qmv_beam_workspace_bytes(int n_req, int beams, int vocab, int n);
+
+/* The n best continuations of each request: of scores[r][k] + log_softmax(logits[r beams + k])[v] over its beams k and tokens v the n
+ * largest, best first, the lowest k vocab + v among equals -> scores_out, parents (k), tokens (v) [n_req][n].  logits: rows row_stride
+ * values apart, of type dtype (QMV_OUT_*), any alignment; NaN counts as -inf, +inf as the largest float; a row of -inf alone and a
+ * score of -inf give -inf throughout (NaN too).  Exponentials in fp32, their sums and everything behind them in fp64, scores_out rounded
+ * once.  n at most 64, beams at most 64, n_req * beams 65535, vocab 2^30, n at most beams * vocab.  workspace: 256-byte aligned.  Two
+ * launches.  Replaces: nothing. */
+int qmv_beam_select(const void* logits, int dtype, long long row_stride, int n_req, int beams, int vocab, const float* scores,
+                    int n, float* scores_out, int* parents, int* tokens, void* workspace, long long workspace_bytes,
+                    void* stream);
+
 /* The norms before and after a block with its gate and residual, any number of rows of n values (dtype QMV_OUT_*
  * for y, h, gate, h_out and xn; norm weights fp32):
  *     z = y rsqrt(mean(y^2) + eps) w_post     (w_post null: z = y)

@@ -54,6 +54,19 @@ _SIGNATURES = {
     "qmv_kv_read": ([P, P, LL, P, P, I, P], I),
     "qmv_kv_attend_workspace_bytes": ([P, I, I, I, I, I, I], LL),
     "qmv_kv_attend": ([P, P, I, LL, I, P, I, P, P, I, LL, I, ctypes.c_float, I, P, P, LL, P], I),
+    "qmv_kv_write_axes": ([P, P, P, I, LL, LL, P, LL, P, P, P, LL, I, I, P, I, P, LL, I, P, P], I),
+    "qmv_kv_copy": ([P, P, P, P, I, P], I),
+    "qmv_kv_bounds": ([P, P, I, P, P, I, I, P, P], I),
+    "qmv_kv_choose_workspace_bytes": ([P, I, LL, I], LL),
+    "qmv_kv_choose": ([P, P, I, LL, I, P, P, I, P, P, I, LL, I, I, I, P, P, P, LL, P], I),
+    "qmv_kv_attend_chosen_workspace_bytes": ([P, I, LL, I, I], LL),
+    "qmv_kv_attend_chosen": ([P, P, I, LL, I, P, I, P, LL, ctypes.c_float, P, P, LL, P], I),
+    "qmv_page_plan": ([P, P, P, I, I, I, P, I, P, LL, P, P, P, P, P, P], I),
+    "qmv_page_release": ([P, P, P, I, I, I, P, I, P, P, P, P], I),
+    "qmv_page_reorder_workspace_bytes": ([I, I, I], LL),
+    "qmv_page_reorder": ([P, P, P, P, I, I, I, I, P, I, P, P, P, P, P, P, P, P, LL, P], I),
+    "qmv_beam_workspace_bytes": ([I, I, I, I], LL),
+    "qmv_beam_select": ([P, I, LL, I, I, I, P, I, P, P, P, P, LL, P], I),
     "qmv_norm_block": ([P, LL, P, LL, P, LL, P, P, I, ctypes.c_float, ctypes.c_float, LL, I, P, P, P, P, P, P, P], I),
 }
 

@@ -44,6 +44,8 @@ struct AttnParams {
     long long q_stride;                   // values between query rows
     void* out;                            // [n_rows][n_heads][dim]
     const int* tables;                    // [n_seq][width] page of each run of P tokens
+    long long row_entries;                // entries between sequences' tables, and between those of a sequence's key heads (0: one
+    int head_entries;                     // table for all)
     const int* lens;                      // [n_seq] tokens in the cache, the new ones among them
     const int* starts;                    // [n_seq + 1] first query row (null: row b is sequence b's)
     int width, n_seq, n_heads, n_rows, max_new, window;
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, (attn_ctas(DT == QMV_OUT_F32,
         if (rows > 0) {
             // ---- the units' copies; the first ones start before the queries are looked at
             const int turns = dead ? 0 : todo;
-            const int* table = P.tables + (long long)b * P.width;
+            const int* table = P.tables + b * P.row_entries + (long long)hk * P.head_entries;
             const int key0 = (S.first_unit + unit) * kUnit;
             const uint32_t lane_k = Slot::lane_k(warp, g, t), lane_v = KT * warp * Slot::kTileV + Slot::lane_v(lane),
                            lane_s = (16 * KT * warp + 2 * t) * Slot::kRowS;

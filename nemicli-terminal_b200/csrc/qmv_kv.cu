@@ -19,9 +19,11 @@ struct KvWriteParams {
     const long long* slots;
     const float* cos_t;                   // [n_pos][rot / 2] (or null: no rotation)
     const float* sin_t;
-    const long long* pos;
+    const long long* pos;                 // [axes][rows]
     long long n_pos;
     int rot, paired, n_q;
+    int n_axes;
+    uint64_t axis_of[4];                  // the axis of each frequency, two bits
     int rows, parts, per_part;            // warps a row, passes a warp
     int* status;
 };
@@ -109,7 +111,9 @@ __device__ __forceinline__ float4 raw4(uint2 w, __half) {
 // key heads of 128 values: 46 us (50 in Q4_0), bound by the 142 instructions for four values a lane; with 32 query heads rotated
 // along 88, where the queries' part moves at 6.4 TB/s.  Five or six CTAs an SM (fewer registers) instead of four: 88 and 94.
 // A decode step is bound by its launch (64 tokens written and read, 12 us for both).
-template <int DT, int J>
+// AXES: a row has a position on each of up to four axes and every frequency its axis, so a frequency's angle is the axis's row of the
+// tables.
+template <int DT, int J, bool AXES>
 __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvWriteParams P) {
     using T = typename Elem<DT>::type;
     using W = typename Raw4<DT>::type;
@@ -129,7 +133,19 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     const float* ct = nullptr;
     const float* st = nullptr;
     const int half = P.rot / 2;
-    if (P.cos_t) {
+    long long from[4] = {0, 0, 0, 0};                             // of each axis, its row of the tables
+    if constexpr (AXES) {
+        ct = P.cos_t, st = P.sin_t;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            if (a >= P.n_axes) continue;
+            const long long p = __ldg(P.pos + (long long)a * P.rows + row);
+            lost |= p < 0 || p >= P.n_pos;
+            from[a] = p * half;
+        }
+        bad |= lost;
+        if (lost) from[0] = from[1] = from[2] = from[3] = 0;
+    } else if (P.cos_t) {
         const long long p = __ldg(P.pos + row);
         lost = p < 0 || p >= P.n_pos;
         bad |= lost;
@@ -138,8 +154,20 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     }
     if (bad && lane == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
     const bool write = slot >= 0 && !bad;
+    auto place = [&](int f) {                                     // of frequency f, in the tables
+        const int a = int(P.axis_of[f >> 5] >> (2 * (f & 31)) & 3);
+        return (a == 0 ? from[0] : a == 1 ? from[1] : a == 2 ? from[2] : from[3]) + f;
+    };
     auto angles = [&](int i0, float4& c, float4& s) {
-        if (P.paired) {
+        if constexpr (AXES) {
+            const int f = P.paired ? i0 / 2 : i0 < half ? i0 : i0 - half;
+            const long long f0 = place(f), f1 = place(f + 1);
+            c.x = __ldg(ct + f0), s.x = __ldg(st + f0), c.y = __ldg(ct + f1), s.y = __ldg(st + f1);
+            if (!P.paired) {
+                const long long f2 = place(f + 2), f3 = place(f + 3);
+                c.z = __ldg(ct + f2), s.z = __ldg(st + f2), c.w = __ldg(ct + f3), s.w = __ldg(st + f3);
+            }
+        } else if (P.paired) {
             const float2 cc = __ldg(reinterpret_cast<const float2*>(ct + i0 / 2)), ss = __ldg(reinterpret_cast<const float2*>(st + i0 / 2));
             c = make_float4(cc.x, cc.y, 0.f, 0.f), s = make_float4(ss.x, ss.y, 0.f, 0.f);
         } else {
@@ -339,14 +367,10 @@ int by_blocks(int J, Fn&& f) {
     return ST_BAD_SHAPE;
 }
 
-}  // namespace
-
-extern "C" {
-
-int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride,
-                 long long v_stride, const long long* slots, long long rows, const float* cos_table,
-                 const float* sin_table, const long long* positions, long long n_positions, int rot_dim, int paired,
-                 const void* q, long long q_stride, int n_q, void* q_out, void* stream) {
+int write_rows(const qmv_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride, long long v_stride,
+               const long long* slots, long long rows, const float* cos_table, const float* sin_table, const long long* positions,
+               long long n_positions, int rot_dim, int paired, const uint8_t* axes, int n_axes, const void* q, long long q_stride,
+               int n_q, void* q_out, void* stream) {
     KvWriteParams P{};
     const int st = kv_view(cache, P.c);
     if (st) return st;
@@ -360,7 +384,12 @@ int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dt
     if (!aligned(k, four) || !aligned(v, four) || k_stride % 4 || v_stride % 4 || !aligned(slots, 8)) return ST_BAD_ALIGN;
     if (q && (!aligned(q, four) || !aligned(q_out, four) || q_stride % 4)) return ST_BAD_ALIGN;
     if (cos_table && (!aligned(cos_table, 16) || !aligned(sin_table, 16) || !aligned(positions, 8))) return ST_BAD_ALIGN;
+    for (int f = 0; axes && f < rot_dim / 2; ++f) {
+        if (axes[f] >= n_axes) return ST_BAD_SHAPE;
+        P.axis_of[f >> 5] |= uint64_t(axes[f]) << (2 * (f & 31));
+    }
     if (rows == 0) return ST_OK;
+    P.n_axes = n_axes;
     P.k = k, P.v = v, P.q = q, P.q_out = q_out;
     P.k_stride = k_stride, P.v_stride = v_stride, P.q_stride = q_stride;
     P.slots = slots;
@@ -372,11 +401,64 @@ int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dt
     if (!ctas) return ST_BAD_TOKENS;
     return by_elem(dtype, [&](auto c) {
         return by_blocks(P.c.J, [&](auto j) {
-            return launch_pdl(kv_write_kernel<decltype(c)::value, decltype(j)::value>, dim3(ctas), dim3(256), static_cast<cudaStream_t>(stream), P);
+            constexpr int DT = decltype(c)::value, J = decltype(j)::value;
+            return axes ? launch_pdl(kv_write_kernel<DT, J, true>, dim3(ctas), dim3(256), static_cast<cudaStream_t>(stream), P)
+                        : launch_pdl(kv_write_kernel<DT, J, false>, dim3(ctas), dim3(256), static_cast<cudaStream_t>(stream), P);
         });
     });
 }
 
+struct KvCopyParams {
+    KvView c;
+    const int* src;
+    const int* dst;
+    const int* used;                      // tokens of each copy (null: whole pages)
+    int n;
+    int* status;
+};
+
+// A CTA a copy and key head: the first tokens' K rows, V pairs and scales, each one run of bytes.
+__global__ void __launch_bounds__(128) kv_copy_kernel(const __grid_constant__ KvCopyParams P) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int i = blockIdx.x / P.c.n_kv, head = blockIdx.x - i * P.c.n_kv, tid = threadIdx.x;
+    const int from = __ldg(P.src + i), to = __ldg(P.dst + i);
+    if (from < 0 || to < 0) return;
+    const int page = P.c.page(), asked = P.used ? __ldg(P.used + i) : page, used = min(max(asked, 0), page);
+    const bool bad = from >= P.c.n_pages || to >= P.c.n_pages;
+    if ((bad || used != asked) && tid == 0 && head == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
+    if (bad) return;
+    auto run = [&](uint8_t* base, long long out, long long in, int bytes) {         // whole words
+        const int whole = bytes / 16;
+        for (int x = tid; x < whole; x += 128) reinterpret_cast<uint4*>(base + out)[x] = reinterpret_cast<const uint4*>(base + in)[x];
+        for (int x = whole * 4 + tid; x < bytes / 4; x += 128) reinterpret_cast<uint32_t*>(base + out)[x] = reinterpret_cast<const uint32_t*>(base + in)[x];
+    };
+    run(P.c.k, P.c.k_row(to, head, 0), P.c.k_row(from, head, 0), used * 4 * P.c.J * P.c.kb);
+    run(P.c.v, P.c.v_pair(to, head, 0), P.c.v_pair(from, head, 0), (used + 1) / 2 * 8 * P.c.J * P.c.vb);
+    run(reinterpret_cast<uint8_t*>(P.c.sc), 2 * P.c.scale_row(to, head, 0), 2 * P.c.scale_row(from, head, 0), used * 4 * P.c.J);
+}
+
+}  // namespace
+
+extern "C" {
+
+int qmv_kv_write(const qmv_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride,
+                 long long v_stride, const long long* slots, long long rows, const float* cos_table,
+                 const float* sin_table, const long long* positions, long long n_positions, int rot_dim, int paired,
+                 const void* q, long long q_stride, int n_q, void* q_out, void* stream) {
+    return write_rows(cache, k, v, dtype, k_stride, v_stride, slots, rows, cos_table, sin_table, positions, n_positions, rot_dim, paired,
+                      nullptr, 0, q, q_stride, n_q, q_out, stream);
+}
+
+int qmv_kv_write_axes(const qmv_kv_cache* cache, const void* k, const void* v, int dtype, long long k_stride, long long v_stride,
+                      const long long* slots, long long rows, const float* cos_table, const float* sin_table, const long long* positions,
+                      long long n_positions, int rot_dim, int paired, const uint8_t* axes, int n_axes, const void* q, long long q_stride,
+                      int n_q, void* q_out, void* stream) {
+    if (!cos_table || !axes) return ST_NULL;
+    if (n_axes < 1 || n_axes > 4) return ST_BAD_SHAPE;
+    return write_rows(cache, k, v, dtype, k_stride, v_stride, slots, rows, cos_table, sin_table, positions, n_positions, rot_dim, paired,
+                      axes, n_axes, q, q_stride, n_q, q_out, stream);
+}
 int qmv_kv_read(const qmv_kv_cache* cache, const long long* slots, long long rows, void* k, void* v, int dtype,
                 void* stream) {
     KvReadParams P{};
@@ -397,6 +479,19 @@ int qmv_kv_read(const qmv_kv_cache* cache, const long long* slots, long long row
             return launch_pdl(kv_read_kernel<decltype(c)::value, decltype(j)::value>, dim3(ctas), dim3(256), static_cast<cudaStream_t>(stream), P);
         });
     });
+}
+
+int qmv_kv_copy(const qmv_kv_cache* cache, const int* src, const int* dst, const int* used, int n, void* stream) {
+    KvCopyParams P{};
+    const int st = kv_view(cache, P.c);
+    if (st) return st;
+    if (!src || !dst) return ST_NULL;
+    if (n < 0 || (long long)n * P.c.n_kv > 0x7FFFFFFFLL) return ST_BAD_TOKENS;
+    if (!aligned(src, 4) || !aligned(dst, 4) || !aligned(used, 4)) return ST_BAD_ALIGN;
+    if (n == 0) return ST_OK;
+    P.src = src, P.dst = dst, P.used = used, P.n = n;
+    P.status = device_status_ptr();
+    return launch_pdl(kv_copy_kernel, dim3(unsigned(n * P.c.n_kv)), dim3(128), static_cast<cudaStream_t>(stream), P);
 }
 
 }  // extern "C"
