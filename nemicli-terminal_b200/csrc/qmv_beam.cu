@@ -56,23 +56,33 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-template <int DT> struct Piece;           // 16 bytes of logits
-template <> struct Piece<QMV_OUT_F32> {
-    static constexpr int N = 4;
-    static __device__ __forceinline__ float get(const uint4& w, int i) { return __uint_as_float((&w.x)[i]); }
-};
-template <> struct Piece<QMV_OUT_BF16> {
-    static constexpr int N = 8;
+// 16 bytes of logits
+template <int DT> struct Piece {
+    static constexpr int N = 16 / elem_bytes(DT);
     static __device__ __forceinline__ float get(const uint4& w, int i) {
-        const uint32_t v = (&w.x)[i / 2];
-        return __uint_as_float(i & 1 ? v & 0xFFFF0000u : v << 16);
+        if constexpr (DT == QMV_OUT_F32) {
+            return __uint_as_float((&w.x)[i]);
+        } else if constexpr (DT == QMV_OUT_BF16) {
+            const uint32_t v = (&w.x)[i / 2];
+            return __uint_as_float(i & 1 ? v & 0xFFFF0000u : v << 16);
+        } else {
+            const __half2 h = *reinterpret_cast<const __half2*>(&(&w.x)[i / 2]);
+            return i & 1 ? __high2float(h) : __low2float(h);
+        }
     }
-};
-template <> struct Piece<QMV_OUT_F16> {
-    static constexpr int N = 8;
-    static __device__ __forceinline__ float get(const uint4& w, int i) {
-        const __half2 h = *reinterpret_cast<const __half2*>(&(&w.x)[i / 2]);
-        return i & 1 ? __high2float(h) : __low2float(h);
+    // the largest of a piece's values; NaN only where all are
+    static __device__ __forceinline__ float top(const uint4& w) {
+        if constexpr (DT == QMV_OUT_F32) {
+            return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+        } else if constexpr (DT == QMV_OUT_BF16) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w.x);
+            const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            return fmaxf(__low2float(m), __high2float(m));
+        } else {
+            const __half2* h = reinterpret_cast<const __half2*>(&w.x);
+            const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            return fmaxf(__low2float(m), __high2float(m));
+        }
     }
 };
 
@@ -113,13 +123,29 @@ __device__ __forceinline__ void take(Held& H, int n, uint64_t& bound, uint64_t k
     if (who >> (threadIdx.x & 31) & 1) H.keys[H.count + __popc(who & ((1u << (threadIdx.x & 31)) - 1))] = key;
     H.count += __popc(who);
 }
+// the lanes' values from the largest down (bitonic exchange)
+__device__ __forceinline__ float sorted_down(float x) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+        for (int j = k / 2; j; j /= 2) {
+            const float y = __shfl_xor_sync(0xffffffffu, x, j);
+            x = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(x, y) : fminf(x, y);
+        }
+    return x;
+}
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_constant__ BeamParams P) {
+// A CTA takes a part of a row: pieces of 16 bytes, U in flight a lane; counted from the row's start whatever its alignment (a shifted row puts
+// each piece together from two), so equal rows have equal sums to the last bit and their candidates tie.
+// (x - top before the product with log2 e, not a fused x log2 e - c: logits of 1e4 would carry log2 e's own rounding into the sum.)
+template <int DT, bool SHIFTED>
+__global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamParams P) {
     using T = typename Elem<DT>::type;
     using Pc = Piece<DT>;
-    constexpr int N = Pc::N, U = 4;       // pieces in flight
+    constexpr int N = Pc::N, U = DT == QMV_OUT_F32 ? 8 : 4;
     __shared__ uint64_t s_keys[kWarps][kRoom];
+    __shared__ uint4 s_stage[kWarps][U][32];                      // pieces with candidates
     __shared__ uint64_t s_bound;
     __shared__ double s_sum[kWarps];
     __shared__ float s_top[kWarps];
@@ -132,21 +158,33 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
     const long long row = blockIdx.x / P.splits;
     const int split = int(blockIdx.x - row * P.splits);
     const T* x = static_cast<const T*>(P.x) + row * P.stride;
-    // the row's 16-byte pieces; the values before and behind them are the first part's
-    const int head = min(P.vocab, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / int(sizeof(T)));
-    const int pieces = (P.vocab - head) / N, tail = P.vocab - head - pieces * N;
+    const int pieces = P.vocab / N, tail = P.vocab - pieces * N;  // the values behind the last whole piece are the first part's
     const int first = int((long long)pieces * split / P.splits), last = int((long long)pieces * (split + 1) / P.splits);
-    const uint4* body = reinterpret_cast<const uint4*>(x + head);
+    const int off = SHIFTED ? int(reinterpret_cast<uintptr_t>(x) & 15) : 0;        // bytes
+    const uint4* body = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(x) - off);
+    auto load = [&](int p) {
+        if constexpr (!SHIFTED) {
+            return __ldg(body + p);
+        } else {
+            // both hold values of the row: the piece ends behind the second one's start (where off is 0 the second is not needed)
+            const uint4 a = __ldg(body + p), b = off ? __ldg(body + p + 1) : a;
+            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            const int o = off >> 2, bits = 8 * (off & 3);
+            uint32_t v[5];
+#pragma unroll
+            for (int i = 0; i < 5; ++i) v[i] = o == 0 ? w[i] : o == 1 ? w[i + 1] : o == 2 ? w[i + 2] : w[min(i + 3, 7)];
+            return make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits), __funnelshift_r(v[2], v[3], bits),
+                              __funnelshift_r(v[3], v[4], bits));
+        }
+    };
 
     Held H{s_keys[warp], 0};
     uint64_t bound = 0;                   // n values seen are at least this
     float top = -kMost;
     double sum = 0.0;
-    auto reaches = [&](float m) { return ordered(m) >= uint32_t(bound >> 32); };
-
-    if (split == 0 && warp == 0) {        // at most 14 values
-        const int i = lane < head ? lane : P.vocab - tail + lane - head;
-        const bool there = lane < head + tail;
+    if (split == 0 && warp == 0 && tail) {                        // at most 7 values
+        const int i = pieces * N + lane;
+        const bool there = lane < tail;
         const float v = there ? clean(to_float(x[i])) : -INFINITY;
         if (there) top = fmaxf(v, -kMost), sum = double(ex2((v - top) * kLog2e));
         take(H, n, bound, there ? key_of(v, i) : 0);
@@ -154,69 +192,78 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
     bool primed = false;
     for (int p0 = first + 32 * U * warp; p0 < last; p0 += 32 * U * kWarps) {
         uint4 w[U];
-        bool there[U];
+        float tops[U], best = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int p = p0 + 32 * u + lane;
-            there[u] = p < last;
-            w[u] = there[u] ? __ldg(body + p) : make_uint4(0, 0, 0, 0);
+            constexpr uint32_t none = DT == QMV_OUT_F32 ? 0xFF800000u : DT == QMV_OUT_BF16 ? 0xFF80FF80u : 0xFC00FC00u;      // -inf
+            w[u] = make_uint4(none, none, none, none);
+            if (p < last) w[u] = load(p);
         }
-        float best = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float m = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < N; ++i) m = fmaxf(m, Pc::get(w[u], i));
-            best = fmaxf(best, there[u] ? m : -INFINITY);
-        }
+        for (int u = 0; u < U; ++u) tops[u] = Pc::top(w[u]), best = fmaxf(best, tops[u]);
         if (best > top) {
-            best = fminf(best, kMost);
-            sum *= double(ex2((top - best) * kLog2e));
-            top = best;
+            const float m = fminf(best, kMost);
+            sum *= double(ex2((top - m) * kLog2e));
+            top = m;
         }
-        float part = 0.f;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < N; ++i) part += there[u] ? ex2((Pc::get(w[u], i) - top) * kLog2e) : 0.f;
-        if (!(part == part) || part > 3e38f) {                    // a NaN or an infinity among them
-            part = 0.f;
+            for (int i = 0; i < N; ++i) part[i & 3] += ex2((Pc::get(w[u], i) - top) * kLog2e);
+        float all = (part[0] + part[1]) + (part[2] + part[3]);
+        if (!(all < 3e38f)) {                                     // a NaN or an infinity among them
+            all = 0.f;
+#pragma unroll
             for (int u = 0; u < U; ++u)
-                for (int i = 0; i < N; ++i) part += there[u] ? ex2((clean(Pc::get(w[u], i)) - top) * kLog2e) : 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) all += ex2((clean(Pc::get(w[u], i)) - top) * kLog2e);
         }
-        sum += double(part);
+        sum += double(all);
         if (!primed) {
-            // the first bound: of 64 maxima (two a lane) the n-th
+            // the first bound: of the lanes' largest the n-th, with more than 32 the least of their halves' largest
             primed = true;
-            uint64_t two[2] = {0, 0};
-            int rank[2] = {0, 0};
+            float m = best;
+            if (n > 32) {
+                float a = -INFINITY, b = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (there[u]) two[u & 1] = max(two[u & 1], key_of(Pc::get(w[u], i), head + (p0 + 32 * u + lane) * N + i));
-            for (int o = 0; o < 32; ++o)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint64_t k = __shfl_sync(0xffffffffu, two[h], o);
-                    rank[0] += k > two[0], rank[1] += k > two[1];
-                }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t who = __ballot_sync(0xffffffffu, two[h] && rank[h] == n - 1);
-                if (who) bound = max(bound, __shfl_sync(0xffffffffu, two[h], __ffs(who) - 1));
+                for (int u = 0; u < U; ++u) (u & 1 ? b : a) = fmaxf(u & 1 ? b : a, tops[u]);
+                m = fminf(a, b);
+            }
+            m = __shfl_sync(0xffffffffu, sorted_down(m), n > 32 ? 31 : n - 1);
+            if (m > -INFINITY) {
+                bound = max(bound, uint64_t(ordered(fminf(m, kMost) + 0.f)) << 32);
+                if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&s_bound), (unsigned long long)bound);
             }
         }
         bound = max(bound, *static_cast<volatile uint64_t*>(&s_bound));       // the other warps'
-        if (__any_sync(0xffffffffu, reaches(best))) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    take(H, n, bound, there[u] ? key_of(Pc::get(w[u], i), head + (p0 + 32 * u + lane) * N + i) : 0);
-            if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&s_bound), (unsigned long long)bound);
-        }
         bound = __shfl_sync(0xffffffffu, bound, 0);
+        const float least = unordered(uint32_t(bound >> 32));     // (no bound: NaN, which nothing is less than)
+        if (__any_sync(0xffffffffu, !(best < least))) {
+            const uint64_t before = bound;
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < U; ++u) s_stage[warp][u][lane] = w[u];
+            __syncwarp();
+#pragma unroll 1
+            for (int u = 0; u < U; ++u) {
+                const int p = p0 + 32 * u + lane;
+                uint32_t who = __ballot_sync(0xffffffffu, p < last && !(Pc::top(s_stage[warp][u][lane]) < least));
+                if (__popc(who) <= 4) {                           // piece by piece, a lane a value
+                    for (; who; who &= who - 1) {
+                        const int l = __ffs(who) - 1;
+                        take(H, n, bound, lane < N ? key_of(to_float(reinterpret_cast<const T*>(&s_stage[warp][u][l])[lane & (N - 1)]), (p0 + 32 * u + l) * N + lane) : 0);
+                    }
+                } else {
+                    const bool mine = who >> lane & 1;
+#pragma unroll 1
+                    for (int i = 0; i < N; ++i)
+                        take(H, n, bound, mine ? key_of(to_float(reinterpret_cast<const T*>(&s_stage[warp][u][lane])[i]), p * N + i) : 0);
+                }
+            }
+            if (bound > before && lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&s_bound), (unsigned long long)bound);
+        }
     }
     // ---- the warps' together
     {
@@ -270,14 +317,21 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const __grid_consta
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, req = blockIdx.x, n = P.n, per = P.splits * n, all = P.K * per;
-    if (tid < P.K) {
-        const long long r = (long long)req * P.K + tid;
+    for (int k = tid >> 5; k < P.K; k += kWarps) {                // a warp a beam
+        const int lane = tid & 31;
+        const long long r = ((long long)req * P.K + k) * P.splits;
         float m = -kMost;
-        for (int s = 0; s < P.splits; ++s) m = fmaxf(m, P.tops[r * P.splits + s]);
+        for (int i = lane; i < P.splits; i += 32) m = fmaxf(m, P.tops[r + i]);
+#pragma unroll
+        for (int o = 16; o; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         double sum = 0.0;
-        for (int s = 0; s < P.splits; ++s) sum += P.sums[r * P.splits + s] * exp(double(P.tops[r * P.splits + s]) - double(m));
-        s_off[tid] = double(m);
-        s_score[tid] = double(P.scores[r]) - log(max(sum, 1e-300));
+        for (int i = lane; i < P.splits; i += 32) sum += P.sums[r + i] * double(ex2((P.tops[r + i] - m) * kLog2e));
+#pragma unroll
+        for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+            s_off[k] = double(m);
+            s_score[k] = double(P.scores[(long long)req * P.K + k]) - log(max(sum, 1e-300));
+        }
     }
     if (tid == 0) s_count = 0, s_limit = Cand{0, INT64_MAX};
     __syncthreads();
@@ -382,9 +436,14 @@ int qmv_beam_select(const void* logits, int dtype, long long row_stride, int n_r
     P.sums = reinterpret_cast<double*>(P.keys + parts * n);
     P.tops = reinterpret_cast<float*>(P.sums + parts);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int e = by_elem(dtype, [&](auto c) { return launch_pdl(beam_part_kernel<decltype(c)::value>, dim3(unsigned(parts)), dim3(kThreads), st, P); });
+    const bool shifted = !aligned(logits, 16) || row_stride * elem_bytes(dtype) % 16;
+    const int e = by_elem(dtype, [&](auto c) {
+        constexpr int DT = decltype(c)::value;
+        return shifted ? launch_pdl(beam_part_kernel<DT, true>, dim3(unsigned(parts)), dim3(kThreads), st, P)
+                       : launch_pdl(beam_part_kernel<DT, false>, dim3(unsigned(parts)), dim3(kThreads), st, P);
+    });
     if (e) return e;
-    return launch_pdl(beam_join_kernel, dim3(n_req), dim3(kThreads), st, P);
+    return launch_behind(beam_join_kernel, dim3(n_req), dim3(kThreads), st, P);
 }
 
 }  // extern "C"

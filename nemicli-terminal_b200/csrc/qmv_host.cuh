@@ -55,6 +55,22 @@ template <class... KArgs, class... Args>
 int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args... args) {
     return launch_pdl_smem(kern, grid, block, 0, st, args...);
 }
+// the second kernel of a call behind its first, which lets it start early (griddepcontrol.launch_dependents): always a programmatic
+// dependent launch, since both are this library's and the second waits (griddepcontrol.wait) before it touches memory
+template <class... KArgs, class... Args>
+int launch_behind(void (*kern)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+    return launched();
+}
 
 // ---- defined per format in qmv_fmt.cu (one object file per format) ----
 // fallback kernel, T = 1..8 tokens

@@ -396,7 +396,7 @@ int qmv_kv_choose(const qmv_kv_cache* cache, const void* q, int dtype, long long
         });
         if (e) return e;
     }
-    return launch_pdl(choose_kernel, dim3(unsigned(n_rows * c.n_kv)), dim3(kThreads), s, P);
+    return launch_behind(choose_kernel, dim3(unsigned(n_rows * c.n_kv)), dim3(kThreads), s, P);
 }
 
 }  // extern "C"
