@@ -143,17 +143,16 @@ template <int DT, bool SHIFTED>
 __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamParams P) {
     using T = typename Elem<DT>::type;
     using Pc = Piece<DT>;
-    constexpr int N = Pc::N, U = DT == QMV_OUT_F32 ? 8 : 4;
+    constexpr int N = Pc::N, U = 32 / N, kSteps = 8;              // 32 values a lane and step
     __shared__ uint64_t s_keys[kWarps][kRoom];
-    __shared__ uint4 s_stage[kWarps][U][32];                      // pieces with candidates
-    __shared__ uint64_t s_bound;
+    __shared__ float s_best[kSteps][kThreads];                    // of a lane's pieces of a step the largest value
+    __shared__ uint64_t s_list[kWarps * kRoom];
     __shared__ double s_sum[kWarps];
-    __shared__ float s_top[kWarps];
-    __shared__ int s_count[kWarps];
+    __shared__ float s_top[kWarps], s_nth[kWarps];
+    __shared__ int s_count;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = P.n;
-    if (tid == 0) s_bound = 0;
-    __syncthreads();
+    if (tid == 0) s_count = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long row = blockIdx.x / P.splits;
     const int split = int(blockIdx.x - row * P.splits);
@@ -189,10 +188,43 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
         if (there) top = fmaxf(v, -kMost), sum = double(ex2((v - top) * kLog2e));
         take(H, n, bound, there ? key_of(v, i) : 0);
     }
-    bool primed = false;
-    for (int p0 = first + 32 * U * warp; p0 < last; p0 += 32 * U * kWarps) {
+    // The bound of all warps: each of those with a whole first step says which value its m largest reach, m its share of n; the least of
+    // these n values reach.  A warp's m-th largest is that of its lanes' largest so far.
+    float seen = -INFINITY;
+    const int full = max(1, min(kWarps, (last - first) / (32 * U))), nth = (n + full - 1) / full - 1;
+    auto tell = [&]() {
+        const float m = __shfl_sync(0xffffffffu, sorted_down(seen), nth & 31);
+        if (lane == 0) *static_cast<volatile float*>(&s_nth[warp]) = warp >= full ? INFINITY : nth < 32 ? m : -INFINITY;
+    };
+    auto hear = [&]() {
+        float m = *static_cast<volatile float*>(&s_nth[lane & (kWarps - 1)]);
+#pragma unroll
+        for (int o = 1; o < kWarps; o *= 2) m = fminf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m > -INFINITY) bound = max(bound, uint64_t(ordered(fminf(m, kMost) + 0.f)) << 32);
+        bound = __shfl_sync(0xffffffffu, bound, 0);
+    };
+    // the candidates of `steps` steps from piece p1 on: a lane's 32 values of a step, read again, where the largest reaches the bound
+    auto flush = [&](int p1, int steps) {
+        for (int t = 0; t < steps; ++t) {
+            const int p0 = p1 + t * (32 * U * kWarps);
+            const uint64_t key = key_of(s_best[t][tid], (p0 + lane) * N);          // no value of the lane's has a larger one
+            const bool any = p0 + lane < last;
+            uint32_t who = __ballot_sync(0xffffffffu, any && key >= bound);
+            while (who) {
+                const int l = __ffs(who) - 1, p = p0 + 32 * (lane / N) + l, place = p * N + lane % N;
+                take(H, n, bound, p < last ? key_of(to_float(x[place]), place) : 0);
+                who &= who - 1;
+                who &= __ballot_sync(0xffffffffu, key >= bound);
+            }
+        }
+    };
+    if (lane == 0) s_nth[warp] = warp >= full ? INFINITY : -INFINITY;
+    __syncthreads();
+    const int begin = first + 32 * U * warp;
+    int p0 = begin, p1 = begin, step = 0;
+    for (; p0 < last; p0 += 32 * U * kWarps) {
         uint4 w[U];
-        float tops[U], best = -INFINITY;
+        float best = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int p = p0 + 32 * u + lane;
@@ -201,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
             if (p < last) w[u] = load(p);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) tops[u] = Pc::top(w[u]), best = fmaxf(best, tops[u]);
+        for (int u = 0; u < U; ++u) best = fmaxf(best, Pc::top(w[u]));
         if (best > top) {
             const float m = fminf(best, kMost);
             sum *= double(ex2((top - m) * kLog2e));
@@ -221,48 +253,14 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
                 for (int i = 0; i < N; ++i) all += ex2((clean(Pc::get(w[u], i)) - top) * kLog2e);
         }
         sum += double(all);
-        if (!primed) {
-            // the first bound: of the lanes' largest the n-th, with more than 32 the least of their halves' largest
-            primed = true;
-            float m = best;
-            if (n > 32) {
-                float a = -INFINITY, b = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < U; ++u) (u & 1 ? b : a) = fmaxf(u & 1 ? b : a, tops[u]);
-                m = fminf(a, b);
-            }
-            m = __shfl_sync(0xffffffffu, sorted_down(m), n > 32 ? 31 : n - 1);
-            if (m > -INFINITY) {
-                bound = max(bound, uint64_t(ordered(fminf(m, kMost) + 0.f)) << 32);
-                if (lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&s_bound), (unsigned long long)bound);
-            }
-        }
-        bound = max(bound, *static_cast<volatile uint64_t*>(&s_bound));       // the other warps'
-        bound = __shfl_sync(0xffffffffu, bound, 0);
-        const float least = unordered(uint32_t(bound >> 32));     // (no bound: NaN, which nothing is less than)
-        if (__any_sync(0xffffffffu, !(best < least))) {
-            const uint64_t before = bound;
+        seen = fmaxf(seen, best);
+        s_best[step][tid] = best;
+        if (++step == kSteps && p0 + 32 * U * kWarps < last) {    // (the last ones come behind the other warps' last word)
             __syncwarp();
-#pragma unroll
-            for (int u = 0; u < U; ++u) s_stage[warp][u][lane] = w[u];
-            __syncwarp();
-#pragma unroll 1
-            for (int u = 0; u < U; ++u) {
-                const int p = p0 + 32 * u + lane;
-                uint32_t who = __ballot_sync(0xffffffffu, p < last && !(Pc::top(s_stage[warp][u][lane]) < least));
-                if (__popc(who) <= 4) {                           // piece by piece, a lane a value
-                    for (; who; who &= who - 1) {
-                        const int l = __ffs(who) - 1;
-                        take(H, n, bound, lane < N ? key_of(to_float(reinterpret_cast<const T*>(&s_stage[warp][u][l])[lane & (N - 1)]), (p0 + 32 * u + l) * N + lane) : 0);
-                    }
-                } else {
-                    const bool mine = who >> lane & 1;
-#pragma unroll 1
-                    for (int i = 0; i < N; ++i)
-                        take(H, n, bound, mine ? key_of(to_float(reinterpret_cast<const T*>(&s_stage[warp][u][lane])[i]), p * N + i) : 0);
-                }
-            }
-            if (bound > before && lane == 0) atomicMax(reinterpret_cast<unsigned long long*>(&s_bound), (unsigned long long)bound);
+            tell();
+            hear();
+            flush(p1, step);
+            step = 0, p1 = p0 + 32 * U * kWarps;
         }
     }
     // ---- the warps' together
@@ -275,20 +273,22 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
         for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         top = m;
     }
-    if (H.count > n) sort_out(H, n, bound);
-    if (lane == 0) s_sum[warp] = sum, s_top[warp] = top, s_count[warp] = H.count;
+    if (lane == 0) s_sum[warp] = sum, s_top[warp] = top;
+    tell();
+    __syncthreads();
+    hear();
+    flush(p1, step);
+    __syncwarp();
+    for (int i = lane; i < H.count; i += 32)
+        if (H.keys[i] >= bound) s_list[atomicAdd(&s_count, 1)] = H.keys[i];
     __syncthreads();
     uint64_t* out = P.keys + (long long)blockIdx.x * n;
-    int total = 0;
-    for (int w = 0; w < kWarps; ++w) total += s_count[w];
+    const int total = s_count;
     for (int i = total + tid; i < n; i += kThreads) out[i] = 0;
-    for (int i = tid; i < kWarps * kMostBest; i += kThreads) {
-        const int w = i / kMostBest, at = i % kMostBest;
-        if (at >= s_count[w]) continue;
-        const uint64_t key = s_keys[w][at];
+    for (int i = tid; i < total; i += kThreads) {
+        const uint64_t key = s_list[i];
         int rank = 0;
-        for (int o = 0; o < kWarps; ++o)
-            for (int j = 0; j < s_count[o]; ++j) rank += s_keys[o][j] > key;
+        for (int j = 0; j < total; ++j) rank += s_list[j] > key;
         if (rank < n) out[rank] = key;
     }
     if (tid == 0) {
@@ -307,18 +307,20 @@ struct Cand {
 };
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.score > b.score || (a.score == b.score && a.place < b.place); }
 
-constexpr int kList = 1024;
+constexpr int kJoin = 1024, kList = 1024;
 
-__global__ void __launch_bounds__(kThreads) beam_join_kernel(const __grid_constant__ BeamParams P) {
+// A CTA a request.  First a bound from the lists, which are in order: of their q-th entries the r-th, q r >= n.  The candidates that
+// reach it are a few more than n; each finds its rank by looking at all others, four threads a candidate.
+__global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant__ BeamParams P) {
     __shared__ double s_off[kMostBest], s_score[kMostBest];        // of a beam: largest logit; score - log of the sum
     __shared__ Cand s_list[kList];
     __shared__ int s_count;
     __shared__ Cand s_limit;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, req = blockIdx.x, n = P.n, per = P.splits * n, all = P.K * per;
-    for (int k = tid >> 5; k < P.K; k += kWarps) {                // a warp a beam
-        const int lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, req = blockIdx.x, n = P.n, lists = P.K * P.splits, all = lists * n;
+    const uint64_t* keys = P.keys + (long long)req * all;
+    for (int k = tid >> 5; k < P.K; k += kJoin / 32) {            // a warp a beam
         const long long r = ((long long)req * P.K + k) * P.splits;
         float m = -kMost;
         for (int i = lane; i < P.splits; i += 32) m = fmaxf(m, P.tops[r + i]);
@@ -335,60 +337,75 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const __grid_consta
     }
     if (tid == 0) s_count = 0, s_limit = Cand{0, INT64_MAX};
     __syncthreads();
-    const uint64_t* keys = P.keys + (long long)req * all;
     auto cand = [&](int i) {
         const uint64_t key = keys[i];
         if (!key) return Cand{0, INT64_MAX};                      // none
-        const int k = i / per;
+        const int k = i / (P.splits * n);
         double s = (double(unordered(uint32_t(key >> 32))) - s_off[k]) + s_score[k];
         if (!(s == s)) s = -INFINITY;
         return Cand{ordered64(s + 0.0), (long long)k * P.vocab + int(~uint32_t(key))};
     };
-    // with many candidates a limit first: of the threads' best ones the n-th
-    if (all > kThreads) {
-        Cand best{0, INT64_MAX};
-        for (int i = tid; i < all; i += kThreads) {
-            const Cand c = cand(i);
-            if (before(c, best)) best = c;
-        }
-        s_list[tid] = best;
-        __syncthreads();
+    // rank of s_list[i] among `count`, in each of the four threads 4 i .. 4 i + 3
+    auto rank_of = [&](int i, int count) {
         int rank = 0;
-        for (int j = 0; j < kThreads; ++j) rank += before(s_list[j], best);
-        if (rank == n - 1 && best.place != INT64_MAX) s_limit = best;
+        if (i < count) {
+            const Cand c = s_list[i];
+            for (int j = lane & 3; j < count; j += 4) rank += before(s_list[j], c);
+        }
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        return rank + __shfl_xor_sync(0xffffffffu, rank, 2);
+    };
+    const int q = (n + lists - 1) / lists, r = (n + q - 1) / q;
+    if (lists <= kList && all > n) {
+        for (int i = tid; i < lists; i += kJoin) s_list[i] = cand(i * n + q - 1);
+        __syncthreads();
+        for (int i0 = 0; i0 < lists; i0 += kJoin / 4) {
+            const int i = i0 + tid / 4, rank = rank_of(i, lists);
+            if (i < lists && (lane & 3) == 0 && rank == r - 1 && s_list[i].place != INT64_MAX) s_limit = s_list[i];
+        }
         __syncthreads();
     }
     const Cand limit = s_limit;
-    // Those that reach it: at most n threads' candidates.  More than the list holds are taken in turns, the n best of each kept.
-    int done = 0;                         // candidates looked at, by all threads
-    while (done < all) {
-        const int end = min(all, done + kList - n);
-        for (int i = done + tid; i < end; i += kThreads) {
+    // where more than the list holds reach it: in turns, of which the n best are kept
+    int turn = all;
+    for (int done = 0; done < all;) {
+        const int kept = s_count;
+        __syncthreads();
+        for (int i = done + tid; i < min(all, done + turn); i += kJoin) {
             const Cand c = cand(i);
-            if (c.place != INT64_MAX && !before(limit, c)) s_list[atomicAdd(&s_count, 1)] = c;
+            if (c.place == INT64_MAX || before(limit, c)) continue;
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kList) s_list[at] = c;
         }
         __syncthreads();
-        done = end;
         const int count = s_count;
-        Cand own[kList / kThreads];
-        int rank[kList / kThreads];
+        if (count > kList) {                                      // (only where turn is all)
+            __syncthreads();
+            if (tid == 0) s_count = kept;
+            turn = kList - n;
+            __syncthreads();
+            continue;
+        }
+        Cand own[4];
+        int rank[4];
 #pragma unroll
-        for (int i = 0; i < kList / kThreads; ++i) {
-            rank[i] = kList;
-            if (kThreads * i + tid >= count) continue;
-            own[i] = s_list[kThreads * i + tid];
-            int r = 0;
-            for (int j = 0; j < count; ++j) r += before(s_list[j], own[i]);
-            rank[i] = r;
+        for (int x = 0; x < 4; ++x) {
+            const int i = kJoin / 4 * x + tid / 4;
+            rank[x] = kList;
+            if (kJoin / 4 * x >= count) continue;
+            rank[x] = rank_of(i, count);
+            if (i < count) own[x] = s_list[i];
+            else rank[x] = kList;
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kList / kThreads; ++i)
-            if (rank[i] < n) s_list[rank[i]] = own[i];
+        for (int x = 0; x < 4; ++x)
+            if ((lane & 3) == 0 && rank[x] < n) s_list[rank[x]] = own[x];
         if (tid == 0) s_count = min(count, n);
         __syncthreads();
+        done += turn;
     }
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid; i < n; i += kJoin) {
         const Cand c = s_list[i];
         const uint64_t o = c.score;
         const double s = __longlong_as_double(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o);
@@ -399,11 +416,11 @@ __global__ void __launch_bounds__(kThreads) beam_join_kernel(const __grid_consta
     }
 }
 
-// Parts a row: two CTAs an SM over all rows, of 2048 values at least.
+// Parts a row: four CTAs an SM over all rows, of 8192 values at least (a step of a CTA).
 int splits_of(int n_req, int K, int vocab) {
     const long long rows = (long long)n_req * K;
     const long long want = (4LL * sm_count() + rows - 1) / rows;
-    return int(std::max<long long>(1, std::min<long long>(want, vocab / 2048)));
+    return int(std::max<long long>(1, std::min<long long>(want, vocab / 8192)));
 }
 bool bad_sizes(int n_req, int K, int vocab, int n) {
     return n_req <= 0 || K <= 0 || K > kMostBest || n_req > 65535 / K || vocab <= 0 || vocab > (1 << 30) || n <= 0 || n > kMostBest || n > (long long)K * vocab;
@@ -443,7 +460,7 @@ int qmv_beam_select(const void* logits, int dtype, long long row_stride, int n_r
                        : launch_pdl(beam_part_kernel<DT, false>, dim3(unsigned(parts)), dim3(kThreads), st, P);
     });
     if (e) return e;
-    return launch_behind(beam_join_kernel, dim3(n_req), dim3(kThreads), st, P);
+    return launch_behind(beam_join_kernel, dim3(n_req), dim3(kJoin), st, P);
 }
 
 }  // extern "C"
