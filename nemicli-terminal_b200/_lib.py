@@ -131,8 +131,8 @@ _HERE = contextlib.nullcontext()
 def on_device(device):
     """Makes `device` the current one for a launch (a stream belongs to its own device only); nothing to do where it
     is already."""
-    index = device.index
-    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(device)
+    index = device.index                     # (a tensor's device: CUDA is up)
+    return _HERE if index is None or index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def addr(t) -> int:

@@ -18,20 +18,20 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n: int = 0):
     beams; twice as many leave room for beams that end.  -> scores float32, parents int32, tokens int32, each (requests, n), best
     first: scores[r, parents] + log_softmax(logits[r, parents])[tokens], the lowest (beam, token) first among equals.  NaN counts as
     -inf, +inf as the largest float.  Two launches."""
-    if logits.dim() != 3 or logits.dtype not in _DTYPES or not _lib.on_gpu(logits):
+    shape, dtype, device = logits.shape, _DTYPES.get(logits.dtype), logits.device
+    if len(shape) != 3 or dtype is None or not logits.is_cuda:
         raise RuntimeError(f"beams.select: logits (requests, beams, vocab) of float32, bfloat16 or float16 on a CUDA device expected, "
-                           f"got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
-    reqs, k, vocab = logits.shape
-    device = logits.device
-    if scores.shape != (reqs, k) or scores.dtype != torch.float32 or scores.device != device or not scores.is_contiguous():
+                           f"got {logits.dtype} {tuple(shape)} on {device}")
+    reqs, k, vocab = shape
+    if scores.shape != (reqs, k) or scores.dtype is not torch.float32 or scores.device != device or not scores.is_contiguous():
         raise RuntimeError(f"beams.select: scores contiguous float32 ({reqs}, {k}) on {device} expected, got {scores.dtype} "
                            f"{tuple(scores.shape)} on {scores.device}")
     n = n or k
     if not 0 < k <= MOST or not 0 < n <= MOST or not 0 < vocab <= 1 << 30 or n > k * vocab or reqs * k > 65535:
         raise RuntimeError(f"beams.select: {reqs} requests of {k} beams over {vocab} tokens, {n} best: up to {MOST} beams and candidates, "
                            f"65535 beams in all")
-    out = torch.empty((reqs, n), dtype=torch.float32, device=device)
-    parents, tokens = (torch.empty((reqs, n), dtype=torch.int32, device=device) for _ in range(2))
+    parents = torch.empty((reqs, n), dtype=torch.int32, device=device)
+    tokens, out = torch.empty_like(parents), torch.empty((reqs, n), dtype=torch.float32, device=device)
     if reqs == 0:
         return out, parents, tokens
     by_req, by_beam, apart = logits.stride()
@@ -43,7 +43,7 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n: int = 0):
     with _lib.on_device(device):
         nbytes = lib.qmv_beam_workspace_bytes(reqs, k, vocab, n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        st = lib.qmv_beam_select(logits.data_ptr(), _DTYPES[logits.dtype], stride, reqs, k, vocab, scores.data_ptr(), n, out.data_ptr(),
+        st = lib.qmv_beam_select(logits.data_ptr(), dtype, stride, reqs, k, vocab, scores.data_ptr(), n, out.data_ptr(),
                                  parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_of(device))
     if st:
         _lib.check(st, "qmv_beam_select")

@@ -30,13 +30,26 @@ struct BoxParams {
     int* status;
 };
 
-// eight codes of a key as values without scale
+// Eight codes of a key times its scale d, exactly: a code's bits below the exponent of 2^e are the float 2^e + code, and
+// d (2^e + code) - d (2^e + offset) is one fused multiply-add without a rounding (d has 11 bits, 2^e + offset at most 13).  (Converted
+// from integers the codes took 16 a clock and SM: 18 us for the pages of 32000 tokens.)
 template <int KB>
-__device__ __forceinline__ void codes8(const uint32_t* w, float (&v)[8]) {
+__device__ __forceinline__ void keys8(const uint32_t* w, float d, float (&v)[8]) {
+    if constexpr (KB == 4) {
+        const float d7 = d * -136.f, d11 = d * -2056.f, d15 = d * -32776.f;      // the code at bits 16, 12, 8: 2^7, 2^11, 2^15
+        auto at16 = [&](uint32_t x) { return fmaf(d, __uint_as_float((x & 0x000F0000u) | 0x43000000u), d7); };
+        auto at12 = [&](uint32_t x) { return fmaf(d, __uint_as_float((x & 0x0000F000u) | 0x45000000u), d11); };
+        auto at8 = [&](uint32_t x) { return fmaf(d, __uint_as_float((x & 0x00000F00u) | 0x47000000u), d15); };
+        const uint32_t up = w[0] << 8, down = w[0] >> 8;          // value n at bit 16 (n & 1) + 4 (n >> 1)
+        v[0] = at8(up), v[2] = at12(up), v[4] = at8(w[0]), v[6] = at12(w[0]);
+        v[1] = at16(w[0]), v[3] = at12(down), v[5] = at16(down), v[7] = at16(w[0] >> 12);
+    } else {
+        const float d15 = d * -32896.f;                           // the code at bit 8: 2^15
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-        const uint32_t c = KB == 4 ? w[0] >> (16 * (n & 1) + 4 * (n >> 1)) & 15u : w[KB == 4 ? 0 : n >> 2] >> (8 * (2 * (n & 1) + ((n & 3) >> 1))) & 255u;
-        v[n] = float(int(c) - (KB == 4 ? 8 : 128));
+        for (int i = 0; i < 2; ++i) {                             // bytes n0 n2 n1 n3
+            auto at8 = [&](uint32_t x) { return fmaf(d, __uint_as_float((x & 0x0000FF00u) | 0x47000000u), d15); };
+            v[4 * i] = at8(w[i] << 8), v[4 * i + 2] = at8(w[i]), v[4 * i + 1] = at8(w[i] >> 8), v[4 * i + 3] = at8(w[i] >> 16);
+        }
     }
 }
 
@@ -70,20 +83,29 @@ __global__ void __launch_bounds__(kThreads) box_kernel(const __grid_constant__ B
 #pragma unroll
     for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
     if (tok < kTok) {
-#pragma unroll 8
-        for (int x = tok; x < P.c.page(); x += kTok) {
-            uint32_t w[2];
-            if constexpr (KB == 4) {
-                w[0] = __ldg(reinterpret_cast<const uint32_t*>(k + x * (kUnits * KB)));
-            } else {
-                const uint2 both = __ldg(reinterpret_cast<const uint2*>(k + x * (kUnits * KB)));
-                w[0] = both.x, w[1] = both.y;
-            }
-            const float d = __half2float(sc[x * 2 * J]);
-            float v[8];
-            codes8<KB>(w, v);
+        constexpr int kAhead = 4;                                 // loads of four tokens go out together (pages hold 16 at least)
+        for (int x0 = tok; x0 < P.c.page(); x0 += kAhead * kTok) {
+            uint32_t w[kAhead][2];
+            __half d[kAhead];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) lo[i] = fminf(lo[i], d * v[i]), hi[i] = fmaxf(hi[i], d * v[i]);
+            for (int a = 0; a < kAhead; ++a) {
+                const int x = x0 + a * kTok;
+                if constexpr (KB == 4) {
+                    w[a][0] = __ldg(reinterpret_cast<const uint32_t*>(k + x * (kUnits * KB)));
+                } else {
+                    const uint2 both = __ldg(reinterpret_cast<const uint2*>(k + x * (kUnits * KB)));
+                    w[a][0] = both.x, w[a][1] = both.y;
+                }
+                d[a] = sc[x * 2 * J];
+            }
+#pragma unroll
+            for (int a = 0; a < kAhead; a += 2) {
+                float u[8], v[8];
+                keys8<KB>(w[a], __half2float(d[a]), u);
+                keys8<KB>(w[a + 1], __half2float(d[a + 1]), v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) lo[i] = fminf(fminf(lo[i], u[i]), v[i]), hi[i] = fmaxf(fmaxf(hi[i], u[i]), v[i]);
+            }
         }
     }
     // the other tokens of the unit
@@ -119,94 +141,183 @@ struct ChooseParams {
     const int* tables;
     const int* lens;
     const int* starts;
-    int n_kv, group, width, shift, n_seq, n_rows, keep, first, last;
-    double* scores;                       // workspace: [rows][n_kv][width]
+    int n_kv, group, dim, width, shift, n_seq, n_rows, keep, first, last;
+    float* near;                          // workspace, each [rows][n_kv][width]: a page's score, nearly
+    float* sizes;                         // what its error is measured by
+    double* scores;                       // in fp64, where many lie next to the border
     int* chosen;                          // [rows][n_kv][keep]
     int* held;                            // [rows]
     int* status;
 };
 
+// the larger one, NaN where one is
+__device__ __forceinline__ float larger(float a, float b) { return b > a || b != b ? b : a; }
+
 struct Row {
     int seq, pos;                         // sequence (-1: none), position in it
 };
-// the row's sequence and place, by the whole CTA
-__device__ __forceinline__ Row find_row(const ChooseParams& P, int row, int* s_seq, bool tell) {
-    if (threadIdx.x == 0) *s_seq = P.starts ? -1 : row < P.n_seq ? row : -1;
-    __syncthreads();
-    if (P.starts)
-        for (int b = threadIdx.x; b < P.n_seq; b += kThreads)
-            if (__ldg(P.starts + b) <= row && row < __ldg(P.starts + b + 1)) *s_seq = b;
-    __syncthreads();
-    const int seq = *s_seq;
+// the row's sequence and place, by each warp
+__device__ __forceinline__ Row find_row(const ChooseParams& P, int row, bool tell) {
+    const int lane = threadIdx.x & 31;
+    int seq = row < P.n_seq ? row : -1, past = 0;
+    if (P.starts) {
+        seq = -1;
+        for (int b0 = 0; b0 < P.n_seq && seq < 0; b0 += 32) {
+            const int b = b0 + lane;
+            const int s0 = b < P.n_seq ? __ldg(P.starts + b) : INT_MAX, s1 = b < P.n_seq ? __ldg(P.starts + b + 1) : 0;
+            const uint32_t who = __ballot_sync(0xffffffffu, s0 <= row && row < s1);
+            if (who) seq = b0 + __ffs(who) - 1, past = __shfl_sync(0xffffffffu, s1, __ffs(who) - 1);
+        }
+    }
     if (seq < 0) return Row{-1, -1};
     const int cap = P.width << P.shift, len = __ldg(P.lens + seq), held = min(max(len, 0), cap);
     if (tell && held != len && threadIdx.x == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
-    return Row{seq, P.starts ? held - (min(__ldg(P.starts + seq + 1), P.n_rows) - row) : held - 1};
+    return Row{seq, P.starts ? held - (min(past, P.n_rows) - row) : held - 1};
 }
 
-constexpr int kPagesCta = 64;             // pages a CTA scores
+constexpr int kScorers = 128;             // threads a CTA
+constexpr int kTiles = 2, kPagesWarp = 16 * kTiles;              // pages a warp scores
 
-// Eight lanes a page, each J runs of 4 channels; heads four at a time.  In fp64: products of a query and an fp16 bound are exact, and
-// pages next to the border between chosen and left have to come out the same way whatever the order of the sums.
+// A warp 16 pages, the rows of mma.m16n8k16 over the 2 dim halves of a box: lo against the queries' negative parts, hi against the
+// positive ones, the key head's query heads as columns (eight at a time).  A lane's 16 bytes of a box are two steps' operands as they
+// lie; the queries are laid out to match.  Queries are fp16 after a power of two a head, fp32 ones two fp16 parts.  So a score is near:
+// off by less than 2^-15 sum_c |q_c| max |box|: 2^-20 of it for the queries' parts, and in each of four chains at most 16 steps of 17
+// terms cut off at 2^-24 of the chain's share of that sum.  The choice computes those that lie nearer to its border again, in fp64.
+// (All in fp64 on the CUDA cores: 27 to 46 us for 64 sequences of 154 pages on average, 184 instructions a page and key head.)
 template <int DT, int J>
-__global__ void __launch_bounds__(kThreads) score_kernel(const __grid_constant__ ChooseParams P) {
+__global__ void __launch_bounds__(kScorers) score_kernel(const __grid_constant__ ChooseParams P) {
     using T = typename Elem<DT>::type;
-    constexpr int D = 32 * J;
-    extern __shared__ __align__(16) double s_q[];                 // [group up to 4s][J][2][8][2]
-    __shared__ int s_seq;
+    constexpr int D = 32 * J, kParts = DT == QMV_OUT_F32 ? 2 : 1, kPieces = 2 * J, kAhead = kPieces < 8 ? kPieces : 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = lane & 7;
-    const int head = blockIdx.y, row = blockIdx.z;
-    const Row r = find_row(P, row, &s_seq, false);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, head = blockIdx.y, row = blockIdx.z;
+    const Row r = find_row(P, row, false);
     const int at = r.pos >> P.shift;                              // the query's own page
-    const int begin = P.first + blockIdx.x * kPagesCta, end = min(at + 1 - P.last, begin + kPagesCta);
+    const int begin = P.first + (blockIdx.x * (kScorers / 32) + warp) * kPagesWarp, end = min(at + 1 - P.last, begin + kPagesWarp);
     if (r.pos < 0 || at + 1 <= P.keep || begin >= end) return;
-    const int groups = (P.group + 3) / 4;
-    for (int i = tid; i < groups * 4 * D; i += kThreads) {
-        const int h = i / D, c = i - h * D;
-        const double v = h < P.group ? double(to_float(static_cast<const T*>(P.q)[row * P.q_stride + (long long)(head * P.group + h) * D + c])) : 0.0;
-        s_q[h * D + ((c / 32 * 2 + (c & 2) / 2) * 8 + (c % 32) / 4) * 2 + (c & 1)] = v;
-    }
-    __syncthreads();
-    for (int i0 = begin + 4 * warp; i0 < end; i0 += 4 * (kThreads / 32)) {
-        const int i = i0 + (lane >> 3);
-        const int page = i < end ? __ldg(P.tables + (long long)r.seq * P.width + i) : -1;
-        const bool there = page >= 0 && page < P.n_pages;
-        uint2 lo[J], hi[J];
-        const __half* box = P.bounds + ((long long)(there ? page : 0) * P.n_kv + head) * (2 * D) + 4 * l;
+    // the boxes of pages begin + g and begin + g + 8 of each tile: this lane's runs of 8 halves
+    bool there[kTiles][2];
+    const uint4* box[kTiles][2];
 #pragma unroll
-        for (int p = 0; p < J; ++p) {
-            lo[p] = there ? __ldg(reinterpret_cast<const uint2*>(box + 32 * p)) : make_uint2(0, 0);
-            hi[p] = there ? __ldg(reinterpret_cast<const uint2*>(box + D + 32 * p)) : make_uint2(0, 0);
+    for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int i = begin + 16 * y + g + 8 * x, page = i < end ? __ldg(P.tables + (long long)r.seq * P.width + i) : -1;
+            there[y][x] = page >= 0 && page < P.n_pages;
+            box[y][x] = reinterpret_cast<const uint4*>(P.bounds + ((long long)(there[y][x] ? page : 0) * P.n_kv + head) * (2 * D)) + t;
         }
-        double best = -INFINITY;
-        for (int g = 0; g < groups; ++g) {
-            double acc[4] = {0.0, 0.0, 0.0, 0.0};
-            const double* q = s_q + 4 * g * D + 2 * l;
+    uint4 a[kAhead][2];
+    auto load = [&](int y, int s0) {
 #pragma unroll
-            for (int p = 0; p < J; ++p)
+        for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float2 a = unpack_h2(h ? lo[p].y : lo[p].x), b = unpack_h2(h ? hi[p].y : hi[p].x);
-                    const double a0 = a.x, a1 = a.y, b0 = b.x, b1 = b.y;
+            for (int x = 0; x < 2; ++x) a[s][x] = there[y][x] ? __ldg(box[y][x] + 4 * (s0 + s)) : make_uint4(0, 0, 0, 0);
+    };
+    load(0, 0);
+    float best[kTiles][2], size = 0.f;                            // of the pages; the heads' largest sum of |q|
+    uint32_t wide[kTiles][2];                                     // largest |half| of the boxes' runs
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const double2 v = *reinterpret_cast<const double2*>(q + n * D + (p * 2 + h) * 16);
-                        acc[n] = fma(v.x, v.x > 0.0 ? b0 : a0, acc[n]);
-                        acc[n] = fma(v.y, v.y > 0.0 ? b1 : a1, acc[n]);
+    for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) best[y][x] = -INFINITY, wide[y][x] = 0;
+    for (int h0 = 0; h0 < P.group; h0 += 8) {
+        // ---- column g: query head h0 + g
+        const bool live = h0 + g < P.group;
+        const T* src = static_cast<const T*>(P.q) + row * P.q_stride + (long long)(head * P.group + (live ? h0 + g : 0)) * D + 8 * t;
+        float4 q[J][2];
+        float top = 0.f, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const float4 v = q[j][m] = live ? load4(src + 32 * j + 4 * m) : make_float4(0.f, 0.f, 0.f, 0.f);
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                sum += (fabsf(v.x) + fabsf(v.y)) + (fabsf(v.z) + fabsf(v.w));
+            }
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o)), sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        size = larger(size, sum);
+        if (top > 0.f && top < 1e-24f) size = INFINITY;           // below what the powers of two here lift: all of it in fp64
+        // 2^14 <= top 2^-e < 2^15; a head of zeros or with an infinity keeps its size
+        const int ex = int((__float_as_uint(top) >> 23) & 255u), e = ex == 0 || ex == 255 ? 0 : max(-100, ex - 127 - 14);
+        const float down = __uint_as_float(uint32_t(127 - e) << 23);
+        uint32_t b[kPieces][2][kParts][2];                        // [piece: lo's, hi's][step][part][half of the step]
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const float v[4] = {q[j][m].x * down, q[j][m].y * down, q[j][m].z * down, q[j][m].w * down};
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    uint32_t w = pack_h2(v[2 * y], v[2 * y + 1]);
+                    const float2 f = unpack_h2(w);
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) {
+                        if (part) w = pack_h2(v[2 * y] - f.x, v[2 * y + 1] - f.y);
+                        // by the sign of the value, not of its second part
+                        const uint32_t minus = (v[2 * y] < 0.f ? 0xFFFFu : 0u) | (v[2 * y + 1] < 0.f ? 0xFFFF0000u : 0u);
+                        b[j][m][part][y] = w & minus, b[J + j][m][part][y] = w & ~minus;
                     }
                 }
+            }
+        const float back = __uint_as_float(uint32_t(127 + e) << 23);
+        const float back0 = __shfl_sync(0xffffffffu, back, 8 * t), back1 = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
-            for (int o = 1; o < 8; o *= 2)
+        for (int y = 0; y < kTiles; ++y) {
+            if (begin + 16 * y >= end) continue;
+            // ---- the products, in four chains
+            float c[4][4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) acc[n] += __shfl_xor_sync(0xffffffffu, acc[n], o);
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                if (4 * g + n < P.group) best = fmax(best, acc[n]);
+                for (int i = 0; i < 4; ++i) c[x][i] = 0.f;
+#pragma unroll
+            for (int s0 = 0; s0 < kPieces; s0 += kAhead) {
+                if (y || s0 || h0) load(y, s0);
+#pragma unroll
+                for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) {
+                        mma16816(c[s & 1], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b[s0 + s][0][part][0], b[s0 + s][0][part][1]);
+                        mma16816(c[2 + (s & 1)], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b[s0 + s][1][part][0], b[s0 + s][1][part][1]);
+                    }
+                    if (h0 == 0)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            wide[y][x] = __vmaxu2(wide[y][x], __vmaxu2(__vmaxu2(a[s][x].x & 0x7FFF7FFFu, a[s][x].y & 0x7FFF7FFFu), __vmaxu2(a[s][x].z & 0x7FFF7FFFu, a[s][x].w & 0x7FFF7FFFu)));
+                }
+            }
+            // ---- columns 2 t, 2 t + 1 of rows g and g + 8: times their heads' powers of two, and the largest
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float u = ((c[0][2 * x] + c[1][2 * x]) + (c[2][2 * x] + c[3][2 * x])) * back0;
+                const float v = ((c[0][2 * x + 1] + c[1][2 * x + 1]) + (c[2][2 * x + 1] + c[3][2 * x + 1])) * back1;
+                if (h0 + 2 * t < P.group) best[y][x] = fmaxf(best[y][x], u);
+                if (h0 + 2 * t + 1 < P.group) best[y][x] = fmaxf(best[y][x], v);
+            }
         }
-        if (i < end && l == 0) P.scores[((long long)row * P.n_kv + head) * P.width + i] = there ? best : -INFINITY;
     }
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2) {
+        size = larger(size, __shfl_xor_sync(0xffffffffu, size, o));      // over the columns
+    }
+    const long long out = ((long long)row * P.n_kv + head) * P.width;
+#pragma unroll
+    for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int o = 1; o < 4; o *= 2) {
+                best[y][x] = fmaxf(best[y][x], __shfl_xor_sync(0xffffffffu, best[y][x], o));
+                wide[y][x] = __vmaxu2(wide[y][x], __shfl_xor_sync(0xffffffffu, wide[y][x], o));
+            }
+            const int i = begin + 16 * y + g + 8 * x;
+            const float2 w = unpack_h2(wide[y][x]);
+            if (t == x && i < end) {
+                P.near[out + i] = there[y][x] ? best[y][x] : -INFINITY;
+                P.sizes[out + i] = there[y][x] ? size * fmaxf(w.x, w.y) : 0.f;
+            }
+        }
 }
 
 // ---- the choice ------------------------------------------------------------------------------------------------
@@ -217,14 +328,64 @@ __device__ __forceinline__ uint64_t ordered64(double x) {
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// A CTA a row and key head.  The k-th largest score by digits of 8 bits from the top: a histogram of those that agree with
-// the digits so far; then the pages from it on, in order.
+// exclusive sums over the CTA's threads; total: of all
+__device__ __forceinline__ int block_sums(int x, int* s_warp, int& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    __syncthreads();                                              // s_warp may still be read
+    if (lane == 31) s_warp[warp] = inc;
+    __syncthreads();
+    total = 0;
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += s_warp[w];
+        total += s_warp[w];
+    }
+    return before + inc - x;
+}
+constexpr int kBins = 4 * kThreads, kList = 512, kHold = 8192;
+
+// Of kPer bins a thread from the top (bin kPer * kThreads - 1 - kPer tid and the ones below) the one in which the count reaches `need`,
+// and how many of it are needed.
+template <int kPer>
+__device__ __forceinline__ void find_bin(const int* s_hist, int need, int* s_warp, int* s_bin, int* s_need) {
+    int sum = 0, total;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += s_hist[kPer * (kThreads - threadIdx.x) - 1 - i];
+    int above = block_sums(sum, s_warp, total);
+    if (above < need && need <= above + sum)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int bin = kPer * (kThreads - threadIdx.x) - 1 - i, n = s_hist[bin];
+            if (above < need && need <= above + n) *s_bin = bin, *s_need = need - above;
+            above += n;
+        }
+    __syncthreads();
+}
+
+// A CTA a row and key head.  A histogram of the near scores in even bins between the least and the largest tells the bin of the k-th
+// largest.  Pages whose score lies above that bin by twice the error are taken, those below it by as much are not; the few others are
+// computed again in fp64, a warp each, and ranked against one another (more than a list holds, scores alike say: by digits of
+// 8 bits).  Then the pages in order.  Bound by latency and by fetching its own instructions (unrolled over scores in registers it took 16 us
+// for 2048 pages), so its loops are rolled, over scores in shared memory.
+template <int DT>
 __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant__ ChooseParams P) {
-    __shared__ int s_seq, s_hist[256], s_digit, s_need, s_warp[kThreads / 32];
+    using T = typename Elem<DT>::type;
+    __shared__ float s_near[kHold];
+    __shared__ int s_hist[kBins], s_bin, s_need, s_warp[kThreads / 32], s_count;
+    __shared__ float s_lo[kThreads / 32], s_hi[kThreads / 32], s_size[kThreads / 32];
+    __shared__ uint64_t s_key[kList];
+    __shared__ int s_place[kList];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.x % P.n_kv, row = blockIdx.x / P.n_kv;
-    const Row r = find_row(P, row, &s_seq, head == 0);
+    const Row r = find_row(P, row, head == 0);
     int* out = P.chosen + (long long)blockIdx.x * P.keep;
     const int* table = P.tables + (long long)max(r.seq, 0) * P.width;
     const int n = r.pos < 0 ? 0 : (r.pos >> P.shift) + 1, kept = min(n, P.keep);
@@ -233,78 +394,152 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant_
         for (int i = tid; i < P.keep; i += kThreads) out[i] = i < n ? __ldg(table + i) : -1;
         return;
     }
-    const int begin = P.first, end = n - P.last, k = P.keep - P.first - P.last;
+    const int middle = n - P.last - P.first, k = P.keep - P.first - P.last;
     for (int i = tid; i < P.first; i += kThreads) out[i] = __ldg(table + i);
-    for (int i = tid; i < P.last; i += kThreads) out[P.keep - P.last + i] = __ldg(table + end + i);
+    for (int i = tid; i < P.last; i += kThreads) out[P.keep - P.last + i] = __ldg(table + n - P.last + i);
     if (k == 0) return;
-    const double* scores = P.scores + (long long)blockIdx.x * P.width;
-    uint64_t prefix = 0, mask = 0;
-    int need = k;                                                 // of those that agree with prefix
-    bool tied = true;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        s_hist[tid] = 0;
-        __syncthreads();
-        for (int i = begin + tid; i < end; i += kThreads) {
-            const uint64_t key = ordered64(scores[i]);
-            if ((key & mask) == prefix) atomicAdd(&s_hist[key >> shift & 255], 1);
+    table += P.first, out += P.first;
+    // ---- the middle's scores, in shared memory where they fit, and their range
+    const long long at0 = (long long)blockIdx.x * P.width + P.first;
+    float* near = middle <= kHold ? s_near : P.near + at0;
+    float lo = INFINITY, hi = -INFINITY, size = 0.f;
+#pragma unroll 4
+    for (int i = tid; i < middle; i += kThreads) {
+        const float s = P.near[at0 + i], y = P.sizes[at0 + i];
+        if (middle <= kHold) s_near[i] = s;
+        if (fabsf(s) < INFINITY) lo = fminf(lo, s), hi = fmaxf(hi, s);
+        size = larger(size, y);
+    }
+    for (int i = tid; i < kBins; i += kThreads) s_hist[i] = 0;
+    if (tid == 0) s_count = 0;
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        size = larger(size, __shfl_xor_sync(0xffffffffu, size, o));
+    }
+    if (lane == 0) s_lo[warp] = lo, s_hi[warp] = hi, s_size[warp] = size;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) lo = fminf(lo, s_lo[w]), hi = fmaxf(hi, s_hi[w]), size = larger(size, s_size[w]);
+    const float per = hi > lo && hi - lo < INFINITY ? kBins / (hi - lo) : 0.f;
+    const float off = size < 1e30f ? size * (1.f / 16384.f) : INFINITY;      // twice the error; with infinities and NaN every page is computed again
+    // grows with the score: each step of it does (NaN: 0)
+    auto bin_of = [&](float f) { return !(f > lo) ? 0 : f >= hi ? kBins - 1 : min(kBins - 1, int((f - lo) * per)); };
+#pragma unroll 1
+    for (int i = tid; i < middle; i += kThreads) atomicAdd(&s_hist[bin_of(near[i])], 1);
+    __syncthreads();
+    find_bin<kBins / kThreads>(s_hist, k, s_warp, &s_bin, &s_need);
+    // ---- taken: +inf, not: -inf; the ones to be computed again are listed
+    const int bin = s_bin;
+    int sure = 0, total;
+#pragma unroll 1
+    for (int i = tid; i < middle; i += kThreads) {
+        const float s = near[i];
+        const bool above = off < INFINITY && bin_of(s - off) > bin, below = off < INFINITY && bin_of(s + off) < bin;
+        sure += above;
+        if (!above && !below) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kList) s_place[at] = i;
         }
-        __syncthreads();
-        if (warp == 0) {
-            int own[8], sum = 0;                                  // lane: digits 255 - 8 lane .. 248 - 8 lane
+        near[i] = above ? INFINITY : below ? -INFINITY : 0.f;
+    }
+    block_sums(sure, s_warp, total);
+    int need = k - total;                                         // of the ones to be computed again: one at least, not more than there are
+    const int members = s_count;
+    // a page's score in fp64, by a warp, four heads at a time
+    auto exact = [&](int i) {
+        const int page = __ldg(table + i), D = P.dim;
+        if (page < 0 || page >= P.n_pages) return -double(INFINITY);
+        const __half* box = P.bounds + ((long long)page * P.n_kv + head) * (2 * D);
+        double best = -INFINITY;
+#pragma unroll 1
+        for (int h0 = 0; h0 < P.group; h0 += 4) {
+            const T* q = static_cast<const T*>(P.q) + row * P.q_stride + (long long)(head * P.group + h0) * D;
+            double sum[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 2
+            for (int c = lane; c < D; c += 32) {
+                const float a = __half2float(box[c]), b = __half2float(box[D + c]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) own[i] = s_hist[255 - 8 * lane - i], sum += own[i];
-            int inc = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const int y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            int above = inc - sum;
-            if (above < need && need <= inc) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (above < need && need <= above + own[i]) s_digit = 255 - 8 * lane - i, s_need = need - above;
-                    above += own[i];
+                for (int h = 0; h < 4; ++h) {
+                    const float x = h0 + h < P.group ? to_float(q[h * D + c]) : 0.f;
+                    sum[h] = fma(double(x), double(x > 0.f ? b : a), sum[h]);
                 }
             }
+#pragma unroll
+            for (int o = 16; o; o /= 2)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+                if (h0 + h < P.group) best = fmax(best, sum[h]);
+        }
+        return best;
+    };
+    if (need == members) {
+#pragma unroll 1
+        for (int i = tid; i < middle; i += kThreads)
+            if (near[i] == 0.f) near[i] = INFINITY;
+    } else if (members <= kList) {
+#pragma unroll 1
+        for (int m = warp; m < members; m += kThreads / 32) {
+            const double s = exact(s_place[m]);
+            if (lane == 0) s_key[m] = ordered64(s);
         }
         __syncthreads();
-        prefix |= uint64_t(s_digit) << shift, mask |= 255ull << shift;
-        need = s_need;
-        if (s_hist[s_digit] == need) {                            // all of them
-            tied = false;
-            break;
+#pragma unroll 1
+        for (int m = tid; m < members; m += kThreads) {
+            const uint64_t key = s_key[m];
+            const int place = s_place[m];
+            int rank = 0;
+            for (int j = 0; j < members; ++j) rank += s_key[j] > key || (s_key[j] == key && s_place[j] < place);
+            near[place] = rank < need ? INFINITY : -INFINITY;
         }
-        __syncthreads();
+    } else {
+        double* scores = P.scores + at0;
+#pragma unroll 1
+        for (int i = warp; i < middle; i += kThreads / 32)
+            if (near[i] == 0.f) {
+                const double s = exact(i);
+                if (lane == 0) scores[i] = s;
+            }
+        uint64_t prefix = 0, mask = 0;
+#pragma unroll 1
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            __syncthreads();
+            s_hist[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < middle; i += kThreads) {
+                if (near[i] != 0.f) continue;
+                const uint64_t key = ordered64(scores[i]);
+                if ((key & mask) == prefix) atomicAdd(&s_hist[key >> shift & 255], 1);
+            }
+            __syncthreads();
+            find_bin<1>(s_hist, need, s_warp, &s_bin, &s_need);
+            prefix |= uint64_t(s_bin) << shift, mask |= 255ull << shift;
+            need = s_need;
+        }
+        // of equal scores the first ones
+        int equal = 0;
+#pragma unroll 1
+        for (int i0 = 0; i0 < middle; i0 += kThreads) {
+            const int i = i0 + tid;
+            const bool open = i < middle && near[i] == 0.f;
+            const uint64_t key = open ? ordered64(scores[i]) : 0;
+            const int before = equal + block_sums(open && key == prefix, s_warp, total);
+            if (open) near[i] = key > prefix || (key == prefix && before < need) ? INFINITY : -INFINITY;
+            equal += total;
+        }
     }
-    // above the prefix every one, with it the first `need`
-    int base = P.first, equal = 0;
-    for (int i0 = begin; i0 < end; i0 += kThreads) {
-        const int i = i0 + tid;
-        const uint64_t key = i < end ? ordered64(scores[i]) & mask : 0;
-        const bool same = i < end && key == prefix;
-        bool take = i < end && key > prefix;
-        const uint32_t ties = __ballot_sync(0xffffffffu, same);
-        __syncthreads();
-        if (lane == 0) s_warp[warp] = __popc(ties);
-        __syncthreads();
-        int before = equal;
-        for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) before += s_warp[w];
-            equal += s_warp[w];
-        }
-        if (same && (!tied || before + __popc(ties & ((1u << lane) - 1)) < need)) take = true;
-        const uint32_t taken = __ballot_sync(0xffffffffu, take);
-        __syncthreads();
-        if (lane == 0) s_warp[warp] = __popc(taken);
-        __syncthreads();
-        int to = base + __popc(taken & ((1u << lane) - 1));
-        for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) to += s_warp[w];
-            base += s_warp[w];
-        }
-        if (take) out[to] = __ldg(table + i);
-    }
+    // ---- the pages, a run of places a thread
+    __syncthreads();
+    const int run = (middle + kThreads - 1) / kThreads, i0 = min(middle, tid * run), i1 = min(middle, i0 + run);
+    int count = 0;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) count += near[i] > 0.f;
+    int to = block_sums(count, s_warp, total);
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i)
+        if (near[i] > 0.f) out[to++] = __ldg(table + i);
 }
 
 bool bad_type(int dtype) { return dtype != QMV_OUT_F32 && dtype != QMV_OUT_BF16 && dtype != QMV_OUT_F16; }
@@ -347,7 +582,7 @@ int qmv_kv_bounds(const qmv_kv_cache* cache, const int* tables, int table_width,
 int64_t qmv_kv_choose_workspace_bytes(const qmv_kv_cache* cache, int table_width, long long n_rows, int keep) {
     KvView c{};
     if (kv_view(cache, c) || table_width <= 0 || table_width > kMostKeys >> c.page_shift || n_rows <= 0 || n_rows > 65535 || keep <= 0) return 0;
-    return table_width <= keep ? 8 : 8LL * n_rows * c.n_kv * table_width;
+    return table_width <= keep ? 8 : 16LL * n_rows * c.n_kv * table_width;
 }
 
 int qmv_kv_choose(const qmv_kv_cache* cache, const void* q, int dtype, long long q_stride, int n_heads, const void* bounds,
@@ -370,20 +605,20 @@ int qmv_kv_choose(const qmv_kv_cache* cache, const void* q, int dtype, long long
     ChooseParams P{};
     P.q = q, P.q_stride = q_stride, P.bounds = static_cast<const __half*>(bounds), P.n_pages = c.n_pages;
     P.tables = tables, P.lens = lens, P.starts = starts;
-    P.n_kv = c.n_kv, P.group = n_heads / c.n_kv, P.width = table_width, P.shift = c.page_shift, P.n_seq = n_seq, P.n_rows = int(n_rows);
+    P.n_kv = c.n_kv, P.group = n_heads / c.n_kv, P.dim = c.dim, P.width = table_width, P.shift = c.page_shift, P.n_seq = n_seq, P.n_rows = int(n_rows);
     P.keep = keep, P.first = first, P.last = last;
-    P.scores = static_cast<double*>(workspace), P.chosen = chosen, P.held = held;
+    const long long pages = n_rows * c.n_kv * table_width;
+    P.scores = static_cast<double*>(workspace), P.near = reinterpret_cast<float*>(P.scores + pages), P.sizes = P.near + pages;
+    P.chosen = chosen, P.held = held;
     P.status = device_status_ptr();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int middle = table_width - first - last;                // pages to score, at most
     if (table_width > keep && middle > 0) {
+        constexpr int kPagesCta = kPagesWarp * (kScorers / 32);
         const dim3 grid((middle + kPagesCta - 1) / kPagesCta, c.n_kv, unsigned(n_rows));
-        const size_t smem = size_t((P.group + 3) / 4 * 4) * c.dim * 8;
         auto go = [&](auto dt, auto j) {
             constexpr int DT = decltype(dt)::value, J = decltype(j)::value;
-            static SmemGrant grant;
-            if (const int e = grant(score_kernel<DT, J>, 64 * 256 * 8)) return e;
-            return launch_pdl_smem(score_kernel<DT, J>, grid, dim3(kThreads), smem, s, P);
+            return launch_pdl(score_kernel<DT, J>, grid, dim3(kScorers), s, P);
         };
         const int e = by_elem(dtype, [&](auto dt) {
             switch (c.J) {
@@ -396,7 +631,7 @@ int qmv_kv_choose(const qmv_kv_cache* cache, const void* q, int dtype, long long
         });
         if (e) return e;
     }
-    return launch_behind(choose_kernel, dim3(unsigned(n_rows * c.n_kv)), dim3(kThreads), s, P);
+    return by_elem(dtype, [&](auto dt) { return launch_behind(choose_kernel<decltype(dt)::value>, dim3(unsigned(n_rows * c.n_kv)), dim3(kThreads), s, P); });
 }
 
 }  // extern "C"

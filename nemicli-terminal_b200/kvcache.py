@@ -96,6 +96,7 @@ class KVCache:
                 raise RuntimeError(f"KVCache: buffers must be contiguous CUDA tensors of shapes {shapes} and types {types}")
         self.k_codes, self.v_codes, self.scales = buffers
         self.device = self.k_codes.device
+        self._where = self.k_codes.get_device()
         self._c = _Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.scales.data_ptr(), n_pages, n_kv, dim, page,
                          TYPE_ID[k_fmt], TYPE_ID[v_fmt])
         self._ref = ctypes.byref(self._c)
@@ -104,7 +105,7 @@ class KVCache:
 
     def _tokens(self, t: torch.Tensor, what: str, heads: Optional[int] = None, like: Optional[torch.Tensor] = None):
         shape = t.shape
-        if t.device != self.device:
+        if t.get_device() != self._where:
             raise RuntimeError(f"{what}: tensor on {t.device}, the cache on {self.device}")
         if len(shape) != 3 or shape[2] != self.dim or t.dtype not in _DTYPES or heads is not None and shape[1] != heads \
                 or shape[1] == 0:
@@ -115,13 +116,23 @@ class KVCache:
 
     def _index(self, t: torch.Tensor, what: str, dtype, *shape):
         got = t.shape
-        ok = t.device == self.device and t.dtype == dtype and len(got) == len(shape) and t.is_contiguous()
-        if ok:
-            for n, want in zip(got, shape):
-                if want is not None and n != want:
-                    ok = False
+        ok = t.dtype is dtype and t.get_device() == self._where and t.is_contiguous()
+        if ok and got != shape:
+            ok = len(got) == len(shape)
+            if ok:
+                for n, want in zip(got, shape):
+                    if want is not None and n != want:
+                        ok = False
         if not ok:
             raise RuntimeError(f"{what}: contiguous {dtype} {shape} on {self.device} expected, got {t.dtype} {tuple(got)}")
+
+    def _room(self, sizes: tuple, nbytes: int) -> int:
+        if nbytes <= 0:
+            raise RuntimeError(f"KVCache: a call of sizes {sizes} is not supported")
+        if len(self._need) >= 4096:           # sizes that never come back
+            self._need.clear()
+        self._need[sizes] = nbytes
+        return nbytes
 
     def _out(self, q: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
         if out is None:
@@ -158,10 +169,12 @@ class KVCache:
             else:
                 self._index(pos, "KVCache.write positions", torch.int64, None, rows)
                 n_axes = pos.shape[0]
-                axes = tuple(axes)
-                if not 1 <= n_axes <= 4 or len(axes) != rot // 2 or not all(0 <= a < n_axes for a in axes):
+                try:
+                    named = bytes(axes)
+                except (TypeError, ValueError):
+                    named = b""
+                if not 1 <= n_axes <= 4 or len(named) != rot // 2 or max(named) >= n_axes:
                     raise RuntimeError(f"KVCache.write: {rot // 2} axes, each below the {n_axes} (at most 4) of positions, expected, got {axes}")
-                axes = bytes(axes)
         elif axes is not None:
             raise RuntimeError("KVCache.write: axes without rope")
         out, qs, n_q = None, 0, 0
@@ -181,7 +194,7 @@ class KVCache:
                 else:
                     st = _lib.load().qmv_kv_write_axes(self._ref, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], ks, vs, slots.data_ptr(),
                                                        rows, cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), n_pos, rot,
-                                                       int(bool(paired)), axes, n_axes, _lib.addr(q), qs, n_q, _lib.addr(out),
+                                                       int(bool(paired)), named, n_axes, _lib.addr(q), qs, n_q, _lib.addr(out),
                                                        _lib.stream_of(self.device))
             if st:
                 _lib.check(st, "qmv_kv_write")
@@ -244,12 +257,7 @@ class KVCache:
             sizes = (heads, n_seq, most, dtype, width, window)
             nbytes = self._need.get(sizes)
             if nbytes is None:
-                nbytes = lib.qmv_kv_attend_workspace_bytes(self._ref, *sizes)
-                if nbytes <= 0:
-                    raise RuntimeError(f"KVCache.attend: {heads} heads, {n_seq} sequences of {most} new tokens not supported")
-                if len(self._need) >= 4096:           # sizes that never come back
-                    self._need.clear()
-                self._need[sizes] = nbytes
+                nbytes = self._room(sizes, lib.qmv_kv_attend_workspace_bytes(self._ref, *sizes))
             if nbytes > 256:
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             else:                                     # used by nothing
@@ -266,9 +274,11 @@ class KVCache:
     def copy(self, src: torch.Tensor, dst: torch.Tensor, used: Optional[torch.Tensor] = None) -> None:
         """Page src[i] copied to page dst[i] (int32, any shape; -1: nothing), its first used[i] tokens or all; for beams that part
         (pages.reorder).  No page is the target of two copies, nor target and source."""
-        n = src.numel()
-        for t, what in ((src, "src"), (dst, "dst")) if used is None else ((src, "src"), (dst, "dst"), (used, "used")):
-            self._index(t, f"KVCache.copy {what}", torch.int32, *src.shape)
+        n, shape = src.numel(), src.shape
+        self._index(src, "KVCache.copy src", torch.int32, *shape)
+        self._index(dst, "KVCache.copy dst", torch.int32, *shape)
+        if used is not None:
+            self._index(used, "KVCache.copy used", torch.int32, *shape)
         if n:
             with _lib.on_device(self.device):
                 st = _lib.load().qmv_kv_copy(self._ref, src.data_ptr(), dst.data_ptr(), _lib.addr(used), n, _lib.stream_of(self.device))
@@ -286,11 +296,11 @@ class KVCache:
             raise RuntimeError(f"{what}: 16-byte aligned bounds expected")
 
     def _tables(self, what: str, tables, lens, starts):
-        self._index(tables, f"{what} tables", torch.int32, None, None)
+        self._index(tables, what + " tables", torch.int32, None, None)
         n_seq, width = tables.shape
-        self._index(lens, f"{what} lens", torch.int32, n_seq)
+        self._index(lens, what + " lens", torch.int32, n_seq)
         if starts is not None:
-            self._index(starts, f"{what} starts", torch.int32, n_seq + 1)
+            self._index(starts, what + " starts", torch.int32, n_seq + 1)
         return n_seq, width
 
     def summarise(self, bounds: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None,
@@ -336,8 +346,11 @@ class KVCache:
             q, qs = _rows(q, heads, self.dim)
             lib = _lib.load()
             with _lib.on_device(self.device):
-                nbytes = lib.qmv_kv_choose_workspace_bytes(self._ref, width, rows, keep)
-                ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
+                sizes = ("choose", width, rows, keep)
+                nbytes = self._need.get(sizes)
+                if nbytes is None:
+                    nbytes = self._room(sizes, lib.qmv_kv_choose_workspace_bytes(self._ref, width, rows, keep))
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
                 st = lib.qmv_kv_choose(self._ref, q.data_ptr(), _DTYPES[q.dtype], qs, heads, bounds.data_ptr(), tables.data_ptr(), width,
                                        lens.data_ptr(), _lib.addr(starts), n_seq, rows, keep, first, last, chosen.data_ptr(), held.data_ptr(),
                                        ws.data_ptr(), nbytes, _lib.stream_of(self.device))
@@ -366,15 +379,10 @@ class KVCache:
         q, qs = _rows(q, heads, self.dim)
         lib, dtype = _lib.load(), _DTYPES[q.dtype]
         with _lib.on_device(self.device):
-            sizes = (heads, rows, dtype, keep)
+            sizes = ("attend_chosen", heads, rows, dtype, keep)
             nbytes = self._need.get(sizes)
             if nbytes is None:
-                nbytes = lib.qmv_kv_attend_chosen_workspace_bytes(self._ref, *sizes)
-                if nbytes <= 0:
-                    raise RuntimeError(f"KVCache.attend_chosen: {heads} heads, {rows} rows of {keep} pages not supported")
-                if len(self._need) >= 4096:
-                    self._need.clear()
-                self._need[sizes] = nbytes
+                nbytes = self._room(sizes, lib.qmv_kv_attend_chosen_workspace_bytes(self._ref, heads, rows, dtype, keep))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             st = lib.qmv_kv_attend_chosen(self._ref, q.data_ptr(), dtype, qs, heads, chosen.data_ptr(), keep, held.data_ptr(), rows,
                                           self.dim ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), nbytes,
