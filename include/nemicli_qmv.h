@@ -386,8 +386,8 @@ int64_t qmv_kv_choose_workspace_bytes(const qmv_kv_cache* cache, int table_width
  * them, and held [n_rows] the tokens in them up to the query's own.  A query at position p has the pages 0 .. p / page of its
  * sequence; where these are more than keep, the first `first`, the last `last` (at least 1: the query's own, whose box need not be
  * written) and of the others those with the largest
- *     max over the key head's query heads of sum_c max(q[c] lo[c], q[c] hi[c])
- * (no product q . k of the page is larger), computed in fp64, the earlier page first among equals; NaN counts as least.  q, tables,
+ *     max over the key head's query heads of sum_c (q[c] > 0 ? q[c] hi[c] : q[c] lo[c])
+ * (no product q . k of the page is larger), as in fp64, the earlier page first among equals; NaN counts as least.  q, tables,
  * lens, starts as for qmv_kv_attend; rows that no sequence covers, or with p < 0, get no page and held 0.  At most 65535 rows and
  * 64 query heads a key head.  workspace: 256-byte aligned, qmv_kv_choose_workspace_bytes long.  Two launches.  Replaces: nothing. */
 int qmv_kv_choose(const qmv_kv_cache* cache, const void* q, int dtype, long long q_stride, int n_heads, const void* bounds,
