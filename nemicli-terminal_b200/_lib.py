@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -16,6 +17,7 @@ from . import build as _build
 
 _lock = threading.Lock()
 _lib = None
+_host = None
 
 P, I, LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 
@@ -98,6 +100,23 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def host():
+    """The module of the small calls' host side (csrc/host/qmv_host.cpp), over the same library."""
+    global _host
+    if _host is not None:
+        return _host
+    load()
+    with _lock:
+        if _host is None:
+            if not os.path.exists(_build.HOST_PATH):
+                raise RuntimeError(f"module missing: {_build.HOST_PATH} (build it with nemicli_terminal_b200.build.build())")
+            spec = importlib.util.spec_from_file_location("_qmv_host", _build.HOST_PATH)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            _host = mod
+    return _host
+
+
 def exported_symbols() -> list:
     return list(_SIGNATURES)
 
@@ -131,8 +150,8 @@ _HERE = contextlib.nullcontext()
 def on_device(device):
     """Makes `device` the current one for a launch (a stream belongs to its own device only); nothing to do where it
     is already."""
-    index = device.index                     # (a tensor's device: CUDA is up)
-    return _HERE if index is None or index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+    index = device.index
+    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def addr(t) -> int:

@@ -24,6 +24,8 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 OBJ_DIR = os.path.join(HERE, "_build")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 PER_FORMAT = "qmv_fmt.cu"
+HOST_SRC = os.path.join(CSRC, "host", "qmv_host.cpp")
+HOST_PATH = os.path.join(HERE, "_qmv_host.so")
 
 
 def nvcc() -> str:
@@ -99,17 +101,47 @@ def up_to_date(out: str = LIB_PATH, obj_dir: str = OBJ_DIR) -> bool:
 
 def build(force: bool = False, verbose: bool = False, extra: tuple = (), out: str = LIB_PATH,
           obj_dir: str = OBJ_DIR, jobs: int = 0) -> str:
-    """Compile the stale objects in parallel and link `out`.  extra: more nvcc flags (e.g. -D...).
-    Processes that build at the same time (one per rank under torchrun) take turns on a lock file in
+    """Compile the stale objects in parallel and link `out`; with the library itself also the Python module
+    over it (build_host).  extra: more nvcc flags (e.g. -D...).  Processes that build at the same time (one per rank under torchrun) take turns on a lock file in
     obj_dir; the later ones find the library up to date."""
-    if not force and up_to_date(out, obj_dir):
+    with_host = out == LIB_PATH
+    if not force and up_to_date(out, obj_dir) and not (with_host and _host_stale()):
         return out
     os.makedirs(obj_dir, exist_ok=True)
     with open(os.path.join(obj_dir, ".lock"), "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
-        if not force and up_to_date(out, obj_dir):
-            return out
-        return _build_locked(force, verbose, extra, out, obj_dir, jobs)
+        if force or not up_to_date(out, obj_dir):
+            _build_locked(force, verbose, extra, out, obj_dir, jobs)
+        if with_host and (force or _host_stale()):
+            build_host(verbose)
+        return out
+
+
+def _host_stale() -> bool:
+    """The Python module is older than its source or the C ABI it calls (the library itself may be newer)."""
+    sources = (HOST_SRC, os.path.join(HERE, "..", "include", "nemicli_qmv.h"))
+    return not os.path.exists(HOST_PATH) or any(os.path.getmtime(p) > os.path.getmtime(HOST_PATH) for p in sources)
+
+
+def build_host(verbose: bool = False) -> str:
+    """The CPython module of the small calls' host side (csrc/host/qmv_host.cpp): host code only, compiled against torch's headers
+    and linked to the library beside it.  torch's own libraries are those of the process that imports it."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", HOST_SRC,
+           "-o", HOST_PATH + ".tmp", f"-L{HERE}", f"-l:{LIB_NAME}", f"-L{root}/lib", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda",
+           "-lc10", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr, flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)} ({res.returncode}):\n{res.stderr[-4000:]}")
+    os.replace(HOST_PATH + ".tmp", HOST_PATH)
+    return HOST_PATH
 
 
 def _build_locked(force: bool, verbose: bool, extra: tuple, out: str, obj_dir: str, jobs: int) -> str:

@@ -100,6 +100,7 @@ class KVCache:
         self._c = _Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.scales.data_ptr(), n_pages, n_kv, dim, page,
                          TYPE_ID[k_fmt], TYPE_ID[v_fmt])
         self._ref = ctypes.byref(self._c)
+        self._at = ctypes.addressof(self._c)
         self._need = {}                     # workspace bytes of the calls so far, by their sizes
         self._none = None                   # stands for the workspace of calls that use none
 
@@ -126,21 +127,6 @@ class KVCache:
         if not ok:
             raise RuntimeError(f"{what}: contiguous {dtype} {shape} on {self.device} expected, got {t.dtype} {tuple(got)}")
 
-    def _room(self, sizes: tuple, nbytes: int) -> int:
-        if nbytes <= 0:
-            raise RuntimeError(f"KVCache: a call of sizes {sizes} is not supported")
-        if len(self._need) >= 4096:           # sizes that never come back
-            self._need.clear()
-        self._need[sizes] = nbytes
-        return nbytes
-
-    def _out(self, q: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
-        if out is None:
-            return torch.empty_like(q, memory_format=torch.contiguous_format)
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
-            raise RuntimeError(f"{what}: out must be a contiguous, 16-byte aligned {tuple(q.shape)} tensor of {q.dtype}")
-        return out
-
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, q: Optional[torch.Tensor] = None, rope=None,
               paired: bool = False, axes=None) -> Optional[torch.Tensor]:
         """k, v: (rows, n_kv, dim) -> quantised into slots (rows,) int64, which are distinct; a negative slot is a
@@ -151,69 +137,19 @@ class KVCache:
         positions outside the tables leave the row unwritten (its queries 0) and set the device status.
         axes: rot / 2 numbers, the axis of each frequency (rope_axes), for tokens with a position on each of up to four axes
         (time, height and width of pictures): positions is then (axes, rows)."""
-        self._tokens(k, "KVCache.write k", self.n_kv)
-        self._tokens(v, "KVCache.write v", self.n_kv, k)
-        rows = k.shape[0]
-        self._index(slots, "KVCache.write slots", torch.int64, rows)
-        cos = sin = pos = None
-        rot = n_pos = 0
-        if rope is not None:
-            cos, sin, pos = rope
-            self._index(cos, "KVCache.write cos", torch.float32, None, None)
-            self._index(sin, "KVCache.write sin", torch.float32, *cos.shape)
-            n_pos, rot = cos.shape[0], 2 * cos.shape[1]
-            if n_pos == 0 or rot % 8 or not 0 < rot <= self.dim:
-                raise RuntimeError(f"KVCache.write: tables (positions, rot / 2), rot a multiple of 8 up to {self.dim}, got {tuple(cos.shape)}")
-            if axes is None:
-                self._index(pos, "KVCache.write positions", torch.int64, rows)
-            else:
-                self._index(pos, "KVCache.write positions", torch.int64, None, rows)
-                n_axes = pos.shape[0]
-                try:
-                    named = bytes(axes)
-                except (TypeError, ValueError):
-                    named = b""
-                if not 1 <= n_axes <= 4 or len(named) != rot // 2 or max(named) >= n_axes:
-                    raise RuntimeError(f"KVCache.write: {rot // 2} axes, each below the {n_axes} (at most 4) of positions, expected, got {axes}")
-        elif axes is not None:
-            raise RuntimeError("KVCache.write: axes without rope")
-        out, qs, n_q = None, 0, 0
-        if q is not None:
-            self._tokens(q, "KVCache.write q", None, k)
-            n_q = q.shape[1]
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            q, qs = _rows(q, n_q, self.dim)
-        k, ks = _rows(k, self.n_kv, self.dim)
-        v, vs = _rows(v, self.n_kv, self.dim)
-        if rows:
-            with _lib.on_device(self.device):
-                if axes is None:
-                    st = _lib.load().qmv_kv_write(self._ref, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], ks, vs, slots.data_ptr(), rows,
-                                                  _lib.addr(cos), _lib.addr(sin), _lib.addr(pos), n_pos, rot, int(bool(paired)),
-                                                  _lib.addr(q), qs, n_q, _lib.addr(out), _lib.stream_of(self.device))
-                else:
-                    st = _lib.load().qmv_kv_write_axes(self._ref, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], ks, vs, slots.data_ptr(),
-                                                       rows, cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), n_pos, rot,
-                                                       int(bool(paired)), named, n_axes, _lib.addr(q), qs, n_q, _lib.addr(out),
-                                                       _lib.stream_of(self.device))
-            if st:
-                _lib.check(st, "qmv_kv_write")
-        return out
+        cos, sin, positions = (None, None, None) if rope is None else rope
+        if axes is not None:
+            try:
+                axes = bytes(tuple(axes))
+            except (TypeError, ValueError):
+                raise RuntimeError(f"KVCache.write: axes {axes} (numbers from 0 on)") from None
+        return _lib.host().write(self._at, self._where, k, v, slots, q, cos, sin, positions, paired, axes)
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
         """The values at slots (rows,) int64 -> k, v (rows, n_kv, dim) of dtype; negative slots give zeros."""
-        self._index(slots, "KVCache.read slots", torch.int64, None)
         if dtype not in _DTYPES:
             raise RuntimeError(f"KVCache.read: dtype {dtype} (float32, bfloat16 or float16)")
-        rows = slots.shape[0]
-        k, v = (self.scales.new_empty((rows, self.n_kv, self.dim), dtype=dtype) for _ in range(2))
-        if rows:
-            with _lib.on_device(self.device):
-                st = _lib.load().qmv_kv_read(self._ref, slots.data_ptr(), rows, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
-                                             _lib.stream_of(self.device))
-            if st:
-                _lib.check(st, "qmv_kv_read")
-        return k, v
+        return _lib.host().read(self._at, self._where, slots, _DTYPES[dtype])
 
     def attend(self, q: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None,
                max_new: Optional[int] = None, scale: Optional[float] = None, window: int = 0,
@@ -245,7 +181,11 @@ class KVCache:
             raise RuntimeError(f"KVCache.attend: scale {scale} is not finite")
         if window < 0 or most < 0:
             raise RuntimeError("KVCache.attend: window and max_new must not be negative")
-        out = self._out(q, out, "KVCache.attend")
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() \
+                or out.data_ptr() % 16:
+            raise RuntimeError(f"KVCache.attend: out must be a contiguous, 16-byte aligned {tuple(q.shape)} tensor of {q.dtype}")
         if rows == 0 or n_seq == 0 or most == 0:
             return out
         if width == 0:
@@ -257,7 +197,12 @@ class KVCache:
             sizes = (heads, n_seq, most, dtype, width, window)
             nbytes = self._need.get(sizes)
             if nbytes is None:
-                nbytes = self._room(sizes, lib.qmv_kv_attend_workspace_bytes(self._ref, *sizes))
+                nbytes = lib.qmv_kv_attend_workspace_bytes(self._ref, *sizes)
+                if nbytes <= 0:
+                    raise RuntimeError(f"KVCache.attend: {heads} heads, {n_seq} sequences of {most} new tokens not supported")
+                if len(self._need) >= 4096:           # sizes that never come back
+                    self._need.clear()
+                self._need[sizes] = nbytes
             if nbytes > 256:
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             else:                                     # used by nothing
@@ -274,52 +219,19 @@ class KVCache:
     def copy(self, src: torch.Tensor, dst: torch.Tensor, used: Optional[torch.Tensor] = None) -> None:
         """Page src[i] copied to page dst[i] (int32, any shape; -1: nothing), its first used[i] tokens or all; for beams that part
         (pages.reorder).  No page is the target of two copies, nor target and source."""
-        n, shape = src.numel(), src.shape
-        self._index(src, "KVCache.copy src", torch.int32, *shape)
-        self._index(dst, "KVCache.copy dst", torch.int32, *shape)
-        if used is not None:
-            self._index(used, "KVCache.copy used", torch.int32, *shape)
-        if n:
-            with _lib.on_device(self.device):
-                st = _lib.load().qmv_kv_copy(self._ref, src.data_ptr(), dst.data_ptr(), _lib.addr(used), n, _lib.stream_of(self.device))
-            if st:
-                _lib.check(st, "qmv_kv_copy")
+        _lib.host().copy(self._at, self._where, src, dst, used)
 
     def bounds(self) -> torch.Tensor:
         """A new, zeroed float16 (n_pages, n_kv, 2, dim) for summarise and choose: the least and largest key of each page, key
         head and channel."""
         return torch.zeros((self.n_pages, self.n_kv, 2, self.dim), dtype=torch.float16, device=self.device)
 
-    def _bounds(self, t: torch.Tensor, what: str):
-        self._index(t, what, torch.float16, self.n_pages, self.n_kv, 2, self.dim)
-        if t.data_ptr() % 16:
-            raise RuntimeError(f"{what}: 16-byte aligned bounds expected")
-
-    def _tables(self, what: str, tables, lens, starts):
-        self._index(tables, what + " tables", torch.int32, None, None)
-        n_seq, width = tables.shape
-        self._index(lens, what + " lens", torch.int32, n_seq)
-        if starts is not None:
-            self._index(starts, what + " starts", torch.int32, n_seq + 1)
-        return n_seq, width
-
     def summarise(self, bounds: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None,
                   max_new: Optional[int] = None) -> None:
         """Writes into bounds (KVCache.bounds) the boxes of the pages that the newest tokens completed, behind their write; tables,
         lens, starts as for attend (one new token a sequence, or starts[b + 1] - starts[b]).  max_new: at least the most new tokens
         of a sequence (default: a whole table of them).  One launch."""
-        self._bounds(bounds, "KVCache.summarise bounds")
-        n_seq, width = self._tables("KVCache.summarise", tables, lens, starts)
-        most = 1 if starts is None else (width * self.page if max_new is None else int(max_new))
-        if most < 0:
-            raise RuntimeError("KVCache.summarise: max_new must not be negative")
-        if n_seq == 0 or width == 0 or most == 0:
-            return
-        with _lib.on_device(self.device):
-            st = _lib.load().qmv_kv_bounds(self._ref, tables.data_ptr(), width, lens.data_ptr(), _lib.addr(starts), n_seq,
-                                           min(most, width * self.page), bounds.data_ptr(), _lib.stream_of(self.device))
-        if st:
-            _lib.check(st, "qmv_kv_bounds")
+        _lib.host().summarise(self._at, self._where, tables, lens, starts, bounds, max_new)
 
     def choose(self, q: torch.Tensor, bounds: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, keep: int,
                starts: Optional[torch.Tensor] = None, first: int = 1, last: int = 1):
@@ -328,65 +240,10 @@ class KVCache:
         `first` first and the `last` last ones (1 at least: its own) are always chosen, of the others those whose box reaches
         furthest along some query head of the key head; all of them where there are no more than keep.  Rows that no sequence covers
         get none.  Boxes of all pages but the query's own must have been written (summarise).  Two launches."""
-        self._tokens(q, "KVCache.choose q")
-        rows, heads, _ = q.shape
-        if heads % self.n_kv or heads > 64 * self.n_kv:
-            raise RuntimeError(f"KVCache.choose: {heads} heads are not a multiple (at most 64) of {self.n_kv} key heads")
-        self._bounds(bounds, "KVCache.choose bounds")
-        n_seq, width = self._tables("KVCache.choose", tables, lens, starts)
-        if starts is None and rows < n_seq:
-            raise RuntimeError(f"KVCache.choose: {rows} query rows for {n_seq} sequences")
-        if first < 0 or last < 1 or keep < first + last or rows > 65535:
-            raise RuntimeError(f"KVCache.choose: keep {keep} holds first {first} (0 at least) and last {last} (1 at least), rows {rows} up to 65535")
-        chosen = lens.new_empty((rows, self.n_kv, keep))
-        held = lens.new_empty((rows,))
-        if n_seq == 0 or width == 0:
-            return chosen.fill_(-1), held.zero_()
-        if rows:
-            q, qs = _rows(q, heads, self.dim)
-            lib = _lib.load()
-            with _lib.on_device(self.device):
-                sizes = ("choose", width, rows, keep)
-                nbytes = self._need.get(sizes)
-                if nbytes is None:
-                    nbytes = self._room(sizes, lib.qmv_kv_choose_workspace_bytes(self._ref, width, rows, keep))
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-                st = lib.qmv_kv_choose(self._ref, q.data_ptr(), _DTYPES[q.dtype], qs, heads, bounds.data_ptr(), tables.data_ptr(), width,
-                                       lens.data_ptr(), _lib.addr(starts), n_seq, rows, keep, first, last, chosen.data_ptr(), held.data_ptr(),
-                                       ws.data_ptr(), nbytes, _lib.stream_of(self.device))
-            if st:
-                _lib.check(st, "qmv_kv_choose")
-        return chosen, held
+        return _lib.host().choose(self._at, self._where, tables, lens, starts, bounds, q, keep, first, last)
 
     def attend_chosen(self, q: torch.Tensor, chosen: torch.Tensor, held: torch.Tensor, scale: Optional[float] = None,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of each row of q over the pages chosen for it (choose): row r's heads of key head h see the first held[r] tokens
         of the pages chosen[r, h].  Rounding, scale and out as for attend; rows with held 0 give zeros."""
-        self._tokens(q, "KVCache.attend_chosen q")
-        rows, heads, _ = q.shape
-        if heads % self.n_kv:
-            raise RuntimeError(f"KVCache.attend_chosen: {heads} heads are not a multiple of {self.n_kv} key heads")
-        self._index(chosen, "KVCache.attend_chosen chosen", torch.int32, rows, self.n_kv, None)
-        self._index(held, "KVCache.attend_chosen held", torch.int32, rows)
-        if scale is not None and not abs(scale) < 3.5e38:
-            raise RuntimeError(f"KVCache.attend_chosen: scale {scale} is not finite")
-        out = self._out(q, out, "KVCache.attend_chosen")
-        keep = chosen.shape[2]
-        if rows == 0:
-            return out
-        if keep == 0:
-            raise RuntimeError("KVCache.attend_chosen: no page a row")
-        q, qs = _rows(q, heads, self.dim)
-        lib, dtype = _lib.load(), _DTYPES[q.dtype]
-        with _lib.on_device(self.device):
-            sizes = ("attend_chosen", heads, rows, dtype, keep)
-            nbytes = self._need.get(sizes)
-            if nbytes is None:
-                nbytes = self._room(sizes, lib.qmv_kv_attend_chosen_workspace_bytes(self._ref, heads, rows, dtype, keep))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            st = lib.qmv_kv_attend_chosen(self._ref, q.data_ptr(), dtype, qs, heads, chosen.data_ptr(), keep, held.data_ptr(), rows,
-                                          self.dim ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr(), nbytes,
-                                          _lib.stream_of(self.device))
-        if st:
-            _lib.check(st, "qmv_kv_attend_chosen")
-        return out
+        return _lib.host().attend_chosen(self._at, self._where, q, chosen, held, scale, out)

@@ -25,8 +25,6 @@ import torch
 
 from . import _lib
 
-MOST_BEAMS = 64
-
 
 class Plan(NamedTuple):
     slots: torch.Tensor                    # int64 (rows,), -1 behind the last token
@@ -51,76 +49,19 @@ def pool(n_pages: int, device=None):
     return free, torch.tensor([n_pages, 0], dtype=torch.int32, device=free.device)
 
 
-_I32 = torch.int32
-_PAGES = (16, 32, 64, 128, 256, 512, 1024)
-
-
-def _fits(t: torch.Tensor, where: int, shape, dtype=_I32) -> bool:
-    return t.dtype is dtype and t.shape == shape and t.get_device() == where and t.is_contiguous()
-
-
-def _refuse(what: str, t: torch.Tensor, name: str, shape, device, dtype=_I32):
-    raise RuntimeError(f"{what} {name}: contiguous {dtype} {tuple(shape)} on {device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
-
-
-def _common(what: str, tables, lens, free, counts, page: int):
-    """The index of the tables' device, the tables and their width."""
-    where = tables.get_device()
-    if where < 0 or not tables.is_cuda:
-        raise RuntimeError(f"{what}: tables on {tables.device}; the tables live on a CUDA device")
-    if tables.dim() != 2 or tables.dtype is not _I32 or not tables.is_contiguous():
-        _refuse(what, tables, "tables", ("sequences", "width"), tables.device)
-    n, width = tables.shape
-    if not _fits(lens, where, (n,)):
-        _refuse(what, lens, "lens", (n,), tables.device)
-    if free.dim() != 1 or not _fits(free, where, free.shape):
-        _refuse(what, free, "free", ("pages",), tables.device)
-    if not _fits(counts, where, (2,)):
-        _refuse(what, counts, "counts", (2,), tables.device)
-    if page not in _PAGES or width == 0 or free.shape[0] == 0 or not 0 < n <= 65535:
-        raise RuntimeError(f"{what}: pages of 16 to 1024 tokens (a power of two), 1 to 65535 tables with a page, and a cache with one "
-                           f"expected, got pages of {page}, tables {tuple(tables.shape)}, free {tuple(free.shape)}")
-    return where, n, width
-
-
 def plan(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page: int,
          rows: int) -> Plan:
     """Sequence b holds lens[b] tokens and gets new[b] (int32, 0 or more); the pages it lacks are taken from free and written into its row
     of tables.  rows: the step's rows, at least the new tokens; the ones behind the last token are padding (slot -1).  Tokens beyond a
     table's end are dropped; tokens whose page is missing get slot -1 and a table entry -1, and counts[1] goes up: both set the
     device status.  One launch."""
-    where, n, width = _common("pages.plan", tables, lens, free, counts, page)
-    if not _fits(new, where, (n,)):
-        _refuse("pages.plan", new, "new", (n,), tables.device)
-    if not 0 <= rows <= 1 << 30:
-        raise RuntimeError(f"pages.plan: {rows} rows")
-    device = tables.device
-    slots = torch.empty(rows, dtype=torch.int64, device=device)
-    out = Plan(slots, torch.empty_like(slots), torch.empty(n + 1, dtype=_I32, device=device), torch.empty_like(lens), torch.empty_like(counts))
-    with _lib.on_device(device):
-        st = _lib.load().qmv_page_plan(lens.data_ptr(), new.data_ptr(), tables.data_ptr(), n, width, page, free.data_ptr(), free.shape[0],
-                                       counts.data_ptr(), rows, slots.data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
-                                       out[4].data_ptr(), _lib.stream_of(device))
-    if st:
-        _lib.check(st, "qmv_page_plan")
-    return out
+    return Plan._make(_lib.host().plan(lens, tables, free, counts, page, new, rows))
 
 
 def release(done: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page: int):
     """The pages of the sequences with done (bool) go back to free; -> lens, 0 for them, and counts.  Their pages must be their own (a
     request's beams share some: `reorder` with parents -1 frees those).  One launch."""
-    where, n, width = _common("pages.release", tables, lens, free, counts, page)
-    if not _fits(done, where, (n,), torch.bool):
-        _refuse("pages.release", done, "done", (n,), tables.device, torch.bool)
-    device = tables.device
-    lens_out, counts_out = torch.empty_like(lens), torch.empty_like(counts)
-    with _lib.on_device(device):
-        st = _lib.load().qmv_page_release(done.data_ptr(), lens.data_ptr(), tables.data_ptr(), n, width, page, free.data_ptr(),
-                                          free.shape[0], counts.data_ptr(), lens_out.data_ptr(), counts_out.data_ptr(),
-                                          _lib.stream_of(device))
-    if st:
-        _lib.check(st, "qmv_page_release")
-    return lens_out, counts_out
+    return _lib.host().release(lens, tables, free, counts, page, done)
 
 
 def reorder(parents: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page: int,
@@ -131,23 +72,4 @@ def reorder(parents: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, fre
     first keeps it, the others get a copy: `KVCache.copy(src, dst, used)` makes it, once a layer and before the next write.
     own int32 (requests,): leading places of the tables whose pages belong to others too (a shared prefix), which are neither freed nor
     written to.  Two launches."""
-    where, n, width = _common("pages.reorder", tables, lens, free, counts, page)
-    if parents.dim() != 2 or not _fits(parents, where, parents.shape):
-        _refuse("pages.reorder", parents, "parents", ("requests", "beams"), tables.device)
-    n_req, beams = parents.shape
-    if not 0 < beams <= MOST_BEAMS or n_req * beams != n:
-        raise RuntimeError(f"pages.reorder: parents {tuple(parents.shape)} for {n} tables, up to {MOST_BEAMS} beams")
-    if own is not None and not _fits(own, where, (n_req,)):
-        _refuse("pages.reorder", own, "own", (n_req,), tables.device)
-    device, lib = tables.device, _lib.load()
-    out = Reordered(torch.empty_like(tables), torch.empty_like(lens), torch.empty_like(counts), torch.empty_like(lens), torch.empty_like(lens),
-                    torch.empty_like(lens))
-    nbytes = lib.qmv_page_reorder_workspace_bytes(n_req, beams, width)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    with _lib.on_device(device):
-        st = lib.qmv_page_reorder(parents.data_ptr(), lens.data_ptr(), tables.data_ptr(), _lib.addr(own), n_req, beams, width, page,
-                                  free.data_ptr(), free.shape[0], counts.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[3].data_ptr(),
-                                  out[4].data_ptr(), out[5].data_ptr(), out[2].data_ptr(), ws.data_ptr(), nbytes, _lib.stream_of(device))
-    if st:
-        _lib.check(st, "qmv_page_reorder")
-    return out
+    return Reordered._make(_lib.host().reorder(lens, tables, free, counts, page, parents, own))
