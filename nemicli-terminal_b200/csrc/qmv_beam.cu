@@ -17,6 +17,7 @@ using namespace qmv;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kResident = 4;              // CTAs an SM
 constexpr int kMostBest = 64;             // candidates kept
 constexpr int kRoom = 128;                // keys a warp holds before it sorts out: kMostBest + a value of every lane, at least
 constexpr float kMost = 3.4028234663852886e38f;
@@ -140,13 +141,13 @@ __device__ __forceinline__ float sorted_down(float x) {
 // each piece together from two), so equal rows have equal sums to the last bit and their candidates tie.
 // (x - top before the product with log2 e, not a fused x log2 e - c: logits of 1e4 would carry log2 e's own rounding into the sum.)
 template <int DT, bool SHIFTED>
-__global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamParams P) {
+__global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __grid_constant__ BeamParams P) {
     using T = typename Elem<DT>::type;
     using Pc = Piece<DT>;
-    constexpr int N = Pc::N, U = 32 / N, kSteps = 8;              // 32 values a lane and step
+    constexpr int N = Pc::N, U = 4, V = U * N, kSteps = 16;      // V values a lane and step
     __shared__ uint64_t s_keys[kWarps][kRoom];
     __shared__ float s_best[kSteps][kThreads];                    // of a lane's pieces of a step the largest value
-    __shared__ uint64_t s_list[kWarps * kRoom];
+    __shared__ uint16_t s_found[kWarps][kSteps * 32];              // lanes and steps with candidates
     __shared__ double s_sum[kWarps];
     __shared__ float s_top[kWarps], s_nth[kWarps];
     __shared__ int s_count;
@@ -203,20 +204,34 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
         if (m > -INFINITY) bound = max(bound, uint64_t(ordered(fminf(m, kMost) + 0.f)) << 32);
         bound = __shfl_sync(0xffffffffu, bound, 0);
     };
-    // the candidates of `steps` steps from piece p1 on: a lane's 32 values of a step, read again, where the largest reaches the bound
+    // The candidates of `steps` steps from piece p1 on: a lane's values of a step, read again, where the largest reaches the bound.  They
+    // are few (some 40 a CTA), so what counts is that their loads go out together.
     auto flush = [&](int p1, int steps) {
+        int found = 0;
         for (int t = 0; t < steps; ++t) {
-            const int p0 = p1 + t * (32 * U * kWarps);
-            const uint64_t key = key_of(s_best[t][tid], (p0 + lane) * N);          // no value of the lane's has a larger one
-            const bool any = p0 + lane < last;
-            uint32_t who = __ballot_sync(0xffffffffu, any && key >= bound);
-            while (who) {
-                const int l = __ffs(who) - 1, p = p0 + 32 * (lane / N) + l, place = p * N + lane % N;
-                take(H, n, bound, p < last ? key_of(to_float(x[place]), place) : 0);
-                who &= who - 1;
-                who &= __ballot_sync(0xffffffffu, key >= bound);
-            }
+            const int p = p1 + t * (32 * U * kWarps) + lane;
+            // (no value of the lane's has a larger key)
+            const uint32_t who = __ballot_sync(0xffffffffu, p < last && key_of(s_best[t][tid], p * N) >= bound);
+            if (who >> lane & 1) s_found[warp][found + __popc(who & ((1u << lane) - 1))] = uint16_t(32 * t + lane);
+            found += __popc(who);
         }
+        __syncwarp();
+        constexpr int kLoads = 4;
+        for (int i = 0; i < found; i += kLoads) {
+            uint64_t key[kLoads];
+#pragma unroll
+            for (int y = 0; y < kLoads; ++y) {
+                key[y] = 0;
+                if (i + y >= found) continue;
+                const int at = s_found[warp][i + y], p0 = p1 + (at >> 5) * (32 * U * kWarps), p = p0 + 32 * (lane / N) + (at & 31), place = p * N + lane % N;
+                // (since the list was made the bound may have passed all of them)
+                if (key_of(s_best[at >> 5][32 * warp + (at & 31)], (p0 + (at & 31)) * N) < bound) continue;
+                if (lane < V && p < last) key[y] = key_of(to_float(x[place]), place);
+            }
+#pragma unroll
+            for (int y = 0; y < kLoads; ++y) take(H, n, bound, key[y]);
+        }
+        __syncwarp();
     };
     if (lane == 0) s_nth[warp] = warp >= full ? INFINITY : -INFINITY;
     __syncthreads();
@@ -225,10 +240,10 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
     for (; p0 < last; p0 += 32 * U * kWarps) {
         uint4 w[U];
         float best = -INFINITY;
+        constexpr uint32_t none = DT == QMV_OUT_F32 ? 0xFF800000u : DT == QMV_OUT_BF16 ? 0xFF80FF80u : 0xFC00FC00u;      // -inf
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int p = p0 + 32 * u + lane;
-            constexpr uint32_t none = DT == QMV_OUT_F32 ? 0xFF800000u : DT == QMV_OUT_BF16 ? 0xFF80FF80u : 0xFC00FC00u;      // -inf
             w[u] = make_uint4(none, none, none, none);
             if (p < last) w[u] = load(p);
         }
@@ -255,6 +270,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
         sum += double(all);
         seen = fmaxf(seen, best);
         s_best[step][tid] = best;
+        if (p0 == begin) tell();                                  // (a first word, for whoever looks before the end)
         if (++step == kSteps && p0 + 32 * U * kWarps < last) {    // (the last ones come behind the other warps' last word)
             __syncwarp();
             tell();
@@ -278,7 +294,9 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
     __syncthreads();
     hear();
     flush(p1, step);
-    __syncwarp();
+    __syncthreads();
+    uint64_t* s_list = reinterpret_cast<uint64_t*>(s_best);
+    static_assert(sizeof(s_best) >= sizeof(s_keys), "room for every key");
     for (int i = lane; i < H.count; i += 32)
         if (H.keys[i] >= bound) s_list[atomicAdd(&s_count, 1)] = H.keys[i];
     __syncthreads();
@@ -309,17 +327,20 @@ __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.
 
 constexpr int kJoin = 1024, kList = 1024;
 
-// A CTA a request.  First a bound from the lists, which are in order: of their q-th entries the r-th, q r >= n.  The candidates that
-// reach it are a few more than n; each finds its rank by looking at all others, four threads a candidate.
+// A CTA a request.  The lists are in order, so n candidates reach the r-th largest of their q-th entries, q r >= n: the largest of these for
+// q = 1, 2, 4 ... is a limit that a few more than n pass (compared as floats: rounding keeps the order).  Each of those finds its rank by
+// looking at all others, four threads a candidate.
 __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant__ BeamParams P) {
     __shared__ double s_off[kMostBest], s_score[kMostBest];        // of a beam: largest logit; score - log of the sum
     __shared__ Cand s_list[kList];
+    __shared__ __align__(16) float s_entry[kList];                // [level][list]
     __shared__ int s_count;
-    __shared__ Cand s_limit;
+    __shared__ uint32_t s_limit;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, lane = tid & 31, req = blockIdx.x, n = P.n, lists = P.K * P.splits, all = lists * n;
+    const int tid = threadIdx.x, lane = tid & 31, req = blockIdx.x, n = P.n, lists = P.K * P.splits, all = lists * n, per = P.splits * n;
     const uint64_t* keys = P.keys + (long long)req * all;
+    const uint64_t first = tid < all ? keys[tid] : 0;             // on its way while the sums are made
     for (int k = tid >> 5; k < P.K; k += kJoin / 32) {            // a warp a beam
         const long long r = ((long long)req * P.K + k) * P.splits;
         float m = -kMost;
@@ -335,47 +356,49 @@ __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant_
             s_score[k] = double(P.scores[(long long)req * P.K + k]) - log(max(sum, 1e-300));
         }
     }
-    if (tid == 0) s_count = 0, s_limit = Cand{0, INT64_MAX};
+    if (tid == 0) s_count = 0, s_limit = 0;
     __syncthreads();
-    auto cand = [&](int i) {
-        const uint64_t key = keys[i];
-        if (!key) return Cand{0, INT64_MAX};                      // none
-        const int k = i / (P.splits * n);
-        double s = (double(unordered(uint32_t(key >> 32))) - s_off[k]) + s_score[k];
-        if (!(s == s)) s = -INFINITY;
-        return Cand{ordered64(s + 0.0), (long long)k * P.vocab + int(~uint32_t(key))};
+    auto score = [&](int i, uint64_t key) {
+        const int k = i / per;
+        const double s = (double(unordered(uint32_t(key >> 32))) - s_off[k]) + s_score[k];
+        return s == s ? s + 0.0 : -INFINITY;
     };
-    // rank of s_list[i] among `count`, in each of the four threads 4 i .. 4 i + 3
-    auto rank_of = [&](int i, int count) {
-        int rank = 0;
-        if (i < count) {
-            const Cand c = s_list[i];
-            for (int j = lane & 3; j < count; j += 4) rank += before(s_list[j], c);
-        }
-        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-        return rank + __shfl_xor_sync(0xffffffffu, rank, 2);
-    };
-    const int q = (n + lists - 1) / lists, r = (n + q - 1) / q;
-    if (lists <= kList && all > n) {
-        for (int i = tid; i < lists; i += kJoin) s_list[i] = cand(i * n + q - 1);
-        __syncthreads();
-        for (int i0 = 0; i0 < lists; i0 += kJoin / 4) {
-            const int i = i0 + tid / 4, rank = rank_of(i, lists);
-            if (i < lists && (lane & 3) == 0 && rank == r - 1 && s_list[i].place != INT64_MAX) s_limit = s_list[i];
-        }
-        __syncthreads();
+    // ---- the limit
+    const int padded = (lists + 3) & ~3;
+    int levels = 0;
+    while (1 << levels <= n && (levels + 1) * padded <= kList) ++levels;
+    for (int i = tid; i < levels * padded; i += kJoin) s_entry[i] = -INFINITY;
+    __syncthreads();
+    for (int i = tid; i < all; i += kJoin) {
+        const int list = i / n, q = i - list * n + 1, level = 31 - __clz(q);
+        const uint64_t key = i == tid ? first : keys[i];
+        if ((q & (q - 1)) == 0 && level < levels && key) s_entry[level * padded + list] = float(score(i, key));
     }
-    const Cand limit = s_limit;
-    // where more than the list holds reach it: in turns, of which the n best are kept
-    int turn = all;
-    for (int done = 0; done < all;) {
+    __syncthreads();
+    for (int i = tid; i < levels * padded; i += kJoin) {
+        const int level = i / padded, r = (n + (1 << level) - 1) >> level;
+        const float mine = s_entry[i];
+        int more = 0, equal = 0;
+        for (int j = 0; j < padded; j += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(s_entry + level * padded + j);
+            more += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+            equal += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
+        }
+        if (more < r && r <= more + equal) atomicMax(&s_limit, ordered(mine));
+    }
+    __syncthreads();
+    const uint32_t limit = s_limit;                               // (-inf and nothing: every candidate passes)
+    // ---- the ones that reach it.  Where more than the list holds do (scores alike): in turns, of which the n best are kept
+    for (int done = 0, turn = all; done < all;) {
         const int kept = s_count;
         __syncthreads();
         for (int i = done + tid; i < min(all, done + turn); i += kJoin) {
-            const Cand c = cand(i);
-            if (c.place == INT64_MAX || before(limit, c)) continue;
+            const uint64_t key = i == tid ? first : keys[i];
+            if (!key) continue;
+            const double s = score(i, key);
+            if (ordered(float(s) + 0.f) < limit) continue;
             const int at = atomicAdd(&s_count, 1);
-            if (at < kList) s_list[at] = c;
+            if (at < kList) s_list[at] = Cand{ordered64(s), (long long)(i / per) * P.vocab + int(~uint32_t(key))};
         }
         __syncthreads();
         const int count = s_count;
@@ -386,6 +409,7 @@ __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant_
             __syncthreads();
             continue;
         }
+        done += turn;
         Cand own[4];
         int rank[4];
 #pragma unroll
@@ -393,34 +417,47 @@ __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant_
             const int i = kJoin / 4 * x + tid / 4;
             rank[x] = kList;
             if (kJoin / 4 * x >= count) continue;
-            rank[x] = rank_of(i, count);
-            if (i < count) own[x] = s_list[i];
-            else rank[x] = kList;
+            int r = 0;
+            if (i < count) {
+                own[x] = s_list[i];
+                for (int j = lane & 3; j < count; j += 4) r += before(s_list[j], own[x]);
+            }
+            r += __shfl_xor_sync(0xffffffffu, r, 1);
+            r += __shfl_xor_sync(0xffffffffu, r, 2);
+            if (i < count && (lane & 3) == 0) rank[x] = r;
+        }
+        if (done >= all) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (rank[x] < n) {
+                    const uint64_t o = own[x].score;
+                    const long long at = (long long)req * n + rank[x];
+                    P.scores_out[at] = float(__longlong_as_double(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
+                    P.parents[at] = int(own[x].place / P.vocab);
+                    P.tokens[at] = int(own[x].place % P.vocab);
+                }
+            return;
         }
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-            if ((lane & 3) == 0 && rank[x] < n) s_list[rank[x]] = own[x];
+            if (rank[x] < n) s_list[rank[x]] = own[x];
         if (tid == 0) s_count = min(count, n);
         __syncthreads();
-        done += turn;
-    }
-    for (int i = tid; i < n; i += kJoin) {
-        const Cand c = s_list[i];
-        const uint64_t o = c.score;
-        const double s = __longlong_as_double(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o);
-        const long long at = (long long)req * n + i;
-        P.scores_out[at] = float(s);
-        P.parents[at] = int(c.place / P.vocab);
-        P.tokens[at] = int(c.place % P.vocab);
     }
 }
 
-// Parts a row: four CTAs an SM over all rows, of 8192 values at least (a step of a CTA).
+// Parts a row: as many as make the fewest steps of 8192 values, with three steps' time for a CTA's start and end, over the CTAs that are
+// resident together.  (512 rows of 128256: one part, 16 steps, one round of CTAs; two parts took two rounds of 8 steps.)
 int splits_of(int n_req, int K, int vocab) {
-    const long long rows = (long long)n_req * K;
-    const long long want = (4LL * sm_count() + rows - 1) / rows;
-    return int(std::max<long long>(1, std::min<long long>(want, vocab / 8192)));
+    const long long rows = (long long)n_req * K, room = (long long)kResident * sm_count();
+    const int most = (vocab + 8191) / 8192;
+    long long best = 1, least = 0;
+    for (long long s = 1; s <= most; ++s) {
+        const long long cost = (rows * s + room - 1) / room * ((most + s - 1) / s + 3);
+        if (s == 1 || cost < least) least = cost, best = s;
+    }
+    return int(best);
 }
 bool bad_sizes(int n_req, int K, int vocab, int n) {
     return n_req <= 0 || K <= 0 || K > kMostBest || n_req > 65535 / K || vocab <= 0 || vocab > (1 << 30) || n <= 0 || n > kMostBest || n > (long long)K * vocab;

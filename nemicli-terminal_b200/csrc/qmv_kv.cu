@@ -428,14 +428,20 @@ __global__ void __launch_bounds__(128) kv_copy_kernel(const __grid_constant__ Kv
     const bool bad = from >= P.c.n_pages || to >= P.c.n_pages;
     if ((bad || used != asked) && tid == 0 && head == 0 && P.status) atomicOr(P.status, DEV_BAD_ADDRESS);
     if (bad) return;
-    auto run = [&](uint8_t* base, long long out, long long in, int bytes) {         // whole words
-        const int whole = bytes / 16;
-        for (int x = tid; x < whole; x += 128) reinterpret_cast<uint4*>(base + out)[x] = reinterpret_cast<const uint4*>(base + in)[x];
-        for (int x = whole * 4 + tid; x < bytes / 4; x += 128) reinterpret_cast<uint32_t*>(base + out)[x] = reinterpret_cast<const uint32_t*>(base + in)[x];
-    };
-    run(P.c.k, P.c.k_row(to, head, 0), P.c.k_row(from, head, 0), used * 4 * P.c.J * P.c.kb);
-    run(P.c.v, P.c.v_pair(to, head, 0), P.c.v_pair(from, head, 0), (used + 1) / 2 * 8 * P.c.J * P.c.vb);
-    run(reinterpret_cast<uint8_t*>(P.c.sc), 2 * P.c.scale_row(to, head, 0), 2 * P.c.scale_row(from, head, 0), used * 4 * P.c.J);
+    // pieces of 16 bytes of K, V and scales in one list, the last words of the scales by themselves: two pieces of a thread in flight
+    uint8_t* sc = reinterpret_cast<uint8_t*>(P.c.sc);
+    const int n_k = used * 4 * P.c.J * P.c.kb / 16, n_v = (used + 1) / 2 * 8 * P.c.J * P.c.vb / 16, words = used * P.c.J, n_s = words / 4;
+    const uint8_t* src[3] = {P.c.k + P.c.k_row(from, head, 0), P.c.v + P.c.v_pair(from, head, 0), sc + 2 * P.c.scale_row(from, head, 0)};
+    uint8_t* dst[3] = {P.c.k + P.c.k_row(to, head, 0), P.c.v + P.c.v_pair(to, head, 0), sc + 2 * P.c.scale_row(to, head, 0)};
+    if (tid < words % 4) reinterpret_cast<uint32_t*>(dst[2])[4 * n_s + tid] = reinterpret_cast<const uint32_t*>(src[2])[4 * n_s + tid];
+    const int all = n_k + n_v + n_s;
+#pragma unroll 4
+    for (int x = tid; x < all; x += 128) {
+        const int y = x < n_k ? x : x < n_k + n_v ? x - n_k : x - n_k - n_v;
+        const uint8_t* f = x < n_k ? src[0] : x < n_k + n_v ? src[1] : src[2];
+        uint8_t* t = x < n_k ? dst[0] : x < n_k + n_v ? dst[1] : dst[2];
+        reinterpret_cast<uint4*>(t)[y] = __ldcg(reinterpret_cast<const uint4*>(f) + y);
+    }
 }
 
 }  // namespace
