@@ -144,12 +144,12 @@ template <int DT, bool SHIFTED>
 __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __grid_constant__ BeamParams P) {
     using T = typename Elem<DT>::type;
     using Pc = Piece<DT>;
-    constexpr int N = Pc::N, U = 4, V = U * N, kSteps = 16;      // V values a lane and step
+    constexpr int N = Pc::N, U = DT == QMV_OUT_F32 ? 8 : 4, V = U * N, kSteps = 16;      // V values a lane and step
     __shared__ uint64_t s_keys[kWarps][kRoom];
     __shared__ float s_best[kSteps][kThreads];                    // of a lane's pieces of a step the largest value
     __shared__ uint16_t s_found[kWarps][kSteps * 32];              // lanes and steps with candidates
     __shared__ double s_sum[kWarps];
-    __shared__ float s_top[kWarps], s_nth[kWarps];
+    __shared__ float s_top[kWarps], s_seen[kWarps][32];
     __shared__ int s_count;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = P.n;
@@ -189,30 +189,42 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
         if (there) top = fmaxf(v, -kMost), sum = double(ex2((v - top) * kLog2e));
         take(H, n, bound, there ? key_of(v, i) : 0);
     }
-    // The bound of all warps: each of those with a whole first step says which value its m largest reach, m its share of n; the least of
-    // these n values reach.  A warp's m-th largest is that of its lanes' largest so far.
+    // The bound of all warps: the n-th largest of the lanes' largest so far (of 256, which n values reach); with more than 32 candidates
+    // the least of what the warps' lanes all reach.  Each warp's lie in order, the 32 largest of two such lists are the larger ones of one
+    // and the other from behind, and seven of these joins are left to each warp.
     float seen = -INFINITY;
-    const int full = max(1, min(kWarps, (last - first) / (32 * U))), nth = (n + full - 1) / full - 1;
-    auto tell = [&]() {
-        const float m = __shfl_sync(0xffffffffu, sorted_down(seen), nth & 31);
-        if (lane == 0) *static_cast<volatile float*>(&s_nth[warp]) = warp >= full ? INFINITY : nth < 32 ? m : -INFINITY;
-    };
+    auto tell = [&]() { static_cast<volatile float*>(s_seen[warp])[lane] = sorted_down(seen); };
     auto hear = [&]() {
-        float m = *static_cast<volatile float*>(&s_nth[lane & (kWarps - 1)]);
+        float m = static_cast<volatile float*>(s_seen[0])[lane];
+        if (n <= 32) {
 #pragma unroll
-        for (int o = 1; o < kWarps; o *= 2) m = fminf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int w = 1; w < kWarps; ++w) {
+                m = fmaxf(m, static_cast<volatile float*>(s_seen[w])[31 - lane]);
+#pragma unroll
+                for (int j = 16; j; j /= 2) {
+                    const float y = __shfl_xor_sync(0xffffffffu, m, j);
+                    m = lane & j ? fminf(m, y) : fmaxf(m, y);
+                }
+            }
+            m = __shfl_sync(0xffffffffu, m, n - 1);
+        } else {
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) m = fminf(m, static_cast<volatile float*>(s_seen[w])[lane]);
+            m = __shfl_sync(0xffffffffu, m, 31);
+        }
         if (m > -INFINITY) bound = max(bound, uint64_t(ordered(fminf(m, kMost) + 0.f)) << 32);
         bound = __shfl_sync(0xffffffffu, bound, 0);
     };
     // The candidates of `steps` steps from piece p1 on: a lane's values of a step, read again, where the largest reaches the bound.  They
-    // are few (some 40 a CTA), so what counts is that their loads go out together.
+    // are few (n and some a CTA), so what counts is that their loads go out together.
     auto flush = [&](int p1, int steps) {
         int found = 0;
-        for (int t = 0; t < steps; ++t) {
-            const int p = p1 + t * (32 * U * kWarps) + lane;
-            // (no value of the lane's has a larger key)
-            const uint32_t who = __ballot_sync(0xffffffffu, p < last && key_of(s_best[t][tid], p * N) >= bound);
-            if (who >> lane & 1) s_found[warp][found + __popc(who & ((1u << lane) - 1))] = uint16_t(32 * t + lane);
+        // (no value of a lane's step has a larger key than its largest in the first place; none of the lane's one than `seen` in place 0)
+        uint32_t lanes = __ballot_sync(0xffffffffu, key_of(seen, 0) >= bound);
+        for (; lanes; lanes &= lanes - 1) {
+            const int l = __ffs(lanes) - 1, p = p1 + lane * (32 * U * kWarps) + l;
+            const uint32_t who = __ballot_sync(0xffffffffu, lane < steps && p < last && key_of(s_best[lane & (kSteps - 1)][32 * warp + l], p * N) >= bound);
+            if (who >> lane & 1) s_found[warp][found + __popc(who & ((1u << lane) - 1))] = uint16_t(32 * lane + l);
             found += __popc(who);
         }
         __syncwarp();
@@ -229,11 +241,12 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
                 if (lane < V && p < last) key[y] = key_of(to_float(x[place]), place);
             }
 #pragma unroll
-            for (int y = 0; y < kLoads; ++y) take(H, n, bound, key[y]);
+            for (int y = 0; y < kLoads; ++y)
+                if (i + y < found) take(H, n, bound, key[y]);
         }
         __syncwarp();
     };
-    if (lane == 0) s_nth[warp] = warp >= full ? INFINITY : -INFINITY;
+    static_cast<volatile float*>(s_seen[warp])[lane] = -INFINITY;
     __syncthreads();
     const int begin = first + 32 * U * warp;
     int p0 = begin, p1 = begin, step = 0;

@@ -350,6 +350,122 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant
     }
 }
 
+// The same in one launch for few beams: a CTA of a warp a request, the sums over the requests behind one barrier.  Bound by dependent
+// reads: lengths and parents, the tables, the freed pages.  Calls in a graph: 4 beams of 14 pages 6.1 us (two launches 9.3), 32 requests of
+// 8 beams of 21 pages 11.0 (15.4); beyond that the two kernels' CTAs win (64 x 8 x 128 entries 45.6 and 16.2).
+constexpr int kFewReqs = 32, kFewBeams = 8, kFewEntries = 1 << 13;    // requests, beams of each, entries of all tables
+__global__ void __launch_bounds__(32 * kFewReqs) reorder_few_kernel(const __grid_constant__ ReorderParams P) {
+    __shared__ int s_freed[kFewReqs], s_wants[kFewReqs];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31, req = threadIdx.x >> 5, K = P.K, cap = P.width << P.shift, tokens = 1 << P.shift;
+    const int given = __ldg(P.counts), n_free = min(max(given, 0), P.n_pages);
+    // ---- lane j: beam j
+    const bool live = lane < K;
+    const int own = P.own ? max(__ldg(P.own + req), 0) : 0;
+    const int len = live ? __ldg(P.lens + req * K + lane) : 0, held = min(max(len, 0), cap), pages = (held + tokens - 1) >> P.shift;
+    int parent = live ? __ldg(P.parents + req * K + lane) : -1;
+    if (held != len || parent < -1 || parent >= K) report(P.status);
+    if (parent >= K) parent = -1;
+    const uint32_t chosen = __reduce_or_sync(0xffffffffu, parent >= 0 ? 1u << parent : 0u);
+    const int from = __shfl_sync(0xffffffffu, held, max(parent, 0)), mine = parent >= 0 ? from : 0;
+    const int* table = P.tables + (long long)req * K * P.width;
+    const int end = mine & (tokens - 1) ? __ldg(table + (long long)parent * P.width + (mine >> P.shift)) : -1;
+    bool copy = end >= 0 && (mine >> P.shift) < own;
+#pragma unroll
+    for (int o = 0; o < kFewBeams - 1; ++o) {
+        const int other = __shfl_sync(0xffffffffu, end, o);       // (by all lanes)
+        copy |= lane > o && end >= 0 && other == end;
+    }
+    const uint32_t copies = __ballot_sync(0xffffffffu, copy);
+    const int asked = copy ? __popc(copies & ((1u << lane) - 1)) : -1, wants = __popc(copies);
+    int n[kFewBeams];                                             // pages of the old beams
+#pragma unroll
+    for (int k = 0; k < kFewBeams; ++k) n[k] = __shfl_sync(0xffffffffu, pages, k);       // (0 from K on)
+    // ---- pages that no beam holds any more, a place a lane
+    const int most = __reduce_max_sync(0xffffffffu, pages);
+    int* list = P.freed + (long long)req * K * P.width;
+    int freed = 0;
+    for (int i0 = own; i0 < most; i0 += 32) {
+        const int i = i0 + lane;
+        int at[kFewBeams];
+#pragma unroll
+        for (int k = 0; k < kFewBeams; ++k) at[k] = i < n[k] ? __ldg(table + (long long)k * P.width + i) : -1;
+        uint32_t gone = 0;
+#pragma unroll
+        for (int k = 0; k < kFewBeams; ++k) {
+            bool kept = at[k] < 0 || at[k] >= P.n_pages || (chosen >> k & 1);
+#pragma unroll
+            for (int o = 0; o < kFewBeams; ++o)
+                if (o != k) kept |= (o < k || (chosen >> o & 1)) && at[o] == at[k];
+            gone |= (kept ? 0u : 1u) << k;
+        }
+        int inc = __popc(gone);
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        int to = freed + inc - __popc(gone);
+#pragma unroll
+        for (int k = 0; k < kFewBeams; ++k)
+            if (gone >> k & 1) list[to++] = at[k];
+        freed += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) s_freed[req] = freed, s_wants[req] = wants;
+    __syncthreads();
+    // ---- what the requests leave and lack, a request a lane, summed up
+    const int spare = lane < P.n_req ? s_freed[lane] - s_wants[lane] : 0;
+    int left = max(spare, 0), lack = max(-spare, 0);
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, left, o), y = __shfl_up_sync(0xffffffffu, lack, o);
+        if (lane >= o) left += x, lack += y;
+    }
+    const int all_left = __shfl_sync(0xffffffffu, left, 31), all_lack = __shfl_sync(0xffffffffu, lack, 31);
+    const int left_before = __shfl_sync(0xffffffffu, left, req) - max(freed - wants, 0), lack_before = __shfl_sync(0xffffffffu, lack, req) - max(wants - freed, 0);
+    const int size = n_free + all_left;
+    for (int f = wants + lane; f < freed; f += 32) {
+        const int at = n_free + left_before + f - wants;
+        if (at < P.n_pages) P.free[at] = list[f];
+        else report(P.status);
+    }
+    // ---- lane j: where beam j's copy goes
+    const int s = size - 1 - (lack_before + asked - freed);
+    int other = 0, before = 0;                                    // the request whose left page that is, and those before it
+#pragma unroll
+    for (int r = 0; r < kFewReqs; ++r) {
+        const int up_to = __shfl_sync(0xffffffffu, left, r);
+        if (up_to <= s - n_free) other = r + 1, before = up_to;
+    }
+    int target = -1;
+    if (asked >= 0) {
+        if (asked < freed) target = list[asked];
+        else if (s >= n_free) target = P.freed[(long long)other * K * P.width + s_wants[other] + s - n_free - before];
+        else if (s >= 0) target = __ldg(P.free + s);
+        if (target < 0 || target >= P.n_pages) target = -1, report(P.status);
+    }
+    if (live) {
+        const int beam = req * K + lane;
+        P.lens_out[beam] = mine;
+        P.src[beam] = asked >= 0 ? end : -1;
+        P.dst[beam] = target;
+        P.used[beam] = asked >= 0 ? mine & (tokens - 1) : 0;
+    }
+    for (int j = 0; j < K; ++j) {
+        const int have = (__shfl_sync(0xffffffffu, mine, j) + tokens - 1) >> P.shift, to = __shfl_sync(0xffffffffu, target, j);
+        const int copied = __shfl_sync(0xffffffffu, asked, j), old = __shfl_sync(0xffffffffu, parent, j);
+        const int* row = table + (long long)max(old, 0) * P.width;
+        int* out = P.tables_out + (long long)(req * K + j) * P.width;
+        for (int i = lane; i < P.width; i += 32) out[i] = i >= have ? -1 : copied >= 0 && i == have - 1 ? to : __ldg(row + i);
+    }
+    if (threadIdx.x == 0) {
+        if (given != n_free) report(P.status);
+        P.counts_out[0] = min(max(size - all_lack, 0), P.n_pages);
+        P.counts_out[1] = P.counts[1] + max(all_lack - size, 0);
+    }
+}
+
 // log2 of the tokens a page, or -1
 int page_shift(int page) {
     for (int s = 4; s <= 10; ++s)
@@ -434,6 +550,8 @@ int qmv_page_reorder(const int* parents, const int* lens, const int* tables, con
     P.freed = P.numbers + 2LL * n_req;
     P.status = device_status_ptr();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (beams <= kFewBeams && n_req <= kFewReqs && (long long)n_req * beams * table_width <= kFewEntries)
+        return launch_pdl(reorder_few_kernel, dim3(1), dim3(32 * n_req), s, P);
     if (const int e = launch_pdl(reorder_free_kernel, dim3(n_req), dim3(kThreads), s, P)) return e;
     return launch_behind(reorder_kernel, dim3(n_req), dim3(kThreads), s, P);
 }

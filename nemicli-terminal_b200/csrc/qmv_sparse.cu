@@ -74,12 +74,11 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const void* p) {
     }
 }
 
-// A warp a page and key head; a lane takes run t of C blocks (16 or 32 bytes of codes, C scales) of every 8th token (4th for 8 blocks), two
-// tokens at a time.  Bound by latency: at 4 bytes a load the 64 tokens of a page were eight dependent rounds of loads, 13.4 us for
+// A warp a page and key head; a lane takes run t of C blocks (8 to 24 bytes of codes, C scales) of every kTok-th token, two tokens at a time.  Bound by latency: at 4 bytes a load the 64 tokens of a page were eight dependent rounds of loads, 13.4 us for
 // 500 pages of 8 heads.
 template <int J, int KB>
 __global__ void __launch_bounds__(kThreads) box_kernel(const __grid_constant__ BoxParams P) {
-    constexpr int C = J < 4 ? J : 4, kLanes = 4 * J / C, kTok = 32 / kLanes, D = 32 * J, W = C * KB / 4, S = (C + 1) / 2;
+    constexpr int C = J == 3 ? 3 : 2, kLanes = 4 * J / C, kTok = 32 / kLanes, D = 32 * J, W = C * KB / 4, S = (C + 1) / 2;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31;
