@@ -466,7 +466,7 @@ int splits_of(int n_req, int K, int vocab) {
     const long long rows = (long long)n_req * K, room = (long long)kResident * sm_count();
     const int most = (vocab + 8191) / 8192;
     long long best = 1, least = 0;
-    for (long long s = 1; s <= most; ++s) {
+    for (long long s = 1; s <= std::min(most, 1024); ++s) {
         const long long cost = (rows * s + room - 1) / room * ((most + s - 1) / s + 3);
         if (s == 1 || cost < least) least = cost, best = s;
     }
