@@ -356,19 +356,20 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant
     }
 }
 
-// The same in one launch for few beams: a CTA of a warp a request, the sums over the requests behind one barrier.  Bound by dependent
-// reads: lengths and parents, the tables, the freed pages.  Calls in a graph: 4 beams of 14 pages 6.1 us (two launches 9.3), 32 requests of
-// 8 beams of 21 pages 11.0 (15.4); beyond that the two kernels' CTAs win (64 x 8 x 128 entries 45.6 and 16.2).
+// The same in one launch for few beams: a warp a request, in a cluster of up to eight CTAs (one SM alone was bound by its own instructions:
+// 1400 a warp, 9.2 us for 32 requests), the sums over the requests behind the cluster's barrier.  Bound by dependent reads: lengths and
+// parents, the tables, the freed pages.  Calls in a graph: 4 beams of 14 pages 4.8 us (two launches 9.3), 32 requests of
+// 8 beams of 21 pages 6.1 (15.4); with more entries a warp walks its request alone (8 x 8 x 130: 15.0, two launches 14.0).
 constexpr int kFewReqs = 32, kFewBeams = 8, kFewEntries = 1 << 13;    // requests, beams of each, entries of all tables
-__global__ void __launch_bounds__(32 * kFewReqs) reorder_few_kernel(const __grid_constant__ ReorderParams P) {
-    __shared__ int s_freed[kFewReqs], s_wants[kFewReqs];
+__global__ void __launch_bounds__(32 * kFewReqs / 8) reorder_few_kernel(const __grid_constant__ ReorderParams P) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31, req = threadIdx.x >> 5, K = P.K, cap = P.width << P.shift, tokens = 1 << P.shift;
+    const int lane = threadIdx.x & 31, req = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), K = P.K, cap = P.width << P.shift, tokens = 1 << P.shift;
+    const bool here = req < P.n_req;                              // (warps behind the last request only meet the barrier)
     const int given = __ldg(P.counts), n_free = min(max(given, 0), P.n_pages);
     // ---- lane j: beam j
-    const bool live = lane < K;
-    const int own = P.own ? max(__ldg(P.own + req), 0) : 0;
+    const bool live = here && lane < K;
+    const int own = here && P.own ? max(__ldg(P.own + req), 0) : 0;
     const int len = live ? __ldg(P.lens + req * K + lane) : 0, held = min(max(len, 0), cap), pages = (held + tokens - 1) >> P.shift;
     int parent = live ? __ldg(P.parents + req * K + lane) : -1;
     if (held != len || parent < -1 || parent >= K) report(P.status);
@@ -418,10 +419,14 @@ __global__ void __launch_bounds__(32 * kFewReqs) reorder_few_kernel(const __grid
             if (gone >> k & 1) list[to++] = at[k];
         freed += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (lane == 0) s_freed[req] = freed, s_wants[req] = wants;
-    __syncthreads();
+    if (here && lane == 0) P.numbers[2 * req] = freed, P.numbers[2 * req + 1] = wants;
+    // every CTA's numbers and lists are written before any is read
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (!here) return;
     // ---- what the requests leave and lack, a request a lane, summed up
-    const int spare = lane < P.n_req ? s_freed[lane] - s_wants[lane] : 0;
+    const int2 its = lane < P.n_req ? __ldcg(reinterpret_cast<const int2*>(P.numbers) + lane) : make_int2(0, 0);
+    const int spare = its.x - its.y;
     int left = max(spare, 0), lack = max(-spare, 0);
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -438,16 +443,17 @@ __global__ void __launch_bounds__(32 * kFewReqs) reorder_few_kernel(const __grid
     }
     // ---- lane j: where beam j's copy goes
     const int s = size - 1 - (lack_before + asked - freed);
-    int other = 0, before = 0;                                    // the request whose left page that is, and those before it
-#pragma unroll
-    for (int r = 0; r < kFewReqs; ++r) {
-        const int up_to = __shfl_sync(0xffffffffu, left, r);
-        if (up_to <= s - n_free) other = r + 1, before = up_to;
-    }
+    int other = 0, before = 0, its_wants = 0;                     // the request whose left page that is, those before it, its copies
+    if (__any_sync(0xffffffffu, asked >= freed && s >= n_free))
+        for (int r = 0; r < P.n_req; ++r) {
+            const int up_to = __shfl_sync(0xffffffffu, left, r), w = __shfl_sync(0xffffffffu, its.y, r);
+            if (up_to <= s - n_free) other = r + 1, before = up_to;
+            else if (other == r) its_wants = w;
+        }
     int target = -1;
     if (asked >= 0) {
         if (asked < freed) target = list[asked];
-        else if (s >= n_free) target = P.freed[(long long)other * K * P.width + s_wants[other] + s - n_free - before];
+        else if (s >= n_free) target = __ldcg(P.freed + (long long)other * K * P.width + its_wants + s - n_free - before);
         else if (s >= 0) target = __ldg(P.free + s);
         if (target < 0 || target >= P.n_pages) target = -1, report(P.status);
     }
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(32 * kFewReqs) reorder_few_kernel(const __grid
         int* out = P.tables_out + (long long)(req * K + j) * P.width;
         for (int i = lane; i < P.width; i += 32) out[i] = i >= have ? -1 : copied >= 0 && i == have - 1 ? to : __ldg(row + i);
     }
-    if (threadIdx.x == 0) {
+    if (req == 0 && lane == 0) {
         if (given != n_free) report(P.status);
         P.counts_out[0] = min(max(size - all_lack, 0), P.n_pages);
         P.counts_out[1] = P.counts[1] + max(all_lack - size, 0);
@@ -556,8 +562,22 @@ int qmv_page_reorder(const int* parents, const int* lens, const int* tables, con
     P.freed = P.numbers + 2LL * n_req;
     P.status = device_status_ptr();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (beams <= kFewBeams && n_req <= kFewReqs && (long long)n_req * beams * table_width <= kFewEntries)
-        return launch_pdl(reorder_few_kernel, dim3(1), dim3(32 * n_req), s, P);
+    if (beams <= kFewBeams && n_req <= kFewReqs && (long long)n_req * beams * table_width <= kFewEntries) {
+        const int ctas = std::min(n_req, 8);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ctas);
+        cfg.blockDim = dim3(32 * ((n_req + ctas - 1) / ctas));
+        cfg.stream = s;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        cudaLaunchKernelEx(&cfg, reorder_few_kernel, P);
+        return launched();
+    }
     if (const int e = launch_pdl(reorder_free_kernel, dim3(n_req), dim3(kFreers), s, P)) return e;
     return launch_behind(reorder_kernel, dim3(n_req), dim3(kThreads), s, P);
 }
