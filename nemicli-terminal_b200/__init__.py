@@ -8,9 +8,12 @@ Module map (reference counterparts in ggufengine/):
     qlinear   -> qlinear.py       QuantLinear, build_quant_linear, quantizable
     layers    -> models/common.py PackedLinear, PackedExperts
     moe       -> models/moe.py    MoE FFN, router (models/baukasten.py:_auswahl)
-    kvcache   -> (new)            key / value cache held in 4 or 8 bits, attention over it
+    kvcache   -> (new)            key / value cache held in 4 or 8 bits, attention over it, over chosen pages too
+    pages     -> (new)            its page tables and slots, built on the GPU; the tables of beams
+    beams     -> (new)            beam search's choice over the beams and the vocabulary
     shard     -> (new)            row-sharded projections and expert-sharded MoE over NCCL
-The CUDA kernels sit in csrc/ behind the C ABI of include/nemicli_qmv.h (libnemiqmv.so).
+The CUDA kernels sit in csrc/ behind the C ABI of include/nemicli_qmv.h (libnemiqmv.so); the small calls' host side is
+csrc/host/qmv_host.cpp (_qmv_host.so).
 """
 from .formats import FORMATS, TYPE_ID, TYPE_NAME  # noqa: F401
 

@@ -9,6 +9,7 @@
 // costs 8 of them (16 a clock and SM), so candidates must cost nothing: a lane compares the maximum of 16 or 32 values, which the
 // softmax needs anyway, with a bound that n values seen so far reach.
 #include <algorithm>
+#include <climits>
 
 #include "qmv_kv.cuh"
 
@@ -18,6 +19,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kResident = 4;              // CTAs an SM
+constexpr int kStep = 8192, kSteps = 16;  // values of a CTA's step, steps of a part
 constexpr int kMostBest = 64;             // candidates kept
 constexpr int kRoom = 128;                // keys a warp holds before it sorts out: kMostBest + a value of every lane, at least
 constexpr float kMost = 3.4028234663852886e38f;
@@ -144,7 +146,8 @@ template <int DT, bool SHIFTED>
 __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __grid_constant__ BeamParams P) {
     using T = typename Elem<DT>::type;
     using Pc = Piece<DT>;
-    constexpr int N = Pc::N, U = DT == QMV_OUT_F32 ? 8 : 4, V = U * N, kSteps = 16;      // V values a lane and step
+    constexpr int N = Pc::N, U = DT == QMV_OUT_F32 ? 8 : 4, V = U * N;                  // V values a lane and step
+    static_assert(V * kThreads == kStep, "splits_of counts in these");
     __shared__ uint64_t s_keys[kWarps][kRoom];
     __shared__ float s_best[kSteps][kThreads];                    // of a lane's pieces of a step the largest value
     __shared__ uint16_t s_found[kWarps][kSteps * 32];              // lanes and steps with candidates
@@ -193,13 +196,13 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
     // the least of what the warps' lanes all reach.  Each warp's lie in order, the 32 largest of two such lists are the larger ones of one
     // and the other from behind, and seven of these joins are left to each warp.
     float seen = -INFINITY;
-    auto tell = [&]() { static_cast<volatile float*>(s_seen[warp])[lane] = sorted_down(seen); };
+    auto tell = [&]() { s_seen[warp][lane] = sorted_down(seen); };
     auto hear = [&]() {
-        float m = static_cast<volatile float*>(s_seen[0])[lane];
+        float m = s_seen[0][lane];
         if (n <= 32) {
 #pragma unroll
             for (int w = 1; w < kWarps; ++w) {
-                m = fmaxf(m, static_cast<volatile float*>(s_seen[w])[31 - lane]);
+                m = fmaxf(m, s_seen[w][31 - lane]);
 #pragma unroll
                 for (int j = 16; j; j /= 2) {
                     const float y = __shfl_xor_sync(0xffffffffu, m, j);
@@ -209,13 +212,13 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
             m = __shfl_sync(0xffffffffu, m, n - 1);
         } else {
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) m = fminf(m, static_cast<volatile float*>(s_seen[w])[lane]);
+            for (int w = 1; w < kWarps; ++w) m = fminf(m, s_seen[w][lane]);
             m = __shfl_sync(0xffffffffu, m, 31);
         }
         if (m > -INFINITY) bound = max(bound, uint64_t(ordered(fminf(m, kMost) + 0.f)) << 32);
         bound = __shfl_sync(0xffffffffu, bound, 0);
     };
-    // The candidates of `steps` steps from piece p1 on: a lane's values of a step, read again, where the largest reaches the bound.  They
+    // The candidates of the steps from piece p1 on: a lane's values of a step, read again, where the largest reaches the bound.  They
     // are few (n and some a CTA), so what counts is that their loads go out together.
     auto flush = [&](int p1, int steps) {
         int found = 0;
@@ -246,11 +249,9 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
         }
         __syncwarp();
     };
-    static_cast<volatile float*>(s_seen[warp])[lane] = -INFINITY;
-    __syncthreads();
     const int begin = first + 32 * U * warp;
-    int p0 = begin, p1 = begin, step = 0;
-    for (; p0 < last; p0 += 32 * U * kWarps) {
+    int step = 0;                                                 // (at most kSteps: splits_of)
+    for (int p0 = begin; p0 < last; p0 += 32 * U * kWarps) {
         uint4 w[U];
         float best = -INFINITY;
         constexpr uint32_t none = DT == QMV_OUT_F32 ? 0xFF800000u : DT == QMV_OUT_BF16 ? 0xFF80FF80u : 0xFC00FC00u;      // -inf
@@ -283,14 +284,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
         sum += double(all);
         seen = fmaxf(seen, best);
         s_best[step][tid] = best;
-        if (p0 == begin) tell();                                  // (a first word, for whoever looks before the end)
-        if (++step == kSteps && p0 + 32 * U * kWarps < last) {    // (the last ones come behind the other warps' last word)
-            __syncwarp();
-            tell();
-            hear();
-            flush(p1, step);
-            step = 0, p1 = p0 + 32 * U * kWarps;
-        }
+        ++step;
     }
     // ---- the warps' together
     {
@@ -306,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
     tell();
     __syncthreads();
     hear();
-    flush(p1, step);
+    flush(begin, step);
     __syncthreads();
     uint64_t* s_list = reinterpret_cast<uint64_t*>(s_best);
     static_assert(sizeof(s_best) >= sizeof(s_keys), "room for every key");
@@ -460,15 +454,16 @@ __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant_
     }
 }
 
-// Parts a row: as many as make the fewest steps of 8192 values, with three steps' time for a CTA's start and end, over the CTAs that are
-// resident together.  (512 rows of 128256: one part, 16 steps, one round of CTAs; two parts took two rounds of 8 steps.)
+// Parts a row: as many as make the fewest steps, with three steps' time for a CTA's start and end, over the CTAs that are resident
+// together, and no part longer than kSteps.  (512 rows of 128256: one part, 16 steps, one round of CTAs: 42.4 us; two parts, two rounds of 8
+// steps 45.8, four 55.)
 int splits_of(int n_req, int K, int vocab) {
     const long long rows = (long long)n_req * K, room = (long long)kResident * sm_count();
-    const int most = (vocab + 8191) / 8192;
-    long long best = 1, least = 0;
-    for (long long s = 1; s <= std::min(most, 1024); ++s) {
-        const long long cost = (rows * s + room - 1) / room * ((most + s - 1) / s + 3);
-        if (s == 1 || cost < least) least = cost, best = s;
+    const int steps = (vocab + kStep - 1) / kStep, least = (steps + kSteps - 1) / kSteps;
+    long long best = least, cost = LLONG_MAX;
+    for (long long s = least; s <= std::min<long long>(steps, least + 1024); ++s) {
+        const long long c = (rows * s + room - 1) / room * ((steps + s - 1) / s + 3);
+        if (c < cost) cost = c, best = s;
     }
     return int(best);
 }

@@ -69,6 +69,22 @@ def test_select(cuda, dtype, reqs, k, vocab, n):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("reqs, k, vocab, dtype, n", [(74, 8, 140001, BF16, 16), (150, 4, 131072, BF16, 64), (2, 2, 400003, F32, 33)])
+def test_long_rows_and_many(cuda, reqs, k, vocab, dtype, n):
+    """Rows of more steps than a part has, with as many rows as there are CTAs at once."""
+    g = gen(vocab, cuda)
+    x = torch.empty(reqs, k, vocab, dtype=dtype, device=cuda)
+    for r in x:
+        r.copy_(torch.randn(k, vocab, generator=g, device=cuda) * 3)
+    s = -torch.rand(reqs, k, generator=g, device=cuda).cumsum(1)
+    whole = beams.select(x, s, n)
+    for r in (0, reqs - 1):                                       # a request's result does not depend on the others
+        one = check(x[r:r + 1], s[r:r + 1], n)
+        near = (one[0] - whole[0][r:r + 1]).abs() <= 1e-4
+        assert near.all()
+    check(x[reqs // 2:reqs // 2 + 8], s[reqs // 2:reqs // 2 + 8], n)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_ties_go_to_the_lowest_place(cuda, dtype):
     """Equal logits in a row; equal rows with equal scores, at every alignment a row can have."""
@@ -131,6 +147,23 @@ def test_orders_that_keep_the_bounds_low(cuda, dtype):
     last[-1] = 50
     x = torch.stack((ramp, ramp.flip(0), flat, last)).to(dtype)[None]
     check(x, torch.tensor([[0.0, -1.5, -2.25, -3.0]], device=cuda), 40)
+
+
+def test_two_streams_at_once(cuda):
+    """Calls that overlap have workspaces of their own."""
+    g = gen(12, cuda)
+    x = [torch.randn(4, 6, 40003, generator=g, device=cuda) for _ in range(2)]
+    s = [torch.zeros(4, 6, device=cuda) for _ in range(2)]
+    want = [beams.select(a, b, 12) for a, b in zip(x, s)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(beams.select(x[i], s[i], 12))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for i in range(2) for o in got[i] for p, q in zip(o, want[i]))
 
 
 def test_strides_and_streams(cuda):

@@ -171,7 +171,7 @@ def test_choose_and_attend(cuda, dtype, dim, heads, n_kv, page, kf, vf):
     starts = torch.tensor(np.cumsum([0] + lens), dtype=torch.int32, device=cuda)
     c.summarise(b, t, n, starts)
     q = (torch.randn(len(lens) + 2, heads, dim, generator=gen(3, cuda), device=cuda) * 0.7).to(dtype)
-    for keep, first, last in ((1, 0, 1), (5, 1, 2), (8, 0, 1), (39, 2, 3), (64, 1, 1)):
+    for keep, first, last in ((1, 0, 1), (3, 1, 2), (5, 1, 2), (8, 0, 1), (39, 2, 3), (64, 1, 1)):
         check(c, q, b, t, n, keep, first, last)
     assert _lib.device_status(device=cuda) == 0
 

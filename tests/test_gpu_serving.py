@@ -3,7 +3,7 @@ and the beams' tables run together as a decoder would use them, against one sequ
 import pytest
 import torch
 
-from nemicli_terminal_b200 import _lib, beams, kvcache, pages
+from nemicli_terminal_b200 import _lib, beams, kvcache, mmvq, pages
 
 from tests.test_gpu_kvcache import gen
 
@@ -16,7 +16,15 @@ def rope_tables(dim, n, cuda):
     return a.cos().float().to(cuda), a.sin().float().to(cuda)
 
 
-def test_steps_of_a_batch(cuda):
+@pytest.fixture(params=[False, True], ids=["plain", "pdl"])
+def launches(request):
+    """The library's programmatic dependent launches off and on."""
+    mmvq.pdl(request.param)
+    yield
+    mmvq.pdl(False)
+
+
+def test_steps_of_a_batch(cuda, launches):
     """Requests of unequal prompts, then a token each; some end and others take their pages.  What each sequence's table holds is what
     it was given, in order; attention over all its pages equals attention over the chosen ones where these are all."""
     dim, n_kv, heads, page, seqs, width = 64, 2, 6, 16, 6, 8
@@ -73,7 +81,7 @@ def test_steps_of_a_batch(cuda):
 
 
 @pytest.mark.parametrize("page, prompt", [(16, 20), (16, 32), (32, 5)])
-def test_beam_search(cuda, page, prompt):
+def test_beam_search(cuda, launches, page, prompt):
     """A toy model: a token's key and value are its embedding, logits the attention's output times the embeddings.  Beam search with paged
     tables keeps for every beam what a search that copies whole caches keeps, step by step."""
     dim, n_kv, reqs, k, vocab, width, steps = 64, 1, 3, 4, 97, 8, 14
