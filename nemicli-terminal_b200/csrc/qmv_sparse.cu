@@ -74,15 +74,17 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const void* p) {
     }
 }
 
-// A warp a page and key head; a lane takes run t of C blocks (8 to 24 bytes of codes, C scales) of every kTok-th token, two tokens at a time.  Bound by latency: at 4 bytes a load the 64 tokens of a page were eight dependent rounds of loads, 13.4 us for
-// 500 pages of 8 heads.
+// A warp a page and key head; a lane takes run t of C blocks (8 to 24 bytes of codes, C scales) of every kTok-th token, two tokens at a time.
+// 500 pages of 64 keys, 8 heads of 128 in Q4_0 (18.5 MB): 10.6 us.  Bound by latency (lengths, table, two rounds of loads) and by the minima
+// and maxima (ALU 44 %).  4 bytes a load, eight dependent rounds: 13.4; 16 bytes, whose registers leave half the warps: 13.0; CTAs of 256: 11.7.
+constexpr int kBoxers = 128;
 template <int J, int KB>
-__global__ void __launch_bounds__(kThreads) box_kernel(const __grid_constant__ BoxParams P) {
+__global__ void __launch_bounds__(kBoxers) box_kernel(const __grid_constant__ BoxParams P) {
     constexpr int C = J == 3 ? 3 : 2, kLanes = 4 * J / C, kTok = 32 / kLanes, D = 32 * J, W = C * KB / 4, S = (C + 1) / 2;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31;
-    const long long id = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const long long id = (long long)blockIdx.x * (kBoxers / 32) + (threadIdx.x >> 5);
     const long long item = id / P.c.n_kv;
     const int head = int(id - item * P.c.n_kv), seq = int(item / P.most), nth = int(item - (long long)seq * P.most);
     if (seq >= P.n_seq) return;                                   // whole warps
@@ -214,7 +216,8 @@ constexpr int kTiles = 2, kPagesWarp = 16 * kTiles;              // pages a warp
 template <int DT, int J>
 __global__ void __launch_bounds__(kScorers) score_kernel(const __grid_constant__ ChooseParams P) {
     using T = typename Elem<DT>::type;
-    constexpr int D = 32 * J, kParts = DT == QMV_OUT_F32 ? 2 : 1, kPieces = 2 * J, kAhead = kPieces < 4 ? kPieces : 4;
+    constexpr int D = 32 * J, kParts = DT == QMV_OUT_F32 ? 2 : 1, kPieces = 2 * J, kAhead = J == 3 ? 3 : 4;
+    static_assert(kPieces % kAhead == 0, "whole rounds of pieces");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, head = blockIdx.y, row = blockIdx.z;
@@ -590,12 +593,12 @@ int qmv_kv_bounds(const qmv_kv_cache* cache, const int* tables, int table_width,
     P.width = table_width, P.n_seq = n_seq;
     P.most = int(std::min<long long>(table_width, ((long long)max_new + P.c.page() - 1) >> P.c.page_shift));
     P.status = device_status_ptr();
-    const long long ctas = ((long long)n_seq * P.most * P.c.n_kv + kThreads / 32 - 1) / (kThreads / 32);
+    const long long ctas = ((long long)n_seq * P.most * P.c.n_kv + kBoxers / 32 - 1) / (kBoxers / 32);
     if (ctas > 0x7FFFFFFFLL) return ST_BAD_TOKENS;
     auto go = [&](auto j) {
         constexpr int J = decltype(j)::value;
-        return P.c.kb == 4 ? launch_pdl(box_kernel<J, 4>, dim3(unsigned(ctas)), dim3(kThreads), static_cast<cudaStream_t>(stream), P)
-                           : launch_pdl(box_kernel<J, 8>, dim3(unsigned(ctas)), dim3(kThreads), static_cast<cudaStream_t>(stream), P);
+        return P.c.kb == 4 ? launch_pdl(box_kernel<J, 4>, dim3(unsigned(ctas)), dim3(kBoxers), static_cast<cudaStream_t>(stream), P)
+                           : launch_pdl(box_kernel<J, 8>, dim3(unsigned(ctas)), dim3(kBoxers), static_cast<cudaStream_t>(stream), P);
     };
     switch (P.c.J) {
     case 2: return go(std::integral_constant<int, 2>{});
