@@ -435,8 +435,8 @@ int64_t qmv_page_reorder_workspace_bytes(int n_req, int beams, int table_width);
  * where the page is not the request's): src, dst, used [n_req][beams] name the page to copy, the new one and its tokens
  * (-1, -1, 0: none), for qmv_kv_copy of each layer.  New pages are the request's own freed ones, in order, then the stack's, onto which all the
  * other freed ones went before; -1 where none is left (counts_out[1] counts them).  tables_out, lens_out: as tables and lens, -1 behind a beam's pages.  Parents
- * outside the request count as -1 and set QMV_DEV_BAD_ADDRESS.  At most 64 beams and 65535 in all.  workspace: 256-byte aligned.  Two launches.
- * Replaces: nothing. */
+ * outside the request count as -1 and set QMV_DEV_BAD_ADDRESS.  At most 64 beams, 65535 in all, and 2^26 entries of a request's tables.  workspace: 256-byte aligned.  One or two
+ * launches.  Replaces: nothing. */
 int qmv_page_reorder(const int* parents, const int* lens, const int* tables, const int* own, int n_req, int beams, int table_width,
                      int page, int* free_pages, int n_pages, const int* counts, int* tables_out, int* lens_out, int* src,
                      int* dst, int* used, int* counts_out, void* workspace, long long workspace_bytes, void* stream);

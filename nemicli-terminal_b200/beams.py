@@ -12,7 +12,7 @@ from . import _lib
 def select(logits: torch.Tensor, scores: torch.Tensor, n: int = 0):
     """The n best continuations of each request.  logits: (requests, beams, vocab) of float32, bfloat16 or float16, the values of a row
     side by side; scores: float32 (requests, beams), the beams' log probabilities so far (-inf: no such beam).  n: default the
-    beams; twice as many leave room for beams that end.  -> scores float32, parents int32, tokens int32, each (requests, n), best
-    first (up to 64, as the beams): scores[r, parents] + log_softmax(logits[r, parents])[tokens], the lowest (beam, token) first among equals.  NaN counts as
-    -inf, +inf as the largest float.  Two launches."""
+    beams; twice as many leave room for beams that end; up to 64 of each.  -> scores float32, parents int32, tokens int32, each
+    (requests, n), best first: scores[r, parents] + log_softmax(logits[r, parents])[tokens], the lowest (beam, token) first among
+    equals.  NaN counts as -inf, +inf as the largest float.  Two launches."""
     return _lib.host().select(logits, scores, n)

@@ -212,7 +212,8 @@ constexpr int kTiles = 2, kPagesWarp = 16 * kTiles;              // pages a warp
 // lie; the queries are laid out to match.  Queries are fp16 after a power of two a head, fp32 ones two fp16 parts.  So a score is near:
 // off by less than 2^-15 sum_c |q_c| max |box|: 2^-20 of it for the queries' parts, and in each of four chains at most 16 steps of 17
 // terms cut off at 2^-24 of the chain's share of that sum.  The choice computes those that lie nearer to its border again, in fp64.
-// (All in fp64 on the CUDA cores: 27 to 46 us for 64 sequences of 154 pages on average, 184 instructions a page and key head.)
+// 64 sequences of 154 pages on average, 8 key heads (40 MB of boxes): 9.8 us, bound by latency (lengths, table, boxes: dependent reads; DRAM
+// 31 %); 47 instructions a page and key head.  (All in fp64 on the CUDA cores: 27 to 46 us, 184 instructions.)
 template <int DT, int J>
 __global__ void __launch_bounds__(kScorers) score_kernel(const __grid_constant__ ChooseParams P) {
     using T = typename Elem<DT>::type;
@@ -400,8 +401,8 @@ __device__ __forceinline__ void find_bin(const int* s_hist, int per, int need, i
 // A CTA a row and key head.  A histogram of the near scores in even bins between the least and the largest tells the bin of the k-th
 // largest.  Pages whose score lies above that bin by twice the error are taken, those below it by as much are not; the few others are
 // computed again in fp64, a warp each, and ranked against one another (more than a list holds, scores alike say: by digits of
-// 8 bits).  Then the pages in order.  Bound by latency and by fetching its own instructions (unrolled over scores in registers it took 16 us
-// for 2048 pages), so its loops are rolled, over scores in shared memory.
+// 8 bits).  Then the pages in order.  2048 pages of 8 key heads: 9.3 us, 11 barriers, each phase 1 to 1.8 us; bound by latency and by fetching its
+// own instructions (unrolled over scores in registers 16 us), so its loops are rolled, over scores in shared memory.
 template <int DT>
 __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant__ ChooseParams P) {
     using T = typename Elem<DT>::type;

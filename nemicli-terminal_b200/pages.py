@@ -71,5 +71,5 @@ def reorder(parents: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, fre
     place of their tables.  Pages that no beam holds any more become free.  Of the beams that would write to one partly filled page the
     first keeps it, the others get a copy: `KVCache.copy(src, dst, used)` makes it, once a layer and before the next write.
     own int32 (requests,): leading places of the tables whose pages belong to others too (a shared prefix), which are neither freed nor
-    written to.  Two launches."""
+    written to.  One launch for up to 32 requests of 8 beams with short tables, else two."""
     return Reordered._make(_lib.host().reorder(lens, tables, free, counts, page, parents, own))
