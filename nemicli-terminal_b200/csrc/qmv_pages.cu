@@ -80,9 +80,15 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
     const long long mine = (long long)blockIdx.x * kThreads + tid, all = (long long)gridDim.x * kThreads;
     const int given = __ldg(P.counts), n_free = min(max(given, 0), P.n_pages);
     if (mine == 0 && given != n_free) report(P.status);
+    // Where pages were asked for in vain, tables may hold entries of -1, which are no pages to give back: then the entries are
+    // counted, a warp a sequence, by every CTA (else only lengths are read).
+    const bool holes = RELEASE && __ldg(P.counts + 1) != 0;
+    const int lane = tid & 31, warp = tid >> 5;
+    auto entry = [&](int b, int i, int had) { return i < had ? __ldg(P.tables + (long long)b * P.width + i) : -1; };
     long long row0 = 0, page0 = 0;                                // rows and pages of the sequences before this chunk
     for (int b0 = 0, turn = 0; b0 < P.n_seq; b0 += kChunk, ++turn) {
         int held[kPer], take[kPer], need[kPer];
+        const int here = min(kChunk, P.n_seq - b0);
         long long rows = 0, pages = 0;
         const bool writes = turn % gridDim.x == blockIdx.x;       // this CTA writes the chunk's lengths
 #pragma unroll
@@ -107,6 +113,22 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
             if (writes && odd) report(P.status);
             rows += take[i], pages += need[i];
         }
+        if (holes) {
+            for (int at = warp; at < here; at += kThreads / 32) {
+                const int had = P.done[b0 + at] ? (min(max(__ldg(P.lens + b0 + at), 0), cap) + (1 << P.shift) - 1) >> P.shift : 0;
+                int n = 0;
+                for (int i = lane; i < had; i += 32) {
+                    const int page = entry(b0 + at, i, had);
+                    n += page >= 0 && page < P.n_pages;
+                }
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (lane == 0) s_had[at] = n;
+            }
+            __syncthreads();
+            pages = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) pages += need[i] = b0 + tid * kPer + i < P.n_seq ? s_had[tid * kPer + i] : 0;
+        }
         long long n_rows = 0, n_need;
         long long r = RELEASE ? 0 : row0 + block_sums(rows, s_warp, n_rows), p = page0 + block_sums(pages, s_warp, n_need);
 #pragma unroll
@@ -117,9 +139,23 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
             r += take[i], p += need[i];
         }
         __syncthreads();
-        const int here = min(kChunk, P.n_seq - b0);
+        if (holes) {
+            for (long long at = blockIdx.x * (kThreads / 32) + warp; at < here; at += all / 32) {
+                const int had = P.done[b0 + at] ? s_had[at] : 0;
+                long long to = n_free + s_page[at];
+                for (int i0 = 0; i0 < had; i0 += 32) {
+                    const int page = entry(b0 + at, i0 + lane, had);
+                    const bool there = page >= 0 && page < P.n_pages;
+                    const uint32_t who = __ballot_sync(0xffffffffu, there);
+                    const long long spot = to + __popc(who & ((1u << lane) - 1));
+                    if (there && spot < P.n_pages) P.free[spot] = page;
+                    if (there ? spot >= P.n_pages : page != -1) report(P.status);
+                    to += __popc(who);
+                }
+            }
+        }
         // pages that change hands: the e-th of this call
-        for (long long e = page0 + mine; e < page0 + n_need; e += all) {
+        for (long long e = page0 + mine; e < page0 + n_need && !holes; e += all) {
             const int i = last_at(s_page, here, e), in = int(e - s_page[i]);
             int* row = P.tables + (long long)(b0 + i) * P.width;
             if constexpr (RELEASE) {

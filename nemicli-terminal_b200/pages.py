@@ -60,7 +60,8 @@ def plan(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torc
 
 def release(done: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page: int):
     """The pages of the sequences with done (bool) go back to free; -> lens, 0 for them, and counts.  Their pages must be their own (a
-    request's beams share some: `reorder` with parents -1 frees those).  One launch."""
+    request's beams share some: `reorder` with parents -1 frees those).  Entries of -1, pages that were missing, are left out while counts[1]
+    is not 0 (so compare it with its last value; do not set it back).  One launch."""
     return _lib.host().release(lens, tables, free, counts, page, done)
 
 

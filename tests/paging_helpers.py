@@ -49,6 +49,8 @@ def release(done, lens, tables, free, counts, page):
         h = min(max(held, 0), width * page)
         if done[b]:
             for i in range(up(h, page)):
+                if counts[1] and not 0 <= tables[b][i] < len(free):
+                    continue
                 if n < len(free):
                     free[n] = tables[b][i]
                     n += 1

@@ -91,6 +91,41 @@ def test_release(cuda, seqs, page, most):
             assert [g.tolist() for g in got] == [want[0], want[1]] and f.tolist() == want[2]
 
 
+@pytest.mark.parametrize("seqs, page, most", [(1, 16, 50), (64, 64, 900), (1500, 16, 90)])
+def test_release_after_pages_were_missing(cuda, seqs, page, most):
+    """Entries of -1 are no pages; without any missing page the entries are not read one by one."""
+    r = random.Random(seqs + 1)
+    lens, tables, rest, total = some_tables(r, seqs, PH.up(most, page) + 1, page, most, 5)
+    free = rest + [0] * (total - len(rest))
+    holes = [[-1 if r.random() < 0.2 else e for e in t] for t in tables]
+    done = [r.random() < 0.6 for _ in range(seqs)]
+    _lib.device_status(device=cuda)
+    for t, missing in ((tables, 0), (holes, 9)):
+        want = PH.release(done, lens, t, free, [len(rest), missing], page)
+        f = ints(free, cuda)
+        got = pages.release(ints(done, cuda, torch.bool), ints(lens, cuda), ints(t, cuda), f, ints([len(rest), missing], cuda), page)
+        assert [g.tolist() for g in got] == [want[0], want[1]] and f.tolist() == want[2]
+    assert _lib.device_status(device=cuda) == 0
+
+
+def test_short_of_pages_and_on(cuda):
+    """Steps that ask for more pages than there are, sequences that end meanwhile: no page is lost and none is there twice."""
+    page, seqs, width, n_pages = 16, 6, 8, 20
+    r = random.Random(8)
+    free, counts = pages.pool(n_pages, cuda)
+    tables, lens = torch.full((seqs, width), -1, dtype=I32, device=cuda), ints([0] * seqs, cuda)
+    missing = False
+    for step in range(60):
+        p = pages.plan(lens, ints([r.randint(0, 20) if n < 90 else 0 for n in lens.tolist()], cuda), tables, free, counts, page, 200)
+        done = [r.random() < 0.2 for _ in range(seqs)]
+        missing |= p.counts[1].item() > 0
+        lens, counts = pages.release(ints(done, cuda, torch.bool), p.lens, tables, free, p.counts, page)
+        held = [e for t, n in zip(tables.tolist(), lens.tolist()) for e in t[:PH.up(n, page)] if e >= 0]
+        assert sorted(held + free[:counts[0].item()].tolist()) == list(range(n_pages)), step
+    assert missing
+    _lib.device_status(device=cuda)
+
+
 def test_release_twice_is_noticed(cuda):
     """More pages than the cache has: the rest is dropped."""
     free, counts = pages.pool(4, cuda)
