@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kScorers) score_kernel(const __grid_constant__
             const float2 w = unpack_h2(wide[y][x]);
             if (t == x && i < end) {
                 P.near[out + i] = there[y][x] ? best[y][x] : -INFINITY;
-                P.sizes[out + i] = there[y][x] ? size * fmaxf(w.x, w.y) : 0.f;
+                P.sizes[out + i] = there[y][x] ? size * larger(w.x, w.y) : 0.f;
             }
         }
 }

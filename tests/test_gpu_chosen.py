@@ -257,6 +257,22 @@ def test_scores_far_apart(cuda):
         assert len(set(got)) == 20 and set(got) <= set(t[0].tolist())
 
 
+@pytest.mark.parametrize("channel", [6, 7])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_boxes_that_are_no_numbers(cuda, channel, value):
+    """A side of a box that is NaN or infinite counts for the heads that read that side."""
+    c, t, n, b = long_cache(cuda, 300)
+    q = torch.randn(1, 4, 64, generator=gen(12, cuda), device=cuda)
+    q[0, :2, channel], q[0, 2:, channel] = 0.5, -0.5
+    q[0, 0] *= 3
+    for side in (0, 1):
+        odd = b.clone()
+        odd[t[0, 20:290:3].long(), :, side, channel] = value
+        chosen, _ = c.choose(q, odd, t, n, 120, first=1, last=2)
+        want = choice(q[0], odd, t[0], 300 * 16 - 1, 16, 120, 1, 2, 1)[0]
+        assert chosen[0, 0].tolist() == t[0, torch.tensor(want, device=cuda)].tolist()
+
+
 def test_bad_pages(cuda):
     """A page outside the cache scores least; chosen all the same it counts as masked, and the status says so."""
     c, t, n, b = long_cache(cuda, 40)
