@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kFreers) reorder_free_kernel(const __grid_cons
     int* list = P.freed + (long long)req * K * P.width;
     long long base = 0;
     auto entry = [&](int i) { return at < places && i < B.pages[k] ? __ldg(table + (long long)k * P.width + i) : -1; };
-    const int first = P.own ? max(__ldg(P.own + req), 0) : 0;
+    const int first = P.own ? min(max(__ldg(P.own + req), 0), P.width) : 0;      // (any number there: first + at stays an int)
     int next = entry(first + at);
     for (int i0 = first; i0 < most; i0 += places) {
         const int page = next;
