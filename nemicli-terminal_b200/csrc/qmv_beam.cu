@@ -3,6 +3,8 @@
 //   s[k][v] = scores[k] + x[k][v] - max_k - log sum_v exp(x[k][v] - max_k);   the n largest of a request's K V, the lowest
 //   k V + v first among equals
 //
+// A beam whose score is -inf or NaN has -inf throughout, so its part is its first places, whatever its logits.
+//
 // One pass over the logits: a beam's order is that of its logits, so each part of a row gives its n best, its largest logit and its
 // sum of exponentials, and a second launch joins the parts, with logarithm and scores in fp64 (candidates of different beams may lie
 // nearer than fp32 tells apart).  Bound by reading the logits: at the HBM's rate an SM sees 12 bf16 values a clock, and of exponentials it
@@ -162,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long row = blockIdx.x / P.splits;
     const int split = int(blockIdx.x - row * P.splits);
+    const float score = __ldg(P.scores + row);                    // looked at behind the sums: here it would hold up the logits' loads
     const T* x = static_cast<const T*>(P.x) + row * P.stride;
     const int pieces = P.vocab / N, tail = P.vocab - pieces * N;  // the values behind the last whole piece are the first part's
     const int first = int((long long)pieces * split / P.splits), last = int((long long)pieces * (split + 1) / P.splits);
@@ -287,6 +290,12 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
         seen = fmaxf(seen, best);
         s_best[step][tid] = best;
         ++step;
+    }
+    if (!(score > -INFINITY)) {                                   // all of the beam's candidates are -inf: the first places (the whole CTA)
+        uint64_t* out = P.keys + (long long)blockIdx.x * n;
+        for (int i = tid; i < n; i += kThreads) out[i] = split == 0 && i < P.vocab ? key_of(-INFINITY, i) : 0;
+        if (tid == 0) P.sums[blockIdx.x] = 1.0, P.tops[blockIdx.x] = -kMost;
+        return;
     }
     // ---- the warps' together
     {

@@ -1,0 +1,52 @@
+"""The order of beam selection's candidates whose scores are alike though their logits are not."""
+import pytest
+import torch
+
+from nemicli_terminal_b200 import beams
+
+from tests.test_gpu_beams import BF16, F16, F32, gen
+
+pytestmark = pytest.mark.gpu
+
+
+def want(logits, scores, n):
+    """Places k vocab + v of a request's n best: beams with a finite score by (score, beam, logit, place), all others and logits of -inf
+    behind them by place.  For scores so far apart that no candidate of one beam comes near another's."""
+    out = []
+    for x, s in zip(logits.double().tolist(), scores.double().tolist()):
+        vocab = len(x[0])
+        live = [k for k in range(len(s)) if s[k] > -float("inf")]
+        order = [(k, v) for k in sorted(live, key=lambda k: (-s[k], k)) for v in sorted(range(vocab), key=lambda v: (-x[k][v], v)) if x[k][v] > -float("inf")]
+        order += sorted((k, v) for k in range(len(s)) for v in range(vocab) if k not in live or x[k][v] == -float("inf"))
+        out.append([k * vocab + v for k, v in order[:n]])
+    return out
+
+
+def places(got, vocab):
+    return (got[1].long() * vocab + got[2]).tolist()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dead", [float("-inf"), float("nan")])
+@pytest.mark.parametrize("reqs, k, vocab, n", [(1, 1, 3, 3), (2, 3, 5, 15), (1, 4, 20001, 8), (3, 2, 131, 64), (40, 3, 9000, 33)])
+def test_beams_without_a_score(cuda, dtype, dead, reqs, k, vocab, n):
+    """Their candidates are all -inf: the lowest places, whatever the logits say, in every batch."""
+    x = (torch.randn(reqs, k, vocab, generator=gen(vocab, cuda), device=cuda) * 3).to(dtype)
+    x[:, -1, 1::2] = -float("inf")
+    s = torch.full((reqs, k), dead, device=cuda)
+    got = beams.select(x, s, n)                                   # all of them
+    assert places(got, vocab) == [list(range(n))] * reqs and (got[0] == -float("inf")).all()
+    s[:, -1] = -1.5                                               # the first ones, the last alive (every other token of it -inf)
+    got = beams.select(x, s, n)
+    assert places(got, vocab) == want(x, s, n)
+    finite = min(n, (vocab + 1) // 2)
+    assert torch.isfinite(got[0][:, :finite]).all() and (got[0][:, finite:] == -float("inf")).all()
+
+
+def test_few_candidates_alive(cuda):
+    """Fewer finite candidates than asked for, behind a beam without a score and before one."""
+    x = torch.randn(1, 3, 40, generator=gen(1, cuda), device=cuda)
+    x[0, 1, 5:] = -float("inf")
+    s = torch.tensor([[-float("inf"), 0.5, -float("inf")]], device=cuda)
+    got = beams.select(x, s, 60)
+    assert places(got, 40) == want(x, s, 60)
