@@ -336,12 +336,12 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_part_kernel(const __
     }
 }
 
-// Joins a request's parts: K * splits lists of n.  Candidates are numbers (score, place), ordered by score, then by the lower place.
+// Joins a request's parts: K * splits lists of n.  Candidates are ordered by score, then by the lower beam, then as in their beam's lists: by
+// the larger logit (fp64 does not tell logits apart beside a score of 1e30), then by the lower place.
 struct Cand {
-    uint64_t score;                       // ordered64
-    int64_t place;                        // k V + v
+    uint64_t score, key;                  // ordered64; key_of
+    int beam;
 };
-__device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.score > b.score || (a.score == b.score && a.place < b.place); }
 
 constexpr int kJoin = 1024, kList = 1024;
 
@@ -350,7 +350,8 @@ constexpr int kJoin = 1024, kList = 1024;
 // looking at all others, four threads a candidate.
 __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant__ BeamParams P) {
     __shared__ double s_off[kMostBest], s_score[kMostBest];        // of a beam: largest logit; score - log of the sum
-    __shared__ Cand s_list[kList];
+    __shared__ uint64_t s_cand[kList], s_key[kList];              // ordered64 of the score; key_of
+    __shared__ uint8_t s_beam[kList];
     __shared__ __align__(16) float s_entry[kList];                // [level][list]
     __shared__ int s_count;
     __shared__ uint32_t s_limit;
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant_
             const double s = score(i, key);
             if (ordered(float(s) + 0.f) < limit) continue;
             const int at = atomicAdd(&s_count, 1);
-            if (at < kList) s_list[at] = Cand{ordered64(s), (long long)(i / per) * P.vocab + int(~uint32_t(key))};
+            if (at < kList) s_cand[at] = ordered64(s), s_key[at] = key, s_beam[at] = uint8_t(i / per);
         }
         __syncthreads();
         const int count = s_count;
@@ -437,8 +438,12 @@ __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant_
             if (kJoin / 4 * x >= count) continue;
             int r = 0;
             if (i < count) {
-                own[x] = s_list[i];
-                for (int j = lane & 3; j < count; j += 4) r += before(s_list[j], own[x]);
+                own[x] = Cand{s_cand[i], s_key[i], s_beam[i]};
+                for (int j = lane & 3; j < count; j += 4) {
+                    const uint64_t o = s_cand[j];
+                    if (o > own[x].score) ++r;
+                    else if (o == own[x].score) r += s_beam[j] < own[x].beam || (s_beam[j] == own[x].beam && s_key[j] > own[x].key);
+                }
             }
             r += __shfl_xor_sync(0xffffffffu, r, 1);
             r += __shfl_xor_sync(0xffffffffu, r, 2);
@@ -451,15 +456,15 @@ __global__ void __launch_bounds__(kJoin) beam_join_kernel(const __grid_constant_
                     const uint64_t o = own[x].score;
                     const long long at = (long long)req * n + rank[x];
                     P.scores_out[at] = float(__longlong_as_double(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
-                    P.parents[at] = int(own[x].place / P.vocab);
-                    P.tokens[at] = int(own[x].place % P.vocab);
+                    P.parents[at] = own[x].beam;
+                    P.tokens[at] = int(~uint32_t(own[x].key));
                 }
             return;
         }
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-            if (rank[x] < n) s_list[rank[x]] = own[x];
+            if (rank[x] < n) s_cand[rank[x]] = own[x].score, s_key[rank[x]] = own[x].key, s_beam[rank[x]] = uint8_t(own[x].beam);
         if (tid == 0) s_count = min(count, n);
         __syncthreads();
     }

@@ -1,4 +1,5 @@
-"""The order of beam selection's candidates whose scores are alike though their logits are not."""
+"""The order of beam selection's candidates whose scores are alike though their logits are not: beams without a score, and scores so
+large that 64 bits no longer tell the logits apart."""
 import pytest
 import torch
 
@@ -50,3 +51,23 @@ def test_few_candidates_alive(cuda):
     s = torch.tensor([[-float("inf"), 0.5, -float("inf")]], device=cuda)
     got = beams.select(x, s, 60)
     assert places(got, 40) == want(x, s, 60)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("score", [-1e30, 3e25, float("inf")])
+def test_scores_that_swallow_the_logits(cuda, dtype, score):
+    """A score beside which fp64 holds no logit: the beam's candidates are still in the order of its logits, equal ones of their places."""
+    x = (torch.randn(2, 2, 6007, generator=gen(6, cuda), device=cuda) * 2).to(dtype)
+    s = torch.tensor([[score, -float("inf")], [-float("inf"), score]], device=cuda)
+    got = beams.select(x, s, 40)
+    assert places(got, 6007) == want(x, s, 40)
+
+
+def test_logits_nearer_than_their_score_tells(cuda):
+    """Logits of 1e-20 and 2e-20 under a largest one of 5: the scores are one number in fp64, the logits are not."""
+    x = torch.full((1, 2, 3000), -9.0, device=cuda)
+    x[0, :, 100] = 5.0
+    x[0, :, 200:210] = torch.arange(10, device=cuda) * 1e-20
+    s = torch.tensor([[0.0, -30.0]], device=cuda)
+    got = beams.select(x, s, 8)
+    assert places(got, 3000) == want(x, s, 8)
