@@ -432,7 +432,8 @@ int64_t qmv_page_reorder_workspace_bytes(int n_req, int beams, int table_width);
 /* The next step's tables of a beam search: beam j of request r goes on from beam parents[r][j] (-1: ends) of the tables [n_req][beams]
  * [table_width] and lens [n_req][beams].  Beams of a request share whole pages, at the same place of their tables; pages that no
  * beam holds any more become free, in the order of place, then beam (the first own[r] places are not the request's and stay; own null:
- * 0).  Of the beams that would write to the same partly filled page the first keeps it and the others get a copy (all of them
+ * 0; where the last of them is partly filled, the beams hold copies of it behind the call, which are the request's: own[r] is one less from
+ * then on, or that page would be copied at every call and the copies be lost).  Of the beams that would write to the same partly filled page the first keeps it and the others get a copy (all of them
  * where the page is not the request's): src, dst, used [n_req][beams] name the page to copy, the new one and its tokens
  * (-1, -1, 0: none), for qmv_kv_copy of each layer.  New pages are the request's own freed ones, in order, then the stack's, onto which all the
  * other freed ones went before; -1 where none is left (counts_out[1] counts them).  tables_out, lens_out: as tables and lens, -1 behind a beam's pages.  Parents

@@ -72,5 +72,7 @@ def reorder(parents: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, fre
     place of their tables.  Pages that no beam holds any more become free.  Of the beams that would write to one partly filled page the
     first keeps it, the others get a copy: `KVCache.copy(src, dst, used)` makes it, once a layer and before the next write.
     own int32 (requests,): leading places of the tables whose pages belong to others too (a shared prefix), which are neither freed nor
-    written to.  One launch for up to 32 requests of 8 beams with short tables, else two."""
+    written to.  Where a prefix ends inside a page, own counts that page for the first call only: every beam gets its copy there, which is
+    the request's own from then on, so later calls pass the whole pages alone (with the same own that page would be copied at every call
+    and its copies be lost to free).  One launch for up to 32 requests of 8 beams with short tables, else two."""
     return Reordered._make(_lib.host().reorder(lens, tables, free, counts, page, parents, own))

@@ -26,3 +26,38 @@ def test_own_of_any_size(cuda, reqs, beams, page, width, shared, own):
     for name, w in zip(("tables", "lens", "counts", "src", "dst", "used"), want):
         assert getattr(got, name).tolist() == w, name
     assert f.tolist() == want[6]
+
+
+@pytest.mark.parametrize("reqs, beams", [(2, 3), (40, 4)])
+@pytest.mark.parametrize("tokens", [40, 48])
+def test_steps_behind_a_shared_prefix(cuda, reqs, beams, tokens):
+    """Requests that go on from one prefix, which ends inside a page or with one: `own` counts the page that it ends in for the first call,
+    which gives every beam a copy, and the whole ones from then on.  At every step each page is the prefix's, a beam's or free."""
+    r = random.Random(reqs + tokens)
+    page, width, n = 16, 9, reqs * beams
+    shared, whole = PH.up(tokens, page), tokens // page
+    n_pages = shared + n * width
+    order = r.sample(range(n_pages), n_pages)
+    prefix = order[:shared]
+    free, counts = ints(order[shared:] + [0] * shared, cuda), ints([n_pages - shared, 0], cuda)
+    tables = ints([prefix + [-1] * (width - shared)] * n, cuda)
+    lens = ints([tokens if b % beams == 0 else 0 for b in range(n)], cuda)      # the prompt is the first beam's
+    parents = [[0] * beams for _ in range(reqs)]
+    for step in range(40):
+        s = pages.reorder(ints(parents, cuda), lens, tables, free, counts, page, ints([shared if step == 0 else whole] * reqs, cuda))
+        if step == 0:
+            assert s.used.tolist() == [tokens % page] * n and (s.src[s.src >= 0] == prefix[-1]).all()
+        p = pages.plan(s.lens, torch.ones_like(s.lens), s.tables, free, s.counts, page, n)
+        tables, lens, counts = s.tables, p.lens, p.counts
+        assert lens.tolist() == [tokens + step + 1] * n and counts[1].item() == 0
+        held = set()
+        for row, k in zip(tables.tolist(), lens.tolist()):
+            assert row[:whole] == prefix[:whole]
+            held |= set(row[whole:PH.up(k, page)])
+        left = free[:counts[0].item()].tolist()
+        assert -1 not in held and not held & set(prefix) and sorted([*prefix, *held, *left]) == list(range(n_pages)), step
+        slots = p.slots.tolist()
+        assert len(set(slots)) == n and not {x // page for x in slots} & set(prefix)      # no two beams write to one page
+        parents = [[r.randrange(beams) for _ in range(beams)] for _ in range(reqs)]
+    s = pages.reorder(ints([[-1] * beams] * reqs, cuda), lens, tables, free, counts, page, ints([whole] * reqs, cuda))
+    assert s.counts.tolist() == [n_pages - shared, 0]
