@@ -1,7 +1,8 @@
 // The host side of the serving loop's small calls (pages.py, beams.py, kvcache.py): argument checks, outputs and workspaces, and the
 // call into the library (include/nemicli_qmv.h).  Their kernels take 2 to 25 us, and through ctypes and torch's Python functions the
 // calls took 14 to 45 us on the host: 1.5 us an output, 0.5 us a checked argument, 1.5 us for ctypes.  A CPython module over
-// libtorch, one function a call; every refusal is a RuntimeError, and nothing is launched before the checks.
+// libtorch, one function a call; every refusal is a RuntimeError, and nothing is launched before the checks.  Arguments are read under the
+// interpreter's lock; allocations, copies and launches, which may wait for memory or for room in the stream, leave it to other threads.
 #include <Python.h>
 
 #include <algorithm>
@@ -121,6 +122,19 @@ PyObject* tuple(T&&... t) {
     return out;
 }
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
+// A call's work on the device: the interpreter's lock is free (no Python object is touched until the end of the scope; an exception leaves
+// it with the lock taken again), and the device is the current one.
+struct OnDevice {
+    struct Unlocked {
+        PyThreadState* state = PyEval_SaveThread();
+        Unlocked() = default;
+        Unlocked(const Unlocked&) = delete;
+        Unlocked& operator=(const Unlocked&) = delete;
+        ~Unlocked() { PyEval_RestoreThread(state); }
+    } unlocked;
+    c10::cuda::OptionalCUDAGuard guard;
+    explicit OnDevice(int device) : guard(c10::Device(c10::kCUDA, device)) {}
+};
 
 // a function of a fixed number of arguments: C++ exceptions become Python's
 template <int N, PyObject* (*F)(PyObject* const*)>
@@ -176,13 +190,16 @@ PyObject* plan(PyObject* const* a) {                              // lens, table
     const Tensor& add = tensor(a[5], "pages.plan new");
     expect(add, "pages.plan new", t.device, ScalarType::Int, {t.n});
     const int64_t rows = number(a[6], "pages.plan rows", 0, 1 << 30);
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, t.device));
-    Outputs o{t.device};
-    o.plan({rows}, ScalarType::Long), o.plan({rows}, ScalarType::Long), o.plan({t.n + 1}, ScalarType::Int), o.plan({t.n}, ScalarType::Int), o.plan({2}, ScalarType::Int);
-    Tensor slots = o.take({rows}, ScalarType::Long), positions = o.take({rows}, ScalarType::Long), starts = o.take({t.n + 1}, ScalarType::Int),
-           lens = o.take({t.n}, ScalarType::Int), counts = o.take({2}, ScalarType::Int);
-    check(qmv_page_plan(ints(t.lens), ints(add), ints(t.tables), t.n, t.width, t.page, ints(t.free), int(t.free.size(0)), ints(t.counts), rows,
-                        longs(slots), longs(positions), ints(starts), ints(lens), ints(counts), stream_of(t.device)), "qmv_page_plan");
+    Tensor slots, positions, starts, lens, counts;
+    {
+        const OnDevice scope(t.device);
+        Outputs o{t.device};
+        o.plan({rows}, ScalarType::Long), o.plan({rows}, ScalarType::Long), o.plan({t.n + 1}, ScalarType::Int), o.plan({t.n}, ScalarType::Int), o.plan({2}, ScalarType::Int);
+        slots = o.take({rows}, ScalarType::Long), positions = o.take({rows}, ScalarType::Long), starts = o.take({t.n + 1}, ScalarType::Int);
+        lens = o.take({t.n}, ScalarType::Int), counts = o.take({2}, ScalarType::Int);
+        check(qmv_page_plan(ints(t.lens), ints(add), ints(t.tables), t.n, t.width, t.page, ints(t.free), int(t.free.size(0)), ints(t.counts), rows,
+                            longs(slots), longs(positions), ints(starts), ints(lens), ints(counts), stream_of(t.device)), "qmv_page_plan");
+    }
     return tuple(std::move(slots), std::move(positions), std::move(starts), std::move(lens), std::move(counts));
 }
 
@@ -190,12 +207,15 @@ PyObject* release(PyObject* const* a) {                           // lens, table
     const Tables t = tables_of(a, "pages.release");
     const Tensor& done = tensor(a[5], "pages.release done");
     expect(done, "pages.release done", t.device, ScalarType::Bool, {t.n});
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, t.device));
-    Outputs o{t.device};
-    o.plan({t.n}, ScalarType::Int), o.plan({2}, ScalarType::Int);
-    Tensor lens = o.take({t.n}, ScalarType::Int), counts = o.take({2}, ScalarType::Int);
-    check(qmv_page_release(static_cast<const uint8_t*>(done.data_ptr()), ints(t.lens), ints(t.tables), t.n, t.width, t.page, ints(t.free),
-                           int(t.free.size(0)), ints(t.counts), ints(lens), ints(counts), stream_of(t.device)), "qmv_page_release");
+    Tensor lens, counts;
+    {
+        const OnDevice scope(t.device);
+        Outputs o{t.device};
+        o.plan({t.n}, ScalarType::Int), o.plan({2}, ScalarType::Int);
+        lens = o.take({t.n}, ScalarType::Int), counts = o.take({2}, ScalarType::Int);
+        check(qmv_page_release(static_cast<const uint8_t*>(done.data_ptr()), ints(t.lens), ints(t.tables), t.n, t.width, t.page, ints(t.free),
+                               int(t.free.size(0)), ints(t.counts), ints(lens), ints(counts), stream_of(t.device)), "qmv_page_release");
+    }
     return tuple(std::move(lens), std::move(counts));
 }
 
@@ -211,17 +231,20 @@ PyObject* reorder(PyObject* const* a) {                           // lens, table
         expect(o, "pages.reorder own", t.device, ScalarType::Int, {reqs});
         own = ints(o);
     }
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, t.device));
-    Outputs o{t.device};
-    o.plan({t.n, t.width}, ScalarType::Int), o.plan({2}, ScalarType::Int);
-    for (int i = 0; i < 4; ++i) o.plan({t.n}, ScalarType::Int);
-    Tensor tables = o.take({t.n, t.width}, ScalarType::Int), counts = o.take({2}, ScalarType::Int), lens = o.take({t.n}, ScalarType::Int),
-           src = o.take({t.n}, ScalarType::Int), dst = o.take({t.n}, ScalarType::Int), used = o.take({t.n}, ScalarType::Int);
-    const int64_t nbytes = qmv_page_reorder_workspace_bytes(int(reqs), int(beams), t.width);
-    const Tensor ws = make({nbytes}, ScalarType::Byte, t.device);
-    check(qmv_page_reorder(ints(parents), ints(t.lens), ints(t.tables), own, int(reqs), int(beams), t.width, t.page, ints(t.free), int(t.free.size(0)),
-                           ints(t.counts), ints(tables), ints(lens), ints(src), ints(dst), ints(used), ints(counts), ws.data_ptr(), nbytes,
-                           stream_of(t.device)), "qmv_page_reorder");
+    Tensor tables, counts, lens, src, dst, used;
+    {
+        const OnDevice scope(t.device);
+        Outputs o{t.device};
+        o.plan({t.n, t.width}, ScalarType::Int), o.plan({2}, ScalarType::Int);
+        for (int i = 0; i < 4; ++i) o.plan({t.n}, ScalarType::Int);
+        tables = o.take({t.n, t.width}, ScalarType::Int), counts = o.take({2}, ScalarType::Int), lens = o.take({t.n}, ScalarType::Int);
+        src = o.take({t.n}, ScalarType::Int), dst = o.take({t.n}, ScalarType::Int), used = o.take({t.n}, ScalarType::Int);
+        const int64_t nbytes = qmv_page_reorder_workspace_bytes(int(reqs), int(beams), t.width);
+        const Tensor ws = make({nbytes}, ScalarType::Byte, t.device);
+        check(qmv_page_reorder(ints(parents), ints(t.lens), ints(t.tables), own, int(reqs), int(beams), t.width, t.page, ints(t.free), int(t.free.size(0)),
+                               ints(t.counts), ints(tables), ints(lens), ints(src), ints(dst), ints(used), ints(counts), ws.data_ptr(), nbytes,
+                               stream_of(t.device)), "qmv_page_reorder");
+    }
     return tuple(std::move(tables), std::move(lens), std::move(counts), std::move(src), std::move(dst), std::move(used));
 }
 
@@ -232,9 +255,23 @@ int dtype_of(const Tensor& t) {
          : t.scalar_type() == ScalarType::Half ? QMV_OUT_F16 : -1;
 }
 
+void choose_best(Tensor logits, const Tensor& scores, int dtype, int n, const Tensor& out, const Tensor& parents, const Tensor& tokens) {
+    const int64_t reqs = logits.size(0), k = logits.size(1), vocab = logits.size(2);
+    int64_t by_req = logits.stride(0), by_beam = logits.stride(1);
+    if ((logits.stride(2) != 1 && vocab > 1) || (k > 1 && by_beam < vocab) || (reqs > 1 && (by_req < vocab || (k > 1 && by_req != k * by_beam)))) {
+        logits = logits.contiguous();
+        by_beam = vocab, by_req = k * vocab;
+    }
+    const int64_t stride = k > 1 ? by_beam : reqs > 1 ? by_req : vocab;
+    const int64_t nbytes = qmv_beam_workspace_bytes(int(reqs), int(k), int(vocab), n);
+    const Tensor ws = make({nbytes}, ScalarType::Byte, logits.get_device());
+    check(qmv_beam_select(logits.data_ptr(), dtype, stride, int(reqs), int(k), int(vocab), static_cast<const float*>(scores.data_ptr()), n,
+                          static_cast<float*>(out.data_ptr()), ints(parents), ints(tokens), ws.data_ptr(), nbytes, stream_of(logits.get_device())),
+          "qmv_beam_select");
+}
+
 PyObject* select(PyObject* const* a) {                            // logits, scores, n
-    Tensor logits = tensor(a[0], "beams.select logits");
-    const Tensor& scores = tensor(a[1], "beams.select scores");
+    const Tensor &logits = tensor(a[0], "beams.select logits"), &scores = tensor(a[1], "beams.select scores");
     const int dtype = dtype_of(logits);
     if (logits.dim() != 3 || dtype < 0 || !logits.is_cuda())
         refuse("beams.select: logits (requests, beams, vocab) of float32, bfloat16 or float16 on a CUDA device expected, got ", shape_of(logits));
@@ -245,21 +282,13 @@ PyObject* select(PyObject* const* a) {                            // logits, sco
     if (n == 0) n = k;
     if (k < 1 || k > 64 || n < 1 || n > 64 || vocab < 1 || vocab > 1 << 30 || n > k * vocab || reqs * k > 65535)
         refuse("beams.select: ", reqs, " requests of ", k, " beams over ", vocab, " tokens, ", n, " best: up to 64 beams and candidates, 65535 beams in all");
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, device));
-    Outputs o{device};
-    o.plan({reqs, n}, ScalarType::Float), o.plan({reqs, n}, ScalarType::Int), o.plan({reqs, n}, ScalarType::Int);
-    Tensor out = o.take({reqs, n}, ScalarType::Float), parents = o.take({reqs, n}, ScalarType::Int), tokens = o.take({reqs, n}, ScalarType::Int);
-    if (reqs) {
-        int64_t by_req = logits.stride(0), by_beam = logits.stride(1);
-        if ((logits.stride(2) != 1 && vocab > 1) || (k > 1 && by_beam < vocab) || (reqs > 1 && (by_req < vocab || (k > 1 && by_req != k * by_beam)))) {
-            logits = logits.contiguous();
-            by_beam = vocab, by_req = k * vocab;
-        }
-        const int64_t stride = k > 1 ? by_beam : reqs > 1 ? by_req : vocab;
-        const int64_t nbytes = qmv_beam_workspace_bytes(int(reqs), int(k), int(vocab), int(n));
-        const Tensor ws = make({nbytes}, ScalarType::Byte, device);
-        check(qmv_beam_select(logits.data_ptr(), dtype, stride, int(reqs), int(k), int(vocab), static_cast<const float*>(scores.data_ptr()), int(n),
-                              static_cast<float*>(out.data_ptr()), ints(parents), ints(tokens), ws.data_ptr(), nbytes, stream_of(device)), "qmv_beam_select");
+    Tensor out, parents, tokens;
+    {
+        const OnDevice scope(device);
+        Outputs o{device};
+        o.plan({reqs, n}, ScalarType::Float), o.plan({reqs, n}, ScalarType::Int), o.plan({reqs, n}, ScalarType::Int);
+        out = o.take({reqs, n}, ScalarType::Float), parents = o.take({reqs, n}, ScalarType::Int), tokens = o.take({reqs, n}, ScalarType::Int);
+        if (reqs) choose_best(logits, scores, dtype, int(n), out, parents, tokens);
     }
     return tuple(std::move(out), std::move(parents), std::move(tokens));
 }
@@ -296,10 +325,24 @@ Tensor rows_of(const Tensor& t, int64_t& stride) {
     return reinterpret_cast<uintptr_t>(x.data_ptr()) % four ? x.clone() : x;
 }
 
+void write_rows(const Cache& c, const Tensor& k_given, const Tensor& v_given, const Tensor& slots, const Tensor& q_given, const Tensor& out, int dtype,
+                const float* cos, const float* sin, const long long* positions, int64_t n_pos, int rot, int paired, const uint8_t* axes, int n_axes) {
+    int64_t ks, vs, qs = 0;
+    const Tensor k = rows_of(k_given, ks), v = rows_of(v_given, vs), q = q_given.defined() ? rows_of(q_given, qs) : q_given;
+    const void* qp = q.defined() ? q.data_ptr() : nullptr;
+    void* op = q.defined() ? out.data_ptr() : nullptr;
+    const int n_q = q.defined() ? int(q.size(1)) : 0;
+    if (axes)
+        check(qmv_kv_write_axes(c.c, k.data_ptr(), v.data_ptr(), dtype, ks, vs, longs(slots), k.size(0), cos, sin, positions, n_pos, rot, paired, axes, n_axes,
+                                qp, qs, n_q, op, stream_of(c.device)), "qmv_kv_write_axes");
+    else
+        check(qmv_kv_write(c.c, k.data_ptr(), v.data_ptr(), dtype, ks, vs, longs(slots), k.size(0), cos, sin, positions, n_pos, rot, paired, qp, qs, n_q, op,
+                           stream_of(c.device)), "qmv_kv_write");
+}
+
 PyObject* write(PyObject* const* a) {                             // cache (2), k, v, slots, q, cos, sin, positions, paired, axes
     const Cache c = cache_of(a);
-    Tensor k = tensor(a[2], "KVCache.write k"), v = tensor(a[3], "KVCache.write v");
-    const Tensor& slots = tensor(a[4], "KVCache.write slots");
+    const Tensor &k = tensor(a[2], "KVCache.write k"), &v = tensor(a[3], "KVCache.write v"), &slots = tensor(a[4], "KVCache.write slots");
     const int dtype = tokens_of(k, "KVCache.write k", c, c.c->n_kv);
     const int64_t rows = k.size(0);
     if (tokens_of(v, "KVCache.write v", c, c.c->n_kv) != dtype || v.size(0) != rows) refuse("KVCache.write v: ", rows, " rows of ", k.scalar_type(), " expected");
@@ -333,26 +376,15 @@ PyObject* write(PyObject* const* a) {                             // cache (2), 
     }
     const int paired = PyObject_IsTrue(a[9]);
     if (paired < 0) throw PythonError{};
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, c.device));
     Tensor q, out;
-    int64_t ks, vs, qs = 0;
     if (!none(a[5])) {
-        const Tensor& given = tensor(a[5], "KVCache.write q");
-        if (tokens_of(given, "KVCache.write q", c) != dtype || given.size(0) != rows) refuse("KVCache.write q: ", rows, " rows of ", k.scalar_type(), " expected");
-        out = make(given.sizes(), given.scalar_type(), c.device);
-        q = rows_of(given, qs);
+        q = tensor(a[5], "KVCache.write q");
+        if (tokens_of(q, "KVCache.write q", c) != dtype || q.size(0) != rows) refuse("KVCache.write q: ", rows, " rows of ", k.scalar_type(), " expected");
     }
-    k = rows_of(k, ks), v = rows_of(v, vs);
-    if (rows) {
-        const void* qp = q.defined() ? q.data_ptr() : nullptr;
-        void* op = q.defined() ? out.data_ptr() : nullptr;
-        const int n_q = q.defined() ? int(q.size(1)) : 0;
-        if (axes)
-            check(qmv_kv_write_axes(c.c, k.data_ptr(), v.data_ptr(), dtype, ks, vs, longs(slots), rows, cos, sin, positions, n_pos, int(rot), paired, axes,
-                                    n_axes, qp, qs, n_q, op, stream_of(c.device)), "qmv_kv_write_axes");
-        else
-            check(qmv_kv_write(c.c, k.data_ptr(), v.data_ptr(), dtype, ks, vs, longs(slots), rows, cos, sin, positions, n_pos, int(rot), paired, qp, qs, n_q,
-                               op, stream_of(c.device)), "qmv_kv_write");
+    {
+        const OnDevice scope(c.device);
+        if (q.defined()) out = make(q.sizes(), q.scalar_type(), c.device);
+        if (rows) write_rows(c, k, v, slots, q, out, dtype, cos, sin, positions, n_pos, int(rot), paired, axes, n_axes);
     }
     if (!out.defined()) Py_RETURN_NONE;
     return wrap(std::move(out));
@@ -365,9 +397,12 @@ PyObject* read(PyObject* const* a) {                              // cache (2), 
     const int dtype = int(number(a[3], "KVCache.read dtype", 0, 2));
     const ScalarType type = dtype == QMV_OUT_F32 ? ScalarType::Float : dtype == QMV_OUT_BF16 ? ScalarType::BFloat16 : ScalarType::Half;
     const int64_t rows = slots.size(0);
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, c.device));
-    Tensor k = make({rows, c.c->n_kv, c.c->dim}, type, c.device), v = make({rows, c.c->n_kv, c.c->dim}, type, c.device);
-    if (rows) check(qmv_kv_read(c.c, longs(slots), rows, k.data_ptr(), v.data_ptr(), dtype, stream_of(c.device)), "qmv_kv_read");
+    Tensor k, v;
+    {
+        const OnDevice scope(c.device);
+        k = make({rows, c.c->n_kv, c.c->dim}, type, c.device), v = make({rows, c.c->n_kv, c.c->dim}, type, c.device);
+        if (rows) check(qmv_kv_read(c.c, longs(slots), rows, k.data_ptr(), v.data_ptr(), dtype, stream_of(c.device)), "qmv_kv_read");
+    }
     return tuple(std::move(k), std::move(v));
 }
 
@@ -380,8 +415,10 @@ PyObject* copy(PyObject* const* a) {                              // cache (2), 
             refuse("KVCache.copy: src, dst and used contiguous int32 of one shape on cuda:", c.device, " expected, got ", shape_of(src), " and ", shape_of(*t));
     const int64_t n = src.numel();
     if (n > 0x7FFFFFFF) refuse("KVCache.copy: ", n, " copies");
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, c.device));
-    if (n) check(qmv_kv_copy(c.c, ints(src), ints(dst), used ? ints(*used) : nullptr, int(n), stream_of(c.device)), "qmv_kv_copy");
+    if (n) {
+        const OnDevice scope(c.device);
+        check(qmv_kv_copy(c.c, ints(src), ints(dst), used ? ints(*used) : nullptr, int(n), stream_of(c.device)), "qmv_kv_copy");
+    }
     Py_RETURN_NONE;
 }
 
@@ -415,10 +452,11 @@ PyObject* summarise(PyObject* const* a) {                         // cache (2), 
     void* bounds = bounds_of(tensor(a[5], "KVCache.summarise bounds"), "KVCache.summarise bounds", c);
     const Held h = held_of(a + 2, c, "KVCache.summarise");
     const int64_t cap = h.width * c.c->page, most = !h.starts ? 1 : none(a[6]) ? cap : number(a[6], "KVCache.summarise max_new", 0, INT64_MAX);
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, c.device));
-    if (h.n_seq && h.width && most)
+    if (h.n_seq && h.width && most) {
+        const OnDevice scope(c.device);
         check(qmv_kv_bounds(c.c, ints(h.tables), int(h.width), ints(h.lens), h.starts, int(h.n_seq), int(std::min(most, cap)), bounds, stream_of(c.device)),
               "qmv_kv_bounds");
+    }
     Py_RETURN_NONE;
 }
 
@@ -434,19 +472,22 @@ PyObject* choose(PyObject* const* a) {                            // cache (2), 
     const int64_t most = (1 << 30) / c.c->page, keep = number(a[7], "KVCache.choose keep", 1, most), first = number(a[8], "KVCache.choose first", 0, most),
                   last = number(a[9], "KVCache.choose last", 1, most);
     if (keep < first + last || rows > 65535) refuse("KVCache.choose: keep ", keep, " holds first ", first, " and last ", last, ", rows ", rows, " up to 65535");
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, c.device));
-    Outputs o{c.device};
-    o.plan({rows, c.c->n_kv, keep}, ScalarType::Int), o.plan({rows}, ScalarType::Int);
-    Tensor chosen = o.take({rows, c.c->n_kv, keep}, ScalarType::Int), held = o.take({rows}, ScalarType::Int);
-    if (rows && (!h.n_seq || !h.width)) {
-        chosen.fill_(-1), held.zero_();
-    } else if (rows) {
-        int64_t qs;
-        const Tensor q = rows_of(given, qs);
-        const int64_t nbytes = qmv_kv_choose_workspace_bytes(c.c, int(h.width), rows, int(keep));
-        const Tensor ws = make({nbytes}, ScalarType::Byte, c.device);
-        check(qmv_kv_choose(c.c, q.data_ptr(), dtype, qs, int(heads), bounds, ints(h.tables), int(h.width), ints(h.lens), h.starts, int(h.n_seq), rows, int(keep),
-                            int(first), int(last), ints(chosen), ints(held), ws.data_ptr(), nbytes, stream_of(c.device)), "qmv_kv_choose");
+    Tensor chosen, held;
+    {
+        const OnDevice scope(c.device);
+        Outputs o{c.device};
+        o.plan({rows, c.c->n_kv, keep}, ScalarType::Int), o.plan({rows}, ScalarType::Int);
+        chosen = o.take({rows, c.c->n_kv, keep}, ScalarType::Int), held = o.take({rows}, ScalarType::Int);
+        if (rows && (!h.n_seq || !h.width)) {
+            chosen.fill_(-1), held.zero_();
+        } else if (rows) {
+            int64_t qs;
+            const Tensor q = rows_of(given, qs);
+            const int64_t nbytes = qmv_kv_choose_workspace_bytes(c.c, int(h.width), rows, int(keep));
+            const Tensor ws = make({nbytes}, ScalarType::Byte, c.device);
+            check(qmv_kv_choose(c.c, q.data_ptr(), dtype, qs, int(heads), bounds, ints(h.tables), int(h.width), ints(h.lens), h.starts, int(h.n_seq), rows,
+                                int(keep), int(first), int(last), ints(chosen), ints(held), ws.data_ptr(), nbytes, stream_of(c.device)), "qmv_kv_choose");
+        }
     }
     return tuple(std::move(chosen), std::move(held));
 }
@@ -469,24 +510,25 @@ PyObject* attend_chosen(PyObject* const* a) {                     // cache (2), 
         if (scale == -1.0 && PyErr_Occurred()) throw PythonError{};
         if (!(std::abs(scale) < 3.4028235e38)) refuse("KVCache.attend_chosen: scale ", scale, " is not finite");
     }
-    const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, c.device));
     Tensor out;
-    if (none(a[6])) {
-        out = make(given.sizes(), given.scalar_type(), c.device);
-    } else {
+    if (!none(a[6])) {
         out = tensor(a[6], "KVCache.attend_chosen out");
         if (out.sizes() != given.sizes() || out.scalar_type() != given.scalar_type() || out.device() != given.device() || !out.is_contiguous() ||
             reinterpret_cast<uintptr_t>(out.data_ptr()) % 16)
             refuse("KVCache.attend_chosen: out must be contiguous, 16-byte aligned and like q (", shape_of(given), "), got ", shape_of(out));
     }
-    if (rows) {
-        int64_t qs;
-        const Tensor q = rows_of(given, qs);
-        const int64_t nbytes = qmv_kv_attend_chosen_workspace_bytes(c.c, int(heads), rows, dtype, int(keep));
-        if (nbytes <= 0) refuse("KVCache.attend_chosen: ", heads, " heads, ", rows, " rows of ", keep, " pages not supported");
-        const Tensor ws = make({nbytes}, ScalarType::Byte, c.device);
-        check(qmv_kv_attend_chosen(c.c, q.data_ptr(), dtype, qs, int(heads), ints(chosen), int(keep), ints(held), rows, float(scale), out.data_ptr(), ws.data_ptr(),
-                                   nbytes, stream_of(c.device)), "qmv_kv_attend_chosen");
+    {
+        const OnDevice scope(c.device);
+        if (!out.defined()) out = make(given.sizes(), given.scalar_type(), c.device);
+        if (rows) {
+            int64_t qs;
+            const Tensor q = rows_of(given, qs);
+            const int64_t nbytes = qmv_kv_attend_chosen_workspace_bytes(c.c, int(heads), rows, dtype, int(keep));
+            if (nbytes <= 0) refuse("KVCache.attend_chosen: ", heads, " heads, ", rows, " rows of ", keep, " pages not supported");
+            const Tensor ws = make({nbytes}, ScalarType::Byte, c.device);
+            check(qmv_kv_attend_chosen(c.c, q.data_ptr(), dtype, qs, int(heads), ints(chosen), int(keep), ints(held), rows, float(scale), out.data_ptr(),
+                                       ws.data_ptr(), nbytes, stream_of(c.device)), "qmv_kv_attend_chosen");
+        }
     }
     if (!none(a[6])) {
         Py_INCREF(a[6]);
