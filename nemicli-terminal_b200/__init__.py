@@ -13,7 +13,7 @@ Module map (reference counterparts in ggufengine/):
     beams     -> (new)            beam search's choice over the beams and the vocabulary
     shard     -> (new)            row-sharded projections and expert-sharded MoE over NCCL
 The CUDA kernels sit in csrc/ behind the C ABI of include/nemicli_qmv.h (libnemiqmv.so); the small calls' host side is
-csrc/host/qmv_host.cpp (_qmv_host.so).
+csrc/host/qmv_host.cpp (_qmv_host.*.so, one for each torch and Python).
 """
 from .formats import FORMATS, TYPE_ID, TYPE_NAME  # noqa: F401
 

@@ -108,9 +108,10 @@ def host():
     load()
     with _lock:
         if _host is None:
-            if not os.path.exists(_build.HOST_PATH):
-                raise RuntimeError(f"module missing: {_build.HOST_PATH} (build it with nemicli_terminal_b200.build.build())")
-            spec = importlib.util.spec_from_file_location("_qmv_host", _build.HOST_PATH)
+            path = _build.host_path()
+            if not os.path.exists(path):
+                raise RuntimeError(f"module missing: {path} (build it with nemicli_terminal_b200.build.build())")
+            spec = importlib.util.spec_from_file_location("_qmv_host", path)
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)
             _host = mod

@@ -25,7 +25,6 @@ OBJ_DIR = os.path.join(HERE, "_build")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 PER_FORMAT = "qmv_fmt.cu"
 HOST_SRC = os.path.join(CSRC, "host", "qmv_host.cpp")
-HOST_PATH = os.path.join(HERE, "_qmv_host.so")
 
 
 def nvcc() -> str:
@@ -117,10 +116,20 @@ def build(force: bool = False, verbose: bool = False, extra: tuple = (), out: st
         return out
 
 
+def host_path() -> str:
+    """The Python module over the library, for this process's torch and Python: it has torch's inline accessors (the layout of a tensor)
+    compiled in, so its name says which it was compiled against, and another environment finds none and builds its own."""
+    import sysconfig
+
+    import torch
+    tag = f"torch-{torch.__version__}-{str(torch.version.git_version)[:12]}-abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    return os.path.join(HERE, f"_qmv_host.{tag}.{sysconfig.get_config_var('SOABI')}.so")
+
+
 def _host_stale() -> bool:
-    """The Python module is older than its source or the C ABI it calls (the library itself may be newer)."""
-    sources = (HOST_SRC, os.path.join(HERE, "..", "include", "nemicli_qmv.h"))
-    return not os.path.exists(HOST_PATH) or any(os.path.getmtime(p) > os.path.getmtime(HOST_PATH) for p in sources)
+    """The Python module is missing or older than its source or the C ABI it calls (the library itself may be newer)."""
+    path, sources = host_path(), (HOST_SRC, os.path.join(HERE, "..", "include", "nemicli_qmv.h"))
+    return not os.path.exists(path) or any(os.path.getmtime(p) > os.path.getmtime(path) for p in sources)
 
 
 def build_host(verbose: bool = False) -> str:
@@ -129,19 +138,20 @@ def build_host(verbose: bool = False) -> str:
     import sysconfig
 
     import torch
+    out = host_path()
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}/include", HOST_SRC,
-           "-o", HOST_PATH + ".tmp", f"-L{HERE}", f"-l:{LIB_NAME}", f"-L{root}/lib", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda",
+           "-o", out + ".tmp", f"-L{HERE}", f"-l:{LIB_NAME}", f"-L{root}/lib", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda",
            "-lc10", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), file=sys.stderr, flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)} ({res.returncode}):\n{res.stderr[-4000:]}")
-    os.replace(HOST_PATH + ".tmp", HOST_PATH)
-    return HOST_PATH
+    os.replace(out + ".tmp", out)
+    return out
 
 
 def _build_locked(force: bool, verbose: bool, extra: tuple, out: str, obj_dir: str, jobs: int) -> str:
