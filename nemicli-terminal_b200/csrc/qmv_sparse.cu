@@ -210,8 +210,9 @@ constexpr int kTiles = 2, kPagesWarp = 16 * kTiles;              // pages a warp
 // A warp 16 pages, the rows of mma.m16n8k16 over the 2 dim halves of a box: lo against the queries' negative parts, hi against the
 // positive ones, the key head's query heads as columns (eight at a time).  A lane's 16 bytes of a box are two steps' operands as they
 // lie; the queries are laid out to match.  Queries are fp16 after a power of two a head, fp32 ones two fp16 parts.  So a score is near:
-// off by less than 2^-15 sum_c |q_c| max |box|: 2^-20 of it for the queries' parts, and in each of four chains at most 16 steps of 17
-// terms cut off at 2^-24 of the chain's share of that sum.  The choice computes those that lie nearer to its border again, in fp64.
+// off by less than 2^-15 sum_c |q_c| max(|box|, 2^-14): 2^-20 of it for the queries' parts, and in each of four chains at most 16 steps of 17
+// terms cut off at 2^-24 of the chain's share of that sum (a denormal side of a box counts there as 2^-14: with all sides 2^-24 scores were
+// off by 7 times 2^-15 of the sum with the sides' own size).  The choice computes those that lie nearer to its border again, in fp64.
 // 64 sequences of 154 pages on average, 8 key heads (40 MB of boxes): 9.8 us, bound by latency (lengths, table, boxes: dependent reads; DRAM
 // 31 %); 47 instructions a page and key head.  (All in fp64 on the CUDA cores: 27 to 46 us, 184 instructions.)
 template <int DT, int J>
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(kScorers) score_kernel(const __grid_constant__
             const float2 w = unpack_h2(wide[y][x]);
             if (t == x && i < end) {
                 P.near[out + i] = there[y][x] ? best[y][x] : -INFINITY;
-                P.sizes[out + i] = there[y][x] ? size * larger(w.x, w.y) : 0.f;
+                P.sizes[out + i] = there[y][x] ? size * larger(6.103515625e-5f, larger(w.x, w.y)) : 0.f;
             }
         }
 }
