@@ -507,7 +507,11 @@ PyObject* attend_chosen(PyObject* const* a) {                     // cache (2), 
     double scale = 1.0 / std::sqrt(double(c.c->dim));
     if (!none(a[5])) {
         scale = PyFloat_AsDouble(a[5]);
-        if (scale == -1.0 && PyErr_Occurred()) throw PythonError{};
+        if (scale == -1.0 && PyErr_Occurred()) {
+            if (!PyErr_ExceptionMatches(PyExc_TypeError) && !PyErr_ExceptionMatches(PyExc_OverflowError)) throw PythonError{};
+            PyErr_Clear();
+            refuse("KVCache.attend_chosen: scale: a number within float32 expected");
+        }
         if (!(std::abs(scale) < 3.4028235e38)) refuse("KVCache.attend_chosen: scale ", scale, " is not finite");
     }
     Tensor out;
