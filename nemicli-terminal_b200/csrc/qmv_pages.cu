@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const __grid_constant__ 
     const int given = __ldg(P.counts), n_free = min(max(given, 0), P.n_pages);
     if (mine == 0 && given != n_free) report(P.status);
     // Where pages were asked for in vain, tables may hold entries of -1, which are no pages to give back: then the entries are
-    // counted, a warp a sequence, by every CTA (else only lengths are read).
+    // counted, a warp a sequence, by every CTA (else only lengths are read: 4.4 us for a quarter of 1021 sequences of up to 512 pages, counted 50,
+    // for all of them 6.1 and 118).
     const bool holes = RELEASE && __ldg(P.counts + 1) != 0;
     const int lane = tid & 31, warp = tid >> 5;
     auto entry = [&](int b, int i, int had) { return i < had ? __ldg(P.tables + (long long)b * P.width + i) : -1; };

@@ -7,7 +7,7 @@ include/nemicli_qmv.h, qmv_page_plan).
 
 Free pages are a stack in two tensors: `free` int32 (pages of the cache,) and `counts` int32 (2,): counts[0] entries of free
 count, the last is taken first; counts[1] is a running number of pages that were asked for in vain, which a caller looks at
-now and then (`pool` makes both).  Everything is read on the device on torch's current stream and CUDA-graph safe.  Lengths and counts come back
+now and then, and sets to 0 when the sequences that lacked them have been released (`pool` makes both).  Everything is read on the device on torch's current stream and CUDA-graph safe.  Lengths and counts come back
 in new tensors, so that a call may be made again; tables and free are changed in place.  A captured step copies them back itself:
 
     step = pages.plan(lens, new, tables, free, counts, cache.page, rows)
@@ -61,7 +61,8 @@ def plan(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torc
 def release(done: torch.Tensor, lens: torch.Tensor, tables: torch.Tensor, free: torch.Tensor, counts: torch.Tensor, page: int):
     """The pages of the sequences with done (bool) go back to free; -> lens, 0 for them, and counts.  Their pages must be their own (a
     request's beams share some: `reorder` with parents -1 frees those).  Entries of -1, pages that were missing, are left out while counts[1]
-    is not 0 (so compare it with its last value; do not set it back).  One launch."""
+    is not 0, which takes a look at every entry of the tables (50 us for 1021 sequences of up to 512 pages, else 4.4): set counts[1] to 0 once the
+    sequences that lacked pages are released, not before.  One launch."""
     return _lib.host().release(lens, tables, free, counts, page, done)
 
 
