@@ -415,7 +415,8 @@ int qmv_kv_attend_chosen(const qmv_kv_cache* cache, const void* q, int dtype, lo
  * first row of each sequence.  Row r < rows is a new token, slots[r] its slot and positions[r] its place in the sequence; rows behind the last token have slot -1
  * and position 0.  Tokens beyond the table's end are dropped (they have no row), as are negative numbers of tokens; tokens beyond `rows`
  * have a page but no row; tokens whose page is missing have slot -1 and a table entry -1: each of these sets
- * QMV_DEV_BAD_ADDRESS.  counts_out: what is left.  One launch.  Replaces: nothing. */
+ * QMV_DEV_BAD_ADDRESS.  counts_out: what is left.  A table's entries behind lens[b] are not read: before a length is made shorter, the pages that
+ * lie behind it alone are given back (qmv_page_release of tables that hold those), or they are lost.  One launch.  Replaces: nothing. */
 int qmv_page_plan(const int* lens, const int* add, int* tables, int n_seq, int table_width, int page, const int* free_pages,
                   int n_pages, const int* counts, long long rows, long long* slots, long long* positions, int* starts,
                   int* lens_out, int* counts_out, void* stream);

@@ -54,7 +54,8 @@ def plan(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torc
     """Sequence b holds lens[b] tokens and gets new[b] (int32, 0 or more); the pages it lacks are taken from free and written into its row
     of tables.  rows: the step's rows, at least the new tokens; the ones behind the last token are padding (slot -1).  Tokens beyond a
     table's end are dropped; tokens whose page is missing get slot -1 and a table entry -1, and counts[1] goes up: both set the
-    device status.  One launch."""
+    device status.  Entries of a table behind its sequence's tokens are written over: where drafted tokens are taken back, the pages that only they
+    had go back first, by a release of tables that hold those pages alone.  One launch."""
     return Plan._make(_lib.host().plan(lens, tables, free, counts, page, new, rows))
 
 
