@@ -452,10 +452,12 @@ int64_t qmv_beam_workspace_bytes(int n_req, int beams, int vocab, int n);
 
 /* The n best continuations of each request: of scores[r][k] + log_softmax(logits[r beams + k])[v] over its beams k and tokens v the n
  * largest, best first, the lowest k vocab + v among equals (a beam's candidates are in the order of its logits also where fp64 no longer
- * tells their scores apart) -> scores_out, parents (k), tokens (v) [n_req][n].  logits: rows row_stride
- * values apart, of type dtype (QMV_OUT_*), any alignment; NaN counts as -inf, +inf as the largest float; a row of -inf alone and a
- * score of -inf give -inf throughout (NaN too), so such a beam's candidates are its first places, whatever its logits.  Exponentials in fp32, their sums and everything behind them in fp64, scores_out rounded
- * once.  n at most 64, beams at most 64, n_req * beams 65535, vocab 2^30, n at most beams * vocab.  workspace: 256-byte aligned.  Two
+ * tells their scores apart) -> scores_out, parents (k), tokens (v) [n_req][n].  logits: rows row_stride values apart, of type dtype
+ * (QMV_OUT_*), any alignment; NaN counts as -inf, +inf as the largest float; a row of -inf alone and a score of -inf give -inf throughout
+ * (NaN too), so such a beam's candidates are its first places, whatever its logits.  Exponentials in fp32, their sums and everything
+ * behind them in fp64, scores_out rounded once.  Rows are cut into parts by how many rows a call has, so a request's scores may differ in
+ * the last bits from one batch to another (and candidates of two beams that lie as near change places); the same call gives the same bits.
+ * n at most 64, beams at most 64, n_req * beams 65535, vocab 2^30, n at most beams * vocab.  workspace: 256-byte aligned.  Two
  * launches.  Replaces: nothing. */
 int qmv_beam_select(const void* logits, int dtype, long long row_stride, int n_req, int beams, int vocab, const float* scores,
                     int n, float* scores_out, int* parents, int* tokens, void* workspace, long long workspace_bytes,

@@ -14,5 +14,6 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n: int = 0):
     side by side; scores: float32 (requests, beams), the beams' log probabilities so far (-inf: no such beam).  n: default the
     beams; twice as many leave room for beams that end; up to 64 of each.  -> scores float32, parents int32, tokens int32, each
     (requests, n), best first: scores[r, parents] + log_softmax(logits[r, parents])[tokens], the lowest (beam, token) first among
-    equals (of a beam whose score is -inf or NaN its first tokens).  NaN counts as -inf, +inf as the largest float.  Two launches."""
+    equals (of a beam whose score is -inf or NaN its first tokens).  NaN counts as -inf, +inf as the largest float.  The
+    same call gives the same bits; in a batch of another size a request's scores may differ in their last ones.  Two launches."""
     return _lib.host().select(logits, scores, n)

@@ -5,7 +5,7 @@ import torch
 
 from nemicli_terminal_b200 import beams
 
-from tests.test_gpu_beams import BF16, F16, F32, gen
+from tests.test_gpu_beams import BF16, F16, F32, define, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,23 @@ def test_logits_nearer_than_their_score_tells(cuda):
     s = torch.tensor([[0.0, -30.0]], device=cuda)
     got = beams.select(x, s, 8)
     assert places(got, 3000) == want(x, s, 8)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [9000, 140001])
+def test_one_request_in_other_batches(cuda, dtype, vocab):
+    """Rows are cut by how many there are, so a request's sums may differ in their last bits from batch to batch: by no more than the errors
+    of two sums, and candidates further apart than that keep their places."""
+    x = (torch.randn(80, 4, vocab, generator=gen(vocab, cuda), device=cuda) * 3).to(dtype)
+    s = -torch.rand(80, 4, generator=gen(2, cuda), device=cuda).cumsum(1)
+    exact, off = define(x[:2], s[:2])                             # (2, 4 vocab), (2, 1)
+    best = torch.sort(exact, dim=1, descending=True)[0][:, :9]
+    gap = torch.minimum((best[:, :-1] - best[:, 1:]), torch.nn.functional.pad(best[:, :-2] - best[:, 1:-1], (1, 0), value=float("inf")))
+    clear = gap > 4 * off
+    sizes = (2, 3, 20, 80)
+    got = [[y[:2] for y in beams.select(x[:n], s[:n], 8)] for n in sizes]
+    for n, here in zip(sizes, got):
+        # twice the error of a sum, and the rounding of each score to float32
+        assert ((here[0].double() - got[0][0].double()).abs() <= 2 * off + best[:, :8].abs() * 2.0 ** -23).all()
+        assert all((a == b)[clear].all() for a, b in zip(here[1:], got[0][1:]))
+        assert all(torch.equal(a[:2], b) for a, b in zip(beams.select(x[:n], s[:n], 8), here))      # the same batch: the same bits
