@@ -15,5 +15,6 @@ def select(logits: torch.Tensor, scores: torch.Tensor, n: int = 0):
     beams; twice as many leave room for beams that end; up to 64 of each.  -> scores float32, parents int32, tokens int32, each
     (requests, n), best first: scores[r, parents] + log_softmax(logits[r, parents])[tokens], the lowest (beam, token) first among
     equals (of a beam whose score is -inf or NaN its first tokens).  NaN counts as -inf, +inf as the largest float.  The
-    same call gives the same bits; in a batch of another size a request's scores may differ in their last ones.  Two launches."""
+    same call gives the same bits; in a batch of another size a request's scores may differ in their last ones.  The three
+    are parts of one allocation: clone what is kept for long, resize none.  Two launches."""
     return _lib.host().select(logits, scores, n)

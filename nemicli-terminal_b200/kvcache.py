@@ -239,7 +239,8 @@ class KVCache:
         tokens in them, for attend_chosen.  q, tables, lens, starts as for attend (a positive scale is meant).  Of a query's pages the
         `first` first and the `last` last ones (1 at least: its own) are always chosen, of the others those whose box reaches
         furthest along some query head of the key head; all of them where there are no more than keep.  Rows that no sequence covers
-        get none.  Boxes of all pages but the query's own must have been written (summarise).  Two launches."""
+        get none.  Boxes of all pages but the query's own must have been written (summarise).  Both are parts of one allocation: clone what is
+        kept for long, resize none.  Two launches."""
         return _lib.host().choose(self._at, self._where, tables, lens, starts, bounds, q, keep, first, last)
 
     def attend_chosen(self, q: torch.Tensor, chosen: torch.Tensor, held: torch.Tensor, scale: Optional[float] = None,

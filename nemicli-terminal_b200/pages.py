@@ -8,7 +8,9 @@ include/nemicli_qmv.h, qmv_page_plan).
 Free pages are a stack in two tensors: `free` int32 (pages of the cache,) and `counts` int32 (2,): counts[0] entries of free
 count, the last is taken first; counts[1] is a running number of pages that were asked for in vain, which a caller looks at
 now and then, and sets to 0 when the sequences that lacked them have been released (`pool` makes both).  Everything is read on the device on torch's current stream and CUDA-graph safe.  Lengths and counts come back
-in new tensors, so that a call may be made again; tables and free are changed in place.  A captured step copies them back itself:
+in new tensors, so that a call may be made again; tables and free are changed in place.  A call's new tensors are parts of one allocation
+(one takes 0.6 us): it lives as long as any of them, and none of them is to be resized (`resize_` would grow into the next); clone what is kept
+for long.  A captured step copies lengths and counts back itself:
 
     step = pages.plan(lens, new, tables, free, counts, cache.page, rows)
     q = cache.write(k, v, step.slots, q=q, rope=(cos, sin, step.positions))
