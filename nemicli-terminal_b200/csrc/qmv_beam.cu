@@ -11,7 +11,7 @@
 // makes 16.  So candidates must cost nothing on the way: a lane notes the largest of its values of each step, which the softmax needs anyway,
 // and behind the last step a bound that n values reach leaves a few of these to be read again (looked for on the way they took twice the
 // instructions).  512 rows of 128256 bf16 logits, 16 candidates of 64 x 8 beams: 40.9 us both kernels (floor 20.1); without the look at the
-// candidates 35.5, without exponentials too 27.  4 rows of fp32 logits: 10.9, of which the join 4.6.
+// candidates 35.5, without exponentials too 27.  4 rows of fp32 logits: 10.9 to 11.4, of which the join 4.6.
 #include <algorithm>
 #include <climits>
 

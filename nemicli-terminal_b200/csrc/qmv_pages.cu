@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant
 
 // The same in one launch for few beams: a warp a request, in a cluster of up to eight CTAs (one SM alone was bound by its own instructions:
 // 1400 a warp, 9.2 us for 32 requests), the sums over the requests behind the cluster's barrier.  Bound by dependent reads: lengths and
-// parents, the tables, the freed pages.  Calls in a graph: 4 beams of 14 pages 4.8 us (two launches 9.3), 32 requests of
-// 8 beams of 21 pages 6.1 (15.4); with more entries a warp walks its request alone (8 x 8 x 130: 15.0, two launches 14.0).
+// parents, the tables, the freed pages.  Calls in a graph: 4 beams of 14 pages 4.0 us (two launches 9.3), 32 requests of
+// 8 beams of 21 pages 5.9 (15.4); with more entries a warp walks its request alone (8 x 8 x 130: 15.0, two launches 14.0).
 constexpr int kFewReqs = 32, kFewBeams = 8, kFewEntries = 1 << 13;    // requests, beams of each, entries of all tables
 __global__ void __launch_bounds__(32 * kFewReqs / 8) reorder_few_kernel(const __grid_constant__ ReorderParams P) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
