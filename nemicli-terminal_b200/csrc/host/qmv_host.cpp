@@ -232,6 +232,8 @@ PyObject* reorder(PyObject* const* a) {                           // lens, table
         expect(o, "pages.reorder own", t.device, ScalarType::Int, {reqs});
         own = ints(o);
     }
+    const int64_t nbytes = qmv_page_reorder_workspace_bytes(int(reqs), int(beams), t.width);
+    if (nbytes <= 0) refuse("pages.reorder: tables ", shape_of(t.tables), " of ", beams, " beams: up to 2^26 entries a request");
     Tensor tables, counts, lens, src, dst, used;
     {
         const OnDevice scope(t.device);
@@ -240,7 +242,6 @@ PyObject* reorder(PyObject* const* a) {                           // lens, table
         for (int i = 0; i < 4; ++i) o.plan({t.n}, ScalarType::Int);
         tables = o.take({t.n, t.width}, ScalarType::Int), counts = o.take({2}, ScalarType::Int), lens = o.take({t.n}, ScalarType::Int);
         src = o.take({t.n}, ScalarType::Int), dst = o.take({t.n}, ScalarType::Int), used = o.take({t.n}, ScalarType::Int);
-        const int64_t nbytes = qmv_page_reorder_workspace_bytes(int(reqs), int(beams), t.width);
         const Tensor ws = make({nbytes}, ScalarType::Byte, t.device);
         check(qmv_page_reorder(ints(parents), ints(t.lens), ints(t.tables), own, int(reqs), int(beams), t.width, t.page, ints(t.free), int(t.free.size(0)),
                                ints(t.counts), ints(tables), ints(lens), ints(src), ints(dst), ints(used), ints(counts), ws.data_ptr(), nbytes,

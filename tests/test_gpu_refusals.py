@@ -33,6 +33,9 @@ def test_numbers(cuda):
         with pytest.raises(RuntimeError, match="beams.select"):
             beams.select(x, s, n)
     t, v, free, counts = torch.zeros(2, 3, dtype=I32, device=cuda), torch.zeros(2, dtype=I32, device=cuda), *pages.pool(4, cuda)
+    wide = torch.zeros(64, (1 << 20) + 1, dtype=I32, device=cuda)
+    with pytest.raises(RuntimeError, match="pages.reorder: tables"):
+        pages.reorder(torch.zeros(1, 64, dtype=I32, device=cuda), torch.zeros(64, dtype=I32, device=cuda), wide, free, counts, 16)
     for page, rows in ((16.0, 2), (None, 2), (24, 2), (16, 2.5), (16, -1), (16, 1 << 31)):
         with pytest.raises(RuntimeError, match="pages.plan"):
             pages.plan(v, v, t, free, counts, page, rows)
